@@ -1,9 +1,10 @@
-"""Build in-tree, from ONE compilation of csrc/quartz_b200.cu for sm_100a:
+"""Build in-tree, from one compilation of the csrc/*.cu files (in parallel) for sm_100a:
   saient-quartz_b200/libquartz_b200.so  the CUDA library (what the tests and the benchmark load)
-  saient-quartz_b200/libkernels.a       the same object as a static archive under the name the reference's
+  saient-quartz_b200/libkernels.a       the same objects as a static archive under the name the reference's
                                         build.rs links (`static=kernels` + `cudart`, build.rs:52-72)
 and saient-quartz_b200/libquartz_host.so (the C++ host side of the decode step, a pure client of the C ABI)."""
 import os
+import re
 import subprocess
 import sys
 
@@ -11,7 +12,6 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libquartz_b200.so")
 ARCHIVE = os.path.join(HERE, "libkernels.a")
-OBJ = os.path.join(HERE, "kernels.o")
 HOST_LIB = os.path.join(HERE, "libquartz_host.so")
 HOST_SRC = os.path.join(HERE, "host", "forward_state.cpp")
 
@@ -26,6 +26,23 @@ def up_to_date():
     t = os.path.getmtime(LIB)
     hdr = os.path.join(HERE, "..", "include", "quartz_b200.h")
     return all(os.path.getmtime(s) <= t for s in sources() + [hdr])
+
+
+def included(src, seen=None):
+    """`src` and every file of this tree that it includes, directly or not."""
+    seen = set() if seen is None else seen
+    if src not in seen:
+        seen.add(src)
+        for name in re.findall(r'^#include "([^"]+)"', open(src).read(), re.M):
+            path = os.path.normpath(os.path.join(os.path.dirname(src), name))
+            if os.path.exists(path):
+                included(path, seen)
+    return seen
+
+
+def object_current(src, obj):
+    """The object is newer than its source, all that it includes and this file (compiler flags)."""
+    return os.path.exists(obj) and all(os.path.getmtime(f) <= os.path.getmtime(obj) for f in included(src) | {os.path.abspath(__file__)})
 
 
 def build_host(force=False):
@@ -50,20 +67,27 @@ def build(force=False, verbose=False):
     nvcc = os.path.join(os.environ.get("CUDA_HOME", "/usr/local/cuda"), "bin", "nvcc")
     arch = os.environ.get("QUARTZ_CUDA_ARCH", "sm_100a")   # same variable as the reference's build.rs:33
     cc = arch.replace("sm_", "compute_")
-    cmd = [nvcc, "-O3", "-std=c++17", "-gencode", f"arch={cc},code={arch}", "-lineinfo", "-Xcompiler", "-fPIC", "-c",
-           "-o", OBJ] + [s for s in sources() if s.endswith(".cu")]
+    cmd = [nvcc, "-O3", "-std=c++17", "-gencode", f"arch={cc},code={arch}", "-lineinfo", "-Xcompiler", "-fPIC", "-c"]
     cmd += os.environ.get("QUARTZ_NVCC_FLAGS", "").split()   # extra compiler flags (e.g. -DNAME=value)
     if verbose:
-        cmd.insert(1, "-Xptxas")
-        cmd.insert(2, "-v")
-    subprocess.check_call(cmd)
+        cmd[1:1] = ["-Xptxas", "-v"]
+    objs, running = [], []
+    for src in (s for s in sources() if s.endswith(".cu")):
+        obj = os.path.join(HERE, os.path.splitext(os.path.basename(src))[0] + ".o")
+        objs.append(obj)
+        if not force and object_current(src, obj):
+            continue
+        running.append((src, subprocess.Popen(cmd + ["-o", obj, src])))
+    failed = [src for src, p in running if p.wait() != 0]
+    if failed:
+        raise RuntimeError("nvcc failed on " + ", ".join(failed))
     tmp = LIB + ".tmp"
-    subprocess.check_call([nvcc, "-gencode", f"arch={cc},code={arch}", "-shared", "-o", tmp, OBJ])
+    subprocess.check_call([nvcc, "-gencode", f"arch={cc},code={arch}", "-shared", "-o", tmp] + objs)
     os.replace(tmp, LIB)   # a reader never sees a half-written library
     tmp = ARCHIVE + ".tmp"
     if os.path.exists(tmp):
         os.remove(tmp)
-    subprocess.check_call(["ar", "rcs", tmp, OBJ])
+    subprocess.check_call(["ar", "rcs", tmp] + objs)
     os.replace(tmp, ARCHIVE)
     build_host(force=True)
     return LIB

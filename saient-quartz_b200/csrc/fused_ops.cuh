@@ -5,6 +5,7 @@
 
 #include "decode_ops.cuh"
 #include "gemv_stream.cuh"
+#include "rope.cuh"
 
 namespace qz {
 
@@ -56,26 +57,6 @@ __global__ void swiglu_q_kernel(const float *__restrict__ gate, const float *__r
         }
     }
     quantize4_store(v, t, valid, o);
-}
-
-// rotation (cos, sin) of pair i at one position, exactly as rope_kv_kernel / src/cuda_kernels.cu:588-620 compute it
-struct RopeArgsLite {
-    int pos;
-    float theta, yarn_scale;
-    int yarn_orig_ctx;
-};
-__device__ __forceinline__ void rope_cs_lite(const RopeArgsLite &r, int i, int head_dim, float &c, float &s)
-{
-    const float PI = 3.14159265358979f;
-    float inv = 1.f / powf(r.theta, 2.f * (float)i / (float)head_dim);
-    float eff = inv;
-    if (r.yarn_scale > 1.f && r.yarn_orig_ctx > 0) {
-        float hi_w = (float)r.yarn_orig_ctx / 32.f, lo_w = (float)r.yarn_orig_ctx / 1.f;
-        float wavelen = 2.f * PI / inv;
-        float ramp = fmaxf(0.f, fminf(1.f, (lo_w - wavelen) / (lo_w - hi_w)));
-        eff = ramp * inv + (1.f - ramp) * (inv / r.yarn_scale);
-    }
-    sincosf((float)r.pos * eff, &s, &c);
 }
 
 // RoPE on q (n_heads) and k (n_kv_heads) in place, then append k, v to the caches at `pos`:
@@ -180,7 +161,6 @@ __global__ void rope_kv_rows_kernel(float *q, float *k, const float *__restrict_
 // handles query heads w, w+4, ...  Each (head, split) leaves (max, sum, unnormalised out[hd])
 // in a scratch buffer; attn_combine_kernel merges the splits.
 constexpr int ATT_CHUNK = 32;
-constexpr int ATT_MAX_HD = 128;
 
 __global__ void __launch_bounds__(128) attn_partial_kernel(float *__restrict__ part, const float *__restrict__ q,
                                                            const float *__restrict__ k_cache,
@@ -341,27 +321,6 @@ __global__ void attn_combine_kernel(float *__restrict__ out, const float *__rest
 // value into the caches and then stages them like any other row.  Partials as in
 // attn_partial_kernel; the CTA that finishes last for a kv head (a counter per kv head) merges that
 // head group's splits and emits the output projection's activation form.
-struct RopeArgs {
-    int pos;
-    float theta, yarn_scale;
-    int yarn_orig_ctx, neox;
-};
-
-// rotation (cos, sin) of pair i, exactly as rope_kv_kernel / src/cuda_kernels.cu:588-620 compute it
-__device__ __forceinline__ void rope_cs(const RopeArgs &r, int i, int head_dim, float &c, float &s)
-{
-    const float PI = 3.14159265358979f;
-    float inv = 1.f / powf(r.theta, 2.f * (float)i / (float)head_dim);
-    float eff = inv;
-    if (r.yarn_scale > 1.f && r.yarn_orig_ctx > 0) {
-        float hi_w = (float)r.yarn_orig_ctx / 32.f, lo_w = (float)r.yarn_orig_ctx / 1.f;
-        float wavelen = 2.f * PI / inv;
-        float ramp = fmaxf(0.f, fminf(1.f, (lo_w - wavelen) / (lo_w - hi_w)));
-        eff = ramp * inv + (1.f - ramp) * (inv / r.yarn_scale);
-    }
-    sincosf((float)r.pos * eff, &s, &c);
-}
-
 // (cos, sin) of every rotation pair at one position: the same for all layers and heads of a decode
 // step, so it is computed once per step instead of in every attention CTA
 __global__ void rope_table_kernel(float2 *__restrict__ tab, RopeArgs r, int head_dim)

@@ -19,6 +19,7 @@
 // copies (bounded) before it exits.
 #pragma once
 
+#include "async_copy.cuh"
 #include "gemv_formats_iq.cuh"
 #include "gemv_formats_k.cuh"
 #include "mgpu.cuh"
@@ -31,7 +32,6 @@ constexpr int TMA_MAX_STAGES = 16;
 #endif
 constexpr int TMA_CONSUMERS = QZ_TMA_CONSUMERS;
 constexpr int XSRC_MAX_IT = 4;             // float4 loads per consumer thread in the fused activation prologue
-constexpr long long TMA_WAIT_CYCLES = 2000000000LL;   // ~1 s at 1.9 GHz
 
 // Where the activation vector comes from.  mode 0: already converted (xq).  mode 1: RMSNorm of the
 // f32 vector a with weights b (src/cuda_kernels.cu:563-575, eps 1e-5 as there), mode 2: SwiGLU of
@@ -54,11 +54,6 @@ struct PrefetchHint {
     unsigned bytes[QZ_MAX_PREFETCH];   // per range, a multiple of 16
     int n;
 };
-
-__device__ __forceinline__ void l2_prefetch_bulk(const void *gmem, uint32_t bytes)
-{
-    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(gmem), "r"(bytes) : "memory");
-}
 
 // 16 KB pieces of every hinted range, piece j issued by CTA j % n_cta: the front of a range (what the successor
 // reads first) is requested first by everybody
@@ -88,49 +83,6 @@ struct TmaArgs {
     size_t sel_stride;
 };
 
-__device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
-
-__device__ __forceinline__ void mbar_init(uint64_t *bar, uint32_t count)
-{
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count));
-}
-__device__ __forceinline__ void mbar_arrive(uint64_t *bar)
-{
-    asm volatile("{ .reg .b64 st; mbarrier.arrive.shared::cta.b64 st, [%0]; }" ::"r"(smem_u32(bar)) : "memory");
-}
-__device__ __forceinline__ void mbar_arrive_expect_tx(uint64_t *bar, uint32_t bytes)
-{
-    asm volatile("{ .reg .b64 st; mbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1; }" ::"r"(smem_u32(bar)),
-                 "r"(bytes)
-                 : "memory");
-}
-__device__ __forceinline__ bool mbar_try_wait(uint64_t *bar, uint32_t parity)
-{
-    uint32_t ok;
-    asm volatile(
-        "{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-// Bounded wait; false = gave up.
-__device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity)
-{
-    if (mbar_try_wait(bar, parity)) return true;
-    const long long t0 = clock64();
-    while (!mbar_try_wait(bar, parity)) {
-        if (clock64() - t0 > TMA_WAIT_CYCLES) return false;
-    }
-    return true;
-}
-__device__ __forceinline__ void tma_load_1d(void *dst_smem, const void *src_gmem, uint32_t bytes, uint64_t *bar)
-{
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                     smem_u32(dst_smem)),
-                 "l"(src_gmem), "r"(bytes), "r"(smem_u32(bar))
-                 : "memory");
-}
 __device__ __forceinline__ void named_bar_sync(int id, int threads)
 {
     asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");

@@ -15,6 +15,7 @@
 #include <vector>
 
 #include "common.cuh"
+#include "host.cuh"
 #include "formats.cuh"
 #include "generic.cuh"
 #include "gemv_stream.cuh"
@@ -44,6 +45,9 @@ void set_error(int code, const char *what)
     }
 }
 cudaStream_t stream() { return g_stream; }
+static cudaStream_t g_graph_stream = nullptr, g_saved_stream = nullptr;
+// the stream the recorded graphs replay on (when there is one), so that the step words are ordered with the replays
+cudaStream_t replay_stream() { return (g_graph_stream && g_stream == 0) ? g_graph_stream : g_stream; }
 int sm_count()
 {
     if (!g_sm_count) {
@@ -55,30 +59,8 @@ int sm_count()
     return g_sm_count;
 }
 
-// ---- launch helper: ordinary launch, or programmatic dependent launch when enabled ----------
 static bool g_pdl = false;
-
-template <class... KArgs, class... Args>
-static void launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, Args... args)
-{
-    g_launch_count++;
-    if (g_pdl) {
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = grid;
-        cfg.blockDim = block;
-        cfg.dynamicSmemBytes = smem;
-        cfg.stream = g_stream;
-        cudaLaunchAttribute at[1];
-        at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        at[0].val.programmaticStreamSerializationAllowed = 1;
-        cfg.attrs = at;
-        cfg.numAttrs = 1;
-        QZ_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...));
-    } else {
-        kernel<<<grid, block, smem, g_stream>>>(KArgs(args)...);
-        QZ_CUDA_CHECK(cudaGetLastError());
-    }
-}
+bool pdl_enabled() { return g_pdl; }
 
 // ---- registry of repacked byte ranges ---------------------------------------------
 struct Range {
@@ -150,7 +132,7 @@ static XQMut xq_slot(uint8_t *base, size_t slot_bytes, int slot, size_t cap_k)
 // set by quartz_mgpu_fuse_next_wait: the next activation conversion first waits for the exchange
 static const MgpuCtrl *g_wait_ctrl = nullptr;
 static int g_wait_ranks = 0;
-static int *status_word();
+
 
 static void launch_quantize(const float *x, const XQMut &q, int K)
 {
@@ -235,7 +217,7 @@ static int stream_layout(uint32_t t)
 
 // ---- device status word written by kernels whose bounded waits gave up ------------------
 static int *g_status = nullptr;
-static int *status_word()
+int *status_word()
 {
     if (!g_status) {
         if (cudaMalloc(&g_status, sizeof(int)) != cudaSuccess) {
@@ -1741,13 +1723,11 @@ __global__ void step_set_kernel(int *step, int token, int pos, RopeSets sets)
     if (i == 0) e.tab[ATT_MAX_HD / 2] = make_float2(__int_as_float(pos), 0.f);
 }
 
-static cudaStream_t g_graph_stream = nullptr, g_saved_stream = nullptr;
 
 void cuda_step_set(int *d_step, int token, int pos)
 {
     if (!d_step) return;
-    // on the stream the recorded graphs replay on (when there is one), so the words are ordered with the replays
-    cudaStream_t s = (g_graph_stream && g_stream == 0) ? g_graph_stream : g_stream;
+    cudaStream_t s = replay_stream();
     RopeSets sets;
     sets.n = 0;
     for (int i = 0; i < g_rope_regs && sets.n < QZ_MAX_ROPE_SETS; i++)
@@ -2694,3 +2674,14 @@ void quartz_mgpu_shutdown(void)
 }
 
 }  // extern "C"
+
+namespace qz {
+
+bool activation_slot(int slot, int n, XQOut *o) { return user_slot(slot, n, o); }
+
+const float2 *step_rope_table(const int *d_step, int head_dim, float theta, float yarn_scale, int yarn_orig_ctx)
+{
+    return d_step ? rope_table_of(d_step, head_dim, theta, yarn_scale, yarn_orig_ctx) : nullptr;
+}
+
+}  // namespace qz
