@@ -239,6 +239,56 @@ void cuda_rope_kv_rows(float *q, float *k, const float *v, float *k_cache, float
 void cuda_attn_prompt(float *out, const float *q, const float *k_cache, const float *v_cache, int n_tok, int n_heads,
                       int n_kv_heads, int head_dim, int max_seq, int pos0, int window, float scale, const float *sinks);
 
+/* ---- A KV cache held in 4 bits, and attention over it (no counterparts in the reference, whose caches are f32,
+ * src/cuda.rs:361-492).  One buffer holds the keys and the values of one layer, 1.25 bytes per (key, value) pair of
+ * dims against 8 in f32.  Every 32 consecutive dims of one (position, kv head) share an f16 minimum m (rounded down)
+ * and an f16 step d (rounded up), a code 0..15 (nearest, ties to even) stands for m + 15 steps at most:
+ * |value - x| <= d / 2.  A group that holds a NaN or an infinity reads back as NaN; magnitudes above 65504 saturate.
+ * head_dim 32, 64, 96 or 128; buffers and rows are 16-byte aligned; a cache needs no initialisation: what lies behind
+ * the last appended position is never used.
+ *   cuda_kv4_bytes          size of a cache of max_seq positions (0: this geometry is not served)
+ *   cuda_kv4_append_rows    quantise rows k, v [n_tok, n_kv_heads*head_dim] into positions pos0 .. pos0+n_tok-1
+ *   cuda_rope_kv4_rows      cuda_rope_kv_rows with such a cache: q and k rotated in place, k and v appended
+ *                           (theta <= 0: nothing is rotated)
+ *   cuda_kv4_read_rows      the values of positions pos0 .. as f32 rows
+ *   cuda_attn_kv4_supported 1 if this head geometry is served: n_heads a multiple of n_kv_heads, at most 16 query
+ *                           heads per kv head
+ *   cuda_attn_step_kv4      cuda_attn_step over such a cache: rotation of q and k_new, append at the position, attention
+ *                           of all heads over [k_start, position], activation form of the result with out_slot >= 0,
+ *                           in one launch whose shape does not depend on the position.  The new position takes part
+ *                           with the values that it has in the cache.  theta <= 0: q and k_new are taken as they are
+ *                           (already rotated, or a layer without rotation); k_new and v_new NULL: nothing is
+ *                           appended, the cache holds the position already.
+ *   cuda_attn_prompt_kv4    cuda_attn_prompt over such a cache (rows appended before, e.g. by cuda_rope_kv4_rows) */
+size_t cuda_kv4_bytes(int max_seq, int n_kv_heads, int head_dim);
+void cuda_kv4_append_rows(void *d_cache, const float *k, const float *v, int n_tok, int n_kv_heads, int head_dim, int max_seq, int pos0);
+void cuda_rope_kv4_rows(float *q, float *k, const float *v, void *d_cache, int n_tok, int n_heads, int n_kv_heads, int head_dim,
+                        int max_seq, int pos0, float theta, float yarn_scale, int yarn_orig_ctx, int neox);
+void cuda_kv4_read_rows(float *k, float *v, const void *d_cache, int n_tok, int n_kv_heads, int head_dim, int max_seq, int pos0);
+int cuda_attn_kv4_supported(int n_heads, int n_kv_heads, int head_dim);
+void cuda_attn_step_kv4(float *out, const float *q, const float *k_new, const float *v_new, void *d_cache, int n_heads, int n_kv_heads,
+                        int head_dim, int max_seq, const int *d_step, int pos, int window, float scale, const float *sinks, float theta,
+                        float yarn_scale, int yarn_orig_ctx, int neox, int out_slot);
+void cuda_attn_prompt_kv4(float *out, const float *q, const void *d_cache, int n_tok, int n_heads, int n_kv_heads, int head_dim,
+                          int max_seq, int pos0, int window, float scale, const float *sinks);
+
+/* ---- The next token, chosen on the device (the reference copies the logits to the host and samples there).
+ * cuda_sample: for each of n_rows rows of d_logits (row r at r * row_stride floats) and a uniform random number d_u[r]
+ * in [0, 1) the token into d_tokens[r] and, with d_probs, its probability among the kept tokens.  Token i weighs
+ * exp((z_i - max z) / temperature); tokens are ordered by logit, ties by the lower index.  Kept are the first top_k of
+ * that order (top_k <= 0: all), of those the shortest prefix whose weights reach top_p of their sum (top_p >= 1: all;
+ * <= 0: the first only), of those the ones that weigh at least min_p (<= 0: all; above 1 counts as 1).  The answer
+ * is the first token in the order of the vocabulary at which the running sum of the kept weights exceeds u times their
+ * total; u below 0 or NaN counts as 0, from 1 on the last token of weight is taken.  Weights are whole numbers of
+ * units of 2^-44: a token below half a unit is never chosen.  temperature 0: the largest logit, ties to the lower index (d_u may be NULL), probability 1.  Logits of -inf
+ * and NaN are never chosen; a row without any other gives token -1, probability 0.  The sums are exact integers: the
+ * same inputs give the same token however the work is split.  vocab <= 524288, finite temperature >= 0.
+ * cuda_step_advance: d_step[0] = *d_token (left as it is if that is negative), d_step[1] += 1, and the registered RoPE
+ * tables of d_step (cuda_step_rope_table) for the new position: the device-side cuda_step_set, on the same stream. */
+void cuda_sample(const float *d_logits, int n_rows, int vocab, size_t row_stride, float temperature, int top_k, float top_p, float min_p,
+                 const float *d_u, int *d_tokens, float *d_probs);
+void cuda_step_advance(int *d_step, const int *d_token);
+
 /* A chain of dependent GEMVs as ONE persistent kernel (one CTA per SM): op k+1's activation vector is
  * computed from op k's outputs after a grid-wide barrier inside the kernel, while the weight rows of
  * op k+1 are already streaming.  In the reference every link is a kernel boundary (src/cuda.rs:548-823:

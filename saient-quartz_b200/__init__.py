@@ -107,6 +107,16 @@ _SIGS = {
     "cuda_rms_norm_rows": (None, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int]),
     "cuda_rope_kv_rows": (None, [C.c_void_p] * 5 + [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_float, C.c_float, C.c_int, C.c_int]),
     "cuda_attn_prompt": (None, [C.c_void_p] * 4 + [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_float, C.c_void_p]),
+    "cuda_kv4_bytes": (C.c_size_t, [C.c_int, C.c_int, C.c_int]),
+    "cuda_kv4_append_rows": (None, [C.c_void_p] * 3 + [C.c_int] * 5),
+    "cuda_rope_kv4_rows": (None, [C.c_void_p] * 4 + [C.c_int] * 6 + [C.c_float, C.c_float, C.c_int, C.c_int]),
+    "cuda_kv4_read_rows": (None, [C.c_void_p] * 3 + [C.c_int] * 5),
+    "cuda_attn_kv4_supported": (C.c_int, [C.c_int, C.c_int, C.c_int]),
+    "cuda_attn_step_kv4": (None, [C.c_void_p] * 5 + [C.c_int] * 4 + [C.c_void_p, C.c_int, C.c_int, C.c_float, C.c_void_p, C.c_float,
+                                  C.c_float, C.c_int, C.c_int, C.c_int]),
+    "cuda_attn_prompt_kv4": (None, [C.c_void_p] * 3 + [C.c_int] * 7 + [C.c_float, C.c_void_p]),
+    "cuda_sample": (None, [C.c_void_p, C.c_int, C.c_int, C.c_size_t, C.c_float, C.c_int, C.c_float, C.c_float] + [C.c_void_p] * 3),
+    "cuda_step_advance": (None, [C.c_void_p, C.c_void_p]),
     "cuda_gemv_experts": (None, [C.c_uint32, C.c_void_p, C.c_size_t, C.c_void_p, C.c_int, C.c_void_p, C.c_size_t, C.c_void_p,
                                  C.c_int, C.c_int]),
     "cuda_moe_decode_act": (None, [C.c_void_p] * 6 + [C.c_int, C.c_int, C.c_int]),

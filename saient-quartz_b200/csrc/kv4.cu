@@ -1,0 +1,154 @@
+// C entry points of the 4-bit KV cache and of the attention over it.
+#include "attn_kv4.cuh"
+#include "host.cuh"
+
+using namespace qz;
+
+namespace {
+
+constexpr const char *GEOMETRY = "head_dim must be 32, 64, 96 or 128";
+
+bool head_dim_ok(int head_dim) { return head_dim > 0 && head_dim % 32 == 0 && head_dim <= ATT_MAX_HD; }
+bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
+// Arguments that every call on a cache shares; records what is wrong.
+bool cache_ok(const char *who, const void *cache, int n_kv_heads, int head_dim, int max_seq)
+{
+    static char msg[160];
+    const char *why = !head_dim_ok(head_dim) ? GEOMETRY
+                      : n_kv_heads <= 0 || max_seq <= 0 ? "n_kv_heads and max_seq must be positive"
+                      : !cache || !aligned16(cache) ? "the cache must be a 16-byte aligned device pointer" : nullptr;
+    if (!why) return true;
+    snprintf(msg, sizeof msg, "%s: %s", who, why);
+    set_error(QZ_ERR_BAD_SHAPE, msg);
+    return false;
+}
+
+bool refuse(const char *why)
+{
+    set_error(QZ_ERR_BAD_SHAPE, why);
+    return false;
+}
+
+// NG = head_dim / 32 as a template argument
+template <class F>
+void by_groups(int head_dim, F f)
+{
+    switch (head_dim / 32) {
+    case 1: f(std::integral_constant<int, 1>()); break;
+    case 2: f(std::integral_constant<int, 2>()); break;
+    case 3: f(std::integral_constant<int, 3>()); break;
+    default: f(std::integral_constant<int, 4>()); break;
+    }
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t cuda_kv4_bytes(int max_seq, int n_kv_heads, int head_dim)
+{
+    if (max_seq <= 0 || n_kv_heads <= 0 || !head_dim_ok(head_dim)) return 0;
+    return (size_t)n_kv_heads * kv4_blocks(max_seq) * kv4_block_bytes(head_dim);
+}
+
+void cuda_kv4_append_rows(void *d_cache, const float *k, const float *v, int n_tok, int n_kv_heads, int head_dim, int max_seq, int pos0)
+{
+    if (n_tok == 0 || !cache_ok("cuda_kv4_append_rows", d_cache, n_kv_heads, head_dim, max_seq)) return;
+    if (n_tok < 0 || pos0 < 0 || (long long)pos0 + n_tok > max_seq) {
+        refuse("cuda_kv4_append_rows: 0 <= pos0 and pos0 + n_tok <= max_seq");
+        return;
+    }
+    if (!k || !v || !aligned16(k) || !aligned16(v)) {
+        refuse("cuda_kv4_append_rows: k and v must be 16-byte aligned");
+        return;
+    }
+    const long long rows = (long long)n_tok * n_kv_heads, threads = rows * (head_dim / 8);
+    by_groups(head_dim, [&](auto ng) {
+        launch(kv4_append_kernel<ng.value>, dim3((unsigned)((threads + 255) / 256), 2), dim3(256), 0, (uint8_t *)d_cache, k, v, rows, n_kv_heads,
+               kv4_blocks(max_seq), pos0);
+    });
+}
+
+void cuda_kv4_read_rows(float *k, float *v, const void *d_cache, int n_tok, int n_kv_heads, int head_dim, int max_seq, int pos0)
+{
+    if (n_tok == 0 || !cache_ok("cuda_kv4_read_rows", d_cache, n_kv_heads, head_dim, max_seq)) return;
+    if (n_tok < 0 || pos0 < 0 || (long long)pos0 + n_tok > max_seq) {
+        refuse("cuda_kv4_read_rows: 0 <= pos0 and pos0 + n_tok <= max_seq");
+        return;
+    }
+    if (!k || !v || !aligned16(k) || !aligned16(v)) {
+        refuse("cuda_kv4_read_rows: k and v must be 16-byte aligned");
+        return;
+    }
+    const long long rows = (long long)n_tok * n_kv_heads, threads = rows * (head_dim / 8);
+    by_groups(head_dim, [&](auto ng) {
+        launch(kv4_read_kernel<ng.value>, dim3((unsigned)((threads + 255) / 256), 2), dim3(256), 0, k, v, (const uint8_t *)d_cache, rows, n_kv_heads,
+               kv4_blocks(max_seq), pos0);
+    });
+}
+
+void cuda_rope_kv4_rows(float *q, float *k, const float *v, void *d_cache, int n_tok, int n_heads, int n_kv_heads, int head_dim, int max_seq,
+                        int pos0, float theta, float yarn_scale, int yarn_orig_ctx, int neox)
+{
+    if (n_tok == 0 || !cache_ok("cuda_rope_kv4_rows", d_cache, n_kv_heads, head_dim, max_seq)) return;
+    if (n_tok < 0 || n_tok > 65535 || n_heads <= 0 || pos0 < 0 || (long long)pos0 + n_tok > max_seq) {
+        refuse("cuda_rope_kv4_rows: 0 <= pos0, pos0 + n_tok <= max_seq, n_tok <= 65535");
+        return;
+    }
+    if (!q || !k || !v) {
+        refuse("cuda_rope_kv4_rows: q, k and v must be device pointers");
+        return;
+    }
+    by_groups(head_dim, [&](auto ng) {
+        launch(rope_kv4_rows_kernel<ng.value>, dim3(n_heads + n_kv_heads, n_tok), dim3(64), 0, q, k, v, (uint8_t *)d_cache, n_heads, n_kv_heads,
+               kv4_blocks(max_seq), pos0, theta, yarn_scale, yarn_orig_ctx, neox);
+    });
+}
+
+int cuda_attn_kv4_supported(int n_heads, int n_kv_heads, int head_dim)
+{
+    return n_heads > 0 && n_kv_heads > 0 && n_heads % n_kv_heads == 0 && n_heads / n_kv_heads <= AK_MAX_G && head_dim_ok(head_dim) ? 1 : 0;
+}
+
+void cuda_attn_step_kv4(float *out, const float *q, const float *k_new, const float *v_new, void *d_cache, int n_heads, int n_kv_heads,
+                        int head_dim, int max_seq, const int *d_step, int pos, int window, float scale, const float *sinks, float theta,
+                        float yarn_scale, int yarn_orig_ctx, int neox, int out_slot)
+{
+    if (!cache_ok("cuda_attn_step_kv4", d_cache, n_kv_heads, head_dim, max_seq)) return;
+    if (!cuda_attn_kv4_supported(n_heads, n_kv_heads, head_dim) || (!d_step && (pos < 0 || pos >= max_seq))) {
+        refuse("cuda_attn_step_kv4: n_heads a multiple of n_kv_heads, at most 16 query heads per kv head, 0 <= pos < max_seq");
+        return;
+    }
+    if (!out || !q || !aligned16(out) || !aligned16(q) || (!k_new) != (!v_new) || !aligned16(k_new) || !aligned16(v_new)) {
+        refuse("cuda_attn_step_kv4: out and q must be 16-byte aligned device pointers, k_new and v_new too or both NULL");
+        return;
+    }
+    AttnKv4Args a = {out, q, k_new, v_new, (uint8_t *)d_cache, d_step, pos, n_heads, n_kv_heads, max_seq, kv4_blocks(max_seq), window, scale, sinks,
+                     theta, yarn_scale, yarn_orig_ctx, neox, XQOut{nullptr, nullptr, nullptr, nullptr}, 0,
+                     theta > 0.f ? step_rope_table(d_step, head_dim, theta, yarn_scale, yarn_orig_ctx) : nullptr};
+    if (out_slot >= 0) {
+        if (!activation_slot(out_slot, n_heads * head_dim, &a.o)) return;
+        a.emit_q = 1;
+    }
+    by_groups(head_dim, [&](auto ng) { launch(attn_kv4_kernel<ng.value>, dim3(n_kv_heads), dim3(AK_THREADS), 0, a); });
+}
+
+void cuda_attn_prompt_kv4(float *out, const float *q, const void *d_cache, int n_tok, int n_heads, int n_kv_heads, int head_dim, int max_seq,
+                          int pos0, int window, float scale, const float *sinks)
+{
+    if (n_tok == 0 || !cache_ok("cuda_attn_prompt_kv4", d_cache, n_kv_heads, head_dim, max_seq)) return;
+    if (!cuda_attn_kv4_supported(n_heads, n_kv_heads, head_dim) || n_tok < 0 || n_tok > 65535 || pos0 < 0 || (long long)pos0 + n_tok > max_seq) {
+        refuse("cuda_attn_prompt_kv4: n_heads a multiple of n_kv_heads, at most 16 query heads per kv head, pos0 + n_tok <= max_seq, n_tok <= 65535");
+        return;
+    }
+    if (!out || !q || !aligned16(out) || !aligned16(q)) {
+        refuse("cuda_attn_prompt_kv4: out and q must be 16-byte aligned device pointers");
+        return;
+    }
+    const AttnKv4Args a = {out, q, nullptr, nullptr, (uint8_t *)d_cache, nullptr, pos0, n_heads, n_kv_heads, max_seq, kv4_blocks(max_seq), window, scale,
+                           sinks, 0.f, 1.f, 0, 0, XQOut{nullptr, nullptr, nullptr, nullptr}, 0, nullptr};
+    by_groups(head_dim, [&](auto ng) { launch(attn_kv4_kernel<ng.value>, dim3(n_kv_heads, n_tok), dim3(AK_THREADS), 0, a); });
+}
+
+}  // extern "C"

@@ -19,7 +19,8 @@
 //   parameters: NG halves m, then NG halves d.
 #pragma once
 
-#include "fused_ops.cuh"
+#include "activation.cuh"
+#include "rope.cuh"
 
 namespace qz {
 
@@ -37,8 +38,8 @@ __device__ __forceinline__ uint8_t *kv4_block(uint8_t *cache, int n_blocks, int 
 // 64 bits, where every quantity is exact for operands within 2^29 of one another.
 __device__ __forceinline__ void kv4_params(float lo, float hi, __half &m, __half &d)
 {
-    m = __float2half_rd(fmaxf(lo, -65504.f));
-    const double span = (double)hi - (double)__half2float(m);
+    m = __float2half_rd(fmaxf(lo, -65504.f) + 0.f);   // (+ 0: a minimum of -0 is stored as 0)
+    const double span = fmax((double)hi - (double)__half2float(m), 0.0);
     float df = __half2float(__float2half_ru(fminf((float)(span * (1.0 / 15.0)), 65504.f)));
     // the product above may be one ulp (of f32) to either side of span / 15: at most one f16 away from the answer
     if (15.0 * (double)df < span && df < 65504.f) df = __half2float(__ushort_as_half((unsigned short)(__half_as_ushort(__float2half_rn(df)) + 1)));

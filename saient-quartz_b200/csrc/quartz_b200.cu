@@ -1701,6 +1701,31 @@ struct RopeReg { const int *step; RopeSetDev d; };
 static RopeReg g_rope_reg[16];
 static int g_rope_regs = 0;
 
+__device__ __forceinline__ void rope_set_write(const RopeSetDev &e, int i, int pos)
+{
+    if (i < e.head_dim / 2) {
+        const RopeArgs r{pos, e.theta, e.yarn_scale, e.yarn_orig_ctx, 0};
+        float c, s;
+        rope_cs(r, i, e.head_dim, c, s);
+        e.tab[i] = make_float2(c, s);
+    }
+    if (i == 0) e.tab[ATT_MAX_HD / 2] = make_float2(__int_as_float(pos), 0.f);
+}
+
+__global__ void step_advance_kernel(int *step, const int *__restrict__ token, RopeSets sets)
+{
+    pdl_wait();
+    pdl_trigger();
+    const int pos = step[1] + 1;
+    __syncthreads();   // every thread has read the position
+    const int set = threadIdx.x / (ATT_MAX_HD / 2);
+    if (set < sets.n) rope_set_write(sets.s[set], threadIdx.x % (ATT_MAX_HD / 2), pos);
+    if (threadIdx.x == 0) {
+        if (*token >= 0) step[0] = *token;
+        step[1] = pos;
+    }
+}
+
 __global__ void step_set_kernel(int *step, int token, int pos, RopeSets sets)
 {
     pdl_wait();
@@ -1712,26 +1737,35 @@ __global__ void step_set_kernel(int *step, int token, int pos, RopeSets sets)
         }
         return;
     }
-    const RopeSetDev &e = sets.s[blockIdx.x - 1];
-    const int i = threadIdx.x;
-    if (i < e.head_dim / 2) {
-        const RopeArgs r{pos, e.theta, e.yarn_scale, e.yarn_orig_ctx, 0};
-        float c, s;
-        rope_cs(r, i, e.head_dim, c, s);
-        e.tab[i] = make_float2(c, s);
-    }
-    if (i == 0) e.tab[ATT_MAX_HD / 2] = make_float2(__int_as_float(pos), 0.f);
+    rope_set_write(sets.s[blockIdx.x - 1], threadIdx.x, pos);
 }
 
+
+static RopeSets rope_sets_of(const int *d_step)
+{
+    RopeSets sets;
+    sets.n = 0;
+    for (int i = 0; i < g_rope_regs && sets.n < QZ_MAX_ROPE_SETS; i++)
+        if (g_rope_reg[i].step == d_step) sets.s[sets.n++] = g_rope_reg[i].d;
+    return sets;
+}
+
+void cuda_step_advance(int *d_step, const int *d_token)
+{
+    if (!d_step || !d_token) {
+        set_error(QZ_ERR_BAD_SHAPE, "cuda_step_advance: d_step and d_token must be device pointers");
+        return;
+    }
+    // one block: the position word is read by all of it before one thread changes it
+    step_advance_kernel<<<1, QZ_MAX_ROPE_SETS * (ATT_MAX_HD / 2), 0, replay_stream()>>>(d_step, d_token, rope_sets_of(d_step));
+    QZ_LAUNCH_CHECK();
+}
 
 void cuda_step_set(int *d_step, int token, int pos)
 {
     if (!d_step) return;
     cudaStream_t s = replay_stream();
-    RopeSets sets;
-    sets.n = 0;
-    for (int i = 0; i < g_rope_regs && sets.n < QZ_MAX_ROPE_SETS; i++)
-        if (g_rope_reg[i].step == d_step) sets.s[sets.n++] = g_rope_reg[i].d;
+    const RopeSets sets = rope_sets_of(d_step);
     step_set_kernel<<<1 + sets.n, ATT_MAX_HD / 2, 0, s>>>(d_step, token, pos, sets);
     QZ_LAUNCH_CHECK();
 }
