@@ -1,6 +1,9 @@
 // Attention over the 4-bit cache (kv4.cuh): one token of a decode step, or the tokens of a prompt.
 #pragma once
 
+#include <cooperative_groups.h>
+
+#include "async_copy.cuh"
 #include "kv4.cuh"
 
 namespace qz {
@@ -23,7 +26,14 @@ struct AttnKv4Args {
     XQOut o;
     int emit_q;
     const float2 *rope_tab;
+    int splits;                          // clusters that share a kv head's query heads
+    int prefetch;                        // the launch may overlap the one before it: fetch into L2 ahead of the wait
+    int *status;
 };
+
+// split cluster barrier (every thread of the CTA executes both halves)
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 // One CTA per (kv head, token); a warp takes every eighth position for one query head after the other.
 template <int NG>
@@ -122,6 +132,584 @@ __global__ void __launch_bounds__(AK_THREADS) attn_kv4_kernel(const AttnKv4Args 
             float v[4] = {0.f, 0.f, 0.f, 0.f};
             for (int j = 0; j < 4 && valid; j++) v[j] = qs[i + j];
             quantize4_store(v, (head * G * HD + i) >> 2, valid, a.o);
+        }
+    }
+}
+
+// ---- one token ---------------------------------------------------------------------------------------------------
+// One launch whose shape does not depend on the position.  A cluster of CL CTAs per kv head (two per kv head when more
+// than eight query heads share it); warp w of CTA r takes the blocks of 32 positions r + CL (w + 8 i), so that a short
+// context is spread over the CTAs first.  A warp works alone: it streams its blocks through a ring of its own (one bulk
+// copy per block: the block is contiguous) and keeps scores, weights and outputs of all heads in registers.
+//
+// Both products run on the tensor cores with the CODES as one operand, exactly, and 22 bits of the other:
+//   scores   s[pos, head] = sum_g d_g ((codes_g - 8) . q_g) + (m_g + 8 d_g) sum(q_g)
+//   outputs  o[dim, head] = sum_pos (codes[dim, pos] - 8) (p d_g)[pos, head]  +  sum_pos (p (m_g + 8 d_g))[pos, head]
+// The codes are taken around 8 because the two terms of either line otherwise cancel (m is a group's minimum).  A nibble
+// becomes the f16 number code - 8, two at a time, by one logical operation (1024 + code or 1024 + 16 code: the nibble in
+// the mantissa) and one exact HADD2 / HFMA2.  (The nibbles alone, as f16 subnormals, would need no second step, but the
+// tensor core aligns products by their nominal exponents: 6 to 10 bits of the sum were lost, 5e-6 of the output.)
+// q and p * d are split into two f16 parts, hi + lo, in neighbouring columns of the 8-column operand, so four heads fill
+// one mma.m16n8k16; both parts are scaled by powers of two (per head for q, per warp for d) that keep them clear of
+// f16's ends.  Sums are f32.
+// The softmax reference of a head is raised only when a score exceeds it by 2^8; until then weights up to 2^8 do no harm.
+constexpr int AK_STAGES = 4;
+
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float ex2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi)
+{
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *(const uint32_t *)&h;
+}
+// The four pairs (i, i + 4) of a word's eight nibbles as pairs of f16 numbers code - 8.
+__device__ __forceinline__ void kv4_pairs(uint32_t w, uint32_t (&x)[4])
+{
+    const __half2 m1032 = __half2half2(__ushort_as_half((unsigned short)0xE408)), m72 = __half2half2(__ushort_as_half((unsigned short)0xD480)),
+                  sixteenth = __half2half2(__ushort_as_half((unsigned short)0x2C00));
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {
+        const uint32_t v = i ? w >> 8 : w;
+        const uint32_t even = (v & 0x000F000Fu) | 0x64006400u, odd = (v & 0x00F000F0u) | 0x64006400u;   // 1024 + c, 1024 + 16 c
+        const __half2 e = __hadd2(*(const __half2 *)&even, m1032), o = __hfma2(*(const __half2 *)&odd, sixteenth, m72);
+        x[i] = *(const uint32_t *)&e;
+        x[i + 1] = *(const uint32_t *)&o;
+    }
+}
+// N halves (N = 1..4) at a 2N-aligned address, as floats
+template <int N>
+__device__ __forceinline__ void lds_halves(const void *p, float (&x)[N])
+{
+    if constexpr (N == 4) {
+        const uint2 w = *(const uint2 *)p;
+        const float2 a = __half22float2(*(const __half2 *)&w.x), b = __half22float2(*(const __half2 *)&w.y);
+        x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y;
+    } else if constexpr (N == 2) {
+        const float2 a = __half22float2(*(const __half2 *)p);
+        x[0] = a.x; x[1] = a.y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) x[i] = __half2float(((const __half *)p)[i]);
+    }
+}
+template <int N>
+__device__ __forceinline__ void lds_words(const void *p, uint32_t (&x)[N])
+{
+    if constexpr (N == 4) {
+        const uint4 w = *(const uint4 *)p;
+        x[0] = w.x; x[1] = w.y; x[2] = w.z; x[3] = w.w;
+    } else if constexpr (N == 2) {
+        const uint2 w = *(const uint2 *)p;
+        x[0] = w.x; x[1] = w.y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) x[i] = ((const uint32_t *)p)[i];
+    }
+}
+// the 16-bit words j of two positions side by side: out[j] = a[j] | b[j] << 16
+template <int N>
+__device__ __forceinline__ void lds_pairs(const void *a, const void *b, uint32_t (&out)[N])
+{
+    if constexpr (N == 4) {
+        const uint2 x = *(const uint2 *)a, y = *(const uint2 *)b;
+        out[0] = __byte_perm(x.x, y.x, 0x5410); out[1] = __byte_perm(x.x, y.x, 0x7632);
+        out[2] = __byte_perm(x.y, y.y, 0x5410); out[3] = __byte_perm(x.y, y.y, 0x7632);
+    } else if constexpr (N == 2) {
+        const uint32_t x = *(const uint32_t *)a, y = *(const uint32_t *)b;
+        out[0] = __byte_perm(x, y, 0x5410); out[1] = __byte_perm(x, y, 0x7632);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) out[i] = (uint32_t)((const uint16_t *)a)[i] | (uint32_t)((const uint16_t *)b)[i] << 16;
+    }
+}
+
+// The running state of a warp over the blocks of one kv head, for 4 NT heads, and one block's turn.
+// lane = 4 gr + t.  Scores: rows gr, gr + 8 of a tile of 16 positions, columns (hi, lo) of head t.  Outputs: dims
+// 32 j + 4 gr + i of head t.  Weights as operand: head gr / 2 (part gr % 2), positions t, t + 4, t + 8, t + 12 of a tile.
+template <int NG, int NT>
+struct Kv4Warp {
+    uint32_t qf[NT][NG][4];   // q as the column operand: dims (0,4) (1,5) (2,6) (3,7) of 32 j + 8 t, column gr
+    float qs[NT][NG];         // sum of q over group j in units of 1 / back, head t
+    float back[NT];           // scores in log2 units = back * what the products give, head t
+    float ref[NT], l[NT];     // reference and partial sum of weights, head t
+    float o[NT][2 * NG][4];
+    float mo[NT][NG];         // partial sums of p * m, head gr / 2
+    float ve;                 // power of two that p * d carries
+
+    __device__ __forceinline__ void clear()
+    {
+        ve = 1.2676506e30f;   // 2^100: the first block with a step above zero sets it
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            ref[n] = -3.0e38f;
+            l[n] = 0.f;
+#pragma unroll
+            for (int j = 0; j < NG; j++) mo[n][j] = 0.f;
+#pragma unroll
+            for (int j = 0; j < 2 * NG; j++) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.f;
+        }
+    }
+
+    // rows lo .. hi of the block are visible (the parameters of the others are finite)
+    __device__ __forceinline__ void block(const uint8_t *blk, int lo, int hi, int lane)
+    {
+        constexpr int HD = 32 * NG, ROW = HD / 2, PAR = 4 * NG;
+        const int gr = lane >> 2, t = lane & 3;
+        float s[2][NT][2];
+        // ---- scores ----
+#pragma unroll
+        for (int tile = 0; tile < 2; tile++) {
+            const int r0 = 16 * tile + gr, r1 = r0 + 8;
+            uint32_t k0[NG], k1[NG];
+            float m0[NG], m1[NG], d0[NG], d1[NG];
+            lds_words<NG>(blk + r0 * ROW + 4 * NG * t, k0);
+            lds_words<NG>(blk + r1 * ROW + 4 * NG * t, k1);
+            const uint8_t *p0 = blk + 16 * HD + r0 * PAR, *p1 = blk + 16 * HD + r1 * PAR;
+            lds_halves<NG>(p0, m0);
+            lds_halves<NG>(p0 + 2 * NG, d0);
+            lds_halves<NG>(p1, m1);
+            lds_halves<NG>(p1 + 2 * NG, d1);
+#pragma unroll
+            for (int j = 0; j < NG; j++) {
+                m0[j] = fmaf(8.f, d0[j], m0[j]);
+                m1[j] = fmaf(8.f, d1[j], m1[j]);
+            }
+#pragma unroll
+            for (int n = 0; n < NT; n++) s[tile][n][0] = s[tile][n][1] = 0.f;
+#pragma unroll
+            for (int j = 0; j < NG; j++) {
+                uint32_t x[4], y[4];
+                kv4_pairs(k0[j], x);
+                kv4_pairs(k1[j], y);
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    float c[4] = {0.f, 0.f, 0.f, 0.f};
+                    mma16816(c, x[0], y[0], x[1], y[1], qf[n][j][0], qf[n][j][1]);
+                    mma16816(c, x[2], y[2], x[3], y[3], qf[n][j][2], qf[n][j][3]);
+                    s[tile][n][0] = fmaf(d0[j], c[0] + c[1], fmaf(m0[j], qs[n][j], s[tile][n][0]));
+                    s[tile][n][1] = fmaf(d1[j], c[2] + c[3], fmaf(m1[j], qs[n][j], s[tile][n][1]));
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                s[tile][n][0] = r0 >= lo && r0 <= hi ? s[tile][n][0] * back[n] : -INFINITY;
+                s[tile][n][1] = r1 >= lo && r1 <= hi ? s[tile][n][1] * back[n] : -INFINITY;
+            }
+        }
+        // ---- reference ----
+        bool raise = false;
+#pragma unroll
+        for (int n = 0; n < NT; n++) raise |= fmaxf(fmaxf(s[0][n][0], s[0][n][1]), fmaxf(s[1][n][0], s[1][n][1])) > ref[n] + 8.f;
+        if (__any_sync(0xFFFFFFFFu, raise)) {
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                float top = fmaxf(fmaxf(s[0][n][0], s[0][n][1]), fmaxf(s[1][n][0], s[1][n][1]));
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, x));
+                top = fmaxf(top, ref[n]);
+                const float corr = ex2(ref[n] - top);
+                ref[n] = top;
+                l[n] *= corr;
+                const float corr_m = __shfl_sync(0xFFFFFFFFu, corr, gr >> 1);   // of the head whose weights this lane carries
+#pragma unroll
+                for (int j = 0; j < NG; j++) mo[n][j] *= corr_m;
+#pragma unroll
+                for (int j = 0; j < 2 * NG; j++) {
+                    o[n][j][0] *= corr; o[n][j][1] *= corr; o[n][j][2] *= corr; o[n][j][3] *= corr;
+                }
+            }
+        }
+        // ---- outputs ----
+        const uint8_t *vb = blk + 20 * HD;
+        const int part = gr & 1;
+        const float lo_part = (float)part;
+#pragma unroll
+        for (int tile = 0; tile < 2; tile++) {
+            const int r = 16 * tile + t;
+            float d[4][NG];
+#pragma unroll
+            for (int i = 0; i < 4; i++) lds_halves<NG>(vb + 16 * HD + (r + 4 * i) * PAR + 2 * NG, d[i]);
+            // the step's scale: largest of d stays below 2^7 (weights are at most 2^8: products below 2^15)
+            float dm = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int j = 0; j < NG; j++) dm = fmaxf(dm, d[i][j]);
+            rescale(dm);
+            float m[2][NG];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                lds_halves<NG>(vb + 16 * HD + (r + 8 * part + 4 * i) * PAR, m[i]);
+#pragma unroll
+                for (int j = 0; j < NG; j++) m[i][j] = fmaf(8.f, part ? d[2 + i][j] : d[i][j], m[i][j]);
+            }
+            uint32_t v01[NG], v23[NG];
+            lds_pairs<NG>(vb + r * ROW + 2 * NG * gr, vb + (r + 4) * ROW + 2 * NG * gr, v01);
+            lds_pairs<NG>(vb + (r + 8) * ROW + 2 * NG * gr, vb + (r + 12) * ROW + 2 * NG * gr, v23);
+            uint32_t x[NG][4], y[NG][4];   // dims 4 gr + 0 .. 3 of positions (t, t + 4) and (t + 8, t + 12)
+#pragma unroll
+            for (int j = 0; j < NG; j++) {
+                kv4_pairs(v01[j], x[j]);
+                kv4_pairs(v23[j], y[j]);
+            }
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                const float w0 = ex2(s[tile][n][0] - ref[n]), w1 = ex2(s[tile][n][1] - ref[n]);
+                l[n] += w0 + w1;
+                const int src = 4 * t + (gr >> 1);
+                float p[4];
+                p[0] = __shfl_sync(0xFFFFFFFFu, w0, src);
+                p[1] = __shfl_sync(0xFFFFFFFFu, w0, src + 16);
+                p[2] = __shfl_sync(0xFFFFFFFFu, w1, src);
+                p[3] = __shfl_sync(0xFFFFFFFFu, w1, src + 16);
+                const float pm0 = part ? p[2] : p[0], pm1 = part ? p[3] : p[1];
+#pragma unroll
+                for (int i = 0; i < 4; i++) p[i] *= ve;
+#pragma unroll
+                for (int j = 0; j < NG; j++) {
+                    mo[n][j] = fmaf(pm0, m[0][j], fmaf(pm1, m[1][j], mo[n][j]));
+                    const float w0j = p[0] * d[0][j], w1j = p[1] * d[1][j], w2j = p[2] * d[2][j], w3j = p[3] * d[3][j];
+                    uint32_t b0 = pack_half2(w0j, w1j), b1 = pack_half2(w2j, w3j);
+                    const float2 h0 = __half22float2(*(const __half2 *)&b0), h1 = __half22float2(*(const __half2 *)&b1);
+                    b0 = pack_half2(fmaf(-lo_part, h0.x, w0j), fmaf(-lo_part, h0.y, w1j));   // hi itself, or what it leaves
+                    b1 = pack_half2(fmaf(-lo_part, h1.x, w2j), fmaf(-lo_part, h1.y, w3j));
+                    mma16816(o[n][2 * j], x[j][0], x[j][1], y[j][0], y[j][1], b0, b1);
+                    mma16816(o[n][2 * j + 1], x[j][2], x[j][3], y[j][2], y[j][3], b0, b1);
+                }
+            }
+        }
+    }
+
+    __device__ __forceinline__ void rescale(float dm)
+    {
+        if (!__any_sync(0xFFFFFFFFu, dm * ve > 128.f)) return;
+#pragma unroll
+        for (int x = 1; x < 32; x <<= 1) dm = fmaxf(dm, __shfl_xor_sync(0xFFFFFFFFu, dm, x));
+        set_scale(dm);
+    }
+    // the power of two that brings dm into [32, 64)
+    __device__ __forceinline__ void set_scale(float dm)
+    {
+        const float to = dm > 0.f ? __uint_as_float((uint32_t)(127 + 5 + 127 - (int)(__float_as_uint(dm) >> 23)) << 23) : 1.f;
+        const float f = to / ve;
+        ve = to;
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int j = 0; j < 2 * NG; j++) {
+                o[n][j][0] *= f; o[n][j][1] *= f; o[n][j][2] *= f; o[n][j][3] *= f;
+            }
+    }
+
+    // unnormalised outputs of dims 32 j + 4 gr .. + 3 of head t; the sum of weights of head t
+    __device__ __forceinline__ float sum(int n) const
+    {
+        float x = l[n];
+#pragma unroll
+        for (int k = 4; k < 32; k <<= 1) x += __shfl_xor_sync(0xFFFFFFFFu, x, k);
+        return x;
+    }
+    __device__ __forceinline__ float4 out(int n, int j, int lane) const
+    {
+        float m = mo[n][j];
+#pragma unroll
+        for (int k = 1; k < 8; k <<= 1) m += __shfl_xor_sync(0xFFFFFFFFu, m, k);
+        m = __shfl_sync(0xFFFFFFFFu, m, 8 * (lane & 3));
+        const float e = 1.f / ve;
+        return make_float4(fmaf(o[n][2 * j][0] + o[n][2 * j][1], e, m), fmaf(o[n][2 * j][2] + o[n][2 * j][3], e, m),
+                           fmaf(o[n][2 * j + 1][0] + o[n][2 * j + 1][1], e, m), fmaf(o[n][2 * j + 1][2] + o[n][2 * j + 1][3], e, m));
+    }
+};
+
+struct AttnKv4Smem {
+    int ring, part, qf, qs, rot, cs, recv, bar, total;   // byte offsets
+};
+__host__ __device__ constexpr AttnKv4Smem attn_kv4_smem(int NG, int NT, int GV, int CL)
+{
+    AttnKv4Smem s = {};
+    const int HD = 32 * NG;
+    s.ring = 0;                                               // [warps][stages] blocks; a warp's results replace its own
+    int at = AK_WARPS * AK_STAGES * 40 * HD;
+    s.qf = at;                                                // [8 NT columns][HD] halves
+    at += 8 * NT * HD * 2;
+    s.qs = at;                                                // [4 NT heads][NG + 1] floats
+    at += 4 * NT * (NG + 1) * 4;
+    s.rot = at;                                               // [warps][HD] floats: rotated rows
+    at += AK_WARPS * HD * 4;
+    s.cs = at;                                                // [HD / 2] (cos, sin)
+    at += HD * 4;
+    s.recv = at;                                              // [slots][CL][34] floats
+    at += ((GV * NG + CL - 1) / CL) * CL * 34 * 4;
+    s.bar = (at + 7) & ~7;
+    s.total = s.bar + AK_WARPS * AK_STAGES * 8;
+    return s;
+}
+
+template <int NG, int NT>
+__global__ void __launch_bounds__(AK_THREADS) attn_step_kv4_kernel(const AttnKv4Args a)
+{
+    namespace cg = cooperative_groups;
+    constexpr int HD = 32 * NG, half = HD / 2, BB = 40 * HD, RS = HD + 2;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int CL = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    extern __shared__ __align__(128) uint8_t smem[];
+    const int G = a.n_heads / a.n_kv, GV = (G + a.splits - 1) / a.splits;   // query heads per kv head, and of a cluster
+    const AttnKv4Smem at = attn_kv4_smem(NG, NT, GV, CL);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int cl = blockIdx.x / CL, kvh = cl / a.splits, split = cl - kvh * a.splits;
+    const int h_lo = kvh * G + split * GV, n_h = min(GV, G - split * GV);   // this cluster's query heads
+    uint8_t *ring = smem + at.ring + warp * (AK_STAGES * BB);
+    uint64_t *bar = (uint64_t *)(smem + at.bar) + warp * AK_STAGES;
+    __half *qf = (__half *)(smem + at.qf);
+    float *qs = (float *)(smem + at.qs);
+    float *rot = (float *)(smem + at.rot) + warp * HD;
+    float2 *cs = (float2 *)(smem + at.cs);
+    float *recv = (float *)(smem + at.recv);
+
+    cluster_arrive();   // another CTA's shared memory may be written once it runs: waited for before the pushes
+    if (lane == 0) {
+        for (int s = 0; s < AK_STAGES; s++) mbar_init(&bar[s], 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncwarp();
+    auto place = [&](int pos, int &first, int &b0, int &n_blk) {   // the blocks of the visible positions
+        pos = max(0, min(pos, a.max_seq - 1));
+        first = a.window > 0 ? max(0, pos + 1 - a.window) : 0;
+        b0 = first / KV4_BLOCK;
+        n_blk = pos / KV4_BLOCK - b0 + 1;
+        return pos;
+    };
+    const uint8_t *head_blocks = kv4_block(a.cache, a.n_blocks, kvh, 0, HD);
+    int first, b0, n_blk;
+    if (a.prefetch) {
+        // Ahead of the kernel that may still be writing q, k_new or the cache: into L2 only, whatever is there
+        const int p = __ldcg(a.step + 1);
+        place(p, first, b0, n_blk);
+        const int b = rank + CL * warp;
+        if (lane < AK_STAGES && b + CL * AK_WARPS * lane < n_blk) l2_prefetch_bulk(head_blocks + (size_t)(b0 + b + CL * AK_WARPS * lane) * BB, BB);
+    }
+    pdl_trigger();
+    pdl_wait();
+    const int pos = place(a.step ? __ldcg(a.step + 1) : a.pos, first, b0, n_blk);
+    const int stride = CL * AK_WARPS, mine = rank + CL * warp;
+    const int n_mine = mine < n_blk ? (n_blk - mine + stride - 1) / stride : 0;
+    auto load = [&](int i) {   // (lane 0) this warp's i-th block into its stage
+        uint64_t *b = &bar[i % AK_STAGES];
+        mbar_arrive_expect_tx(b, BB);
+        tma_load_1d(ring + (i % AK_STAGES) * BB, head_blocks + (size_t)(b0 + mine + i * stride) * BB, BB, b);
+    };
+    if (lane == 0)
+        for (int i = 0; i < min(n_mine, AK_STAGES); i++) load(i);
+    const bool rotate = a.theta > 0.f;
+    if (rotate) {
+        if (threadIdx.x < half) {
+            float c, s;
+            if (a.rope_tab && __float_as_int(__ldcg(&a.rope_tab[ATT_MAX_HD / 2].x)) == pos) {
+                const float2 v = __ldcg(&a.rope_tab[threadIdx.x]);
+                c = v.x;
+                s = v.y;
+            } else {
+                rope_cs(RopeArgs{pos, a.theta, a.yarn_scale, a.yarn_orig_ctx, a.neox}, threadIdx.x, HD, c, s);
+            }
+            cs[threadIdx.x] = make_float2(c, s);
+        }
+        __syncthreads();
+    }
+    // a row of q or k, rotated, into this warp's `rot`
+    auto rotated = [&](const float *src) {
+        for (int i = lane; i < half; i += 32) {
+            const int i0 = a.neox ? i : 2 * i, i1 = a.neox ? i + half : 2 * i + 1;
+            float x0 = __ldcg(src + i0), x1 = __ldcg(src + i1);
+            if (rotate) {
+                const float2 v = cs[i];
+                const float r0 = x0 * v.x - x1 * v.y, r1 = x0 * v.y + x1 * v.x;
+                x0 = r0;
+                x1 = r1;
+            }
+            rot[i0] = x0;
+            rot[i1] = x1;
+        }
+        __syncwarp();
+    };
+    // ---- q as the column operand: warp w prepares head w (columns 2 w and 2 w + 1) ----
+    if (warp < 4 * NT) {
+        float x[NG], top = 0.f;
+        if (warp < n_h) {
+            rotated(a.q + (size_t)(h_lo + warp) * HD);
+#pragma unroll
+            for (int j = 0; j < NG; j++) {
+                x[j] = rot[32 * j + lane] * (a.scale * 1.44269504f);
+                top = fmaxf(top, fabsf(x[j]));
+            }
+#pragma unroll
+            for (int s = 16; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, s));
+        } else {
+#pragma unroll
+            for (int j = 0; j < NG; j++) x[j] = 0.f;
+        }
+        // 2^e brings the largest element into [2^13, 2^14)
+        const int e = top > 0.f ? max(-100, min(100, 127 + 13 - (int)(__float_as_uint(top) >> 23))) : 0;
+        const float up = __uint_as_float((uint32_t)(127 + e) << 23);
+        float *head_qs = qs + warp * (NG + 1);
+        if (lane == 0) head_qs[NG] = 1.f / up;
+#pragma unroll
+        for (int j = 0; j < NG; j++) {
+            const float total = warp_sum(x[j]);
+            if (lane == 0) head_qs[j] = total * up;
+            // dim 32 j + lane = 8 tt + i: halves of word (j, tt): pairs (0,4) (1,5) (2,6) (3,7)
+            const int tt = lane >> 3, i = lane & 7;
+            const float y = x[j] * up;
+            const __half hi = __float2half_rn(y), lo = __float2half_rn(y - __half2float(hi));
+            const int slot = (j * 4 + tt) * 8 + (i & 3) * 2 + (i >> 2);
+            qf[(2 * warp) * HD + slot] = hi;
+            qf[(2 * warp + 1) * HD + slot] = lo;
+        }
+    }
+    __syncthreads();
+    Kv4Warp<NG, NT> w;
+    w.clear();
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        const float *head_qs = qs + (4 * n + (lane & 3)) * (NG + 1);
+        w.back[n] = head_qs[NG];
+#pragma unroll
+        for (int j = 0; j < NG; j++) {
+            w.qs[n][j] = head_qs[j];
+            const uint4 v = *(const uint4 *)(qf + (8 * n + (lane >> 2)) * HD + (j * 4 + (lane & 3)) * 8);
+            w.qf[n][j][0] = v.x; w.qf[n][j][1] = v.y; w.qf[n][j][2] = v.z; w.qf[n][j][3] = v.w;
+        }
+    }
+    // ---- this warp's blocks ----
+    for (int i = 0; i < n_mine; i++) {
+        const int stage = i % AK_STAGES;
+        if (!__all_sync(0xFFFFFFFFu, mbar_wait(&bar[stage], (i / AK_STAGES) & 1))) {
+            if (lane == 0) {
+                if (a.status) *a.status = QZ_ERR_TIMEOUT;
+                for (int k = i; k < min(n_mine, i + AK_STAGES); k++) mbar_wait(&bar[k % AK_STAGES], (k / AK_STAGES) & 1);   // copies in flight
+            }
+            break;
+        }
+        uint8_t *blk = ring + stage * BB;
+        const int base = (b0 + mine + i * stride) * KV4_BLOCK;
+        const int lo = max(0, first - base), hi = min(KV4_BLOCK - 1, pos - base);
+        if (lo > 0 || hi < KV4_BLOCK - 1 || (a.k_new && base + hi == pos)) {
+            if (a.k_new && base + hi == pos) {
+                // the new position: lanes 0.. quantise its key, lanes 16.. its value, into the staged block; split 0
+                // copies the row to the cache
+                rotated(a.k_new + (size_t)kvh * HD);
+                const int e = lane & 15;
+                const bool is_v = lane >= 16;
+                if (e < 4 * NG) {
+                    float x[8];
+                    const float *v = a.v_new + (size_t)kvh * HD + 8 * e;
+#pragma unroll
+                    for (int c = 0; c < 8; c++) x[c] = is_v ? __ldcg(v + c) : rot[8 * e + c];
+                    kv4_store8<NG>(x, blk, hi, e >> 2, e & 3, is_v, ((1u << (4 * NG)) - 1u) * 0x00010001u);
+                }
+                __syncwarp();
+                if (split == 0) {
+                    uint32_t *dst = (uint32_t *)(kv4_block(a.cache, a.n_blocks, kvh, pos / KV4_BLOCK, HD));
+                    const uint32_t *src = (const uint32_t *)blk;
+                    for (int c = lane; c < 10 * NG; c += 32) {   // K codes, K parameters, V codes, V parameters of the row
+                        const int side = c / (5 * NG), k = c - side * 5 * NG;
+                        const int word = side * 5 * HD + (k < 4 * NG ? hi * 4 * NG + k : 4 * HD + hi * NG + (k - 4 * NG));
+                        dst[word] = src[word];
+                    }
+                }
+            }
+            // rows outside [lo, hi] hold anything: their parameters become 0
+            if (lane < lo || lane > hi) {
+#pragma unroll
+                for (int j = 0; j < NG; j++) {
+                    ((uint32_t *)(blk + 16 * HD))[lane * NG + j] = 0;
+                    ((uint32_t *)(blk + 36 * HD))[lane * NG + j] = 0;
+                }
+            }
+            __syncwarp();
+        }
+        w.block(blk, lo, hi, lane);
+        __syncwarp();   // every lane is done with the stage
+        if (lane == 0 && i + AK_STAGES < n_mine) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // (a patched block is overwritten by the copy)
+            load(i + AK_STAGES);
+        }
+    }
+    // ---- results of this warp over its own ring, then of the CTA ----
+    float *part = (float *)(smem + at.ring);
+    constexpr int WS = AK_STAGES * BB / 4;   // floats from one warp's results to the next
+    __syncwarp();
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        const float total = w.sum(n);
+        const int h = 4 * n + (lane & 3);
+        float *dst = part + warp * WS + h * RS;
+#pragma unroll
+        for (int j = 0; j < NG; j++) {
+            const float4 v = w.out(n, j, lane);
+            if (h < n_h) {
+                *(float2 *)(dst + 2 + 32 * j + 4 * (lane >> 2)) = make_float2(v.x, v.y);
+                *(float2 *)(dst + 4 + 32 * j + 4 * (lane >> 2)) = make_float2(v.z, v.w);
+            }
+        }
+        if (lane < 4 && h < n_h) {
+            dst[0] = w.ref[n];
+            dst[1] = total;
+        }
+    }
+    __syncthreads();
+    // runs of 32 outputs: run e belongs to CTA e % CL, in its slot e / CL
+    const int n_runs = n_h * NG, active = min(AK_WARPS, max(1, (n_blk - rank + CL - 1) / CL));
+    cluster_wait();   // (arrived at the top) every CTA of the cluster has started
+    for (int e = warp; e < n_runs; e += AK_WARPS) {
+        const int h = e / NG, j = e - h * NG;
+        float top = -3.0e38f;
+        for (int k = 0; k < active; k++) top = fmaxf(top, part[k * WS + h * RS]);
+        float l = 0.f, o = 0.f;
+        for (int k = 0; k < active; k++) {
+            const float *src = part + k * WS + h * RS;
+            const float f = ex2(src[0] - top);
+            l = fmaf(src[1], f, l);
+            o = fmaf(src[2 + 32 * j + lane], f, o);
+        }
+        float *dst = cluster.map_shared_rank(recv, e % CL) + ((e / CL) * CL + rank) * 34;
+        dst[2 + lane] = o;
+        if (lane == 0) {
+            dst[0] = top;
+            dst[1] = l;
+        }
+    }
+    cluster_arrive();
+    cluster_wait();   // every push has landed
+    for (int e = rank + CL * warp; e < n_runs; e += CL * AK_WARPS) {
+        const float *src = recv + (e / CL) * CL * 34;
+        const int head = h_lo + e / NG;
+        const float sink = a.sinks ? a.sinks[head] * 1.44269504f : -INFINITY;
+        float top = fmaxf(sink, -3.0e38f);
+        for (int c = 0; c < CL; c++) top = fmaxf(top, src[34 * c]);
+        float l = ex2(sink - top), o = 0.f;
+        for (int c = 0; c < CL; c++) {
+            const float f = ex2(src[34 * c] - top);
+            l = fmaf(src[34 * c + 1], f, l);
+            o = fmaf(src[34 * c + 2 + lane], f, o);
+        }
+        const float r = o / l;
+        const int first_out = head * HD + 32 * (e % NG);
+        a.out[first_out + lane] = r;
+        if (a.emit_q) {
+            float v[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) v[k] = __shfl_sync(0xFFFFFFFFu, r, (4 * lane + k) & 31);
+            quantize4_store(v, (first_out >> 2) + (lane & 7), lane < 8, a.o);
         }
     }
 }

@@ -30,6 +30,42 @@ bool refuse(const char *why)
     return false;
 }
 
+// Cluster width of the step kernel: as many CTAs per kv head as leave all clusters on the chip at once, no more than the
+// cache has blocks, at most what the device can schedule (16 needs the non-portable size).
+template <int NG, int NT>
+int step_cluster(int clusters, int n_blocks, int GV)
+{
+    static bool ready = false;
+    if (!ready) {
+        const auto kernel = attn_step_kv4_kernel<NG, NT>;
+        QZ_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, attn_kv4_smem(NG, NT, 4 * NT, 16).total));
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) cudaGetLastError();
+        ready = true;
+    }
+    static int widest[4 * NT + 1] = {};   // by query heads per cluster (they size the shared memory a little)
+    if (!widest[GV]) {
+        int cl = 16;
+        for (int n = 0; cl > 1; cl /= 2) {
+            cudaLaunchConfig_t cfg = {};
+            cudaLaunchAttribute at[1];
+            at[0].id = cudaLaunchAttributeClusterDimension;
+            at[0].val.clusterDim.x = (unsigned)cl;
+            at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+            cfg.gridDim = dim3(cl);
+            cfg.blockDim = dim3(AK_THREADS);
+            cfg.dynamicSmemBytes = attn_kv4_smem(NG, NT, GV, cl).total;
+            cfg.attrs = at;
+            cfg.numAttrs = 1;
+            if (cudaOccupancyMaxActiveClusters(&n, attn_step_kv4_kernel<NG, NT>, &cfg) == cudaSuccess && n >= 1) break;
+            cudaGetLastError();
+        }
+        widest[GV] = cl;
+    }
+    int cl = widest[GV];
+    while (cl > 1 && (clusters * cl > sm_count() || cl / 2 >= n_blocks)) cl /= 2;
+    return cl;
+}
+
 // NG = head_dim / 32 as a template argument
 template <class F>
 void by_groups(int head_dim, F f)
@@ -131,7 +167,20 @@ void cuda_attn_step_kv4(float *out, const float *q, const float *k_new, const fl
         if (!activation_slot(out_slot, n_heads * head_dim, &a.o)) return;
         a.emit_q = 1;
     }
-    by_groups(head_dim, [&](auto ng) { launch(attn_kv4_kernel<ng.value>, dim3(n_kv_heads), dim3(AK_THREADS), 0, a); });
+    const int G = n_heads / n_kv_heads;
+    a.splits = (G + 7) / 8;
+    a.prefetch = pdl_enabled() && d_step;
+    a.status = status_word_if_ready();
+    const int GV = (G + a.splits - 1) / a.splits, clusters = n_kv_heads * a.splits;
+    by_groups(head_dim, [&](auto ng) {
+        auto go = [&](auto nt) {
+            const int cl = step_cluster<ng.value, nt.value>(clusters, a.n_blocks, GV);
+            launch_cluster(attn_step_kv4_kernel<ng.value, nt.value>, dim3(clusters * cl), dim3(AK_THREADS),
+                           (size_t)attn_kv4_smem(ng.value, nt.value, GV, cl).total, cl, a);
+        };
+        if (GV <= 4) go(std::integral_constant<int, 1>());
+        else go(std::integral_constant<int, 2>());
+    });
 }
 
 void cuda_attn_prompt_kv4(float *out, const float *q, const void *d_cache, int n_tok, int n_heads, int n_kv_heads, int head_dim, int max_seq,

@@ -230,6 +230,15 @@ int *status_word()
     }
     return g_status;
 }
+int *status_word_if_ready()
+{
+    if (!g_status) {   // creating it would break a capture on this stream
+        cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+        if (cudaStreamIsCapturing(g_stream, &st) != cudaSuccess) cudaGetLastError();
+        else if (st == cudaStreamCaptureStatusNone) return status_word();
+    }
+    return g_status;
+}
 static GridBarrier *g_grid_barrier = nullptr;   // count / generation / abort words of the chained-GEMV kernel
 static void poll_status()
 {
