@@ -10,6 +10,9 @@ namespace qz {
 
 constexpr int AK_THREADS = 256, AK_WARPS = AK_THREADS / 32;
 constexpr int AK_MAX_G = 16;
+constexpr int AK_MAX_CLUSTERS = 128;                  // of all units together when a unit has several
+constexpr int AK_COUNTERS = AK_MAX_CLUSTERS * 32;     // one per run of 32 outputs of a unit
+constexpr size_t AK_WORKSPACE = sizeof(float) * (AK_COUNTERS + (size_t)AK_MAX_CLUSTERS * 32 * 34);
 
 struct AttnKv4Args {
     float *out;
@@ -26,7 +29,9 @@ struct AttnKv4Args {
     XQOut o;
     int emit_q;
     const float2 *rope_tab;
-    int splits;                          // clusters that share a kv head's query heads
+    int splits;                          // units that share a kv head's query heads
+    int clusters;                        // clusters per unit
+    float *workspace;                    // clusters > 1: AK_COUNTERS zeroed counters, then [units * 32 runs][clusters][34]
     int prefetch;                        // the launch may overlap the one before it: fetch into L2 ahead of the wait
     int *status;
 };
@@ -137,10 +142,14 @@ __global__ void __launch_bounds__(AK_THREADS) attn_kv4_kernel(const AttnKv4Args 
 }
 
 // ---- one token ---------------------------------------------------------------------------------------------------
-// One launch whose shape does not depend on the position.  A cluster of CL CTAs per kv head (two per kv head when more
-// than eight query heads share it); warp w of CTA r takes the blocks of 32 positions r + CL (w + 8 i), so that a short
-// context is spread over the CTAs first.  A warp works alone: it streams its blocks through a ring of its own (one bulk
-// copy per block: the block is contiguous) and keeps scores, weights and outputs of all heads in registers.
+// One launch whose shape does not depend on the position.  A unit is a kv head (two units when more than eight query heads
+// share it); it has NC clusters of CL CTAs, of which as many work as the context has a block for every warp of.  Warp w of
+// CTA r (of all R working ones) takes the blocks of 32 positions r + R (w + 8 i), so that a short context is spread over the
+// CTAs first.  A warp works alone: it streams its blocks through a ring of its own (one bulk copy per block: the block is
+// contiguous) and keeps scores, weights and outputs of all heads in registers.  A cluster's CTAs push their results into
+// the CTA that finishes a run of 32 outputs; with several clusters at work, that CTA leaves the run in a workspace and the
+// last one to arrive merges them in the clusters' order (clusters of 16 need no workspace, but only 7 of them fit on the
+// chip at once, 8 kv heads took two turns).
 //
 // Both products run on the tensor cores with the CODES as one operand, exactly, and 22 bits of the other:
 //   scores   s[pos, head] = sum_g d_g ((codes_g - 8) . q_g) + (m_g + 8 d_g) sum(q_g)
@@ -153,11 +162,11 @@ __global__ void __launch_bounds__(AK_THREADS) attn_kv4_kernel(const AttnKv4Args 
 // one mma.m16n8k16; both parts are scaled by powers of two (per head for q, per warp for d) that keep them clear of
 // f16's ends.  Sums are f32.
 // The softmax reference of a head is raised only when a score exceeds it by 2^8; until then weights up to 2^8 do no harm.
-constexpr int AK_STAGES = 4;
+__host__ __device__ constexpr int attn_kv4_stages(int NG) { return NG == 1 ? 8 : NG == 2 ? 4 : 2; }   // ~10 KB in flight per warp
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
 {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -233,17 +242,35 @@ __device__ __forceinline__ void lds_pairs(const void *a, const void *b, uint32_t
     }
 }
 
+// N floats at a 4N-aligned address (16 N = 64: one vector)
+template <int N>
+__device__ __forceinline__ void lds_floats(const float *p, float (&x)[N])
+{
+    if constexpr (N == 4) {
+        const float4 v = *(const float4 *)p;
+        x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+    } else if constexpr (N == 2) {
+        const float2 v = *(const float2 *)p;
+        x[0] = v.x; x[1] = v.y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) x[i] = p[i];
+    }
+}
+
 // The running state of a warp over the blocks of one kv head, for 4 NT heads, and one block's turn.
 // lane = 4 gr + t.  Scores: rows gr, gr + 8 of a tile of 16 positions, columns (hi, lo) of head t.  Outputs: dims
 // 32 j + 4 gr + i of head t.  Weights as operand: head gr / 2 (part gr % 2), positions t, t + 4, t + 8, t + 12 of a tile.
 template <int NG, int NT>
 struct Kv4Warp {
+    static constexpr int SCRATCH = 4 * 32 * NG;   // floats of shared memory a warp needs: d, m + 8 d of K and of V per position
     uint32_t qf[NT][NG][4];   // q as the column operand: dims (0,4) (1,5) (2,6) (3,7) of 32 j + 8 t, column gr
-    float qs[NT][NG];         // sum of q over group j in units of 1 / back, head t
+    float qs[NT][NG];         // sum of q over group j, head t
     float back[NT];           // scores in log2 units = back * what the products give, head t
     float ref[NT], l[NT];     // reference and partial sum of weights, head t
-    float o[NT][2 * NG][4];
-    float mo[NT][NG];         // partial sums of p * m, head gr / 2
+    float o[NT][2 * NG][4];   // sums of the tensor core since the last flush
+    float acc[NT][2 * NG][2]; // flushed sums (hi + lo)
+    float mo[NT][NG];         // partial sums of p * (m + 8 d), head gr / 2
     float ve;                 // power of two that p * d carries
 
     __device__ __forceinline__ void clear()
@@ -256,17 +283,67 @@ struct Kv4Warp {
 #pragma unroll
             for (int j = 0; j < NG; j++) mo[n][j] = 0.f;
 #pragma unroll
-            for (int j = 0; j < 2 * NG; j++) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.f;
+            for (int j = 0; j < 2 * NG; j++) {
+                o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.f;
+                acc[n][j][0] = acc[n][j][1] = 0.f;
+            }
         }
     }
 
-    // rows lo .. hi of the block are visible (the parameters of the others are finite)
-    __device__ __forceinline__ void block(const uint8_t *blk, int lo, int hi, int lane)
+    // The tensor core rounds its running f32 sums towards zero, half an ulp too low at each step on average: 64 steps cost
+    // 2e-6.  Sums of at most 8 steps are therefore moved to ordinary ones (1e-7), which round to nearest.
+    __device__ __forceinline__ void flush()
+    {
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int j = 0; j < 2 * NG; j++) {
+                acc[n][j][0] += o[n][j][0] + o[n][j][1];
+                acc[n][j][1] += o[n][j][2] + o[n][j][3];
+                o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.f;
+            }
+    }
+
+    // rows lo .. hi of the block are visible; the others may hold anything
+    __device__ __forceinline__ void block(const uint8_t *blk, float *scratch, int lo, int hi, int lane)
     {
         constexpr int HD = 32 * NG, ROW = HD / 2, PAR = 4 * NG;
         const int gr = lane >> 2, t = lane & 3;
-        float s[2][NT][2];
+        float *kd = scratch, *km = kd + 32 * NG, *vd = km + 32 * NG, *vm = vd + 32 * NG;
+        // ---- parameters: lane = position, converted once for the warp ----
+        const bool whole = lo == 0 && hi == KV4_BLOCK - 1;
+        {
+            float m[NG], d[NG], dm = 0.f;
+            const bool seen = lane >= lo && lane <= hi;
+#pragma unroll
+            for (int side = 0; side < 2; side++) {
+                const uint8_t *p = blk + (side ? 36 : 16) * HD + lane * PAR;
+                lds_halves<NG>(p, m);
+                lds_halves<NG>(p + 2 * NG, d);
+                if (!whole && !seen) {
+#pragma unroll
+                    for (int j = 0; j < NG; j++) m[j] = d[j] = 0.f;
+                }
+                float *dd = (side ? vd : kd) + lane * NG, *mm = (side ? vm : km) + lane * NG;
+                if constexpr (NG == 4) {
+                    *(float4 *)dd = make_float4(d[0], d[1], d[2], d[3]);
+                    *(float4 *)mm = make_float4(fmaf(8.f, d[0], m[0]), fmaf(8.f, d[1], m[1]), fmaf(8.f, d[2], m[2]), fmaf(8.f, d[3], m[3]));
+                } else {
+#pragma unroll
+                    for (int j = 0; j < NG; j++) {
+                        dd[j] = d[j];
+                        mm[j] = fmaf(8.f, d[j], m[j]);
+                    }
+                }
+            }
+            // scale of p * d: the largest d stays below 2^7 (weights are at most 2^8: products below 2^15)
+#pragma unroll
+            for (int j = 0; j < NG; j++) dm = fmaxf(dm, d[j]);
+            if (__any_sync(0xFFFFFFFFu, dm * ve > 128.f)) set_scale(dm);
+        }
+        __syncwarp();
         // ---- scores ----
+        float s[2][NT][2];
 #pragma unroll
         for (int tile = 0; tile < 2; tile++) {
             const int r0 = 16 * tile + gr, r1 = r0 + 8;
@@ -274,16 +351,10 @@ struct Kv4Warp {
             float m0[NG], m1[NG], d0[NG], d1[NG];
             lds_words<NG>(blk + r0 * ROW + 4 * NG * t, k0);
             lds_words<NG>(blk + r1 * ROW + 4 * NG * t, k1);
-            const uint8_t *p0 = blk + 16 * HD + r0 * PAR, *p1 = blk + 16 * HD + r1 * PAR;
-            lds_halves<NG>(p0, m0);
-            lds_halves<NG>(p0 + 2 * NG, d0);
-            lds_halves<NG>(p1, m1);
-            lds_halves<NG>(p1 + 2 * NG, d1);
-#pragma unroll
-            for (int j = 0; j < NG; j++) {
-                m0[j] = fmaf(8.f, d0[j], m0[j]);
-                m1[j] = fmaf(8.f, d1[j], m1[j]);
-            }
+            lds_floats<NG>(kd + r0 * NG, d0);
+            lds_floats<NG>(km + r0 * NG, m0);
+            lds_floats<NG>(kd + r1 * NG, d1);
+            lds_floats<NG>(km + r1 * NG, m1);
 #pragma unroll
             for (int n = 0; n < NT; n++) s[tile][n][0] = s[tile][n][1] = 0.f;
 #pragma unroll
@@ -300,20 +371,25 @@ struct Kv4Warp {
                     s[tile][n][1] = fmaf(d1[j], c[2] + c[3], fmaf(m1[j], qs[n][j], s[tile][n][1]));
                 }
             }
+        }
+        if (!whole) {
 #pragma unroll
-            for (int n = 0; n < NT; n++) {
-                s[tile][n][0] = r0 >= lo && r0 <= hi ? s[tile][n][0] * back[n] : -INFINITY;
-                s[tile][n][1] = r1 >= lo && r1 <= hi ? s[tile][n][1] * back[n] : -INFINITY;
+            for (int i = 0; i < 4; i++) {
+                const int r = gr + 8 * i;
+                if (r < lo || r > hi) {
+#pragma unroll
+                    for (int n = 0; n < NT; n++) s[i >> 1][n][i & 1] = -INFINITY;   // (back is positive)
+                }
             }
         }
-        // ---- reference ----
+        // ---- weights ----
         bool raise = false;
 #pragma unroll
-        for (int n = 0; n < NT; n++) raise |= fmaxf(fmaxf(s[0][n][0], s[0][n][1]), fmaxf(s[1][n][0], s[1][n][1])) > ref[n] + 8.f;
+        for (int n = 0; n < NT; n++) raise |= fmaxf(fmaxf(s[0][n][0], s[0][n][1]), fmaxf(s[1][n][0], s[1][n][1])) * back[n] > ref[n] + 8.f;
         if (__any_sync(0xFFFFFFFFu, raise)) {
 #pragma unroll
             for (int n = 0; n < NT; n++) {
-                float top = fmaxf(fmaxf(s[0][n][0], s[0][n][1]), fmaxf(s[1][n][0], s[1][n][1]));
+                float top = fmaxf(fmaxf(s[0][n][0], s[0][n][1]), fmaxf(s[1][n][0], s[1][n][1])) * back[n];
 #pragma unroll
                 for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, x));
                 top = fmaxf(top, ref[n]);
@@ -323,95 +399,90 @@ struct Kv4Warp {
                 const float corr_m = __shfl_sync(0xFFFFFFFFu, corr, gr >> 1);   // of the head whose weights this lane carries
 #pragma unroll
                 for (int j = 0; j < NG; j++) mo[n][j] *= corr_m;
-#pragma unroll
-                for (int j = 0; j < 2 * NG; j++) {
-                    o[n][j][0] *= corr; o[n][j][1] *= corr; o[n][j][2] *= corr; o[n][j][3] *= corr;
-                }
+                scale_outputs(n, corr);
             }
         }
-        // ---- outputs ----
-        const uint8_t *vb = blk + 20 * HD;
-        const int part = gr & 1;
-        const float lo_part = (float)part;
-#pragma unroll
-        for (int tile = 0; tile < 2; tile++) {
-            const int r = 16 * tile + t;
-            float d[4][NG];
-#pragma unroll
-            for (int i = 0; i < 4; i++) lds_halves<NG>(vb + 16 * HD + (r + 4 * i) * PAR + 2 * NG, d[i]);
-            // the step's scale: largest of d stays below 2^7 (weights are at most 2^8: products below 2^15)
-            float dm = 0.f;
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int j = 0; j < NG; j++) dm = fmaxf(dm, d[i][j]);
-            rescale(dm);
-            float m[2][NG];
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                lds_halves<NG>(vb + 16 * HD + (r + 8 * part + 4 * i) * PAR, m[i]);
-#pragma unroll
-                for (int j = 0; j < NG; j++) m[i][j] = fmaf(8.f, part ? d[2 + i][j] : d[i][j], m[i][j]);
-            }
-            uint32_t v01[NG], v23[NG];
-            lds_pairs<NG>(vb + r * ROW + 2 * NG * gr, vb + (r + 4) * ROW + 2 * NG * gr, v01);
-            lds_pairs<NG>(vb + (r + 8) * ROW + 2 * NG * gr, vb + (r + 12) * ROW + 2 * NG * gr, v23);
-            uint32_t x[NG][4], y[NG][4];   // dims 4 gr + 0 .. 3 of positions (t, t + 4) and (t + 8, t + 12)
-#pragma unroll
-            for (int j = 0; j < NG; j++) {
-                kv4_pairs(v01[j], x[j]);
-                kv4_pairs(v23[j], y[j]);
-            }
-#pragma unroll
-            for (int n = 0; n < NT; n++) {
-                const float w0 = ex2(s[tile][n][0] - ref[n]), w1 = ex2(s[tile][n][1] - ref[n]);
-                l[n] += w0 + w1;
-                const int src = 4 * t + (gr >> 1);
-                float p[4];
-                p[0] = __shfl_sync(0xFFFFFFFFu, w0, src);
-                p[1] = __shfl_sync(0xFFFFFFFFu, w0, src + 16);
-                p[2] = __shfl_sync(0xFFFFFFFFu, w1, src);
-                p[3] = __shfl_sync(0xFFFFFFFFu, w1, src + 16);
-                const float pm0 = part ? p[2] : p[0], pm1 = part ? p[3] : p[1];
-#pragma unroll
-                for (int i = 0; i < 4; i++) p[i] *= ve;
-#pragma unroll
-                for (int j = 0; j < NG; j++) {
-                    mo[n][j] = fmaf(pm0, m[0][j], fmaf(pm1, m[1][j], mo[n][j]));
-                    const float w0j = p[0] * d[0][j], w1j = p[1] * d[1][j], w2j = p[2] * d[2][j], w3j = p[3] * d[3][j];
-                    uint32_t b0 = pack_half2(w0j, w1j), b1 = pack_half2(w2j, w3j);
-                    const float2 h0 = __half22float2(*(const __half2 *)&b0), h1 = __half22float2(*(const __half2 *)&b1);
-                    b0 = pack_half2(fmaf(-lo_part, h0.x, w0j), fmaf(-lo_part, h0.y, w1j));   // hi itself, or what it leaves
-                    b1 = pack_half2(fmaf(-lo_part, h1.x, w2j), fmaf(-lo_part, h1.y, w3j));
-                    mma16816(o[n][2 * j], x[j][0], x[j][1], y[j][0], y[j][1], b0, b1);
-                    mma16816(o[n][2 * j + 1], x[j][2], x[j][3], y[j][2], y[j][3], b0, b1);
-                }
-            }
-        }
-    }
-
-    __device__ __forceinline__ void rescale(float dm)
-    {
-        if (!__any_sync(0xFFFFFFFFu, dm * ve > 128.f)) return;
-#pragma unroll
-        for (int x = 1; x < 32; x <<= 1) dm = fmaxf(dm, __shfl_xor_sync(0xFFFFFFFFu, dm, x));
-        set_scale(dm);
-    }
-    // the power of two that brings dm into [32, 64)
-    __device__ __forceinline__ void set_scale(float dm)
-    {
-        const float to = dm > 0.f ? __uint_as_float((uint32_t)(127 + 5 + 127 - (int)(__float_as_uint(dm) >> 23)) << 23) : 1.f;
-        const float f = to / ve;
-        ve = to;
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int j = 0; j < 2 * NG; j++) {
-                o[n][j][0] *= f; o[n][j][1] *= f; o[n][j][2] *= f; o[n][j][3] *= f;
+            for (int i = 0; i < 4; i++) {
+                float &x = s[i >> 1][n][i & 1];
+                x = ex2(fmaf(x, back[n], -ref[n]));
+                l[n] += x;
             }
+        // ---- outputs ----
+        const uint8_t *vb = blk + 20 * HD;
+        const int part = gr & 1;
+        const float is_lo = (float)part;
+        const uint32_t flip = (uint32_t)part << 31;
+#pragma unroll
+        for (int tile = 0; tile < 2; tile++) {
+            const int r = 16 * tile + t;
+            float d[4][NG], m[2][NG];
+#pragma unroll
+            for (int i = 0; i < 4; i++) lds_floats<NG>(vd + (r + 4 * i) * NG, d[i]);
+#pragma unroll
+            for (int i = 0; i < 2; i++) lds_floats<NG>(vm + (r + 8 * part + 4 * i) * NG, m[i]);
+            uint32_t v01[NG], v23[NG];
+            lds_pairs<NG>(vb + r * ROW + 2 * NG * gr, vb + (r + 4) * ROW + 2 * NG * gr, v01);
+            lds_pairs<NG>(vb + (r + 8) * ROW + 2 * NG * gr, vb + (r + 12) * ROW + 2 * NG * gr, v23);
+            float p[NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                const int src = 4 * t + (gr >> 1);
+                p[n][0] = __shfl_sync(0xFFFFFFFFu, s[tile][n][0], src);
+                p[n][1] = __shfl_sync(0xFFFFFFFFu, s[tile][n][0], src + 16);
+                p[n][2] = __shfl_sync(0xFFFFFFFFu, s[tile][n][1], src);
+                p[n][3] = __shfl_sync(0xFFFFFFFFu, s[tile][n][1], src + 16);
+                const float a = part ? p[n][2] : p[n][0], b = part ? p[n][3] : p[n][1];
+#pragma unroll
+                for (int j = 0; j < NG; j++) mo[n][j] = fmaf(a, m[0][j], fmaf(b, m[1][j], mo[n][j]));
+#pragma unroll
+                for (int i = 0; i < 4; i++) p[n][i] *= ve;
+            }
+#pragma unroll
+            for (int j = 0; j < NG; j++) {
+                uint32_t x[4], y[4];   // dims 4 gr + 0 .. 3 of positions (t, t + 4) and (t + 8, t + 12)
+                kv4_pairs(v01[j], x);
+                kv4_pairs(v23[j], y);
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    float w[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        // hi: the leading 11 bits; lo: the rest
+                        const float v = p[n][i] * d[i][j];
+                        w[i] = fmaf(is_lo, v, __uint_as_float((__float_as_uint(v) & 0xFFFFE000u) ^ flip));
+                    }
+                    const uint32_t b0 = pack_half2(w[0], w[1]), b1 = pack_half2(w[2], w[3]);
+                    mma16816(o[n][2 * j], x[0], x[1], y[0], y[1], b0, b1);
+                    mma16816(o[n][2 * j + 1], x[2], x[3], y[2], y[3], b0, b1);
+                }
+            }
+        }
     }
 
-    // unnormalised outputs of dims 32 j + 4 gr .. + 3 of head t; the sum of weights of head t
+    __device__ __forceinline__ void scale_outputs(int n, float f)
+    {
+#pragma unroll
+        for (int j = 0; j < 2 * NG; j++) {
+            o[n][j][0] *= f; o[n][j][1] *= f; o[n][j][2] *= f; o[n][j][3] *= f;
+            acc[n][j][0] *= f; acc[n][j][1] *= f;
+        }
+    }
+    // the power of two that brings the warp's largest dm into [32, 64)
+    __device__ __forceinline__ void set_scale(float dm)
+    {
+#pragma unroll
+        for (int x = 1; x < 32; x <<= 1) dm = fmaxf(dm, __shfl_xor_sync(0xFFFFFFFFu, dm, x));
+        const float to = __uint_as_float((uint32_t)(127 + 5 + 127 - (int)(__float_as_uint(dm) >> 23)) << 23);
+        const float f = to / ve;
+        ve = to;
+#pragma unroll
+        for (int n = 0; n < NT; n++) scale_outputs(n, f);
+    }
+
+    // after the last flush: the sum of weights of head t, and outputs (times it) of dims 32 j + 4 gr .. + 3 of head t
     __device__ __forceinline__ float sum(int n) const
     {
         float x = l[n];
@@ -426,20 +497,22 @@ struct Kv4Warp {
         for (int k = 1; k < 8; k <<= 1) m += __shfl_xor_sync(0xFFFFFFFFu, m, k);
         m = __shfl_sync(0xFFFFFFFFu, m, 8 * (lane & 3));
         const float e = 1.f / ve;
-        return make_float4(fmaf(o[n][2 * j][0] + o[n][2 * j][1], e, m), fmaf(o[n][2 * j][2] + o[n][2 * j][3], e, m),
-                           fmaf(o[n][2 * j + 1][0] + o[n][2 * j + 1][1], e, m), fmaf(o[n][2 * j + 1][2] + o[n][2 * j + 1][3], e, m));
+        return make_float4(fmaf(acc[n][2 * j][0], e, m), fmaf(acc[n][2 * j][1], e, m), fmaf(acc[n][2 * j + 1][0], e, m),
+                           fmaf(acc[n][2 * j + 1][1], e, m));
     }
 };
 
 struct AttnKv4Smem {
-    int ring, part, qf, qs, rot, cs, recv, bar, total;   // byte offsets
+    int ring, params, qf, qs, rot, cs, recv, bar, total;   // byte offsets
 };
 __host__ __device__ constexpr AttnKv4Smem attn_kv4_smem(int NG, int NT, int GV, int CL)
 {
     AttnKv4Smem s = {};
     const int HD = 32 * NG;
     s.ring = 0;                                               // [warps][stages] blocks; a warp's results replace its own
-    int at = AK_WARPS * AK_STAGES * 40 * HD;
+    int at = AK_WARPS * attn_kv4_stages(NG) * 40 * HD;
+    s.params = at;                                            // [warps][4][32][NG] floats
+    at += AK_WARPS * 4 * 32 * NG * 4;
     s.qf = at;                                                // [8 NT columns][HD] halves
     at += 8 * NT * HD * 2;
     s.qs = at;                                                // [4 NT heads][NG + 1] floats
@@ -451,25 +524,26 @@ __host__ __device__ constexpr AttnKv4Smem attn_kv4_smem(int NG, int NT, int GV, 
     s.recv = at;                                              // [slots][CL][34] floats
     at += ((GV * NG + CL - 1) / CL) * CL * 34 * 4;
     s.bar = (at + 7) & ~7;
-    s.total = s.bar + AK_WARPS * AK_STAGES * 8;
+    s.total = s.bar + AK_WARPS * attn_kv4_stages(NG) * 8;
     return s;
 }
 
 template <int NG, int NT>
-__global__ void __launch_bounds__(AK_THREADS) attn_step_kv4_kernel(const AttnKv4Args a)
+__global__ void __launch_bounds__(AK_THREADS, NT == 1 ? 2 : 1) attn_step_kv4_kernel(const AttnKv4Args a)
 {
     namespace cg = cooperative_groups;
-    constexpr int HD = 32 * NG, half = HD / 2, BB = 40 * HD, RS = HD + 2;
+    constexpr int HD = 32 * NG, half = HD / 2, BB = 40 * HD, RS = HD + 2, STAGES = attn_kv4_stages(NG);
     cg::cluster_group cluster = cg::this_cluster();
     const int CL = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     extern __shared__ __align__(128) uint8_t smem[];
     const int G = a.n_heads / a.n_kv, GV = (G + a.splits - 1) / a.splits;   // query heads per kv head, and of a cluster
     const AttnKv4Smem at = attn_kv4_smem(NG, NT, GV, CL);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int cl = blockIdx.x / CL, kvh = cl / a.splits, split = cl - kvh * a.splits;
+    const int unit = blockIdx.x / CL / a.clusters, nth = blockIdx.x / CL - unit * a.clusters;   // which cluster of its unit
+    const int kvh = unit / a.splits, split = unit - kvh * a.splits;
     const int h_lo = kvh * G + split * GV, n_h = min(GV, G - split * GV);   // this cluster's query heads
-    uint8_t *ring = smem + at.ring + warp * (AK_STAGES * BB);
-    uint64_t *bar = (uint64_t *)(smem + at.bar) + warp * AK_STAGES;
+    uint8_t *ring = smem + at.ring + warp * (STAGES * BB);
+    uint64_t *bar = (uint64_t *)(smem + at.bar) + warp * STAGES;
     __half *qf = (__half *)(smem + at.qf);
     float *qs = (float *)(smem + at.qs);
     float *rot = (float *)(smem + at.rot) + warp * HD;
@@ -478,7 +552,7 @@ __global__ void __launch_bounds__(AK_THREADS) attn_step_kv4_kernel(const AttnKv4
 
     cluster_arrive();   // another CTA's shared memory may be written once it runs: waited for before the pushes
     if (lane == 0) {
-        for (int s = 0; s < AK_STAGES; s++) mbar_init(&bar[s], 1);
+        for (int s = 0; s < STAGES; s++) mbar_init(&bar[s], 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncwarp();
@@ -489,27 +563,34 @@ __global__ void __launch_bounds__(AK_THREADS) attn_step_kv4_kernel(const AttnKv4
         n_blk = pos / KV4_BLOCK - b0 + 1;
         return pos;
     };
+    auto at_work = [&](int n_blk) { return max(1, min(a.clusters, n_blk / (CL * AK_WARPS))); };
     const uint8_t *head_blocks = kv4_block(a.cache, a.n_blocks, kvh, 0, HD);
     int first, b0, n_blk;
     if (a.prefetch) {
         // Ahead of the kernel that may still be writing q, k_new or the cache: into L2 only, whatever is there
         const int p = __ldcg(a.step + 1);
         place(p, first, b0, n_blk);
-        const int b = rank + CL * warp;
-        if (lane < AK_STAGES && b + CL * AK_WARPS * lane < n_blk) l2_prefetch_bulk(head_blocks + (size_t)(b0 + b + CL * AK_WARPS * lane) * BB, BB);
+        const int R = CL * at_work(n_blk), b = nth * CL + rank + R * warp;
+        if (nth < at_work(n_blk) && lane < STAGES && b + R * AK_WARPS * lane < n_blk)
+            l2_prefetch_bulk(head_blocks + (size_t)(b0 + b + R * AK_WARPS * lane) * BB, BB);
     }
     pdl_trigger();
     pdl_wait();
     const int pos = place(a.step ? __ldcg(a.step + 1) : a.pos, first, b0, n_blk);
-    const int stride = CL * AK_WARPS, mine = rank + CL * warp;
+    const int NC = at_work(n_blk), R = CL * NC, cta = nth * CL + rank;
+    if (nth >= NC) {
+        cluster_wait();
+        return;
+    }
+    const int stride = R * AK_WARPS, mine = cta + R * warp;
     const int n_mine = mine < n_blk ? (n_blk - mine + stride - 1) / stride : 0;
     auto load = [&](int i) {   // (lane 0) this warp's i-th block into its stage
-        uint64_t *b = &bar[i % AK_STAGES];
+        uint64_t *b = &bar[i % STAGES];
         mbar_arrive_expect_tx(b, BB);
-        tma_load_1d(ring + (i % AK_STAGES) * BB, head_blocks + (size_t)(b0 + mine + i * stride) * BB, BB, b);
+        tma_load_1d(ring + (i % STAGES) * BB, head_blocks + (size_t)(b0 + mine + i * stride) * BB, BB, b);
     };
     if (lane == 0)
-        for (int i = 0; i < min(n_mine, AK_STAGES); i++) load(i);
+        for (int i = 0; i < min(n_mine, STAGES); i++) load(i);
     const bool rotate = a.theta > 0.f;
     if (rotate) {
         if (threadIdx.x < half) {
@@ -591,19 +672,19 @@ __global__ void __launch_bounds__(AK_THREADS) attn_step_kv4_kernel(const AttnKv4
     }
     // ---- this warp's blocks ----
     for (int i = 0; i < n_mine; i++) {
-        const int stage = i % AK_STAGES;
-        if (!__all_sync(0xFFFFFFFFu, mbar_wait(&bar[stage], (i / AK_STAGES) & 1))) {
+        const int stage = i % STAGES;
+        if (!__all_sync(0xFFFFFFFFu, mbar_wait(&bar[stage], (i / STAGES) & 1))) {
             if (lane == 0) {
                 if (a.status) *a.status = QZ_ERR_TIMEOUT;
-                for (int k = i; k < min(n_mine, i + AK_STAGES); k++) mbar_wait(&bar[k % AK_STAGES], (k / AK_STAGES) & 1);   // copies in flight
+                for (int k = i; k < min(n_mine, i + STAGES); k++) mbar_wait(&bar[k % STAGES], (k / STAGES) & 1);   // copies in flight
             }
             break;
         }
         uint8_t *blk = ring + stage * BB;
         const int base = (b0 + mine + i * stride) * KV4_BLOCK;
         const int lo = max(0, first - base), hi = min(KV4_BLOCK - 1, pos - base);
-        if (lo > 0 || hi < KV4_BLOCK - 1 || (a.k_new && base + hi == pos)) {
-            if (a.k_new && base + hi == pos) {
+        if (a.k_new && base + hi == pos) {
+            {
                 // the new position: lanes 0.. quantise its key, lanes 16.. its value, into the staged block; split 0
                 // copies the row to the cache
                 rotated(a.k_new + (size_t)kvh * HD);
@@ -627,26 +708,20 @@ __global__ void __launch_bounds__(AK_THREADS) attn_step_kv4_kernel(const AttnKv4
                     }
                 }
             }
-            // rows outside [lo, hi] hold anything: their parameters become 0
-            if (lane < lo || lane > hi) {
-#pragma unroll
-                for (int j = 0; j < NG; j++) {
-                    ((uint32_t *)(blk + 16 * HD))[lane * NG + j] = 0;
-                    ((uint32_t *)(blk + 36 * HD))[lane * NG + j] = 0;
-                }
-            }
             __syncwarp();
         }
-        w.block(blk, lo, hi, lane);
+        w.block(blk, (float *)(smem + at.params) + warp * w.SCRATCH, lo, hi, lane);
+        if ((i & 3) == 3) w.flush();
         __syncwarp();   // every lane is done with the stage
-        if (lane == 0 && i + AK_STAGES < n_mine) {
+        if (lane == 0 && i + STAGES < n_mine) {
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // (a patched block is overwritten by the copy)
-            load(i + AK_STAGES);
+            load(i + STAGES);
         }
     }
+    w.flush();
     // ---- results of this warp over its own ring, then of the CTA ----
     float *part = (float *)(smem + at.ring);
-    constexpr int WS = AK_STAGES * BB / 4;   // floats from one warp's results to the next
+    constexpr int WS = STAGES * BB / 4;   // floats from one warp's results to the next
     __syncwarp();
 #pragma unroll
     for (int n = 0; n < NT; n++) {
@@ -668,7 +743,7 @@ __global__ void __launch_bounds__(AK_THREADS) attn_step_kv4_kernel(const AttnKv4
     }
     __syncthreads();
     // runs of 32 outputs: run e belongs to CTA e % CL, in its slot e / CL
-    const int n_runs = n_h * NG, active = min(AK_WARPS, max(1, (n_blk - rank + CL - 1) / CL));
+    const int n_runs = n_h * NG, active = min(AK_WARPS, max(1, (n_blk - cta + R - 1) / R));
     cluster_wait();   // (arrived at the top) every CTA of the cluster has started
     for (int e = warp; e < n_runs; e += AK_WARPS) {
         const int h = e / NG, j = e - h * NG;
@@ -693,14 +768,39 @@ __global__ void __launch_bounds__(AK_THREADS) attn_step_kv4_kernel(const AttnKv4
     for (int e = rank + CL * warp; e < n_runs; e += CL * AK_WARPS) {
         const float *src = recv + (e / CL) * CL * 34;
         const int head = h_lo + e / NG;
-        const float sink = a.sinks ? a.sinks[head] * 1.44269504f : -INFINITY;
-        float top = fmaxf(sink, -3.0e38f);
+        float top = -3.0e38f, l = 0.f, o = 0.f;
         for (int c = 0; c < CL; c++) top = fmaxf(top, src[34 * c]);
-        float l = ex2(sink - top), o = 0.f;
         for (int c = 0; c < CL; c++) {
             const float f = ex2(src[34 * c] - top);
             l = fmaf(src[34 * c + 1], f, l);
             o = fmaf(src[34 * c + 2 + lane], f, o);
+        }
+        if (NC > 1) {
+            float *ws = a.workspace + AK_COUNTERS + (size_t)(unit * 32 + e) * a.clusters * 34;
+            __stcg(ws + nth * 34 + 2 + lane, o);
+            if (lane < 2) __stcg(ws + nth * 34 + lane, lane ? l : top);
+            __threadfence();
+            __syncwarp();
+            int *count = (int *)a.workspace + unit * 32 + e;
+            int before = 0;
+            if (lane == 0) before = atomicAdd(count, 1);
+            if (__shfl_sync(0xFFFFFFFFu, before, 0) != NC - 1) continue;
+            __threadfence();
+            if (lane == 0) *count = 0;   // for the next call
+            float all_top = -3.0e38f;
+            for (int c = 0; c < NC; c++) all_top = fmaxf(all_top, __ldcg(ws + 34 * c));
+            l = o = 0.f;
+            top = all_top;
+            for (int c = 0; c < NC; c++) {
+                const float f = ex2(__ldcg(ws + 34 * c) - top);
+                l = fmaf(__ldcg(ws + 34 * c + 1), f, l);
+                o = fmaf(__ldcg(ws + 34 * c + 2 + lane), f, o);
+            }
+        }
+        if (a.sinks) {
+            const float sink = a.sinks[head] * 1.44269504f, all = fmaxf(sink, top), f = ex2(top - all);
+            l = fmaf(l, f, ex2(sink - all));
+            o *= f;
         }
         const float r = o / l;
         const int first_out = head * HD + 32 * (e % NG);

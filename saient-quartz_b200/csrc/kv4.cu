@@ -1,4 +1,9 @@
 // C entry points of the 4-bit KV cache and of the attention over it.
+#include <algorithm>
+#include <atomic>
+#include <memory>
+#include <vector>
+
 #include "attn_kv4.cuh"
 #include "host.cuh"
 
@@ -30,40 +35,101 @@ bool refuse(const char *why)
     return false;
 }
 
-// Cluster width of the step kernel: as many CTAs per kv head as leave all clusters on the chip at once, no more than the
-// cache has blocks, at most what the device can schedule (16 needs the non-portable size).
+// Shape of the step kernel: clusters of CL <= 8 CTAs, `clusters` of them per unit.  8 is the widest size that leaves (almost)
+// no SM without a cluster; narrower when the units alone would not fit on the chip at once or the cache has fewer blocks.
+struct StepShape {
+    int cl, clusters;
+};
 template <int NG, int NT>
-int step_cluster(int clusters, int n_blocks, int GV)
+StepShape step_shape(int units, int n_blocks, int GV)
 {
-    static bool ready = false;
-    if (!ready) {
+    static int fit[4 * NT + 1][4] = {};   // clusters of 1, 2, 4, 8 CTAs that the device holds at once
+    int (&f)[4] = fit[GV];
+    if (!f[0]) {
         const auto kernel = attn_step_kv4_kernel<NG, NT>;
-        QZ_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, attn_kv4_smem(NG, NT, 4 * NT, 16).total));
-        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) cudaGetLastError();
-        ready = true;
-    }
-    static int widest[4 * NT + 1] = {};   // by query heads per cluster (they size the shared memory a little)
-    if (!widest[GV]) {
-        int cl = 16;
-        for (int n = 0; cl > 1; cl /= 2) {
+        QZ_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, attn_kv4_smem(NG, NT, 4 * NT, 8).total));
+        for (int i = 0; i < 4; i++) {
             cudaLaunchConfig_t cfg = {};
             cudaLaunchAttribute at[1];
             at[0].id = cudaLaunchAttributeClusterDimension;
-            at[0].val.clusterDim.x = (unsigned)cl;
+            at[0].val.clusterDim.x = 1u << i;
             at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-            cfg.gridDim = dim3(cl);
+            cfg.gridDim = dim3(1u << i);
             cfg.blockDim = dim3(AK_THREADS);
-            cfg.dynamicSmemBytes = attn_kv4_smem(NG, NT, GV, cl).total;
+            cfg.dynamicSmemBytes = attn_kv4_smem(NG, NT, GV, 1 << i).total;
             cfg.attrs = at;
             cfg.numAttrs = 1;
-            if (cudaOccupancyMaxActiveClusters(&n, attn_step_kv4_kernel<NG, NT>, &cfg) == cudaSuccess && n >= 1) break;
-            cudaGetLastError();
+            if (cudaOccupancyMaxActiveClusters(&f[i], kernel, &cfg) != cudaSuccess || f[i] < 1) {
+                cudaGetLastError();
+                f[i] = i ? 0 : 1;
+            }
         }
-        widest[GV] = cl;
     }
-    int cl = widest[GV];
-    while (cl > 1 && (clusters * cl > sm_count() || cl / 2 >= n_blocks)) cl /= 2;
-    return cl;
+    int i = 3;
+    while (i > 0 && (f[i] < units || (1 << (i - 1)) >= n_blocks)) i--;
+    const int useful = std::max(1, n_blocks / (AK_WARPS << i));
+    return {1 << i, std::max(1, std::min({f[i] / units, useful, AK_MAX_CLUSTERS / units}))};
+}
+
+// The workspace in which the clusters of a unit meet.  Calls on one stream follow one another and share one; every graph
+// that is being captured gets one of its own (graphs may be replayed side by side), which returns to the pool when the
+// last executable form of the graph is gone.  NULL if it cannot be had (then one cluster per unit works).
+struct Workspace {
+    int device;
+    cudaStream_t stream;
+    unsigned long long capture;   // 0: calls that run at once
+    float *ptr;
+    std::atomic<bool> in_use;
+};
+float *merge_workspace()
+{
+    static std::vector<std::unique_ptr<Workspace>> all;
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    cudaGraph_t graph = nullptr;
+    if (cudaStreamGetCaptureInfo_v2(stream(), &status, &id, &graph, nullptr, nullptr) != cudaSuccess) cudaGetLastError();
+    if (status == cudaStreamCaptureStatusInvalidated) return nullptr;
+    const bool capturing = status == cudaStreamCaptureStatusActive;
+    if (!capturing) id = 0;
+    int device = 0;
+    cudaGetDevice(&device);
+    Workspace *w = nullptr;
+    for (auto &e : all)
+        if (e->device == device && e->in_use && e->stream == stream() && e->capture == id) return e->ptr;
+    for (auto &e : all)
+        if (e->device == device && !e->in_use) w = e.get();
+    if (!w) {
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;   // allocating does not disturb a capture
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        float *p = nullptr;
+        cudaStream_t side = nullptr;
+        bool ok = cudaMalloc(&p, AK_WORKSPACE) == cudaSuccess && cudaStreamCreateWithFlags(&side, cudaStreamNonBlocking) == cudaSuccess &&
+                  cudaMemsetAsync(p, 0, AK_COUNTERS * sizeof(int), side) == cudaSuccess && cudaStreamSynchronize(side) == cudaSuccess;
+        if (side) cudaStreamDestroy(side);
+        if (!ok) {
+            cudaGetLastError();
+            if (p) cudaFree(p);
+        }
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        if (!ok) return nullptr;
+        all.push_back(std::make_unique<Workspace>());
+        w = all.back().get();
+        w->device = device;
+        w->ptr = p;
+    }
+    if (capturing) {
+        cudaUserObject_t owner = nullptr;
+        const auto release = [](void *e) { ((Workspace *)e)->in_use = false; };
+        if (cudaUserObjectCreate(&owner, w, release, 1, cudaUserObjectNoDestructorSync) != cudaSuccess ||
+            cudaGraphRetainUserObject(graph, owner, 1, cudaGraphUserObjectMove) != cudaSuccess) {
+            cudaGetLastError();
+            return nullptr;
+        }
+    }
+    w->stream = stream();
+    w->capture = id;
+    w->in_use = true;
+    return w->ptr;
 }
 
 // NG = head_dim / 32 as a template argument
@@ -171,12 +237,14 @@ void cuda_attn_step_kv4(float *out, const float *q, const float *k_new, const fl
     a.splits = (G + 7) / 8;
     a.prefetch = pdl_enabled() && d_step;
     a.status = status_word_if_ready();
-    const int GV = (G + a.splits - 1) / a.splits, clusters = n_kv_heads * a.splits;
+    const int GV = (G + a.splits - 1) / a.splits, units = n_kv_heads * a.splits;
     by_groups(head_dim, [&](auto ng) {
         auto go = [&](auto nt) {
-            const int cl = step_cluster<ng.value, nt.value>(clusters, a.n_blocks, GV);
-            launch_cluster(attn_step_kv4_kernel<ng.value, nt.value>, dim3(clusters * cl), dim3(AK_THREADS),
-                           (size_t)attn_kv4_smem(ng.value, nt.value, GV, cl).total, cl, a);
+            StepShape s = step_shape<ng.value, nt.value>(units, a.n_blocks, GV);
+            if (s.clusters > 1 && !(a.workspace = merge_workspace())) s.clusters = 1;
+            a.clusters = s.clusters;
+            launch_cluster(attn_step_kv4_kernel<ng.value, nt.value>, dim3(units * s.clusters * s.cl), dim3(AK_THREADS),
+                           (size_t)attn_kv4_smem(ng.value, nt.value, GV, s.cl).total, s.cl, a);
         };
         if (GV <= 4) go(std::integral_constant<int, 1>());
         else go(std::integral_constant<int, 2>());
