@@ -8,7 +8,8 @@
 
 namespace qz {
 
-constexpr int AK_THREADS = 256, AK_WARPS = AK_THREADS / 32;
+// six warps: two CTAs of them per SM leave 168 registers a thread (eight: 128, which spill; 131072 positions take 58 us, not 51)
+constexpr int AK_THREADS = 192, AK_WARPS = AK_THREADS / 32;
 constexpr int AK_MAX_G = 16;
 constexpr int AK_MAX_CLUSTERS = 128;                  // of all units together when a unit has several
 constexpr int AK_COUNTERS = AK_MAX_CLUSTERS * 32;     // one per run of 32 outputs of a unit
@@ -144,7 +145,7 @@ __global__ void __launch_bounds__(AK_THREADS) attn_kv4_kernel(const AttnKv4Args 
 // ---- one token ---------------------------------------------------------------------------------------------------
 // One launch whose shape does not depend on the position.  A unit is a kv head (two units when more than eight query heads
 // share it); it has NC clusters of CL CTAs, of which as many work as the context has a block for every warp of.  Warp w of
-// CTA r (of all R working ones) takes the blocks of 32 positions r + R (w + 8 i), so that a short context is spread over the
+// CTA r (of all R working ones) takes the blocks of 32 positions r + R (w + 6 i), so that a short context is spread over the
 // CTAs first.  A warp works alone: it streams its blocks through a ring of its own (one bulk copy per block: the block is
 // contiguous) and keeps scores, weights and outputs of all heads in registers.  A cluster's CTAs push their results into
 // the CTA that finishes a run of 32 outputs; with several clusters at work, that CTA leaves the run in a workspace and the
@@ -170,6 +171,12 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma16816_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
+{
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ float ex2(float x)
 {
     float y;
@@ -181,20 +188,36 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi)
     const __half2 h = __floats2half2_rn(lo, hi);
     return *(const uint32_t *)&h;
 }
-// The four pairs (i, i + 4) of a word's eight nibbles as pairs of f16 numbers code - 8.
-__device__ __forceinline__ void kv4_pairs(uint32_t w, uint32_t (&x)[4])
+// (v & mask) | magic as ONE instruction: both constants live in registers (two immediates would make it two)
+__device__ __forceinline__ uint32_t and_or(uint32_t v, uint32_t mask, uint32_t magic)
 {
-    const __half2 m1032 = __half2half2(__ushort_as_half((unsigned short)0xE408)), m72 = __half2half2(__ushort_as_half((unsigned short)0xD480)),
-                  sixteenth = __half2half2(__ushort_as_half((unsigned short)0x2C00));
-#pragma unroll
-    for (int i = 0; i < 4; i += 2) {
-        const uint32_t v = i ? w >> 8 : w;
-        const uint32_t even = (v & 0x000F000Fu) | 0x64006400u, odd = (v & 0x00F000F0u) | 0x64006400u;   // 1024 + c, 1024 + 16 c
-        const __half2 e = __hadd2(*(const __half2 *)&even, m1032), o = __hfma2(*(const __half2 *)&odd, sixteenth, m72);
-        x[i] = *(const uint32_t *)&e;
-        x[i + 1] = *(const uint32_t *)&o;
-    }
+    uint32_t y;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(v), "r"(mask), "r"(magic));
+    return y;
 }
+struct Nibbles {
+    uint32_t even, odd, magic;
+    __device__ __forceinline__ Nibbles()
+    {
+        asm volatile("mov.b32 %0, 0x000F000F;" : "=r"(even));   // (volatile: kept in registers, not rebuilt at each use)
+        asm volatile("mov.b32 %0, 0x00F000F0;" : "=r"(odd));
+        asm volatile("mov.b32 %0, 0x64006400;" : "=r"(magic));
+    }
+    // The four pairs (i, i + 4) of a word's eight nibbles as pairs of f16 numbers code - 8.
+    __device__ __forceinline__ void pairs(uint32_t w, uint32_t (&x)[4]) const
+    {
+        const __half2 m1032 = __half2half2(__ushort_as_half((unsigned short)0xE408)), m72 = __half2half2(__ushort_as_half((unsigned short)0xD480)),
+                      sixteenth = __half2half2(__ushort_as_half((unsigned short)0x2C00));
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+            const uint32_t v = i ? w >> 8 : w;
+            const uint32_t e = and_or(v, even, magic), o = and_or(v, odd, magic);   // 1024 + c, 1024 + 16 c
+            const __half2 he = __hadd2(*(const __half2 *)&e, m1032), ho = __hfma2(*(const __half2 *)&o, sixteenth, m72);
+            x[i] = *(const uint32_t *)&he;
+            x[i + 1] = *(const uint32_t *)&ho;
+        }
+    }
+};
 // N halves (N = 1..4) at a 2N-aligned address, as floats
 template <int N>
 __device__ __forceinline__ void lds_halves(const void *p, float (&x)[N])
@@ -272,6 +295,7 @@ struct Kv4Warp {
     float acc[NT][2 * NG][2]; // flushed sums (hi + lo)
     float mo[NT][NG];         // partial sums of p * (m + 8 d), head gr / 2
     float ve;                 // power of two that p * d carries
+    Nibbles nib;
 
     __device__ __forceinline__ void clear()
     {
@@ -360,12 +384,12 @@ struct Kv4Warp {
 #pragma unroll
             for (int j = 0; j < NG; j++) {
                 uint32_t x[4], y[4];
-                kv4_pairs(k0[j], x);
-                kv4_pairs(k1[j], y);
+                nib.pairs(k0[j], x);
+                nib.pairs(k1[j], y);
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
-                    float c[4] = {0.f, 0.f, 0.f, 0.f};
-                    mma16816(c, x[0], y[0], x[1], y[1], qf[n][j][0], qf[n][j][1]);
+                    float c[4];
+                    mma16816_first(c, x[0], y[0], x[1], y[1], qf[n][j][0], qf[n][j][1]);
                     mma16816(c, x[2], y[2], x[3], y[3], qf[n][j][2], qf[n][j][3]);
                     s[tile][n][0] = fmaf(d0[j], c[0] + c[1], fmaf(m0[j], qs[n][j], s[tile][n][0]));
                     s[tile][n][1] = fmaf(d1[j], c[2] + c[3], fmaf(m1[j], qs[n][j], s[tile][n][1]));
@@ -443,8 +467,8 @@ struct Kv4Warp {
 #pragma unroll
             for (int j = 0; j < NG; j++) {
                 uint32_t x[4], y[4];   // dims 4 gr + 0 .. 3 of positions (t, t + 4) and (t + 8, t + 12)
-                kv4_pairs(v01[j], x);
-                kv4_pairs(v23[j], y);
+                nib.pairs(v01[j], x);
+                nib.pairs(v23[j], y);
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
                     float w[4];
@@ -622,11 +646,11 @@ __global__ void __launch_bounds__(AK_THREADS, NT == 1 ? 2 : 1) attn_step_kv4_ker
         }
         __syncwarp();
     };
-    // ---- q as the column operand: warp w prepares head w (columns 2 w and 2 w + 1) ----
-    if (warp < 4 * NT) {
+    // ---- q as the column operand: head h is columns 2 h and 2 h + 1 ----
+    for (int h = warp; h < 4 * NT; h += AK_WARPS) {
         float x[NG], top = 0.f;
-        if (warp < n_h) {
-            rotated(a.q + (size_t)(h_lo + warp) * HD);
+        if (h < n_h) {
+            rotated(a.q + (size_t)(h_lo + h) * HD);
 #pragma unroll
             for (int j = 0; j < NG; j++) {
                 x[j] = rot[32 * j + lane] * (a.scale * 1.44269504f);
@@ -641,7 +665,7 @@ __global__ void __launch_bounds__(AK_THREADS, NT == 1 ? 2 : 1) attn_step_kv4_ker
         // 2^e brings the largest element into [2^13, 2^14)
         const int e = top > 0.f ? max(-100, min(100, 127 + 13 - (int)(__float_as_uint(top) >> 23))) : 0;
         const float up = __uint_as_float((uint32_t)(127 + e) << 23);
-        float *head_qs = qs + warp * (NG + 1);
+        float *head_qs = qs + h * (NG + 1);
         if (lane == 0) head_qs[NG] = 1.f / up;
 #pragma unroll
         for (int j = 0; j < NG; j++) {
@@ -652,8 +676,8 @@ __global__ void __launch_bounds__(AK_THREADS, NT == 1 ? 2 : 1) attn_step_kv4_ker
             const float y = x[j] * up;
             const __half hi = __float2half_rn(y), lo = __float2half_rn(y - __half2float(hi));
             const int slot = (j * 4 + tt) * 8 + (i & 3) * 2 + (i >> 2);
-            qf[(2 * warp) * HD + slot] = hi;
-            qf[(2 * warp + 1) * HD + slot] = lo;
+            qf[(2 * h) * HD + slot] = hi;
+            qf[(2 * h + 1) * HD + slot] = lo;
         }
     }
     __syncthreads();
@@ -779,13 +803,12 @@ __global__ void __launch_bounds__(AK_THREADS, NT == 1 ? 2 : 1) attn_step_kv4_ker
             float *ws = a.workspace + AK_COUNTERS + (size_t)(unit * 32 + e) * a.clusters * 34;
             __stcg(ws + nth * 34 + 2 + lane, o);
             if (lane < 2) __stcg(ws + nth * 34 + lane, lane ? l : top);
-            __threadfence();
             __syncwarp();
             int *count = (int *)a.workspace + unit * 32 + e;
             int before = 0;
-            if (lane == 0) before = atomicAdd(count, 1);
+            // releases the warp's stores (ordered before it by the warp barrier), acquires the other clusters'
+            if (lane == 0) asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(before) : "l"(count) : "memory");
             if (__shfl_sync(0xFFFFFFFFu, before, 0) != NC - 1) continue;
-            __threadfence();
             if (lane == 0) *count = 0;   // for the next call
             float all_top = -3.0e38f;
             for (int c = 0; c < NC; c++) all_top = fmaxf(all_top, __ldcg(ws + 34 * c));
