@@ -4,6 +4,28 @@
 
 using namespace qz;
 
+namespace {
+
+size_t sample_smem(int chunk) { return ((sizeof(SampleShared) + 15) & ~(size_t)15) + (size_t)chunk * 4; }
+
+// CTAs per row: enough for a CTA's part of the row to fit an SM, then, while that leaves SMs idle, more of them as long as a
+// thread keeps four tokens (the device holds 7 clusters of 16).
+int sample_cluster(int n_rows, int vocab)
+{
+    static bool ready = false;
+    if (!ready) {
+        QZ_CUDA_CHECK(cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
+        if (cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) cudaGetLastError();
+        ready = true;
+    }
+    int cl = 1;
+    while (cl < SMP_MAX_CLUSTER && sample_smem((vocab + cl - 1) / cl + 3) > 227 * 1024) cl *= 2;
+    while (cl < SMP_MAX_CLUSTER && (long long)n_rows * cl * 2 <= (cl == 8 ? 112 : sm_count()) && vocab / (cl * 2) >= 4 * SMP_THREADS) cl *= 2;
+    return cl;
+}
+
+}  // namespace
+
 extern "C" void cuda_sample(const float *d_logits, int n_rows, int vocab, size_t row_stride, float temperature, int top_k, float top_p,
                             float min_p, const float *d_u, int *d_tokens, float *d_probs)
 {
@@ -20,6 +42,7 @@ extern "C" void cuda_sample(const float *d_logits, int n_rows, int vocab, size_t
         set_error(QZ_ERR_BAD_SHAPE, "cuda_sample: d_logits, d_tokens and (temperature > 0) d_u must be device pointers");
         return;
     }
-    const SampleArgs a = {d_logits, row_stride, vocab, temperature, top_k, top_p, min_p, d_u, d_tokens, d_probs};
-    launch(sample_kernel, dim3((unsigned)n_rows), dim3(SMP_THREADS), 0, a);
+    const int cl = sample_cluster(n_rows, vocab), chunk = ((vocab + cl - 1) / cl + 3) & ~3;
+    const SampleArgs a = {d_logits, row_stride, vocab, temperature, top_k, top_p, min_p, d_u, d_tokens, d_probs, chunk};
+    launch_cluster(sample_kernel, dim3((unsigned)n_rows * cl), dim3(SMP_THREADS), sample_smem(chunk), cl, a);
 }

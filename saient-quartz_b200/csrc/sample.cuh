@@ -10,6 +10,8 @@
 // 2^19 tokens of weight 1 still fit.  A logit of -inf or NaN has no weight and is never chosen.
 #pragma once
 
+#include <cooperative_groups.h>
+
 #include "common.cuh"
 
 namespace qz {
@@ -29,9 +31,11 @@ struct SampleArgs {
     const float *u;
     int *tokens;
     float *probs;
+    int chunk;   // tokens per CTA, a multiple of 4
 };
 
-// order of f32 values as unsigned integers; -0 counts as +0, NaN comes last
+// Order of f32 values as unsigned integers; -0 counts as +0, NaN comes last.  A token's place in its row is the number
+// key << 32 | ~index: larger = earlier.
 __device__ __forceinline__ uint32_t smp_key(float z)
 {
     if (!(z == z)) return 0;
@@ -40,7 +44,10 @@ __device__ __forceinline__ uint32_t smp_key(float z)
 }
 constexpr uint32_t SMP_KEY_MIN = 0x00800000u;   // keys from here on are logits above -inf
 
-// weight of logit z in units of 2^-44.  Weights above 2^-13 carry the sums and are taken in 64 bits; below, the f32
+__device__ __forceinline__ float smp_unkey(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k); }
+
+__device__ __noinline__ u64 smp_weight64(float z, float M, double inv_t) { return (u64)__double2ull_rn(exp(((double)z - (double)M) * inv_t) * SMP_ONE); }
+// Weight of logit z in units of 2^-44.  Weights above 2^-13 carry the sums and are taken in 64 bits; below, the f32
 // error (1e-6 of a weight under 1e-4) is lost in the total.
 __device__ __forceinline__ u64 smp_weight(float z, float M, float inv_t, double inv_t64)
 {
@@ -48,147 +55,406 @@ __device__ __forceinline__ u64 smp_weight(float z, float M, float inv_t, double 
     const float x = (z - M) * inv_t;
     if (x < -31.5f) return 0;
     if (x < -9.f) return (u64)__float2uint_rn(expf(x) * (float)SMP_ONE);
-    return (u64)__double2ull_rn(exp(((double)z - (double)M) * inv_t64) * SMP_ONE);
+    return smp_weight64(z, M, inv_t64);
 }
 
-template <class T, class Op>
-__device__ __forceinline__ T smp_block_reduce(T v, T *sm, Op op)
+// ---- the kernel -------------------------------------------------------------------------------------------------
+// A cluster of CL CTAs per row; each keeps a contiguous part of the row in shared memory, read once from HBM.  Nothing is
+// sorted: a threshold is the number of the last token kept, and is found by counting.
+//   1. the largest number of the row (M; at temperature 0 the answer)
+//   2. a histogram of the logits over 1024 bins of 1/32 of the temperature below M
+//   3. top_k: the bin of the k-th token follows from the counts; its tokens are gathered and ranked against one another.
+//      When all tokens down to that bin fit the list (k up to some hundreds), everything else is done on the list.
+//   4. top_p: the counts bracket the bin in which the weights reach their goal (a bin's tokens weigh the same within 1/32);
+//      one pass sums the weights above the bracket and below it, and those inside bin by bin; the tokens of the right
+//      bin are gathered and ranked.
+//   5. the kept weights are summed warp by warp in the order of the vocabulary; the warp in whose range u falls walks it.
+// A bin with more tokens than the list takes (ties, high temperatures) is divided further, by the number itself.
+// A histogram is reduced in slices, one per CTA, that are pushed to every CTA: all find the same bin without asking.
+constexpr int SMP_BINS = 1024, SMP_LIST = 512, SMP_WARPS = SMP_THREADS / 32, SMP_MAX_CLUSTER = 16;
+
+struct SampleShared {
+    uint32_t cnt[SMP_BINS], part[3][SMP_BINS];    // this CTA's histogram: tokens, and their weights in parts of 15 bits
+    uint32_t all_cnt[SMP_BINS];                   // the row's
+    u64 all_w[SMP_BINS];
+    u64 mine[SMP_LIST], list[SMP_LIST];           // gathered tokens: this CTA's; (CTA 0) the row's
+    u64 list_w[SMP_LIST];
+    u64 from[2][SMP_MAX_CLUSTER][3];              // what the cluster's CTAs pushed last, and before
+    u64 red[SMP_WARPS];
+    u64 result;
+    u64 before;
+    int n_mine, n_list, at, bin;
+};
+
+// sum, or largest, over the block; every thread gets it
+template <bool MAX>
+__device__ __forceinline__ u64 smp_reduce(u64 v, u64 *sm)
 {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+    for (int o = 16; o > 0; o >>= 1) {
+        const u64 y = __shfl_xor_sync(0xFFFFFFFFu, v, o);
+        v = MAX ? (v > y ? v : y) : v + y;
+    }
     __syncthreads();
     if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = v;
     __syncthreads();
     v = sm[threadIdx.x & 31];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+    for (int o = 16; o > 0; o >>= 1) {
+        const u64 y = __shfl_xor_sync(0xFFFFFFFFu, v, o);
+        v = MAX ? (v > y ? v : y) : v + y;
+    }
     return v;
 }
-__device__ __forceinline__ u64 smp_block_sum(u64 v, u64 *sm)
+template <class T>
+__device__ __forceinline__ T smp_warp_inclusive(T v)
 {
-    return smp_block_reduce(v, sm, [](u64 a, u64 b) { return a + b; });
-}
-// sum over the threads before this one; *total over all
-__device__ __forceinline__ u64 smp_block_before(u64 v, u64 *sm, u64 *total)
-{
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    u64 inc = v;
+    const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const u64 y = __shfl_up_sync(0xFFFFFFFFu, inc, o);
-        if (lane >= o) inc += y;
+        const T y = __shfl_up_sync(0xFFFFFFFFu, v, o);
+        if (lane >= o) v += y;
     }
+    return v;
+}
+// sum over the threads before this one; *total over all (T of 8 bytes)
+template <class T>
+__device__ __forceinline__ T smp_before(T v, u64 *scratch, T *total)
+{
+    T *sm = (T *)scratch;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const T inc = smp_warp_inclusive(v);
     __syncthreads();
     if (lane == 31) sm[warp] = inc;
     __syncthreads();
-    u64 w = sm[lane], winc = w;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const u64 y = __shfl_up_sync(0xFFFFFFFFu, winc, o);
-        if (lane >= o) winc += y;
-    }
+    const T w = sm[lane], winc = smp_warp_inclusive(w);
     *total = __shfl_sync(0xFFFFFFFFu, winc, 31);
     return __shfl_sync(0xFFFFFFFFu, winc - w, warp) + inc - v;
 }
 
-// One CTA per row; thresholds found by bisecting the 32 bits of the key.
+struct Sampler {
+    SampleShared &s;
+    const float *z;       // this CTA's part of the row
+    int n, base;          // tokens in it, index of the first
+    int CL, rank, turn;
+    float M, inv, per_bin;
+    double inv64;
+    u64 keep;             // number of the last token of the set
+
+    __device__ __forceinline__ SampleShared *peer(int r) const { return cooperative_groups::this_cluster().map_shared_rank(&s, r); }
+    __device__ __forceinline__ void sync() const { cooperative_groups::this_cluster().sync(); }
+    __device__ __forceinline__ u64 number(int i) const { return (u64)smp_key(z[i]) << 32 | (uint32_t)~(base + i); }
+    __device__ __forceinline__ int bin(float x) const
+    {
+        const float t = (M - x) * per_bin;
+        return x == M ? 0 : t < (float)(SMP_BINS - 1) ? (int)t : SMP_BINS - 1;
+    }
+    __device__ __forceinline__ u64 weight(float x) const { return smp_weight(x, M, inv, inv64); }
+    __device__ __forceinline__ u64 weight_of(u64 number) const { return weight(smp_unkey((uint32_t)(number >> 32))); }
+
+    // three values of this CTA to every CTA: afterwards s.from[turn][r] holds those of CTA r (two turns' worth are kept:
+    // a CTA may still read the last ones while another pushes the next)
+    __device__ __forceinline__ void exchange(u64 a, u64 b, u64 c)
+    {
+        turn ^= 1;
+        if ((int)threadIdx.x < CL) {
+            u64 *to = peer(threadIdx.x)->from[turn][rank];
+            to[0] = a;
+            to[1] = b;
+            to[2] = c;
+        }
+        sync();
+    }
+    __device__ __forceinline__ void clear(bool weights)
+    {
+        s.cnt[threadIdx.x] = 0;
+        if (weights) s.part[0][threadIdx.x] = s.part[1][threadIdx.x] = s.part[2][threadIdx.x] = 0;
+        if (threadIdx.x == 0) s.bin = -1;
+        __syncthreads();
+    }
+    __device__ __forceinline__ void add(int b, bool weights, float x)
+    {
+        atomicAdd(&s.cnt[b], 1u);
+        if (weights) {
+            const u64 w = weight(x);
+            atomicAdd(&s.part[0][b], (uint32_t)(w & 0x7FFF));
+            atomicAdd(&s.part[1][b], (uint32_t)(w >> 15 & 0x7FFF));
+            atomicAdd(&s.part[2][b], (uint32_t)(w >> 30));
+        }
+    }
+    // the row's histogram into every CTA: a thread reads one bin of one CTA, CL lanes make a bin's sum and push it
+    __device__ __forceinline__ void collect(bool weights)
+    {
+        sync();
+        const int p = threadIdx.x % CL, b = rank * (SMP_BINS / CL) + threadIdx.x / CL;
+        const SampleShared *from = peer(p);
+        uint32_t c = from->cnt[b];
+        u64 w = 0;
+        if (weights) w = (u64)from->part[0][b] + ((u64)from->part[1][b] << 15) + ((u64)from->part[2][b] << 30);
+        for (int o = 1; o < CL; o <<= 1) {
+            c += __shfl_xor_sync(0xFFFFFFFFu, c, o);
+            if (weights) w += __shfl_xor_sync(0xFFFFFFFFu, w, o);
+        }
+        peer(p)->all_cnt[b] = c;
+        if (weights) peer(p)->all_w[b] = w;
+        sync();
+    }
+    // The first bin at which `above` plus the sum up to and with it reaches the goal; *before: the sum above it.
+    // (The last bin that holds anything where the goal is not reached: fewer tokens than top_k.)
+    __device__ __forceinline__ int boundary(bool weights, u64 above, double goal, u64 *before)
+    {
+        const u64 v = weights ? s.all_w[threadIdx.x] : s.all_cnt[threadIdx.x];
+        u64 total;
+        const u64 sum = above + smp_before(v, s.red, &total);
+        if (v && (double)sum < goal && (goal <= (double)(sum + v) || sum + v == above + total)) {
+            s.bin = threadIdx.x;
+            s.before = sum;
+        }
+        __syncthreads();
+        const int b = s.bin;
+        *before = s.before;
+        __syncthreads();   // (read before the next clear)
+        return b;
+    }
+    // The tokens for which pred holds, as numbers, in CTA 0's list (it takes them all: the caller has counted)
+    template <class Pred>
+    __device__ __forceinline__ void gather(Pred pred)
+    {
+        if (threadIdx.x == 0) s.n_mine = s.n_list = 0;
+        sync();
+        for (int i = threadIdx.x; i < n; i += SMP_THREADS)
+            if (pred(i)) s.mine[atomicAdd(&s.n_mine, 1)] = number(i);
+        __syncthreads();
+        if (threadIdx.x == 0) s.at = atomicAdd(&peer(0)->n_list, s.n_mine);
+        __syncthreads();
+        for (int i = threadIdx.x; i < s.n_mine; i += SMP_THREADS) peer(0)->list[s.at + i] = s.mine[i];
+        sync();
+    }
+    // Number of the last token with `above` + (weights, or count, of the set's tokens before it) < goal, given that it is
+    // among the `count` tokens of bin b.
+    __device__ __forceinline__ u64 last_in_bin(int b, uint32_t count, u64 above, double goal, bool weights)
+    {
+        u64 lo = 0, hi = ~(u64)0;
+        if (count > SMP_LIST) {
+            u64 small = 0, large = 0;   // largest of ~number and of number
+            for (int i = threadIdx.x; i < n; i += SMP_THREADS) {
+                const u64 x = number(i);
+                if (x >= keep && bin(z[i]) == b) {
+                    small = max(small, ~x);
+                    large = max(large, x);
+                }
+            }
+            small = smp_reduce<true>(small, s.red);
+            large = smp_reduce<true>(large, s.red);
+            exchange(small, large, 0);
+            for (int r = 0; r < CL; r++) {
+                small = max(small, s.from[turn][r][0]);
+                large = max(large, s.from[turn][r][1]);
+            }
+            lo = ~small;
+            hi = large;
+            while (count > SMP_LIST && lo < hi) {
+                const int shift = max(0, 54 - __clzll((long long)(hi - lo)));   // (hi - lo) >> shift < 1024
+                clear(weights);
+                for (int i = threadIdx.x; i < n; i += SMP_THREADS) {
+                    const u64 x = number(i);
+                    if (x >= lo && x <= hi) add((int)((hi - x) >> shift), weights, z[i]);
+                }
+                collect(weights);
+                const int sub = boundary(weights, above, goal, &above);
+                count = s.all_cnt[sub];
+                hi -= (u64)sub << shift;
+                lo = max(lo, hi - (((u64)1 << shift) - 1));
+            }
+            if (lo == hi) return hi;
+            b = -1;
+        }
+        gather([&](int i) {
+            const u64 x = number(i);
+            return x >= keep && (b < 0 ? x >= lo && x <= hi : bin(z[i]) == b);
+        });
+        if (rank == 0) {
+            const int c = s.n_list;
+            const u64 x = (int)threadIdx.x < c ? s.list[threadIdx.x] : 0;
+            if ((int)threadIdx.x < c) s.list_w[threadIdx.x] = weights ? weight_of(x) : 1;
+            __syncthreads();
+            u64 before = above;
+            if ((int)threadIdx.x < c)
+                for (int j = 0; j < c; j++) before += s.list[j] > x ? s.list_w[j] : 0;
+            const u64 last = ~smp_reduce<true>((int)threadIdx.x < c && (double)before < goal ? ~x : 0, s.red);
+            if ((int)threadIdx.x < CL) peer(threadIdx.x)->result = last;
+        }
+        sync();
+        return s.result;
+    }
+};
+
 __global__ void __launch_bounds__(SMP_THREADS) sample_kernel(const SampleArgs a)
 {
-    __shared__ u64 sm[32];
+    extern __shared__ __align__(16) unsigned char smem[];
+    SampleShared &s = *(SampleShared *)smem;
+    float *z = (float *)(smem + ((sizeof(SampleShared) + 15) & ~(size_t)15));
+    const cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    Sampler c = {s, z};
+    c.CL = (int)cluster.num_blocks();
+    c.rank = (int)cluster.block_rank();
+    c.turn = 0;
+    c.base = c.rank * a.chunk;
+    c.n = max(0, min(a.chunk, a.vocab - c.base));
+    const int row = blockIdx.x / c.CL, n = c.n;
     pdl_wait();
     pdl_trigger();
-    const float *z = a.logits + (size_t)blockIdx.x * a.ld;
-    const int n = a.vocab, tid = threadIdx.x;
-    // strided passes for sums, a contiguous chunk per thread where the order of the indices matters
-    auto sum = [&](auto f) {
-        u64 s = 0;
-        for (int i = tid; i < n; i += SMP_THREADS) s += f(z[i]);
-        return smp_block_sum(s, sm);
-    };
-    u64 best = 0;
-    for (int i = tid; i < n; i += SMP_THREADS) {
-        const uint32_t k = smp_key(z[i]);
-        if (k >= SMP_KEY_MIN) best = max(best, (u64)k << 32 | (uint32_t)~i);
+    // ---- 1. the row into shared memory; its first token ----
+    const float *src = a.logits + (size_t)row * a.ld + c.base;
+    if (((uintptr_t)src & 15) == 0) {
+        for (int i = tid; i < n / 4; i += SMP_THREADS) ((float4 *)z)[i] = __ldcs((const float4 *)src + i);
+        if (tid < (n & 3)) z[(n & ~3) + tid] = src[(n & ~3) + tid];
+    } else {
+        for (int i = tid; i < n; i += SMP_THREADS) z[i] = __ldcs(src + i);
     }
-    best = smp_block_reduce(best, sm, [](u64 x, u64 y) { return x > y ? x : y; });
-    if (best == 0 || a.temperature == 0.f) {
-        if (tid == 0) {
-            a.tokens[blockIdx.x] = best ? (int)~(uint32_t)best : -1;
-            if (a.probs) a.probs[blockIdx.x] = best ? 1.f : 0.f;
+    c.clear(false);   // (synchronises)
+    u64 best = 0;
+    for (int i = tid; i < n; i += SMP_THREADS) best = max(best, c.number(i));
+    best = smp_reduce<true>(best, s.red);
+    c.exchange(best, 0, 0);
+    for (int r = 0; r < c.CL; r++) best = max(best, s.from[c.turn][r][0]);
+    const bool none = best < (u64)SMP_KEY_MIN << 32;
+    if (none || a.temperature == 0.f) {
+        if (c.rank == 0 && tid == 0) {
+            a.tokens[row] = none ? -1 : (int)~(uint32_t)best;
+            if (a.probs) a.probs[row] = none ? 0.f : 1.f;
         }
         return;
     }
-    const float M = z[~(uint32_t)best];
-    const uint32_t key_max = (uint32_t)(best >> 32);
-    const double inv64 = 1.0 / (double)a.temperature;
-    const float inv = (float)inv64;
-    // ---- top_k: the smallest key of the set, and how many tokens of that key belong to it ----
-    uint32_t t_k = SMP_KEY_MIN;
-    u64 r_k = (u64)n;
-    if (a.top_k > 0 && a.top_k < n && sum([&](float x) { return (u64)(smp_key(x) >= SMP_KEY_MIN); }) > (u64)a.top_k) {
-        t_k = 0;
-        for (int bit = 31; bit >= 0; bit--) {
-            const uint32_t c = t_k | 1u << bit;
-            if (sum([&](float x) { return (u64)(smp_key(x) >= c); }) >= (u64)a.top_k) t_k = c;
-        }
-        r_k = (u64)a.top_k - sum([&](float x) { return (u64)(smp_key(x) > t_k); });
-    }
-    // ---- top_p ----
-    uint32_t t_f = t_k;
-    u64 r_f = r_k;
-    if (a.top_p <= 0.f) {
-        t_f = key_max;
-        r_f = 1;
-    } else if (a.top_p < 1.f) {
-        const u64 ties = sum([&](float x) { return (u64)(smp_key(x) == t_k); });
-        const u64 above_k = sum([&](float x) { return smp_key(x) > t_k ? smp_weight(x, M, inv, inv64) : 0; });
-        const u64 tie_w = sum([&](float x) { return smp_key(x) == t_k ? smp_weight(x, M, inv, inv64) : 0; });
-        const double goal = (double)a.top_p * (double)(above_k + (ties ? tie_w / ties * min(ties, r_k) : 0));
-        // the largest key whose tokens above it do not reach the goal yet is one more than the largest that do
-        uint32_t t = 0;
-        for (int bit = 31; bit >= 0; bit--) {
-            const uint32_t c = t | 1u << bit;
-            if (c <= t_k || (double)sum([&](float x) { return smp_key(x) > c - 1 ? smp_weight(x, M, inv, inv64) : 0; }) >= goal) t = c;
-        }
-        // (weight of the tokens with key >= t reaches the goal, that of key >= t + 1 does not)
-        if (t > t_k) {
-            t_f = t;
-            r_f = (u64)n;
-        }
-        const u64 eq = sum([&](float x) { return (u64)(smp_key(x) == t_f); });
-        const double above = (double)sum([&](float x) { return smp_key(x) > t_f ? smp_weight(x, M, inv, inv64) : 0; });
-        const u64 w = eq ? sum([&](float x) { return smp_key(x) == t_f ? smp_weight(x, M, inv, inv64) : 0; }) / eq : 0;
-        if (w > 0 && above < goal) r_f = min(r_f, max((u64)1, (u64)ceil((goal - above) / (double)w)));
-    }
-    // ---- min_p is a lower bound of the weight ----
-    const double lowest = fmin((double)a.min_p, 1.0);
-    const int per = (n + SMP_THREADS - 1) / SMP_THREADS, lo = min(n, tid * per), hi = min(n, lo + per);
-    u64 eq = 0, total;
-    for (int i = lo; i < hi; i++) eq += smp_key(z[i]) == t_f;
-    const u64 eq_before = smp_block_before(eq, sm, &total);
-    auto kept = [&](float x, u64 &rank) -> u64 {
-        const uint32_t k = smp_key(x);
-        if (k < t_f || k < SMP_KEY_MIN || (k == t_f && rank++ >= r_f)) return 0;
-        if (lowest > 0.0 && k != key_max && exp(((double)x - (double)M) * inv64) < lowest) return 0;
-        return smp_weight(x, M, inv, inv64);
+    c.M = smp_unkey((uint32_t)(best >> 32));
+    c.inv64 = 1.0 / (double)a.temperature;
+    c.inv = (float)c.inv64;
+    c.per_bin = (float)(32.0 * c.inv64);
+    c.keep = (u64)SMP_KEY_MIN << 32;
+    const double u = (double)fminf(fmaxf(a.u[row], 0.f), 1.f), lowest = fmin((double)a.min_p, 1.0);
+    const float log_lowest = lowest > 0.0 ? (float)log(lowest) : -INFINITY;
+    auto heavy = [&](float x) {   // weight >= min_p: decided in 64 bits where 32 could be wrong
+        const float y = (x - c.M) * c.inv;
+        if (x == c.M || y > log_lowest + 1e-3f) return true;
+        if (y < log_lowest - 1e-3f) return false;
+        return exp(((double)x - (double)c.M) * c.inv64) >= lowest;
     };
-    u64 s = 0, rank = eq_before;
-    for (int i = lo; i < hi; i++) s += kept(z[i], rank);
-    const u64 before = smp_block_before(s, sm, &total);
-    const float u = fminf(fmaxf(a.u[blockIdx.x], 0.f), 1.f);
-    const u64 goal = min((u64)floor((double)u * (double)total), total - 1);
-    if (before <= goal && goal < before + s) {
-        u64 run = before;
-        rank = eq_before;
-        for (int i = lo; i < hi; i++) {
-            const u64 w = kept(z[i], rank);
-            run += w;
-            if (run > goal) {
-                a.tokens[blockIdx.x] = i;
-                if (a.probs) a.probs[blockIdx.x] = (float)((double)w / (double)total);
-                break;
+    const bool by_k = a.top_k > 0 && a.top_k < a.vocab, by_p = a.top_p > 0.f && a.top_p < 1.f;
+    if (by_k || by_p) {
+        // ---- 2. counts ----
+        for (int i = tid; i < n; i += SMP_THREADS)
+            if (smp_key(z[i]) >= SMP_KEY_MIN) c.add(c.bin(z[i]), false, z[i]);
+        c.collect(false);
+    }
+    if (a.top_p <= 0.f) {
+        c.keep = best;
+    } else if (by_k) {
+        // ---- 3. top_k ----
+        u64 before;
+        const int b = c.boundary(false, 0, (double)a.top_k, &before);
+        const uint32_t in_bin = s.all_cnt[b];
+        if (before + in_bin <= SMP_LIST) {
+            c.gather([&](int i) { return smp_key(z[i]) >= SMP_KEY_MIN && c.bin(z[i]) <= b; });
+            if (c.rank != 0) return;   // (nobody pushes to this CTA or reads from it any more)
+            const int m = s.n_list;
+            const u64 x = tid < m ? s.list[tid] : 0;
+            int place = 0;
+            if (tid < m)
+                for (int j = 0; j < m; j++) place += s.list[j] > x;
+            const u64 w = tid < m && place < a.top_k ? c.weight_of(x) : 0;
+            if (tid < m) s.list_w[tid] = w;
+            u64 total = smp_reduce<false>(w, s.red), earlier = 0;
+            if (w && a.top_p < 1.f)
+                for (int j = 0; j < m; j++) earlier += s.list[j] > x ? s.list_w[j] : 0;
+            const bool in = w && (a.top_p >= 1.f || (double)earlier < (double)a.top_p * (double)total) && heavy(smp_unkey((uint32_t)(x >> 32)));
+            __syncthreads();
+            if (tid < m) s.list_w[tid] = in ? w : 0;
+            total = smp_reduce<false>(in ? w : 0, s.red);
+            const u64 goal = min((u64)floor(u * (double)total), total - 1);
+            if (in) {
+                u64 run = 0;   // weights of lower indices (larger low words)
+                for (int j = 0; j < m; j++) run += (uint32_t)s.list[j] > (uint32_t)x ? s.list_w[j] : 0;
+                if (run <= goal && goal < run + w) {
+                    a.tokens[row] = (int)~(uint32_t)x;
+                    if (a.probs) a.probs[row] = (float)((double)w / (double)total);
+                }
             }
+            return;
         }
+        c.keep = c.last_in_bin(b, in_bin, before, (double)a.top_k, false);
+    }
+    if (by_p) {
+        // ---- 4. top_p ----
+        if (by_k) {   // the counts of the set (last_in_bin may have used the histogram)
+            c.clear(false);
+            for (int i = tid; i < n; i += SMP_THREADS)
+                if (c.number(i) >= c.keep) c.add(c.bin(z[i]), false, z[i]);
+            c.collect(false);
+        }
+        // a token of bin b weighs between exp(-(b + 1) / 32) and exp(-b / 32); 1e-4 covers the rounding of its bin
+        const double count = (double)s.all_cnt[tid];
+        const double most = count * exp(-(double)tid / 32.0) * 1.0001, least = tid < SMP_BINS - 1 ? count * exp(-(double)(tid + 1) / 32.0) * 0.9999 : 0.0;
+        double most_all, least_all;
+        const double most_before = smp_before(most, s.red, &most_all), least_before = smp_before(least, s.red, &least_all);
+        // first bin that may hold the boundary: the last with most_before < goal; last: the first with least up to it >= goal
+        const int first = (int)smp_reduce<true>(most_before < (double)a.top_p * least_all ? (u64)tid : 0, s.red);
+        const int last = SMP_BINS - 1 - (int)smp_reduce<true>(least_before + least >= (double)a.top_p * most_all ? (u64)(SMP_BINS - 1 - tid) : 0, s.red);
+        c.clear(true);
+        u64 above = 0, below = 0;
+        for (int i = tid; i < n; i += SMP_THREADS) {
+            if (c.number(i) < c.keep) continue;
+            const int b = c.bin(z[i]);
+            if (b < first) above += c.weight(z[i]);
+            else if (b > last) below += c.weight(z[i]);
+            else c.add(b, true, z[i]);
+        }
+        above = smp_reduce<false>(above, s.red);
+        below = smp_reduce<false>(below, s.red);
+        c.exchange(above, below, 0);
+        above = below = 0;
+        for (int r = 0; r < c.CL; r++) {
+            above += s.from[c.turn][r][0];
+            below += s.from[c.turn][r][1];
+        }
+        c.collect(true);
+        u64 inside;
+        smp_before(s.all_w[tid], s.red, &inside);
+        const double goal = (double)a.top_p * (double)(above + inside + below);
+        u64 before;
+        const int b = c.boundary(true, above, goal, &before);
+        if (b >= 0) c.keep = c.last_in_bin(b, s.all_cnt[b], before, goal, true);
+    }
+    // ---- 5. the token ----
+    const int seg = ((n + SMP_WARPS - 1) / SMP_WARPS + 31) & ~31, lo = min(n, warp * seg), hi = min(n, lo + seg);
+    auto kept = [&](int i) -> u64 { return c.number(i) >= c.keep && heavy(z[i]) ? c.weight(z[i]) : 0; };
+    u64 mine = 0, cta;
+    for (int i = lo + lane; i < hi; i += 32) mine += kept(i);
+    u64 warp_sum = mine;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) warp_sum += __shfl_xor_sync(0xFFFFFFFFu, warp_sum, o);
+    u64 run = smp_before(lane == 0 ? warp_sum : 0, s.red, &cta);
+    run = __shfl_sync(0xFFFFFFFFu, run, 0);
+    c.exchange(cta, 0, 0);
+    u64 total = 0;
+    for (int r = 0; r < c.CL; r++) {
+        if (r < c.rank) run += s.from[c.turn][r][0];
+        total += s.from[c.turn][r][0];
+    }
+    const u64 goal = min((u64)floor(u * (double)total), total - 1);
+    if (goal < run || goal >= run + warp_sum) return;
+    for (int i0 = lo; i0 < hi; i0 += 32) {
+        const u64 w = i0 + lane < hi ? kept(i0 + lane) : 0;
+        const u64 inc = run + smp_warp_inclusive(w);
+        const unsigned hit = __ballot_sync(0xFFFFFFFFu, inc > goal);
+        if (hit) {
+            if (lane == __ffs(hit) - 1) {
+                a.tokens[row] = c.base + i0 + lane;
+                if (a.probs) a.probs[row] = (float)((double)w / (double)total);
+            }
+            return;
+        }
+        run = __shfl_sync(0xFFFFFFFFu, inc, 31);
     }
 }
 
