@@ -8,7 +8,7 @@ namespace {
 
 size_t sample_smem(int chunk) { return ((sizeof(SampleShared) + 15) & ~(size_t)15) + (size_t)chunk * 4; }
 
-// CTAs per row: enough for a CTA's part of the row to fit an SM, then, while that leaves SMs idle, more of them as long as a
+// CTAs per row: enough for two CTAs and their parts of rows to fit an SM (16 for the longest rows), then, while that leaves SMs idle, more of them as long as a
 // thread keeps four tokens (the device holds 7 clusters of 16).
 int sample_cluster(int n_rows, int vocab)
 {
@@ -19,7 +19,7 @@ int sample_cluster(int n_rows, int vocab)
         ready = true;
     }
     int cl = 1;
-    while (cl < SMP_MAX_CLUSTER && sample_smem((vocab + cl - 1) / cl + 3) > 227 * 1024) cl *= 2;
+    while (cl < SMP_MAX_CLUSTER && sample_smem((vocab + cl - 1) / cl + 3) > 112 * 1024) cl *= 2;
     while (cl < SMP_MAX_CLUSTER && (long long)n_rows * cl * 2 <= (cl == 8 ? 112 : sm_count()) && vocab / (cl * 2) >= 4 * SMP_THREADS) cl *= 2;
     return cl;
 }

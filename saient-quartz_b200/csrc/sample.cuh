@@ -17,7 +17,7 @@
 namespace qz {
 
 typedef unsigned long long u64;
-constexpr int SMP_THREADS = 1024;
+constexpr int SMP_THREADS = 512;
 constexpr int SMP_MAX_VOCAB = 1 << 19;
 constexpr double SMP_ONE = 17592186044416.0;   // 2^44
 
@@ -42,20 +42,30 @@ __device__ __forceinline__ uint32_t smp_key(float z)
     const uint32_t b = __float_as_uint(z + 0.f);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
-constexpr uint32_t SMP_KEY_MIN = 0x00800000u;   // keys from here on are logits above -inf
 
 __device__ __forceinline__ float smp_unkey(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k); }
 
-__device__ __noinline__ u64 smp_weight64(float z, float M, double inv_t) { return (u64)__double2ull_rn(exp(((double)z - (double)M) * inv_t) * SMP_ONE); }
-// Weight of logit z in units of 2^-44.  Weights above 2^-13 carry the sums and are taken in 64 bits; below, the f32
-// error (1e-6 of a weight under 1e-4) is lost in the total.
-__device__ __forceinline__ u64 smp_weight(float z, float M, float inv_t, double inv_t64)
+// exp of a weight's argument in units of 2^-44.  In 64 bits: with thousands of tokens kept, an error of 1e-7 in their sums
+// moves the border of top_p, or the token that u falls on, once in some thousand rows. 2^(n / 16) from a table, the rest (below ln 2 / 32) by its
+// Taylor series up to the fifth power (1.4e-13).  (CUDA's exp: 730 us, not 610, for 256 rows of 128256.)
+struct SampleExp {
+    double M, scale;        // scale = 16 log2(e) / temperature
+    const double *table;    // 2^(k / 16), k < 16
+    __device__ __forceinline__ u64 operator()(float z) const
+    {
+        const double t = ((double)z - M) * scale, whole = t + 6755399441055744.0;   // 1.5 * 2^52: the sum's low word is t's nearest integer
+        const int n = __double2loint(whole);
+        constexpr double A = 0.04332169878499658;   // ln(2) / 16
+        const double f = (t - (whole - 6755399441055744.0)) * A;
+        const double p = fma(f, fma(f, fma(f, fma(f, fma(f, 1.0 / 120, 1.0 / 24), 1.0 / 6), 0.5), 1.0), 1.0) * table[n & 15];
+        const double w = __hiloint2double(__double2hiint(p) + (((n >> 4) + 44) << 20), __double2loint(p));
+        return (u64)__double_as_longlong(w + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;   // + 2^52: rounded to a whole number
+    }
+};
+// Weight of logit z in units of 2^-44
+__device__ __forceinline__ u64 smp_weight(float z, float M, float inv_t, const SampleExp &e)
 {
-    if (z == M) return (u64)SMP_ONE;
-    const float x = (z - M) * inv_t;
-    if (x < -31.5f) return 0;
-    if (x < -9.f) return (u64)__float2uint_rn(expf(x) * (float)SMP_ONE);
-    return smp_weight64(z, M, inv_t64);
+    return z == M ? (u64)SMP_ONE : (z - M) * inv_t < -31.5f ? 0 : e(z);
 }
 
 // ---- the kernel -------------------------------------------------------------------------------------------------
@@ -71,16 +81,21 @@ __device__ __forceinline__ u64 smp_weight(float z, float M, float inv_t, double 
 //   5. the kept weights are summed warp by warp in the order of the vocabulary; the warp in whose range u falls walks it.
 // A bin with more tokens than the list takes (ties, high temperatures) is divided further, by the number itself.
 // A histogram is reduced in slices, one per CTA, that are pushed to every CTA: all find the same bin without asking.
-constexpr int SMP_BINS = 1024, SMP_LIST = 512, SMP_WARPS = SMP_THREADS / 32, SMP_MAX_CLUSTER = 16;
+constexpr int SMP_BINS = 2 * SMP_THREADS, SMP_LIST = 512,   // (a thread looks after two bins, and one token of the list)
+              SMP_WARPS = SMP_THREADS / 32, SMP_MAX_CLUSTER = 16;
 
 struct SampleShared {
     uint32_t cnt[SMP_BINS], part[3][SMP_BINS];    // this CTA's histogram: tokens, and their weights in parts of 15 bits
     uint32_t all_cnt[SMP_BINS];                   // the row's
     u64 all_w[SMP_BINS];
-    u64 mine[SMP_LIST], list[SMP_LIST];           // gathered tokens: this CTA's; (CTA 0) the row's
+    union {
+        u64 slice[SMP_BINS];                      // while a histogram is collected: this CTA's slice of everybody's
+        struct { u64 mine[SMP_LIST], list[SMP_LIST]; };   // gathered tokens: this CTA's; (CTA 0) the row's
+    };
     u64 list_w[SMP_LIST];
     u64 from[2][SMP_MAX_CLUSTER][3];              // what the cluster's CTAs pushed last, and before
     u64 red[SMP_WARPS];
+    double exp2_16[16];
     u64 result;
     u64 before;
     int n_mine, n_list, at, bin;
@@ -98,7 +113,7 @@ __device__ __forceinline__ u64 smp_reduce(u64 v, u64 *sm)
     __syncthreads();
     if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = v;
     __syncthreads();
-    v = sm[threadIdx.x & 31];
+    v = (threadIdx.x & 31) < SMP_WARPS ? sm[threadIdx.x & 31] : 0;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         const u64 y = __shfl_xor_sync(0xFFFFFFFFu, v, o);
@@ -127,7 +142,7 @@ __device__ __forceinline__ T smp_before(T v, u64 *scratch, T *total)
     __syncthreads();
     if (lane == 31) sm[warp] = inc;
     __syncthreads();
-    const T w = sm[lane], winc = smp_warp_inclusive(w);
+    const T w = lane < SMP_WARPS ? sm[lane] : T(0), winc = smp_warp_inclusive(w);
     *total = __shfl_sync(0xFFFFFFFFu, winc, 31);
     return __shfl_sync(0xFFFFFFFFu, winc - w, warp) + inc - v;
 }
@@ -138,18 +153,25 @@ struct Sampler {
     int n, base;          // tokens in it, index of the first
     int CL, rank, turn;
     float M, inv, per_bin;
-    double inv64;
-    u64 keep;             // number of the last token of the set
+    SampleExp e;
+    float keep_z;         // the set: logits above keep_z, and those equal to it with an index up to keep_i
+    int keep_i;
 
     __device__ __forceinline__ SampleShared *peer(int r) const { return cooperative_groups::this_cluster().map_shared_rank(&s, r); }
     __device__ __forceinline__ void sync() const { cooperative_groups::this_cluster().sync(); }
+    __device__ __forceinline__ bool in_set(int i) const { return z[i] > keep_z || (z[i] == keep_z && base + i <= keep_i); }
+    __device__ __forceinline__ void keep_to(u64 last)
+    {
+        keep_z = smp_unkey((uint32_t)(last >> 32));
+        keep_i = (int)~(uint32_t)last;
+    }
     __device__ __forceinline__ u64 number(int i) const { return (u64)smp_key(z[i]) << 32 | (uint32_t)~(base + i); }
     __device__ __forceinline__ int bin(float x) const
     {
         const float t = (M - x) * per_bin;
         return x == M ? 0 : t < (float)(SMP_BINS - 1) ? (int)t : SMP_BINS - 1;
     }
-    __device__ __forceinline__ u64 weight(float x) const { return smp_weight(x, M, inv, inv64); }
+    __device__ __forceinline__ u64 weight(float x) const { return smp_weight(x, M, inv, e); }
     __device__ __forceinline__ u64 weight_of(u64 number) const { return weight(smp_unkey((uint32_t)(number >> 32))); }
 
     // three values of this CTA to every CTA: afterwards s.from[turn][r] holds those of CTA r (two turns' worth are kept:
@@ -167,48 +189,58 @@ struct Sampler {
     }
     __device__ __forceinline__ void clear(bool weights)
     {
-        s.cnt[threadIdx.x] = 0;
-        if (weights) s.part[0][threadIdx.x] = s.part[1][threadIdx.x] = s.part[2][threadIdx.x] = 0;
+        for (int b = threadIdx.x; b < SMP_BINS; b += SMP_THREADS) {
+            s.cnt[b] = 0;
+            if (weights) s.part[0][b] = s.part[1][b] = s.part[2][b] = 0;
+        }
         if (threadIdx.x == 0) s.bin = -1;
         __syncthreads();
     }
-    __device__ __forceinline__ void add(int b, bool weights, float x)
+    __device__ __forceinline__ void add(int b, bool weights, u64 w)
     {
         atomicAdd(&s.cnt[b], 1u);
         if (weights) {
-            const u64 w = weight(x);
             atomicAdd(&s.part[0][b], (uint32_t)(w & 0x7FFF));
             atomicAdd(&s.part[1][b], (uint32_t)(w >> 15 & 0x7FFF));
             atomicAdd(&s.part[2][b], (uint32_t)(w >> 30));
         }
     }
-    // the row's histogram into every CTA: a thread reads one bin of one CTA, CL lanes make a bin's sum and push it
+    // the row's histogram into every CTA: this one sums a slice of all CTAs' bins and pushes it (lanes run over bins)
     __device__ __forceinline__ void collect(bool weights)
     {
         sync();
-        const int p = threadIdx.x % CL, b = rank * (SMP_BINS / CL) + threadIdx.x / CL;
-        const SampleShared *from = peer(p);
-        uint32_t c = from->cnt[b];
-        u64 w = 0;
-        if (weights) w = (u64)from->part[0][b] + ((u64)from->part[1][b] << 15) + ((u64)from->part[2][b] << 30);
-        for (int o = 1; o < CL; o <<= 1) {
-            c += __shfl_xor_sync(0xFFFFFFFFu, c, o);
-            if (weights) w += __shfl_xor_sync(0xFFFFFFFFu, w, o);
+        const int per = SMP_BINS / CL;
+        for (int what = weights ? 1 : 0; what >= 0; what--) {   // weights, then tokens
+            for (int t = threadIdx.x; t < SMP_BINS; t += SMP_THREADS) {
+                const SampleShared *from = peer(t / per);
+                const int b = rank * per + t % per;
+                s.slice[t] = what ? (u64)from->part[0][b] + ((u64)from->part[1][b] << 15) + ((u64)from->part[2][b] << 30) : from->cnt[b];
+            }
+            __syncthreads();
+            for (int t = threadIdx.x; t < SMP_BINS; t += SMP_THREADS) {
+                const int k = t % per, b = rank * per + k;
+                u64 sum = 0;
+                for (int r = 0; r < CL; r++) sum += s.slice[r * per + k];
+                if (what) peer(t / per)->all_w[b] = sum;
+                else peer(t / per)->all_cnt[b] = (uint32_t)sum;
+            }
+            if (what) __syncthreads();
         }
-        peer(p)->all_cnt[b] = c;
-        if (weights) peer(p)->all_w[b] = w;
         sync();
     }
     // The first bin at which `above` plus the sum up to and with it reaches the goal; *before: the sum above it.
     // (The last bin that holds anything where the goal is not reached: fewer tokens than top_k.)
     __device__ __forceinline__ int boundary(bool weights, u64 above, double goal, u64 *before)
     {
-        const u64 v = weights ? s.all_w[threadIdx.x] : s.all_cnt[threadIdx.x];
-        u64 total;
-        const u64 sum = above + smp_before(v, s.red, &total);
-        if (v && (double)sum < goal && (goal <= (double)(sum + v) || sum + v == above + total)) {
-            s.bin = threadIdx.x;
-            s.before = sum;
+        u64 v[2], total;
+        for (int k = 0; k < 2; k++) v[k] = weights ? s.all_w[2 * threadIdx.x + k] : s.all_cnt[2 * threadIdx.x + k];
+        u64 sum = above + smp_before(v[0] + v[1], s.red, &total);
+        for (int k = 0; k < 2; k++) {
+            if (v[k] && (double)sum < goal && (goal <= (double)(sum + v[k]) || sum + v[k] == above + total)) {
+                s.bin = 2 * threadIdx.x + k;
+                s.before = sum;
+            }
+            sum += v[k];
         }
         __syncthreads();
         const int b = s.bin;
@@ -239,7 +271,7 @@ struct Sampler {
             u64 small = 0, large = 0;   // largest of ~number and of number
             for (int i = threadIdx.x; i < n; i += SMP_THREADS) {
                 const u64 x = number(i);
-                if (x >= keep && bin(z[i]) == b) {
+                if (in_set(i) && bin(z[i]) == b) {
                     small = max(small, ~x);
                     large = max(large, x);
                 }
@@ -258,7 +290,7 @@ struct Sampler {
                 clear(weights);
                 for (int i = threadIdx.x; i < n; i += SMP_THREADS) {
                     const u64 x = number(i);
-                    if (x >= lo && x <= hi) add((int)((hi - x) >> shift), weights, z[i]);
+                    if (x >= lo && x <= hi) add((int)((hi - x) >> shift), weights, weights ? weight(z[i]) : 0);
                 }
                 collect(weights);
                 const int sub = boundary(weights, above, goal, &above);
@@ -270,8 +302,9 @@ struct Sampler {
             b = -1;
         }
         gather([&](int i) {
+            if (b >= 0) return in_set(i) && bin(z[i]) == b;
             const u64 x = number(i);
-            return x >= keep && (b < 0 ? x >= lo && x <= hi : bin(z[i]) == b);
+            return x >= lo && x <= hi;
         });
         if (rank == 0) {
             const int c = s.n_list;
@@ -313,13 +346,23 @@ __global__ void __launch_bounds__(SMP_THREADS) sample_kernel(const SampleArgs a)
     } else {
         for (int i = tid; i < n; i += SMP_THREADS) z[i] = __ldcs(src + i);
     }
+    if (tid < 16) s.exp2_16[tid] = exp2((double)tid / 16.0);
     c.clear(false);   // (synchronises)
     u64 best = 0;
-    for (int i = tid; i < n; i += SMP_THREADS) best = max(best, c.number(i));
+    {
+        float top = -INFINITY;
+        int at = -1;
+        for (int i = tid; i < n; i += SMP_THREADS)
+            if (z[i] > top) {
+                top = z[i];
+                at = i;
+            }
+        if (at >= 0) best = c.number(at);
+    }
     best = smp_reduce<true>(best, s.red);
     c.exchange(best, 0, 0);
     for (int r = 0; r < c.CL; r++) best = max(best, s.from[c.turn][r][0]);
-    const bool none = best < (u64)SMP_KEY_MIN << 32;
+    const bool none = best == 0;
     if (none || a.temperature == 0.f) {
         if (c.rank == 0 && tid == 0) {
             a.tokens[row] = none ? -1 : (int)~(uint32_t)best;
@@ -328,34 +371,36 @@ __global__ void __launch_bounds__(SMP_THREADS) sample_kernel(const SampleArgs a)
         return;
     }
     c.M = smp_unkey((uint32_t)(best >> 32));
-    c.inv64 = 1.0 / (double)a.temperature;
-    c.inv = (float)c.inv64;
-    c.per_bin = (float)(32.0 * c.inv64);
-    c.keep = (u64)SMP_KEY_MIN << 32;
+    const double inv64 = 1.0 / (double)a.temperature;
+    c.inv = (float)inv64;
+    c.per_bin = (float)(32.0 * inv64);
+    c.e = {(double)c.M, 16.0 * 1.4426950408889634 * inv64, s.exp2_16};
+    c.keep_z = -INFINITY;
+    c.keep_i = -1;
     const double u = (double)fminf(fmaxf(a.u[row], 0.f), 1.f), lowest = fmin((double)a.min_p, 1.0);
     const float log_lowest = lowest > 0.0 ? (float)log(lowest) : -INFINITY;
     auto heavy = [&](float x) {   // weight >= min_p: decided in 64 bits where 32 could be wrong
         const float y = (x - c.M) * c.inv;
         if (x == c.M || y > log_lowest + 1e-3f) return true;
         if (y < log_lowest - 1e-3f) return false;
-        return exp(((double)x - (double)c.M) * c.inv64) >= lowest;
+        return exp(((double)x - (double)c.M) * inv64) >= lowest;
     };
     const bool by_k = a.top_k > 0 && a.top_k < a.vocab, by_p = a.top_p > 0.f && a.top_p < 1.f;
     if (by_k || by_p) {
         // ---- 2. counts ----
         for (int i = tid; i < n; i += SMP_THREADS)
-            if (smp_key(z[i]) >= SMP_KEY_MIN) c.add(c.bin(z[i]), false, z[i]);
+            if (c.in_set(i)) c.add(c.bin(z[i]), false, 0);
         c.collect(false);
     }
     if (a.top_p <= 0.f) {
-        c.keep = best;
+        c.keep_to(best);
     } else if (by_k) {
         // ---- 3. top_k ----
         u64 before;
         const int b = c.boundary(false, 0, (double)a.top_k, &before);
         const uint32_t in_bin = s.all_cnt[b];
         if (before + in_bin <= SMP_LIST) {
-            c.gather([&](int i) { return smp_key(z[i]) >= SMP_KEY_MIN && c.bin(z[i]) <= b; });
+            c.gather([&](int i) { return c.in_set(i) && c.bin(z[i]) <= b; });
             if (c.rank != 0) return;   // (nobody pushes to this CTA or reads from it any more)
             const int m = s.n_list;
             const u64 x = tid < m ? s.list[tid] : 0;
@@ -382,32 +427,43 @@ __global__ void __launch_bounds__(SMP_THREADS) sample_kernel(const SampleArgs a)
             }
             return;
         }
-        c.keep = c.last_in_bin(b, in_bin, before, (double)a.top_k, false);
+        c.keep_to(c.last_in_bin(b, in_bin, before, (double)a.top_k, false));
     }
     if (by_p) {
         // ---- 4. top_p ----
         if (by_k) {   // the counts of the set (last_in_bin may have used the histogram)
             c.clear(false);
             for (int i = tid; i < n; i += SMP_THREADS)
-                if (c.number(i) >= c.keep) c.add(c.bin(z[i]), false, z[i]);
+                if (c.in_set(i)) c.add(c.bin(z[i]), false, 0);
             c.collect(false);
         }
         // a token of bin b weighs between exp(-(b + 1) / 32) and exp(-b / 32); 1e-4 covers the rounding of its bin
-        const double count = (double)s.all_cnt[tid];
-        const double most = count * exp(-(double)tid / 32.0) * 1.0001, least = tid < SMP_BINS - 1 ? count * exp(-(double)(tid + 1) / 32.0) * 0.9999 : 0.0;
-        double most_all, least_all;
-        const double most_before = smp_before(most, s.red, &most_all), least_before = smp_before(least, s.red, &least_all);
-        // first bin that may hold the boundary: the last with most_before < goal; last: the first with least up to it >= goal
-        const int first = (int)smp_reduce<true>(most_before < (double)a.top_p * least_all ? (u64)tid : 0, s.red);
-        const int last = SMP_BINS - 1 - (int)smp_reduce<true>(least_before + least >= (double)a.top_p * most_all ? (u64)(SMP_BINS - 1 - tid) : 0, s.red);
+        double most[2], least[2], most_all, least_all;
+        for (int k = 0; k < 2; k++) {
+            const int b = 2 * tid + k;
+            const double count = (double)s.all_cnt[b];
+            most[k] = count * exp(-(double)b / 32.0) * 1.0001;
+            least[k] = b < SMP_BINS - 1 ? count * exp(-(double)(b + 1) / 32.0) * 0.9999 : 0.0;
+        }
+        double most_before = smp_before(most[0] + most[1], s.red, &most_all), least_before = smp_before(least[0] + least[1], s.red, &least_all);
+        // the first bin that may hold the border is the last with most_before < goal, the last one the first with least up to it >= goal
+        int first = 0, from_end = 0;
+        for (int k = 0; k < 2; k++) {
+            if (most_before < (double)a.top_p * least_all) first = 2 * tid + k;
+            least_before += least[k];
+            if (least_before >= (double)a.top_p * most_all) from_end = max(from_end, SMP_BINS - 1 - (2 * tid + k));
+            most_before += most[k];
+        }
+        first = (int)smp_reduce<true>((u64)first, s.red);
+        const int last = SMP_BINS - 1 - (int)smp_reduce<true>((u64)from_end, s.red);
         c.clear(true);
         u64 above = 0, below = 0;
         for (int i = tid; i < n; i += SMP_THREADS) {
-            if (c.number(i) < c.keep) continue;
             const int b = c.bin(z[i]);
-            if (b < first) above += c.weight(z[i]);
-            else if (b > last) below += c.weight(z[i]);
-            else c.add(b, true, z[i]);
+            const u64 w = c.in_set(i) ? c.weight(z[i]) : 0;   // (one evaluation for the three cases)
+            if (b < first) above += w;
+            else if (b > last) below += w;
+            else if (c.in_set(i)) c.add(b, true, w);
         }
         above = smp_reduce<false>(above, s.red);
         below = smp_reduce<false>(below, s.red);
@@ -419,15 +475,15 @@ __global__ void __launch_bounds__(SMP_THREADS) sample_kernel(const SampleArgs a)
         }
         c.collect(true);
         u64 inside;
-        smp_before(s.all_w[tid], s.red, &inside);
+        smp_before(s.all_w[2 * tid] + s.all_w[2 * tid + 1], s.red, &inside);
         const double goal = (double)a.top_p * (double)(above + inside + below);
         u64 before;
         const int b = c.boundary(true, above, goal, &before);
-        if (b >= 0) c.keep = c.last_in_bin(b, s.all_cnt[b], before, goal, true);
+        if (b >= 0) c.keep_to(c.last_in_bin(b, s.all_cnt[b], before, goal, true));
     }
     // ---- 5. the token ----
     const int seg = ((n + SMP_WARPS - 1) / SMP_WARPS + 31) & ~31, lo = min(n, warp * seg), hi = min(n, lo + seg);
-    auto kept = [&](int i) -> u64 { return c.number(i) >= c.keep && heavy(z[i]) ? c.weight(z[i]) : 0; };
+    auto kept = [&](int i) -> u64 { return c.in_set(i) && heavy(z[i]) ? c.weight(z[i]) : 0; };
     u64 mine = 0, cta;
     for (int i = lo + lane; i < hi; i += 32) mine += kept(i);
     u64 warp_sum = mine;
