@@ -1,0 +1,408 @@
+// Causal attention of a prompt's tokens over the 4-bit cache (kv4.cuh), on the 5th-generation tensor cores.
+//
+// One CTA per (kv head, 128 query rows: 128 / G tokens by the G query heads of the kv head), one KV tile of 64 positions
+// after the other, longest CTAs first.  f32 in and out means 22 bits in both products, so every operand is split into two
+// f16 parts and a product takes three MMAs, the two small ones first (lo hi + hi lo + hi hi):
+//   S[row, pos]  = Q K^T   A = Q in tensor memory (rows scaled by a power of two), B = K tile in shared memory, K-major
+//   O[row, dim]  = P V     A = P in tensor memory, over S's own columns, B = V tile in shared memory, dims contiguous
+// A operands live in tensor memory because a 64-wide MMA that fetched them from shared memory would be bound by that.
+// The tensor core rounds its sums towards zero, so O is never carried across tiles there: each tile's O starts from zero
+// and is added to f32 registers, where a raised softmax reference is also paid for (one factor per row and tile).
+//
+//   warps 0-3   one row per thread: S from tensor memory, mask, weights 64 exp2(s - ref), their sum, P back.  The
+//               reference is raised only when a score exceeds it by 2^8.
+//   warps 4-11  fill a ring of three (K, V) stages from the cache: a thread unpacks 8 dims of a position at a time,
+//               value = m + d * code in f32, scaled per tile by a power of two that keeps both parts clear of f16's ends;
+//               between two stages they add a finished O tile to their 64 columns of a row.
+//   warp 12     one thread issues S(j), then P V of tile j - 1: the tensor core works while the weights are computed.
+// Columns of tensor memory: Q 128 (hi, lo), S / P 2 x 64, O 2 x 128.
+// Within every 8 dims the tiles' order is (0,4,1,5,2,6,3,7), which unpacking produces for free; Q is put in that order,
+// and O's columns are written out by it.
+// Positions outside [first visible, last visible] of the CTA count as zero whatever the cache holds there; a visible V
+// group that is NaN is taken as zero by the MMA (0 * NaN would reach rows that do not see it) and noted in a bit mask,
+// from which the rows that see it are set to NaN.
+#pragma once
+
+#include "attn_kv4.cuh"
+#include "tcgen05.cuh"
+
+namespace qz {
+
+constexpr int APK_BN = 64, APK_STAGES = 3, APK_THREADS = 416;
+
+struct AttnPromptKv4Args {
+    float *out;
+    const float *q;
+    const uint8_t *cache;
+    int n_tok, n_heads, n_kv, n_blocks, pos0, window, tq;   // tq: tokens per CTA
+    float scale;
+    const float *sinks;
+    int *status;
+};
+
+struct AttnPromptKv4Shared {
+    uint64_t full[APK_STAGES], free_[APK_STAGES], s_full[2], p_full[2], o_free[2];
+    float corr[4][UMMA_M];           // factor of a row's earlier outputs at tile j (slot j % 4)
+    float scale_k[4], scale_v[4];    // 1 / what the tile's K and V were multiplied with
+    uint32_t nan_v[4][4][2];         // positions of the tile whose V group is NaN, by group
+    uint32_t top[2][2][8];           // largest magnitude per warp, as bits
+    float inv[UMMA_M];               // 1 / sum of weights
+    uint32_t nan_row[UMMA_M];        // groups of the row's output that are NaN
+    uint32_t tmem;
+};
+
+__host__ __device__ constexpr size_t attn_prompt_kv4_smem(int NG)
+{
+    return (size_t)APK_STAGES * 4 * ((NG + 1) / 2) * APK_BN * 128 + 1024 + sizeof(AttnPromptKv4Shared);
+}
+
+// eight values m + d * code of a word as two 16-byte rows of f16, hi and lo, in the order (0,4,1,5,2,6,3,7)
+__device__ __forceinline__ void kv4_split8(const Nibbles &nib, uint32_t w, float m, float d, uint4 &hi, uint4 &lo)
+{
+    uint32_t x[4], h[4], l[4];
+    nib.pairs(w, x);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float2 c = __half22float2(*(const __half2 *)&x[i]);
+        const float a = fmaf(d, c.x, m), b = fmaf(d, c.y, m);
+        const float ah = __uint_as_float(__float_as_uint(a) & 0xFFFFE000u), bh = __uint_as_float(__float_as_uint(b) & 0xFFFFE000u);
+        h[i] = pack_half2(ah, bh);
+        l[i] = pack_half2(a - ah, b - bh);
+    }
+    hi = make_uint4(h[0], h[1], h[2], h[3]);
+    lo = make_uint4(l[0], l[1], l[2], l[3]);
+}
+
+template <int N>
+__device__ __forceinline__ void ldg_words(const void *p, uint32_t (&x)[N])
+{
+    if constexpr (N == 4) {
+        const uint4 w = __ldcg((const uint4 *)p);
+        x[0] = w.x; x[1] = w.y; x[2] = w.z; x[3] = w.w;
+    } else if constexpr (N == 2) {
+        const uint2 w = __ldcg((const uint2 *)p);
+        x[0] = w.x; x[1] = w.y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) x[i] = __ldcg((const uint32_t *)p + i);
+    }
+}
+// half k of an array of words
+template <int N>
+__device__ __forceinline__ float half_of(const uint32_t (&x)[N], int k) { return __half2float(__ushort_as_half((unsigned short)(x[k >> 1] >> (16 * (k & 1))))); }
+
+template <int NG>
+__global__ void __launch_bounds__(APK_THREADS, 1) attn_prompt_kv4_kernel(const AttnPromptKv4Args a)
+{
+    constexpr int HD = 32 * NG, NH = (NG + 1) / 2, HALF = APK_BN * 128, SIDE = NH * HALF, STAGE = 4 * SIDE;   // bytes: 64 dims, a part, K and V
+    constexpr uint32_t T_Q = 0, T_S = 128, T_O = 256;   // tensor-memory columns
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char *ring = (unsigned char *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    AttnPromptKv4Shared &s = *(AttnPromptKv4Shared *)(ring + APK_STAGES * STAGE);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int kvh = blockIdx.x, G = a.n_heads / a.n_kv;
+    const int t0 = ((int)gridDim.y - 1 - (int)blockIdx.y) * a.tq, nt = min(a.tq, a.n_tok - t0);
+    const int p_first = a.pos0 + t0, p_last = p_first + nt - 1;
+    const int k_lo = a.window > 0 ? max(0, p_first + 1 - a.window) : 0, b0 = k_lo / KV4_BLOCK;
+    const int base0 = b0 * KV4_BLOCK, n_tiles = (p_last - base0) / APK_BN + 1;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < APK_STAGES; i++) {
+            mbar_init(&s.full[i], 8);
+            mbar_init(&s.free_[i], 1);
+        }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&s.s_full[i], 1);
+            mbar_init(&s.p_full[i], 4);
+            mbar_init(&s.o_free[i], 8);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (threadIdx.x < 32) ((uint32_t *)s.nan_v)[threadIdx.x] = 0;
+    if (warp == 12) tmem_alloc(&s.tmem, 512);
+    pdl_trigger();
+    pdl_wait();   // q and the cache's rows come from the launches before
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s.tmem;
+    bool ok = true;
+    const int row = 32 * (warp & 3) + lane;   // (warps 0 to 11) this thread's row, and its token and head
+    const int tok = row / G, head = kvh * G + row % G;
+    const bool is_row = row < nt * G;
+
+    if (warp < 4) {
+        // ---- Q into tensor memory ----
+        const uint32_t lanes = (uint32_t)(32 * warp) << 16;
+        const float *q = a.q + ((size_t)(t0 + tok) * a.n_heads + head) * HD;
+        const float to_log2 = a.scale * 1.44269504f;
+        float top = 0.f;
+        if (is_row)
+            for (int i = 0; i < HD / 4; i++) {
+                const float4 v = __ldcg((const float4 *)q + i);
+                top = fmaxf(top, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
+            }
+        top *= fabsf(to_log2);
+        const int e = top > 0.f ? max(-100, min(100, 127 + 13 - (int)(__float_as_uint(top) >> 23))) : 0;   // the largest element into [2^13, 2^14)
+        const float up = __uint_as_float((uint32_t)(127 + e) << 23), back = __uint_as_float((uint32_t)(127 - e) << 23);
+        for (int g = 0; g < NG; g++) {
+            uint32_t hi[16], lo[16];
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                float4 u = make_float4(0.f, 0.f, 0.f, 0.f), v = u;
+                if (is_row) {
+                    u = __ldcg((const float4 *)q + 8 * g + 2 * c);
+                    v = __ldcg((const float4 *)q + 8 * g + 2 * c + 1);
+                }
+                const float x[4] = {u.x, u.y, u.z, u.w}, y[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float p = x[i] * to_log2 * up, r = y[i] * to_log2 * up;
+                    const uint32_t h = pack_half2(p, r);
+                    const float2 f = __half22float2(*(const __half2 *)&h);
+                    hi[4 * c + i] = h;
+                    lo[4 * c + i] = pack_half2(p - f.x, r - f.y);
+                }
+            }
+            tc_st16(tmem + lanes + T_Q + 16 * g, hi);
+            tc_st16(tmem + lanes + T_Q + 64 + 16 * g, lo);
+        }
+        tc_wait_st();
+        tc_fence_before();
+        asm volatile("bar.sync 1, 160;" ::: "memory");   // with the issuing warp: Q is in place
+        // ---- tiles ----
+        const int p_row = p_first + tok, lo_row = a.window > 0 ? max(0, p_row + 1 - a.window) : 0;
+        float ref = -3.0e38f, l = 0.f;
+        uint32_t nan_groups = 0;
+        for (int j = 0; j < n_tiles; j++) {
+            const uint32_t t_s = tmem + lanes + T_S + 64 * (j & 1);
+            ok = ok && mbar_wait(&s.s_full[j & 1], (j >> 1) & 1) && mbar_wait(&s.full[j % APK_STAGES], (j / APK_STAGES) & 1);
+            if (!__all_sync(0xFFFFFFFFu, ok)) break;
+            tc_fence_after();
+            const float f = back * s.scale_k[j & 3];
+            const int lo = lo_row - (base0 + APK_BN * j), hi = p_row - (base0 + APK_BN * j);   // visible columns
+            const bool partial = __any_sync(0xFFFFFFFFu, lo > 0 || hi < APK_BN - 1);
+            auto load = [&](int c, uint32_t (&v)[32]) {   // (twice: 64 values do not fit the registers beside the rest)
+                tc_ld32(t_s + 32 * c, v);
+                if (partial) {
+#pragma unroll
+                    for (int i = 0; i < 32; i++)
+                        if (32 * c + i < lo || 32 * c + i > hi) v[i] = 0xFF800000u;
+                }
+            };
+            float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                uint32_t v[32];
+                load(c, v);
+#pragma unroll
+                for (int i = 0; i < 32; i++) top4[i & 3] = fmaxf(top4[i & 3], __uint_as_float(v[i]));
+            }
+            const float y = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * f;
+            float corr = 1.f;
+            if (y > ref + 8.f) {
+                corr = ex2(ref - y);
+                l *= corr;
+                ref = y;
+            }
+            s.corr[j & 3][row] = corr;
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+                const uint32_t n0 = s.nan_v[j & 3][g][0], n1 = s.nan_v[j & 3][g][1];
+                if (n0 | n1) {   // rare: does this row see one of them?
+                    const uint64_t seen = hi < 0 || lo > 63 ? 0 : (~0ull >> (63 - min(63, hi))) & (~0ull << max(0, lo));
+                    if (seen & ((uint64_t)n1 << 32 | n0)) nan_groups |= 1u << g;
+                }
+            }
+            float l4[4] = {0.f, 0.f, 0.f, 0.f};
+            const float minus = 6.f - ref;   // weights carry 2^6: their lo parts stay clear of f16's subnormals
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                uint32_t v[32], ph[16], pl[16];
+                load(c, v);
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const float p0 = ex2(fmaf(__uint_as_float(v[2 * i]), f, minus)), p1 = ex2(fmaf(__uint_as_float(v[2 * i + 1]), f, minus));
+                    l4[(2 * i) & 3] += p0;
+                    l4[(2 * i + 1) & 3] += p1;
+                    const float h0 = __uint_as_float(__float_as_uint(p0) & 0xFFFFE000u), h1 = __uint_as_float(__float_as_uint(p1) & 0xFFFFE000u);
+                    ph[i] = pack_half2(h0, h1);
+                    pl[i] = pack_half2(p0 - h0, p1 - h1);
+                }
+                tc_st16(t_s + 32 * c, ph);
+                tc_st16(t_s + 32 * c + 16, pl);
+            }
+            l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+            tc_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s.p_full[j & 1]);
+        }
+        if (a.sinks && is_row) {
+            const float sink = a.sinks[head] * 1.44269504f, all = fmaxf(ref, sink), down = ex2(ref - all);
+            s.inv[row] = down / fmaf(l, down, ex2(sink - all + 6.f));
+        } else {
+            s.inv[row] = 1.f / l;
+        }
+        s.nan_row[row] = nan_groups;
+        asm volatile("bar.sync 2, 384;" ::: "memory");
+    } else if (warp < 12) {
+        const int tid = threadIdx.x - 128, w8 = warp - 4, p_tile = tid >> 2, t = tid & 3;
+        const uint8_t *head_blocks = kv4_block(const_cast<uint8_t *>(a.cache), a.n_blocks, kvh, 0, HD);
+        const Nibbles nib;
+        float acc[16 * NG];   // columns [part * HD / 2, ...) of row
+#pragma unroll
+        for (int i = 0; i < 16 * NG; i++) acc[i] = 0.f;
+        const int part = w8 >> 2;
+        // O of tile j is finished: add it
+        auto collect = [&](int j) {
+            ok = ok && mbar_wait(&s.free_[j % APK_STAGES], (j / APK_STAGES) & 1);
+            if (!__all_sync(0xFFFFFFFFu, ok)) {
+                ok = false;
+                return;
+            }
+            tc_fence_after();
+            const float corr = s.corr[j & 3][row], f = s.scale_v[j & 3];
+            const uint32_t t_o = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + T_O + 128 * (j & 1) + part * (HD / 2);
+#pragma unroll
+            for (int c = 0; c < NG; c++) {
+                uint32_t o[16];
+                tc_ld16(t_o + 16 * c, o);
+#pragma unroll
+                for (int i = 0; i < 16; i++) acc[16 * c + i] = fmaf(__uint_as_float(o[i]), f, acc[16 * c + i] * corr);
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s.o_free[j & 1]);
+        };
+        uint32_t kw[NG], vw[NG], kp[NG], vp[NG];   // 8 dims of NG groups, and the position's parameters (m .., d ..)
+        auto fetch = [&](int j) {
+            const int pos = base0 + APK_BN * j + p_tile;
+            const bool seen = pos >= k_lo && pos <= p_last;
+            const uint8_t *blk = head_blocks + (size_t)((seen ? pos : p_last) / KV4_BLOCK) * (40 * HD);
+            const int r = (seen ? pos : p_last) % KV4_BLOCK;
+            ldg_words<NG>(blk + 16 * HD + r * 4 * NG, kp);
+            ldg_words<NG>(blk + 36 * HD + r * 4 * NG, vp);
+            ldg_words<NG>(blk + r * (HD / 2) + 4 * NG * t, kw);
+            ldg_words<NG>(blk + 20 * HD + r * (HD / 2) + 4 * NG * t, vw);
+            if (!seen) {
+#pragma unroll
+                for (int i = 0; i < NG; i++) kp[i] = vp[i] = 0;   // m = d = 0
+            }
+        };
+        fetch(0);
+        for (int j = 0; j < n_tiles; j++) {
+            if (j >= APK_STAGES) collect(j - APK_STAGES);   // (a wait that gave up does not leave the loop: the barrier below is for all)
+            // the tile's largest magnitudes
+            float top_k = 0.f, top_v = 0.f;
+            if (tid < 8) s.nan_v[(j + 1) & 3][tid >> 1][tid & 1] = 0;   // (its last readers have finished: tile j - 3 is)
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+                const float dk = half_of(kp, NG + g), dv = half_of(vp, NG + g), mv = half_of(vp, g);
+                if (mv != mv && t == 0) atomicOr(&s.nan_v[j & 3][g][p_tile >> 5], 1u << (p_tile & 31));
+                top_k = fmaxf(top_k, fabsf(fmaf(8.f, dk, half_of(kp, g))) + 8.f * dk);
+                top_v = fmaxf(top_v, fabsf(fmaf(8.f, dv, mv)) + 8.f * dv);
+            }
+            const uint32_t wk = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(top_k)), wv = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(top_v));
+            if (lane == 0) {
+                s.top[j & 1][0][w8] = wk;
+                s.top[j & 1][1][w8] = wv;
+            }
+            asm volatile("bar.sync 3, 256;" ::: "memory");
+            uint32_t tk = 0, tv = 0;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                tk = max(tk, s.top[j & 1][0][i]);
+                tv = max(tv, s.top[j & 1][1][i]);
+            }
+            // powers of two that bring them into [2^13, 2^14)
+            const int ek = tk ? 127 + 13 - (int)(tk >> 23) : 0, ev = tv ? 127 + 13 - (int)(tv >> 23) : 0;
+            const float uk = __uint_as_float((uint32_t)(127 + ek) << 23), uv = __uint_as_float((uint32_t)(127 + ev) << 23);
+            if (tid == 0) {
+                s.scale_k[j & 3] = __uint_as_float((uint32_t)(127 - ek) << 23);
+                s.scale_v[j & 3] = __uint_as_float((uint32_t)(127 - ev) << 23);
+            }
+            unsigned char *stage = ring + (j % APK_STAGES) * STAGE;
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+                const uint32_t at = (g >> 1) * HALF + sw128(p_tile, (g & 1) * 4 + t);
+                uint4 hi, lo;
+                float d = half_of(kp, NG + g) * uk;
+                kv4_split8(nib, kw[g], fmaf(8.f, d, half_of(kp, g) * uk), d, hi, lo);
+                *(uint4 *)(stage + at) = hi;
+                *(uint4 *)(stage + SIDE + at) = lo;
+                const uint32_t a16 = vw[g >> 1] >> (16 * (g & 1)), b16 = vw[(NG + g) >> 1] >> (16 * ((NG + g) & 1));   // dims 8 t .., and 8 t + 4 ..
+                d = half_of(vp, NG + g) * uv;
+                float m = fmaf(8.f, d, half_of(vp, g) * uv);
+                if (m != m) m = d = 0.f;
+                kv4_split8(nib, (a16 & 0xFFFFu) | b16 << 16, m, d, hi, lo);
+                *(uint4 *)(stage + 2 * SIDE + at) = hi;
+                *(uint4 *)(stage + 3 * SIDE + at) = lo;
+            }
+            if (j + 1 < n_tiles) fetch(j + 1);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s.full[j % APK_STAGES]);
+        }
+        for (int j = max(0, n_tiles - APK_STAGES); j < n_tiles; j++) collect(j);
+        asm volatile("bar.sync 2, 384;" ::: "memory");
+        if (is_row && ok) {
+            const float inv = s.inv[row];
+            const uint32_t bad = s.nan_row[row];
+            float *dst = a.out + ((size_t)(t0 + tok) * a.n_heads + head) * HD + part * (HD / 2);
+#pragma unroll
+            for (int c = 0; c < 2 * NG; c++) {   // eight columns: dims (0,4,1,5,2,6,3,7)
+                const float f = bad >> ((part * (HD / 2) + 8 * c) >> 5) & 1 ? __int_as_float(0x7FC00000) : inv;
+                const float *o = acc + 8 * c;
+                *(float4 *)(dst + 8 * c) = make_float4(o[0] * f, o[2] * f, o[4] * f, o[6] * f);
+                *(float4 *)(dst + 8 * c + 4) = make_float4(o[1] * f, o[3] * f, o[5] * f, o[7] * f);
+            }
+        }
+    } else {
+        asm volatile("bar.sync 1, 160;" ::: "memory");
+        if (lane == 0) {
+            tc_fence_after();
+            const uint32_t i_s = umma_idesc_f16(APK_BN, false), i_o = umma_idesc_f16(HD, true);
+            const uint32_t ring_addr = smem_u32(ring);
+            int done = -1;   // last tile whose P V was issued
+            for (int j = 0; j <= n_tiles && ok; j++) {
+                if (j < n_tiles) {
+                    // S(j) may overwrite P(j - 2): the MMAs that read it were issued before and execute in order
+                    ok = mbar_wait(&s.full[j % APK_STAGES], (j / APK_STAGES) & 1);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t k_hi = ring_addr + (j % APK_STAGES) * STAGE, d = tmem + T_S + 64 * (j & 1);
+#pragma unroll
+                    for (int m = 0; m < 3; m++)
+#pragma unroll
+                        for (int k = 0; k < HD / 16; k++)
+                            tc_mma_f16_ta(d, tmem + T_Q + (m == 0 ? 64 : 0) + 8 * k,
+                                          umma_desc_sw128(k_hi + (m == 1 ? SIDE : 0) + (k >> 2) * HALF + 32 * (k & 3)), i_s, (m | k) ? 1u : 0u);
+                    tc_commit(&s.s_full[j & 1]);
+                }
+                if (j > 0) {
+                    const int i = j - 1;
+                    ok = mbar_wait(&s.p_full[i & 1], (i >> 1) & 1) && (i < 2 || mbar_wait(&s.o_free[i & 1], ((i >> 1) - 1) & 1));
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t v_hi = ring_addr + (i % APK_STAGES) * STAGE + 2 * SIDE, d = tmem + T_O + 128 * (i & 1), p = tmem + T_S + 64 * (i & 1);
+#pragma unroll
+                    for (int m = 0; m < 3; m++)
+#pragma unroll
+                        for (int k = 0; k < APK_BN / 16; k++)
+                            tc_mma_f16_ta(d, p + 32 * (k >> 1) + 8 * (k & 1) + (m == 0 ? 16 : 0),
+                                          umma_desc_sw128_mn(v_hi + (m == 1 ? SIDE : 0) + 2048 * k, HALF), i_o, (m | k) ? 1u : 0u);
+                    tc_commit(&s.free_[i % APK_STAGES]);
+                    done = i;
+                }
+            }
+            if (done >= 0) mbar_wait(&s.free_[done % APK_STAGES], (done / APK_STAGES) & 1);   // nothing in flight at the exit
+        }
+        __syncwarp();
+    }
+    if (!ok && a.status) *a.status = QZ_ERR_TIMEOUT;
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 12) tmem_dealloc(tmem, 512);
+}
+
+}  // namespace qz

@@ -4,7 +4,7 @@
 #include <memory>
 #include <vector>
 
-#include "attn_kv4.cuh"
+#include "attn_prompt_kv4.cuh"
 #include "host.cuh"
 
 using namespace qz;
@@ -263,9 +263,16 @@ void cuda_attn_prompt_kv4(float *out, const float *q, const void *d_cache, int n
         refuse("cuda_attn_prompt_kv4: out and q must be 16-byte aligned device pointers");
         return;
     }
-    const AttnKv4Args a = {out, q, nullptr, nullptr, (uint8_t *)d_cache, nullptr, pos0, n_heads, n_kv_heads, max_seq, kv4_blocks(max_seq), window, scale,
-                           sinks, 0.f, 1.f, 0, 0, XQOut{nullptr, nullptr, nullptr, nullptr}, 0, nullptr};
-    by_groups(head_dim, [&](auto ng) { launch(attn_kv4_kernel<ng.value>, dim3(n_kv_heads, n_tok), dim3(AK_THREADS), 0, a); });
+    AttnPromptKv4Args a = {out, q, (const uint8_t *)d_cache, n_tok, n_heads, n_kv_heads, kv4_blocks(max_seq), pos0, window, UMMA_M / (n_heads / n_kv_heads),
+                           scale, sinks, status_word_if_ready()};
+    by_groups(head_dim, [&](auto ng) {
+        static bool ready = false;
+        if (!ready) {
+            QZ_CUDA_CHECK(cudaFuncSetAttribute(attn_prompt_kv4_kernel<ng.value>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)attn_prompt_kv4_smem(ng.value)));
+            ready = true;
+        }
+        launch(attn_prompt_kv4_kernel<ng.value>, dim3(n_kv_heads, (n_tok + a.tq - 1) / a.tq), dim3(APK_THREADS), attn_prompt_kv4_smem(ng.value), a);
+    });
 }
 
 }  // extern "C"
