@@ -28,7 +28,7 @@
 
 namespace qz {
 
-constexpr int APK_BN = 64, APK_STAGES = 3, APK_THREADS = 416;
+constexpr int APK_BN = 64, APK_STAGES = 3, APK_THREADS = 512;
 
 struct AttnPromptKv4Args {
     float *out;
@@ -130,6 +130,11 @@ __global__ void __launch_bounds__(APK_THREADS, 1) attn_prompt_kv4_kernel(const A
     const int tok = row / G, head = kvh * G + row % G;
     const bool is_row = row < nt * G;
 
+    // registers: 128 a thread at launch; the issuing warpgroup gives 64 of each of its threads away (8192), the others
+    // take 16 (2048) and 24 (2 x 3072)
+    if (warp < 4) asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
+    else if (warp < 12) asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     if (warp < 4) {
         // ---- Q into tensor memory ----
         const uint32_t lanes = (uint32_t)(32 * warp) << 16;
@@ -262,13 +267,17 @@ __global__ void __launch_bounds__(APK_THREADS, 1) attn_prompt_kv4_kernel(const A
             }
             tc_fence_after();
             const float corr = s.corr[j & 3][row], f = s.scale_v[j & 3];
+            const bool same = __all_sync(0xFFFFFFFFu, corr == 1.f);   // (a reference is raised a few times in all)
             const uint32_t t_o = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + T_O + 128 * (j & 1) + part * (HD / 2);
 #pragma unroll
             for (int c = 0; c < NG; c++) {
                 uint32_t o[16];
                 tc_ld16(t_o + 16 * c, o);
 #pragma unroll
-                for (int i = 0; i < 16; i++) acc[16 * c + i] = fmaf(__uint_as_float(o[i]), f, acc[16 * c + i] * corr);
+                for (int i = 0; i < 16; i++) {
+                    if (!same) acc[16 * c + i] *= corr;
+                    acc[16 * c + i] = fmaf(__uint_as_float(o[i]), f, acc[16 * c + i]);
+                }
             }
             tc_fence_before();
             __syncwarp();
@@ -357,7 +366,7 @@ __global__ void __launch_bounds__(APK_THREADS, 1) attn_prompt_kv4_kernel(const A
                 *(float4 *)(dst + 8 * c + 4) = make_float4(o[1] * f, o[3] * f, o[5] * f, o[7] * f);
             }
         }
-    } else {
+    } else if (warp == 12) {   // (warps 13 to 15 only lend their registers)
         asm volatile("bar.sync 1, 160;" ::: "memory");
         if (lane == 0) {
             tc_fence_after();
