@@ -14,7 +14,7 @@
 //   warps 4-11  fill a ring of three (K, V) stages from the cache: a thread unpacks 8 dims of a position at a time,
 //               value = m + d * code in f32, scaled per tile by a power of two that keeps both parts clear of f16's ends;
 //               between two stages they add a finished O tile to their 64 columns of a row.
-//   warp 12     one thread issues S(j), then P V of tile j - 1: the tensor core works while the weights are computed.
+//   warp 12     issues S(j), then P V of tile j - 1: the tensor core works while the weights are computed.
 // Columns of tensor memory: Q 128 (hi, lo), S / P 2 x 64, O 2 x 128.
 // Within every 8 dims the tiles' order is (0,4,1,5,2,6,3,7), which unpacking produces for free; Q is put in that order,
 // and O's columns are written out by it.
@@ -368,44 +368,45 @@ __global__ void __launch_bounds__(APK_THREADS, 1) attn_prompt_kv4_kernel(const A
         }
     } else if (warp == 12) {   // (warps 13 to 15 only lend their registers)
         asm volatile("bar.sync 1, 160;" ::: "memory");
-        if (lane == 0) {
-            tc_fence_after();
-            const uint32_t i_s = umma_idesc_f16(APK_BN, false), i_o = umma_idesc_f16(HD, true);
-            const uint32_t ring_addr = smem_u32(ring);
-            int done = -1;   // last tile whose P V was issued
-            for (int j = 0; j <= n_tiles && ok; j++) {
-                if (j < n_tiles) {
-                    // S(j) may overwrite P(j - 2): the MMAs that read it were issued before and execute in order
-                    ok = mbar_wait(&s.full[j % APK_STAGES], (j / APK_STAGES) & 1);
-                    if (!ok) break;
-                    tc_fence_after();
-                    const uint32_t k_hi = ring_addr + (j % APK_STAGES) * STAGE, d = tmem + T_S + 64 * (j & 1);
+        tc_fence_after();
+        const bool leader = elect_one();
+        constexpr uint32_t i_s = umma_idesc_f16(APK_BN, false), i_o = umma_idesc_f16(HD, true);
+        const uint32_t ring_addr = smem_u32(ring), t_base = __shfl_sync(0xFFFFFFFFu, tmem, 0);
+        int done = -1;   // last tile whose P V was issued
+        for (int j = 0; j <= n_tiles; j++) {
+            if (j < n_tiles) {
+                // S(j) may overwrite P(j - 2): the MMAs that read it were issued before and execute in order
+                ok = __all_sync(0xFFFFFFFFu, mbar_wait(&s.full[j % APK_STAGES], (j / APK_STAGES) & 1));
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t d = t_base + T_S + 64 * (j & 1);
+                const uint64_t k_hi = umma_desc_sw128(ring_addr + (j % APK_STAGES) * STAGE);   // (its low word counts 16 bytes)
 #pragma unroll
-                    for (int m = 0; m < 3; m++)
+                for (int m = 0; m < 3; m++)
 #pragma unroll
-                        for (int k = 0; k < HD / 16; k++)
-                            tc_mma_f16_ta(d, tmem + T_Q + (m == 0 ? 64 : 0) + 8 * k,
-                                          umma_desc_sw128(k_hi + (m == 1 ? SIDE : 0) + (k >> 2) * HALF + 32 * (k & 3)), i_s, (m | k) ? 1u : 0u);
-                    tc_commit(&s.s_full[j & 1]);
-                }
-                if (j > 0) {
-                    const int i = j - 1;
-                    ok = mbar_wait(&s.p_full[i & 1], (i >> 1) & 1) && (i < 2 || mbar_wait(&s.o_free[i & 1], ((i >> 1) - 1) & 1));
-                    if (!ok) break;
-                    tc_fence_after();
-                    const uint32_t v_hi = ring_addr + (i % APK_STAGES) * STAGE + 2 * SIDE, d = tmem + T_O + 128 * (i & 1), p = tmem + T_S + 64 * (i & 1);
-#pragma unroll
-                    for (int m = 0; m < 3; m++)
-#pragma unroll
-                        for (int k = 0; k < APK_BN / 16; k++)
-                            tc_mma_f16_ta(d, p + 32 * (k >> 1) + 8 * (k & 1) + (m == 0 ? 16 : 0),
-                                          umma_desc_sw128_mn(v_hi + (m == 1 ? SIDE : 0) + 2048 * k, HALF), i_o, (m | k) ? 1u : 0u);
-                    tc_commit(&s.free_[i % APK_STAGES]);
-                    done = i;
-                }
+                    for (int k = 0; k < HD / 16; k++)
+                        tc_mma_f16_ta(leader, d, t_base + T_Q + (m == 0 ? 64 : 0) + 8 * k,
+                                      k_hi + (((m == 1 ? SIDE : 0) + (k >> 2) * HALF + 32 * (k & 3)) >> 4), i_s, (m | k) ? 1u : 0u);
+                if (leader) tc_commit(&s.s_full[j & 1]);
             }
-            if (done >= 0) mbar_wait(&s.free_[done % APK_STAGES], (done / APK_STAGES) & 1);   // nothing in flight at the exit
+            if (j > 0) {
+                const int i = j - 1;
+                ok = __all_sync(0xFFFFFFFFu, mbar_wait(&s.p_full[i & 1], (i >> 1) & 1) && (i < 2 || mbar_wait(&s.o_free[i & 1], ((i >> 1) - 1) & 1)));
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t d = t_base + T_O + 128 * (i & 1), p = t_base + T_S + 64 * (i & 1);
+                const uint64_t v_hi = umma_desc_sw128_mn(ring_addr + (i % APK_STAGES) * STAGE + 2 * SIDE, HALF);
+#pragma unroll
+                for (int m = 0; m < 3; m++)
+#pragma unroll
+                    for (int k = 0; k < APK_BN / 16; k++)
+                        tc_mma_f16_ta(leader, d, p + 32 * (k >> 1) + 8 * (k & 1) + (m == 0 ? 16 : 0), v_hi + (((m == 1 ? SIDE : 0) + 2048 * k) >> 4), i_o,
+                                      (m | k) ? 1u : 0u);
+                if (leader) tc_commit(&s.free_[i % APK_STAGES]);
+                done = i;
+            }
         }
+        if (done >= 0) mbar_wait(&s.free_[done % APK_STAGES], (done / APK_STAGES) & 1);   // nothing in flight at the exit
         __syncwarp();
     }
     if (!ok && a.status) *a.status = QZ_ERR_TIMEOUT;

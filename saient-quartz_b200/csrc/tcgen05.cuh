@@ -98,13 +98,22 @@ __device__ __forceinline__ uint32_t umma_idesc_bf16(int n)
 __device__ __forceinline__ uint32_t sw128(int r, int c) { return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4)); }
 
 // ---- forms that the attention uses: f16 operands, A in tensor memory ----
-__device__ __forceinline__ void tc_mma_f16_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate)
+// Called by a whole warp in step, carried out by the lane for which `leader` holds: the operands are then the same in all
+// lanes and stay in uniform registers.  (A lone thread moves each of them there before every instruction; 36 of them took
+// it 4500 cycles.)
+__device__ __forceinline__ void tc_mma_f16_ta(bool leader, uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate)
 {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}\n" ::"r"(d_tmem),
-        "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(0u)
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"((uint32_t)leader)
         : "memory");
+}
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t x;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(x));
+    return x != 0;
 }
 // B stored with its n index contiguous: 64 n by 8 k atoms of 128-byte rows, `n_step` bytes from one 64-wide atom to the next
 __device__ __forceinline__ uint64_t umma_desc_sw128_mn(uint32_t smem_addr, uint32_t n_step)
@@ -118,7 +127,7 @@ __device__ __forceinline__ uint64_t umma_desc_sw128_mn(uint32_t smem_addr, uint3
     return d;
 }
 // D = f32, A = B = f16, A K-major, B K-major or (b_mn) n-contiguous, M = 128, N = n
-__device__ __forceinline__ uint32_t umma_idesc_f16(int n, bool b_mn)
+__device__ constexpr uint32_t umma_idesc_f16(int n, bool b_mn)
 {
     return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(UMMA_M >> 4) << 24);
 }
