@@ -5,17 +5,21 @@
 // f16 parts and a product takes three MMAs, the two small ones first (lo hi + hi lo + hi hi):
 //   S[row, pos]  = Q K^T   A = Q in tensor memory (rows scaled by a power of two), B = K tile in shared memory, K-major
 //   O[row, dim]  = P V     A = P in tensor memory, over S's own columns, B = V tile in shared memory, dims contiguous
+// A value is d (code - 8) + (m + 8 d).  The first term's two parts are exact and cost two packed instructions for two
+// values (hi = d c rounded, lo = d c - hi by one HFMA2: d has 11 bits, c four); the second is the same for the 32 dims of a
+// group, so it is a product of its own, with m and 8 d as they are: 8 more k of S against the sums of q over the groups, 8
+// more columns of O.  (Values split in f32, ten instructions for two, made unpacking the bottleneck: 182 us, not %s.)
 // A operands live in tensor memory because a 64-wide MMA that fetched them from shared memory would be bound by that.
 // The tensor core rounds its sums towards zero, so O is never carried across tiles there: each tile's O starts from zero
 // and is added to f32 registers, where a raised softmax reference is also paid for (one factor per row and tile).
 //
 //   warps 0-3   one row per thread: S from tensor memory, mask, weights 64 exp2(s - ref), their sum, P back.  The
 //               reference is raised only when a score exceeds it by 2^8.
-//   warps 4-11  fill a ring of three (K, V) stages from the cache: a thread unpacks 8 dims of a position at a time,
-//               value = m + d * code in f32, scaled per tile by a power of two that keeps both parts clear of f16's ends;
-//               between two stages they add a finished O tile to their 64 columns of a row.
+//   warps 4-11  fill a ring of three (K, V) stages from the cache, 8 dims of a position at a time.  A tile with a step
+//               that is subnormal or above 8188 (8 d would overflow) is scaled by a power of two.  Between two stages
+//               they add a finished O tile to their half of a row.
 //   warp 12     issues S(j), then P V of tile j - 1: the tensor core works while the weights are computed.
-// Columns of tensor memory: Q 128 (hi, lo), S / P 2 x 64, O 2 x 128.
+// Columns of tensor memory: Q 144 (hi, lo, sums over groups), S / P 2 x 64, O 144 (two halves of 64 dims, 16 for m and 8 d).
 // Within every 8 dims the tiles' order is (0,4,1,5,2,6,3,7), which unpacking produces for free; Q is put in that order,
 // and O's columns are written out by it.
 // Positions outside [first visible, last visible] of the CTA count as zero whatever the cache holds there; a visible V
@@ -41,7 +45,7 @@ struct AttnPromptKv4Args {
 };
 
 struct AttnPromptKv4Shared {
-    uint64_t full[APK_STAGES], free_[APK_STAGES], s_full[2], p_full[2], o_free[2];
+    uint64_t full[APK_STAGES], free_[APK_STAGES], s_full[2], p_full[2], o_free;
     float corr[4][UMMA_M];           // factor of a row's earlier outputs at tile j (slot j % 4)
     float scale_k[4], scale_v[4];    // 1 / what the tile's K and V were multiplied with
     uint32_t nan_v[4][4][2];         // positions of the tile whose V group is NaN, by group
@@ -53,21 +57,19 @@ struct AttnPromptKv4Shared {
 
 __host__ __device__ constexpr size_t attn_prompt_kv4_smem(int NG)
 {
-    return (size_t)APK_STAGES * 4 * ((NG + 1) / 2) * APK_BN * 128 + 1024 + sizeof(AttnPromptKv4Shared);
+    return (size_t)APK_STAGES * (4 * ((NG + 1) / 2) + 1) * APK_BN * 128 + 1024 + sizeof(AttnPromptKv4Shared);
 }
 
-// eight values m + d * code of a word as two 16-byte rows of f16, hi and lo, in the order (0,4,1,5,2,6,3,7)
-__device__ __forceinline__ void kv4_split8(const Nibbles &nib, uint32_t w, float m, float d, uint4 &hi, uint4 &lo)
+// eight products d (code - 8) of a word as two 16-byte rows of f16, hi and lo, in the order (0,4,1,5,2,6,3,7)
+__device__ __forceinline__ void kv4_split8(const Nibbles &nib, uint32_t w, __half2 d, uint4 &hi, uint4 &lo)
 {
     uint32_t x[4], h[4], l[4];
     nib.pairs(w, x);
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const float2 c = __half22float2(*(const __half2 *)&x[i]);
-        const float a = fmaf(d, c.x, m), b = fmaf(d, c.y, m);
-        const float ah = __uint_as_float(__float_as_uint(a) & 0xFFFFE000u), bh = __uint_as_float(__float_as_uint(b) & 0xFFFFE000u);
-        h[i] = pack_half2(ah, bh);
-        l[i] = pack_half2(a - ah, b - bh);
+        const __half2 c = *(const __half2 *)&x[i], p = __hmul2_rn(d, c), r = __hfma2(d, c, __hneg2(p));
+        h[i] = *(const uint32_t *)&p;
+        l[i] = *(const uint32_t *)&r;
     }
     hi = make_uint4(h[0], h[1], h[2], h[3]);
     lo = make_uint4(l[0], l[1], l[2], l[3]);
@@ -89,13 +91,16 @@ __device__ __forceinline__ void ldg_words(const void *p, uint32_t (&x)[N])
 }
 // half k of an array of words
 template <int N>
-__device__ __forceinline__ float half_of(const uint32_t (&x)[N], int k) { return __half2float(__ushort_as_half((unsigned short)(x[k >> 1] >> (16 * (k & 1))))); }
+__device__ __forceinline__ uint32_t bits_of(const uint32_t (&x)[N], int k) { return (x[k >> 1] >> (16 * (k & 1))) & 0xFFFFu; }
+template <int N>
+__device__ __forceinline__ float half_of(const uint32_t (&x)[N], int k) { return __half2float(__ushort_as_half((unsigned short)bits_of(x, k))); }
 
 template <int NG>
 __global__ void __launch_bounds__(APK_THREADS, 1) attn_prompt_kv4_kernel(const AttnPromptKv4Args a)
 {
-    constexpr int HD = 32 * NG, NH = (NG + 1) / 2, HALF = APK_BN * 128, SIDE = NH * HALF, STAGE = 4 * SIDE;   // bytes: 64 dims, a part, K and V
-    constexpr uint32_t T_Q = 0, T_S = 128, T_O = 256;   // tensor-memory columns
+    constexpr int HD = 32 * NG, NH = (NG + 1) / 2, HALF = APK_BN * 128, SIDE = NH * HALF, STAGE = 4 * SIDE + HALF;   // bytes: 64 dims, a part, K and V and their m and 8 d
+    constexpr int AT_K = 0, AT_V_LO = 2 * SIDE, AT_V = 3 * SIDE, AT_X = 4 * SIDE;   // (the m and 8 d follow V's hi part as its next columns)
+    constexpr uint32_t T_Q = 0, T_S = 160, T_O = 288, T_X = T_O + 64 * NH;          // tensor-memory columns
     extern __shared__ unsigned char smem_raw[];
     unsigned char *ring = (unsigned char *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     AttnPromptKv4Shared &s = *(AttnPromptKv4Shared *)(ring + APK_STAGES * STAGE);
@@ -113,11 +118,14 @@ __global__ void __launch_bounds__(APK_THREADS, 1) attn_prompt_kv4_kernel(const A
         for (int i = 0; i < 2; i++) {
             mbar_init(&s.s_full[i], 1);
             mbar_init(&s.p_full[i], 4);
-            mbar_init(&s.o_free[i], 8);
         }
+        mbar_init(&s.o_free, 8);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (threadIdx.x < 32) ((uint32_t *)s.nan_v)[threadIdx.x] = 0;
+    for (int i = threadIdx.x; i < APK_STAGES * HALF / 16; i += APK_THREADS)   // what the m and 8 d do not fill stays zero
+        *(uint4 *)(ring + (i / (HALF / 16)) * STAGE + AT_X + 16 * (i % (HALF / 16))) = make_uint4(0, 0, 0, 0);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     if (warp == 12) tmem_alloc(&s.tmem, 512);
     pdl_trigger();
     pdl_wait();   // q and the cache's rows come from the launches before
@@ -147,8 +155,10 @@ __global__ void __launch_bounds__(APK_THREADS, 1) attn_prompt_kv4_kernel(const A
                 top = fmaxf(top, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
             }
         top *= fabsf(to_log2);
-        const int e = top > 0.f ? max(-100, min(100, 127 + 13 - (int)(__float_as_uint(top) >> 23))) : 0;   // the largest element into [2^13, 2^14)
+        const int e = top > 0.f ? max(-100, min(100, 127 + 8 - (int)(__float_as_uint(top) >> 23))) : 0;   // the largest element into [2^8, 2^9): 32 of them fit f16
         const float up = __uint_as_float((uint32_t)(127 + e) << 23), back = __uint_as_float((uint32_t)(127 - e) << 23);
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};   // of q over the groups
+#pragma unroll
         for (int g = 0; g < NG; g++) {
             uint32_t hi[16], lo[16];
 #pragma unroll
@@ -164,12 +174,24 @@ __global__ void __launch_bounds__(APK_THREADS, 1) attn_prompt_kv4_kernel(const A
                     const float p = x[i] * to_log2 * up, r = y[i] * to_log2 * up;
                     const uint32_t h = pack_half2(p, r);
                     const float2 f = __half22float2(*(const __half2 *)&h);
+                    sum[g] += p + r;
                     hi[4 * c + i] = h;
                     lo[4 * c + i] = pack_half2(p - f.x, r - f.y);
                 }
             }
             tc_st16(tmem + lanes + T_Q + 16 * g, hi);
             tc_st16(tmem + lanes + T_Q + 64 + 16 * g, lo);
+        }
+        {
+            uint32_t x[16] = {};   // hi: (0,1) (2,3) for m, the same for 8 d, zeros; then lo
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const uint32_t h = pack_half2(sum[2 * i], sum[2 * i + 1]);
+                const float2 f = __half22float2(*(const __half2 *)&h);
+                x[i] = x[2 + i] = h;
+                x[8 + i] = x[10 + i] = pack_half2(sum[2 * i] - f.x, sum[2 * i + 1] - f.y);
+            }
+            tc_st16(tmem + lanes + T_Q + 128, x);
         }
         tc_wait_st();
         tc_fence_before();
@@ -258,6 +280,9 @@ __global__ void __launch_bounds__(APK_THREADS, 1) attn_prompt_kv4_kernel(const A
 #pragma unroll
         for (int i = 0; i < 16 * NG; i++) acc[i] = 0.f;
         const int part = w8 >> 2;
+        float acc_x[2] = {0.f, 0.f};                    // sum of p (m + 8 d) of the one or two groups they lie in
+        constexpr int GROUPS = NG == 1 ? 1 : 2;
+        const int g0 = part * (HD / 2) / 32;
         // O of tile j is finished: add it
         auto collect = [&](int j) {
             ok = ok && mbar_wait(&s.free_[j % APK_STAGES], (j / APK_STAGES) & 1);
@@ -267,21 +292,31 @@ __global__ void __launch_bounds__(APK_THREADS, 1) attn_prompt_kv4_kernel(const A
             }
             tc_fence_after();
             const float corr = s.corr[j & 3][row], f = s.scale_v[j & 3];
-            const bool same = __all_sync(0xFFFFFFFFu, corr == 1.f);   // (a reference is raised a few times in all)
-            const uint32_t t_o = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + T_O + 128 * (j & 1) + part * (HD / 2);
+            const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+            if (!__all_sync(0xFFFFFFFFu, corr == 1.f)) {   // (a reference is raised a few times in all)
+#pragma unroll
+                for (int i = 0; i < 16 * NG; i++) acc[i] *= corr;
+                acc_x[0] *= corr;
+                acc_x[1] *= corr;
+            }
+            uint32_t o[16];
+            tc_ld8(tmem + lanes + T_X, o);
+#pragma unroll
+            for (int g = 0; g < GROUPS; g++) {
+                float m = 0.f;
+#pragma unroll
+                for (int i = 0; i < NG; i++) m = i == g0 + g ? __uint_as_float(o[i]) + __uint_as_float(o[4 + i]) : m;
+                acc_x[g] = fmaf(m, f, acc_x[g]);
+            }
 #pragma unroll
             for (int c = 0; c < NG; c++) {
-                uint32_t o[16];
-                tc_ld16(t_o + 16 * c, o);
+                tc_ld16(tmem + lanes + T_O + part * (HD / 2) + 16 * c, o);
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    if (!same) acc[16 * c + i] *= corr;
-                    acc[16 * c + i] = fmaf(__uint_as_float(o[i]), f, acc[16 * c + i]);
-                }
+                for (int i = 0; i < 16; i++) acc[16 * c + i] = fmaf(__uint_as_float(o[i]), f, acc[16 * c + i]);
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&s.o_free[j & 1]);
+            if (lane == 0) mbar_arrive(&s.o_free);
         };
         uint32_t kw[NG], vw[NG], kp[NG], vp[NG];   // 8 dims of NG groups, and the position's parameters (m .., d ..)
         auto fetch = [&](int j) {
@@ -298,18 +333,13 @@ __global__ void __launch_bounds__(APK_THREADS, 1) attn_prompt_kv4_kernel(const A
                 for (int i = 0; i < NG; i++) kp[i] = vp[i] = 0;   // m = d = 0
             }
         };
-        fetch(0);
-        for (int j = 0; j < n_tiles; j++) {
-            if (j >= APK_STAGES) collect(j - APK_STAGES);   // (a wait that gave up does not leave the loop: the barrier below is for all)
-            // the tile's largest magnitudes
+        // (rare) bring the tile's parameters into range: times the power of two that takes its largest magnitude to [2^12, 2^13)
+        auto rescale_params = [&](int j, float &uk, float &uv) {
             float top_k = 0.f, top_v = 0.f;
-            if (tid < 8) s.nan_v[(j + 1) & 3][tid >> 1][tid & 1] = 0;   // (its last readers have finished: tile j - 3 is)
 #pragma unroll
             for (int g = 0; g < NG; g++) {
-                const float dk = half_of(kp, NG + g), dv = half_of(vp, NG + g), mv = half_of(vp, g);
-                if (mv != mv && t == 0) atomicOr(&s.nan_v[j & 3][g][p_tile >> 5], 1u << (p_tile & 31));
-                top_k = fmaxf(top_k, fabsf(fmaf(8.f, dk, half_of(kp, g))) + 8.f * dk);
-                top_v = fmaxf(top_v, fabsf(fmaf(8.f, dv, mv)) + 8.f * dv);
+                top_k = fmaxf(top_k, fabsf(half_of(kp, g)) + 15.f * half_of(kp, NG + g));
+                top_v = fmaxf(top_v, fabsf(half_of(vp, g)) + 15.f * half_of(vp, NG + g));
             }
             const uint32_t wk = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(top_k)), wv = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(top_v));
             if (lane == 0) {
@@ -318,34 +348,74 @@ __global__ void __launch_bounds__(APK_THREADS, 1) attn_prompt_kv4_kernel(const A
             }
             asm volatile("bar.sync 3, 256;" ::: "memory");
             uint32_t tk = 0, tv = 0;
-#pragma unroll
             for (int i = 0; i < 8; i++) {
                 tk = max(tk, s.top[j & 1][0][i]);
                 tv = max(tv, s.top[j & 1][1][i]);
             }
-            // powers of two that bring them into [2^13, 2^14)
-            const int ek = tk ? 127 + 13 - (int)(tk >> 23) : 0, ev = tv ? 127 + 13 - (int)(tv >> 23) : 0;
-            const float uk = __uint_as_float((uint32_t)(127 + ek) << 23), uv = __uint_as_float((uint32_t)(127 + ev) << 23);
+            const int ek = tk ? 127 + 12 - (int)(tk >> 23) : 0, ev = tv ? 127 + 12 - (int)(tv >> 23) : 0;
+            uk = __uint_as_float((uint32_t)(127 + ek) << 23);
+            uv = __uint_as_float((uint32_t)(127 + ev) << 23);
+            auto times = [](uint32_t w, float u) {
+                const float2 x = __half22float2(*(const __half2 *)&w);
+                return pack_half2(x.x * u, x.y * u);
+            };
+#pragma unroll
+            for (int i = 0; i < NG; i++) {
+                kp[i] = times(kp[i], uk);
+                vp[i] = times(vp[i], uv);
+            }
+        };
+        fetch(0);
+        for (int j = 0; j < n_tiles; j++) {
+            if (j >= APK_STAGES) collect(j - APK_STAGES);   // (a wait that gave up does not leave the loop: the barrier below is for all)
+            if (tid < 8) s.nan_v[(j + 1) & 3][tid >> 1][tid & 1] = 0;   // (its last readers have finished: tile j - 3 is)
+            bool odd = false;   // a step that is subnormal, or whose eightfold overflows
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+                const uint32_t dk = bits_of(kp, NG + g), dv = bits_of(vp, NG + g);
+                odd |= (dk && dk - 0x400u > 0x6BFFu) || (dv && dv - 0x400u > 0x6BFFu);
+                if ((bits_of(vp, g) & 0x7FFFu) > 0x7C00u) {   // NaN
+                    if (t == 0) atomicOr(&s.nan_v[j & 3][g][p_tile >> 5], 1u << (p_tile & 31));
+                    vp[g >> 1] &= g & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+                }
+            }
+            uint32_t any;
+            asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 3, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}\n"
+                         : "=r"(any) : "r"((uint32_t)odd) : "memory");
+            float uk = 1.f, uv = 1.f;
+            if (any) rescale_params(j, uk, uv);
             if (tid == 0) {
-                s.scale_k[j & 3] = __uint_as_float((uint32_t)(127 - ek) << 23);
-                s.scale_v[j & 3] = __uint_as_float((uint32_t)(127 - ev) << 23);
+                s.scale_k[j & 3] = 1.f / uk;
+                s.scale_v[j & 3] = 1.f / uv;
             }
             unsigned char *stage = ring + (j % APK_STAGES) * STAGE;
 #pragma unroll
             for (int g = 0; g < NG; g++) {
                 const uint32_t at = (g >> 1) * HALF + sw128(p_tile, (g & 1) * 4 + t);
                 uint4 hi, lo;
-                float d = half_of(kp, NG + g) * uk;
-                kv4_split8(nib, kw[g], fmaf(8.f, d, half_of(kp, g) * uk), d, hi, lo);
-                *(uint4 *)(stage + at) = hi;
-                *(uint4 *)(stage + SIDE + at) = lo;
-                const uint32_t a16 = vw[g >> 1] >> (16 * (g & 1)), b16 = vw[(NG + g) >> 1] >> (16 * ((NG + g) & 1));   // dims 8 t .., and 8 t + 4 ..
-                d = half_of(vp, NG + g) * uv;
-                float m = fmaf(8.f, d, half_of(vp, g) * uv);
-                if (m != m) m = d = 0.f;
-                kv4_split8(nib, (a16 & 0xFFFFu) | b16 << 16, m, d, hi, lo);
-                *(uint4 *)(stage + 2 * SIDE + at) = hi;
-                *(uint4 *)(stage + 3 * SIDE + at) = lo;
+                kv4_split8(nib, kw[g], __half2half2(__ushort_as_half((unsigned short)bits_of(kp, NG + g))), hi, lo);
+                *(uint4 *)(stage + AT_K + at) = hi;
+                *(uint4 *)(stage + AT_K + SIDE + at) = lo;
+                const uint32_t w = bits_of(vw, g) | bits_of(vw, NG + g) << 16;   // dims 8 t .., and 8 t + 4 ..
+                kv4_split8(nib, w, __half2half2(__ushort_as_half((unsigned short)bits_of(vp, NG + g))), hi, lo);
+                *(uint4 *)(stage + AT_V + at) = hi;
+                *(uint4 *)(stage + AT_V_LO + at) = lo;
+            }
+            if (t < 2) {   // m and 8 d of the position: K's as k 32 .. of the extra tile, V's as its first columns
+                uint32_t x[4];
+                const __half2 eight = __half2half2(__ushort_as_half((unsigned short)0x4800));
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const uint32_t mk = (2 * i < NG ? bits_of(kp, min(2 * i, NG - 1)) : 0) | (2 * i + 1 < NG ? bits_of(kp, min(2 * i + 1, NG - 1)) << 16 : 0);
+                    const uint32_t mv = (2 * i < NG ? bits_of(vp, min(2 * i, NG - 1)) : 0) | (2 * i + 1 < NG ? bits_of(vp, min(2 * i + 1, NG - 1)) << 16 : 0);
+                    const uint32_t dk = (2 * i < NG ? bits_of(kp, NG + min(2 * i, NG - 1)) : 0) | (2 * i + 1 < NG ? bits_of(kp, NG + min(2 * i + 1, NG - 1)) << 16 : 0);
+                    const uint32_t dv = (2 * i < NG ? bits_of(vp, NG + min(2 * i, NG - 1)) : 0) | (2 * i + 1 < NG ? bits_of(vp, NG + min(2 * i + 1, NG - 1)) << 16 : 0);
+                    const uint32_t d = t ? dv : dk;
+                    const __half2 d8 = __hmul2(*(const __half2 *)&d, eight);
+                    x[i] = t ? mv : mk;
+                    x[2 + i] = *(const uint32_t *)&d8;
+                }
+                *(uint4 *)(stage + AT_X + sw128(p_tile, t ? 0 : 4)) = make_uint4(x[0], x[1], x[2], x[3]);
             }
             if (j + 1 < n_tiles) fetch(j + 1);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -360,17 +430,18 @@ __global__ void __launch_bounds__(APK_THREADS, 1) attn_prompt_kv4_kernel(const A
             float *dst = a.out + ((size_t)(t0 + tok) * a.n_heads + head) * HD + part * (HD / 2);
 #pragma unroll
             for (int c = 0; c < 2 * NG; c++) {   // eight columns: dims (0,4,1,5,2,6,3,7)
-                const float f = bad >> ((part * (HD / 2) + 8 * c) >> 5) & 1 ? __int_as_float(0x7FC00000) : inv;
+                const int g = (part * (HD / 2) + 8 * c) >> 5;
+                const float f = bad >> g & 1 ? __int_as_float(0x7FC00000) : inv, x = g == g0 ? acc_x[0] : acc_x[1];
                 const float *o = acc + 8 * c;
-                *(float4 *)(dst + 8 * c) = make_float4(o[0] * f, o[2] * f, o[4] * f, o[6] * f);
-                *(float4 *)(dst + 8 * c + 4) = make_float4(o[1] * f, o[3] * f, o[5] * f, o[7] * f);
+                *(float4 *)(dst + 8 * c) = make_float4((o[0] + x) * f, (o[2] + x) * f, (o[4] + x) * f, (o[6] + x) * f);
+                *(float4 *)(dst + 8 * c + 4) = make_float4((o[1] + x) * f, (o[3] + x) * f, (o[5] + x) * f, (o[7] + x) * f);
             }
         }
     } else if (warp == 12) {   // (warps 13 to 15 only lend their registers)
         asm volatile("bar.sync 1, 160;" ::: "memory");
         tc_fence_after();
         const bool leader = elect_one();
-        constexpr uint32_t i_s = umma_idesc_f16(APK_BN, false), i_o = umma_idesc_f16(HD, true);
+        constexpr uint32_t i_s = umma_idesc_f16(APK_BN, false), i_o = umma_idesc_f16(64 * NH + 16, true), i_lo = umma_idesc_f16(64 * NH, true);
         const uint32_t ring_addr = smem_u32(ring), t_base = __shfl_sync(0xFFFFFFFFu, tmem, 0);
         int done = -1;   // last tile whose P V was issued
         for (int j = 0; j <= n_tiles; j++) {
@@ -380,28 +451,30 @@ __global__ void __launch_bounds__(APK_THREADS, 1) attn_prompt_kv4_kernel(const A
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t d = t_base + T_S + 64 * (j & 1);
-                const uint64_t k_hi = umma_desc_sw128(ring_addr + (j % APK_STAGES) * STAGE);   // (its low word counts 16 bytes)
+                const uint64_t stage = umma_desc_sw128(ring_addr + (j % APK_STAGES) * STAGE);   // (its low word counts 16 bytes)
 #pragma unroll
-                for (int m = 0; m < 3; m++)
+                for (int m = 0; m < 3; m++) {   // lo hi, hi lo, hi hi
 #pragma unroll
                     for (int k = 0; k < HD / 16; k++)
                         tc_mma_f16_ta(leader, d, t_base + T_Q + (m == 0 ? 64 : 0) + 8 * k,
-                                      k_hi + (((m == 1 ? SIDE : 0) + (k >> 2) * HALF + 32 * (k & 3)) >> 4), i_s, (m | k) ? 1u : 0u);
+                                      stage + ((AT_K + (m == 1 ? SIDE : 0) + (k >> 2) * HALF + 32 * (k & 3)) >> 4), i_s, (m | k) ? 1u : 0u);
+                    if (m != 1) tc_mma_f16_ta(leader, d, t_base + T_Q + (m == 0 ? 136 : 128), stage + ((AT_X + 64) >> 4), i_s, 1u);
+                }
                 if (leader) tc_commit(&s.s_full[j & 1]);
             }
             if (j > 0) {
                 const int i = j - 1;
-                ok = __all_sync(0xFFFFFFFFu, mbar_wait(&s.p_full[i & 1], (i >> 1) & 1) && (i < 2 || mbar_wait(&s.o_free[i & 1], ((i >> 1) - 1) & 1)));
+                ok = __all_sync(0xFFFFFFFFu, mbar_wait(&s.p_full[i & 1], (i >> 1) & 1) && (i < 1 || mbar_wait(&s.o_free, (i - 1) & 1)));
                 if (!ok) break;
                 tc_fence_after();
-                const uint32_t d = t_base + T_O + 128 * (i & 1), p = t_base + T_S + 64 * (i & 1);
-                const uint64_t v_hi = umma_desc_sw128_mn(ring_addr + (i % APK_STAGES) * STAGE + 2 * SIDE, HALF);
+                const uint32_t d = t_base + T_O, p = t_base + T_S + 64 * (i & 1);
+                const uint64_t stage = umma_desc_sw128_mn(ring_addr + (i % APK_STAGES) * STAGE, HALF);
 #pragma unroll
                 for (int m = 0; m < 3; m++)
 #pragma unroll
                     for (int k = 0; k < APK_BN / 16; k++)
-                        tc_mma_f16_ta(leader, d, p + 32 * (k >> 1) + 8 * (k & 1) + (m == 0 ? 16 : 0), v_hi + (((m == 1 ? SIDE : 0) + 2048 * k) >> 4), i_o,
-                                      (m | k) ? 1u : 0u);
+                        tc_mma_f16_ta(leader, d, p + 32 * (k >> 1) + 8 * (k & 1) + (m == 0 ? 16 : 0), stage + (((m == 1 ? AT_V_LO : AT_V) + 2048 * k) >> 4),
+                                      m == 1 ? i_lo : i_o, (m | k) ? 1u : 0u);
                 if (leader) tc_commit(&s.free_[i % APK_STAGES]);
                 done = i;
             }
