@@ -299,38 +299,46 @@ __global__ void __launch_bounds__(APK_THREADS, 1) attn_prompt_kv4_kernel(const A
                 acc_x[0] *= corr;
                 acc_x[1] *= corr;
             }
-            uint32_t o[16];
-            tc_ld8(tmem + lanes + T_X, o);
+            uint32_t x[8];
+            tc_ld8(tmem + lanes + T_X, x);
 #pragma unroll
             for (int g = 0; g < GROUPS; g++) {
-                float m = 0.f;
-#pragma unroll
-                for (int i = 0; i < NG; i++) m = i == g0 + g ? __uint_as_float(o[i]) + __uint_as_float(o[4 + i]) : m;
+                constexpr int G1 = HD / 64;   // (indexes known to the compiler: the values stay in registers)
+                const float m0 = __uint_as_float(x[g]) + __uint_as_float(x[4 + g]), m1 = __uint_as_float(x[G1 + g]) + __uint_as_float(x[4 + G1 + g]);
+                const float m = part ? m1 : m0;
                 acc_x[g] = fmaf(m, f, acc_x[g]);
             }
 #pragma unroll
-            for (int c = 0; c < NG; c++) {
-                tc_ld16(tmem + lanes + T_O + part * (HD / 2) + 16 * c, o);
+            for (int c = 0; c < NG / 2; c++) {
+                uint32_t o[32];
+                tc_ld32(tmem + lanes + T_O + part * (HD / 2) + 32 * c, o);
 #pragma unroll
-                for (int i = 0; i < 16; i++) acc[16 * c + i] = fmaf(__uint_as_float(o[i]), f, acc[16 * c + i]);
+                for (int i = 0; i < 32; i++) acc[32 * c + i] = fmaf(__uint_as_float(o[i]), f, acc[32 * c + i]);
+            }
+            if constexpr (NG % 2 == 1) {
+                uint32_t o[16];
+                tc_ld16(tmem + lanes + T_O + part * (HD / 2) + 16 * (NG - 1), o);
+#pragma unroll
+                for (int i = 0; i < 16; i++) acc[16 * (NG - 1) + i] = fmaf(__uint_as_float(o[i]), f, acc[16 * (NG - 1) + i]);
             }
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&s.o_free);
         };
-        uint32_t kw[NG], vw[NG], kp[NG], vp[NG];   // 8 dims of NG groups, and the position's parameters (m .., d ..)
+        // 8 dims of NG groups, and the position's parameters (m .., d ..): of this tile, and of the next, on its way
+        uint32_t kw[NG], vw[NG], kp[NG], vp[NG], kw1[NG], vw1[NG], kp1[NG], vp1[NG];
         auto fetch = [&](int j) {
             const int pos = base0 + APK_BN * j + p_tile;
             const bool seen = pos >= k_lo && pos <= p_last;
             const uint8_t *blk = head_blocks + (size_t)((seen ? pos : p_last) / KV4_BLOCK) * (40 * HD);
             const int r = (seen ? pos : p_last) % KV4_BLOCK;
-            ldg_words<NG>(blk + 16 * HD + r * 4 * NG, kp);
-            ldg_words<NG>(blk + 36 * HD + r * 4 * NG, vp);
-            ldg_words<NG>(blk + r * (HD / 2) + 4 * NG * t, kw);
-            ldg_words<NG>(blk + 20 * HD + r * (HD / 2) + 4 * NG * t, vw);
+            ldg_words<NG>(blk + 16 * HD + r * 4 * NG, kp1);
+            ldg_words<NG>(blk + 36 * HD + r * 4 * NG, vp1);
+            ldg_words<NG>(blk + r * (HD / 2) + 4 * NG * t, kw1);
+            ldg_words<NG>(blk + 20 * HD + r * (HD / 2) + 4 * NG * t, vw1);
             if (!seen) {
 #pragma unroll
-                for (int i = 0; i < NG; i++) kp[i] = vp[i] = 0;   // m = d = 0
+                for (int i = 0; i < NG; i++) kp1[i] = vp1[i] = 0;   // m = d = 0
             }
         };
         // (rare) bring the tile's parameters into range: times the power of two that takes its largest magnitude to [2^12, 2^13)
@@ -368,6 +376,14 @@ __global__ void __launch_bounds__(APK_THREADS, 1) attn_prompt_kv4_kernel(const A
         fetch(0);
         for (int j = 0; j < n_tiles; j++) {
             if (j >= APK_STAGES) collect(j - APK_STAGES);   // (a wait that gave up does not leave the loop: the barrier below is for all)
+#pragma unroll
+            for (int i = 0; i < NG; i++) {
+                kw[i] = kw1[i];
+                vw[i] = vw1[i];
+                kp[i] = kp1[i];
+                vp[i] = vp1[i];
+            }
+            if (j + 1 < n_tiles) fetch(j + 1);
             if (tid < 8) s.nan_v[(j + 1) & 3][tid >> 1][tid & 1] = 0;   // (its last readers have finished: tile j - 3 is)
             bool odd = false;   // a step that is subnormal, or whose eightfold overflows
 #pragma unroll
@@ -391,13 +407,17 @@ __global__ void __launch_bounds__(APK_THREADS, 1) attn_prompt_kv4_kernel(const A
             unsigned char *stage = ring + (j % APK_STAGES) * STAGE;
 #pragma unroll
             for (int g = 0; g < NG; g++) {
-                const uint32_t at = (g >> 1) * HALF + sw128(p_tile, (g & 1) * 4 + t);
+                // odd positions take a pair of groups the other way round: eight lanes then fill eight different 16-byte columns
+                const int other = (g ^ 1) < NG ? g ^ 1 : g;
+                const bool swap = (p_tile & 1) && other != g;
+                const uint32_t at = (g >> 1) * HALF + sw128(p_tile, ((swap ? other : g) & 1) * 4 + t);
                 uint4 hi, lo;
-                kv4_split8(nib, kw[g], __half2half2(__ushort_as_half((unsigned short)bits_of(kp, NG + g))), hi, lo);
+                kv4_split8(nib, swap ? kw[other] : kw[g], __half2half2(__ushort_as_half((unsigned short)(swap ? bits_of(kp, NG + other) : bits_of(kp, NG + g)))), hi, lo);
                 *(uint4 *)(stage + AT_K + at) = hi;
                 *(uint4 *)(stage + AT_K + SIDE + at) = lo;
-                const uint32_t w = bits_of(vw, g) | bits_of(vw, NG + g) << 16;   // dims 8 t .., and 8 t + 4 ..
-                kv4_split8(nib, w, __half2half2(__ushort_as_half((unsigned short)bits_of(vp, NG + g))), hi, lo);
+                // dims 8 t .., and 8 t + 4 ..
+                const uint32_t w = swap ? bits_of(vw, other) | bits_of(vw, NG + other) << 16 : bits_of(vw, g) | bits_of(vw, NG + g) << 16;
+                kv4_split8(nib, w, __half2half2(__ushort_as_half((unsigned short)(swap ? bits_of(vp, NG + other) : bits_of(vp, NG + g)))), hi, lo);
                 *(uint4 *)(stage + AT_V + at) = hi;
                 *(uint4 *)(stage + AT_V_LO + at) = lo;
             }
@@ -417,7 +437,6 @@ __global__ void __launch_bounds__(APK_THREADS, 1) attn_prompt_kv4_kernel(const A
                 }
                 *(uint4 *)(stage + AT_X + sw128(p_tile, t ? 0 : 4)) = make_uint4(x[0], x[1], x[2], x[3]);
             }
-            if (j + 1 < n_tiles) fetch(j + 1);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(&s.full[j % APK_STAGES]);
