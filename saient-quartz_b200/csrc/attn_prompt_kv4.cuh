@@ -16,7 +16,7 @@
 //   warps 0-3   one row per thread: S from tensor memory, mask, weights 64 exp2(s - ref), their sum, P back.  The
 //               reference is raised only when a score exceeds it by 2^8.
 //   warps 4-11  fill a ring of three (K, V) stages from the cache, 8 dims of a position at a time.  A tile with a step
-//               that is subnormal or above 8188 (8 d would overflow) is scaled by a power of two.  Between two stages
+//               above 8188 (8 d would overflow) is scaled by a power of two.  Between two stages
 //               they add a finished O tile to their half of a row.
 //   warp 12     issues S(j), then P V of tile j - 1: the tensor core works while the weights are computed.
 // Columns of tensor memory: Q 144 (hi, lo, sums over groups), S / P 2 x 64, O 144 (two halves of 64 dims, 16 for m and 8 d).
@@ -327,23 +327,31 @@ __global__ void __launch_bounds__(APK_THREADS, 1) attn_prompt_kv4_kernel(const A
         };
         // 8 dims of NG groups, and the position's parameters (m .., d ..): of this tile, and of the next, on its way
         uint32_t kw[NG], vw[NG], kp[NG], vp[NG], kw1[NG], vw1[NG], kp1[NG], vp1[NG];
+        const uint8_t *at0 = head_blocks + (size_t)(b0 + p_tile / KV4_BLOCK) * (40 * HD) + 4 * NG * (p_tile % KV4_BLOCK);   // (a tile is two blocks on)
         auto fetch = [&](int j) {
             const int pos = base0 + APK_BN * j + p_tile;
-            const bool seen = pos >= k_lo && pos <= p_last;
-            const uint8_t *blk = head_blocks + (size_t)((seen ? pos : p_last) / KV4_BLOCK) * (40 * HD);
-            const int r = (seen ? pos : p_last) % KV4_BLOCK;
-            ldg_words<NG>(blk + 16 * HD + r * 4 * NG, kp1);
-            ldg_words<NG>(blk + 36 * HD + r * 4 * NG, vp1);
-            ldg_words<NG>(blk + r * (HD / 2) + 4 * NG * t, kw1);
-            ldg_words<NG>(blk + 20 * HD + r * (HD / 2) + 4 * NG * t, vw1);
-            if (!seen) {
+            if ((unsigned)(pos - k_lo) <= (unsigned)(p_last - k_lo)) {
+                const uint8_t *at = at0 + (size_t)j * (2 * 40 * HD);
+                ldg_words<NG>(at + 16 * HD, kp1);
+                ldg_words<NG>(at + 36 * HD, vp1);
+                at += 4 * NG * (3 * (p_tile % KV4_BLOCK) + t);   // (a row of codes is four rows of parameters long)
+                ldg_words<NG>(at, kw1);
+                ldg_words<NG>(at + 20 * HD, vw1);
+            } else {
 #pragma unroll
-                for (int i = 0; i < NG; i++) kp1[i] = vp1[i] = 0;   // m = d = 0
+                for (int i = 0; i < NG; i++) kp1[i] = vp1[i] = kw1[i] = vw1[i] = 0;   // m = d = 0
             }
         };
-        // (rare) bring the tile's parameters into range: times the power of two that takes its largest magnitude to [2^12, 2^13)
-        auto rescale_params = [&](int j, float &uk, float &uv) {
+        // (rare) note V groups that are NaN and take them as zero; bring the tile's parameters into range: times the power of
+        // two that takes its largest magnitude to [2^12, 2^13)
+        auto mend = [&](int j, float &uk, float &uv) {
             float top_k = 0.f, top_v = 0.f;
+#pragma unroll
+            for (int g = 0; g < NG; g++)
+                if ((bits_of(vp, g) & 0x7FFFu) > 0x7C00u) {
+                    if (t == 0) atomicOr(&s.nan_v[j & 3][g][p_tile >> 5], 1u << (p_tile & 31));
+                    vp[g >> 1] &= g & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+                }
 #pragma unroll
             for (int g = 0; g < NG; g++) {
                 top_k = fmaxf(top_k, fabsf(half_of(kp, g)) + 15.f * half_of(kp, NG + g));
@@ -385,21 +393,30 @@ __global__ void __launch_bounds__(APK_THREADS, 1) attn_prompt_kv4_kernel(const A
             }
             if (j + 1 < n_tiles) fetch(j + 1);
             if (tid < 8) s.nan_v[(j + 1) & 3][tid >> 1][tid & 1] = 0;   // (its last readers have finished: tile j - 3 is)
-            bool odd = false;   // a step that is subnormal, or whose eightfold overflows
+            // a step whose eightfold overflows f16, or a NaN among V's minima (a sum of them that is NaN)?  Subnormal steps do no
+            // harm: their multiples are exact.
+            bool odd;
+            if constexpr (NG % 2 == 0) {
+                uint32_t top = 0;
+                __half2 sum = __half2half2(__ushort_as_half((unsigned short)0));
 #pragma unroll
-            for (int g = 0; g < NG; g++) {
-                const uint32_t dk = bits_of(kp, NG + g), dv = bits_of(vp, NG + g);
-                odd |= (dk && dk - 0x400u > 0x6BFFu) || (dv && dv - 0x400u > 0x6BFFu);
-                if ((bits_of(vp, g) & 0x7FFFu) > 0x7C00u) {   // NaN
-                    if (t == 0) atomicOr(&s.nan_v[j & 3][g][p_tile >> 5], 1u << (p_tile & 31));
-                    vp[g >> 1] &= g & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+                for (int i = 0; i < NG / 2; i++) {
+                    top = __vmaxu2(top, __vmaxu2(kp[NG / 2 + i], vp[NG / 2 + i]));
+                    sum = __hadd2(sum, *(const __half2 *)&vp[i]);
                 }
+                const uint32_t w = *(const uint32_t *)&sum & 0x7FFF7FFFu;
+                odd = (__vmaxu2(top, 0x6FFF6FFFu) != 0x6FFF6FFFu) | (__vmaxu2(w, 0x7C007C00u) != 0x7C007C00u);
+            } else {
+                odd = false;
+#pragma unroll
+                for (int g = 0; g < NG; g++)
+                    odd |= bits_of(kp, NG + g) > 0x6FFFu || bits_of(vp, NG + g) > 0x6FFFu || (bits_of(vp, g) & 0x7FFFu) > 0x7C00u;
             }
             uint32_t any;
             asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 3, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}\n"
                          : "=r"(any) : "r"((uint32_t)odd) : "memory");
             float uk = 1.f, uv = 1.f;
-            if (any) rescale_params(j, uk, uv);
+            if (any) mend(j, uk, uv);
             if (tid == 0) {
                 s.scale_k[j & 3] = 1.f / uk;
                 s.scale_v[j & 3] = 1.f / uv;
@@ -422,17 +439,23 @@ __global__ void __launch_bounds__(APK_THREADS, 1) attn_prompt_kv4_kernel(const A
                 *(uint4 *)(stage + AT_V_LO + at) = lo;
             }
             if (t < 2) {   // m and 8 d of the position: K's as k 32 .. of the extra tile, V's as its first columns
-                uint32_t x[4];
+                uint32_t x[4] = {0, 0, 0, 0};
                 const __half2 eight = __half2half2(__ushort_as_half((unsigned short)0x4800));
 #pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const uint32_t mk = (2 * i < NG ? bits_of(kp, min(2 * i, NG - 1)) : 0) | (2 * i + 1 < NG ? bits_of(kp, min(2 * i + 1, NG - 1)) << 16 : 0);
-                    const uint32_t mv = (2 * i < NG ? bits_of(vp, min(2 * i, NG - 1)) : 0) | (2 * i + 1 < NG ? bits_of(vp, min(2 * i + 1, NG - 1)) << 16 : 0);
-                    const uint32_t dk = (2 * i < NG ? bits_of(kp, NG + min(2 * i, NG - 1)) : 0) | (2 * i + 1 < NG ? bits_of(kp, NG + min(2 * i + 1, NG - 1)) << 16 : 0);
-                    const uint32_t dv = (2 * i < NG ? bits_of(vp, NG + min(2 * i, NG - 1)) : 0) | (2 * i + 1 < NG ? bits_of(vp, NG + min(2 * i + 1, NG - 1)) << 16 : 0);
-                    const uint32_t d = t ? dv : dk;
+                for (int i = 0; i < (NG + 1) / 2; i++) {
+                    uint32_t m, d;
+                    if constexpr (NG % 2 == 0) {
+                        m = t ? vp[i] : kp[i];
+                        d = t ? vp[NG / 2 + i] : kp[NG / 2 + i];
+                    } else {
+                        const bool two = 2 * i + 1 < NG;
+                        constexpr int L = NG - 1;
+                        m = t ? bits_of(vp, 2 * i) | (two ? bits_of(vp, min(2 * i + 1, L)) << 16 : 0) : bits_of(kp, 2 * i) | (two ? bits_of(kp, min(2 * i + 1, L)) << 16 : 0);
+                        d = t ? bits_of(vp, NG + 2 * i) | (two ? bits_of(vp, NG + min(2 * i + 1, L)) << 16 : 0)
+                              : bits_of(kp, NG + 2 * i) | (two ? bits_of(kp, NG + min(2 * i + 1, L)) << 16 : 0);
+                    }
                     const __half2 d8 = __hmul2(*(const __half2 *)&d, eight);
-                    x[i] = t ? mv : mk;
+                    x[i] = m;
                     x[2 + i] = *(const uint32_t *)&d8;
                 }
                 *(uint4 *)(stage + AT_X + sw128(p_tile, t ? 0 : 4)) = make_uint4(x[0], x[1], x[2], x[3]);
