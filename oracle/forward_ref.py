@@ -60,6 +60,10 @@ class RefModel:
     def set_kv(self, layer, k, v):
         self.kv[layer] = (k.astype(f32).copy(), v.astype(f32).copy())
 
+    def cached(self, x):
+        """The values that a row of k or v has once it is in the cache (f32 caches: its own)."""
+        return x
+
     def _mv(self, role, layer, x, K, N, expert=None):
         t, a = self.t[(role, layer)]
         a = a.view(np.uint8).reshape(-1)
@@ -95,8 +99,8 @@ class RefModel:
         for hh in range(kvh):
             rope_yarn(k[hh * hd:(hh + 1) * hd], pos, hd, c["rope_theta"], ys, yo, c.get("rope_neox", 0))
         K_, V_ = self.kv[l]
-        K_ = np.concatenate([K_[:pos], k[None, :]], 0)
-        V_ = np.concatenate([V_[:pos], v[None, :]], 0)
+        K_ = np.concatenate([K_[:pos], self.cached(k)[None, :]], 0)
+        V_ = np.concatenate([V_[:pos], self.cached(v)[None, :]], 0)
         self.kv[l] = (K_, V_)
         seq = pos + 1
         mscale2 = f32(1.0)

@@ -1,4 +1,4 @@
-// Attention over the 4-bit cache (kv4.cuh): one token of a decode step, or the tokens of a prompt.
+// Attention over the 4-bit cache (kv4.cuh) for one token of a decode step, or a few tokens of a prompt one by one.
 #pragma once
 
 #include <cooperative_groups.h>
@@ -17,7 +17,7 @@ constexpr size_t AK_WORKSPACE = sizeof(float) * (AK_COUNTERS + (size_t)AK_MAX_CL
 
 struct AttnKv4Args {
     float *out;
-    const float *q, *k_new, *v_new;      // step: before rotation; prompt: already rotated, k_new / v_new NULL
+    const float *q, *k_new, *v_new;      // before rotation; token blockIdx.y (at pos + blockIdx.y) has row blockIdx.y of q and out
     uint8_t *cache;
     const int *step;                     // device words {token, pos}, or NULL: pos
     int pos;
@@ -40,107 +40,6 @@ struct AttnKv4Args {
 // split cluster barrier (every thread of the CTA executes both halves)
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-
-// One CTA per (kv head, token); a warp takes every eighth position for one query head after the other.
-template <int NG>
-__global__ void __launch_bounds__(AK_THREADS) attn_kv4_kernel(const AttnKv4Args a)
-{
-    constexpr int HD = 32 * NG, half = HD / 2;
-    __shared__ __align__(16) float qs[AK_MAX_G * HD];
-    __shared__ __align__(16) float kn[HD];
-    __shared__ float part[AK_WARPS][HD + 2];
-    const int head = blockIdx.x, tok = blockIdx.y, G = a.n_heads / a.n_kv;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    pdl_wait();
-    pdl_trigger();
-    int pos = (a.step ? __ldcg(a.step + 1) : a.pos) + tok;
-    pos = max(0, min(pos, a.max_seq - 1));
-    const int first = a.window > 0 ? max(0, pos + 1 - a.window) : 0;
-    const RopeArgs rope{pos, a.theta, a.yarn_scale, a.yarn_orig_ctx, a.neox};
-    for (int e = threadIdx.x; e < (G + 1) * half; e += AK_THREADS) {
-        const int g = e / half, i = e - g * half;
-        const int i0 = a.neox ? i : 2 * i, i1 = a.neox ? i + half : 2 * i + 1;
-        if (g == G && !a.k_new) break;
-        const float *src = g == G ? a.k_new + (size_t)head * HD : a.q + ((size_t)tok * a.n_heads + (size_t)head * G + g) * HD;
-        float x0 = __ldcg(src + i0), x1 = __ldcg(src + i1);
-        if (a.theta > 0.f) {
-            float c, s;
-            rope_cs(rope, i, HD, c, s);
-            const float r0 = x0 * c - x1 * s, r1 = x0 * s + x1 * c;
-            x0 = r0;
-            x1 = r1;
-        }
-        float *dst = g == G ? kn : qs + g * HD;
-        dst[i0] = x0;
-        dst[i1] = x1;
-    }
-    __syncthreads();
-    if (a.k_new && warp < 2 && lane < 4 * NG) {
-        const float *src = warp ? a.v_new + (size_t)head * HD : kn;
-        float x[8];
-#pragma unroll
-        for (int e = 0; e < 8; e++) x[e] = src[8 * lane + e];
-        kv4_store8<NG>(x, kv4_block(a.cache, a.n_blocks, head, pos / KV4_BLOCK, HD), pos % KV4_BLOCK, lane >> 2, lane & 3, warp == 1,
-                       4 * NG == 32 ? 0xFFFFFFFFu : (1u << (4 * NG)) - 1u);
-    }
-    __syncthreads();
-    for (int g = 0; g < G; g++) {
-        float m_run = -INFINITY, l_run = 0.f, acc[NG];
-#pragma unroll
-        for (int j = 0; j < NG; j++) acc[j] = 0.f;
-        for (int p = first + warp; p <= pos; p += AK_WARPS) {
-            const uint8_t *blk = kv4_block(a.cache, a.n_blocks, head, p / KV4_BLOCK, HD);
-            const int row = p % KV4_BLOCK;
-            const uint32_t *kc = (const uint32_t *)(blk + row * half);
-            const uint16_t *vc = (const uint16_t *)(blk + 20 * HD + row * half);
-            const __half *kp = (const __half *)(blk + 16 * HD) + row * 2 * NG, *vp = (const __half *)(blk + 36 * HD) + row * 2 * NG;
-            float s = 0.f;
-#pragma unroll
-            for (int j = 0; j < NG; j++) {
-                const float c = (float)((kc[(lane >> 3) * NG + j] >> (4 * (lane & 7))) & 15u);
-                s = fmaf(fmaf(__half2float(kp[NG + j]), c, __half2float(kp[j])), qs[g * HD + 32 * j + lane], s);
-            }
-            s = warp_sum(s) * a.scale;
-            const float m_new = fmaxf(m_run, s), corr = m_run == m_new ? 1.f : expf(m_run - m_new), w = expf(s - m_new);
-            l_run = l_run * corr + w;
-#pragma unroll
-            for (int j = 0; j < NG; j++) {
-                const float c = (float)((vc[(lane >> 2) * NG + j] >> (4 * (lane & 3))) & 15u);
-                acc[j] = fmaf(w, fmaf(__half2float(vp[NG + j]), c, __half2float(vp[j])), acc[j] * corr);
-            }
-            m_run = m_new;
-        }
-        if (lane == 0) {
-            part[warp][HD] = m_run;
-            part[warp][HD + 1] = l_run;
-        }
-#pragma unroll
-        for (int j = 0; j < NG; j++) part[warp][32 * j + lane] = acc[j];
-        __syncthreads();
-        const int h = head * G + g;
-        float top = a.sinks ? a.sinks[h] : -INFINITY;
-        for (int w = 0; w < AK_WARPS; w++) top = fmaxf(top, part[w][HD]);
-        float total = a.sinks ? expf(a.sinks[h] - top) : 0.f;
-        for (int w = 0; w < AK_WARPS; w++) total += part[w][HD + 1] * expf(part[w][HD] - top);
-        for (int d = threadIdx.x; d < HD; d += AK_THREADS) {
-            float o = 0.f;
-            for (int w = 0; w < AK_WARPS; w++) o = fmaf(part[w][d], expf(part[w][HD] - top), o);
-            o /= total;
-            a.out[((size_t)tok * a.n_heads + h) * HD + d] = o;
-            qs[g * HD + d] = o;   // (this head's query is no longer read)
-        }
-        __syncthreads();
-    }
-    if (a.emit_q) {
-        for (int e = warp * 128; e < G * HD; e += AK_WARPS * 128) {
-            const int i = e + 4 * lane;
-            const bool valid = i < G * HD;
-            float v[4] = {0.f, 0.f, 0.f, 0.f};
-            for (int j = 0; j < 4 && valid; j++) v[j] = qs[i + j];
-            quantize4_store(v, (head * G * HD + i) >> 2, valid, a.o);
-        }
-    }
-}
 
 // ---- one token ---------------------------------------------------------------------------------------------------
 // One launch whose shape does not depend on the position.  A unit is a kv head (two units when more than eight query heads
@@ -565,6 +464,7 @@ __global__ void __launch_bounds__(AK_THREADS, NT == 1 ? 2 : 1) attn_step_kv4_ker
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int unit = blockIdx.x / CL / a.clusters, nth = blockIdx.x / CL - unit * a.clusters;   // which cluster of its unit
     const int kvh = unit / a.splits, split = unit - kvh * a.splits;
+    const int tok = blockIdx.y;
     const int h_lo = kvh * G + split * GV, n_h = min(GV, G - split * GV);   // this cluster's query heads
     uint8_t *ring = smem + at.ring + warp * (STAGES * BB);
     uint64_t *bar = (uint64_t *)(smem + at.bar) + warp * STAGES;
@@ -600,7 +500,7 @@ __global__ void __launch_bounds__(AK_THREADS, NT == 1 ? 2 : 1) attn_step_kv4_ker
     }
     pdl_trigger();
     pdl_wait();
-    const int pos = place(a.step ? __ldcg(a.step + 1) : a.pos, first, b0, n_blk);
+    const int pos = place(a.step ? __ldcg(a.step + 1) : a.pos + tok, first, b0, n_blk);
     const int NC = at_work(n_blk), R = CL * NC, cta = nth * CL + rank;
     if (nth >= NC) {
         cluster_wait();
@@ -650,7 +550,7 @@ __global__ void __launch_bounds__(AK_THREADS, NT == 1 ? 2 : 1) attn_step_kv4_ker
     for (int h = warp; h < 4 * NT; h += AK_WARPS) {
         float x[NG], top = 0.f;
         if (h < n_h) {
-            rotated(a.q + (size_t)(h_lo + h) * HD);
+            rotated(a.q + ((size_t)tok * a.n_heads + h_lo + h) * HD);
 #pragma unroll
             for (int j = 0; j < NG; j++) {
                 x[j] = rot[32 * j + lane] * (a.scale * 1.44269504f);
@@ -800,11 +700,12 @@ __global__ void __launch_bounds__(AK_THREADS, NT == 1 ? 2 : 1) attn_step_kv4_ker
             o = fmaf(src[34 * c + 2 + lane], f, o);
         }
         if (NC > 1) {
-            float *ws = a.workspace + AK_COUNTERS + (size_t)(unit * 32 + e) * a.clusters * 34;
+            const int run = (tok * a.n_kv * a.splits + unit) * 32 + e;
+            float *ws = a.workspace + AK_COUNTERS + (size_t)run * a.clusters * 34;
             __stcg(ws + nth * 34 + 2 + lane, o);
             if (lane < 2) __stcg(ws + nth * 34 + lane, lane ? l : top);
             __syncwarp();
-            int *count = (int *)a.workspace + unit * 32 + e;
+            int *count = (int *)a.workspace + run;
             int before = 0;
             // releases the warp's stores (ordered before it by the warp barrier), acquires the other clusters'
             if (lane == 0) asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(before) : "l"(count) : "memory");
@@ -827,7 +728,7 @@ __global__ void __launch_bounds__(AK_THREADS, NT == 1 ? 2 : 1) attn_step_kv4_ker
         }
         const float r = o / l;
         const int first_out = head * HD + 32 * (e % NG);
-        a.out[first_out + lane] = r;
+        a.out[(size_t)tok * a.n_heads * HD + first_out + lane] = r;
         if (a.emit_q) {
             float v[4];
 #pragma unroll

@@ -1,6 +1,7 @@
 // C entry points of the 4-bit KV cache and of the attention over it.
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <memory>
 #include <vector>
 
@@ -144,6 +145,27 @@ void by_groups(int head_dim, F f)
     }
 }
 
+// The step kernel for n_tok tokens at consecutive positions.
+void launch_step(AttnKv4Args &a, int n_tok, int head_dim)
+{
+    const int G = a.n_heads / a.n_kv;
+    a.splits = (G + 7) / 8;
+    a.prefetch = pdl_enabled() && a.step;
+    a.status = status_word_if_ready();
+    const int GV = (G + a.splits - 1) / a.splits, units = a.n_kv * a.splits;
+    by_groups(head_dim, [&](auto ng) {
+        auto go = [&](auto nt) {
+            StepShape s = step_shape<ng.value, nt.value>(units * n_tok, a.n_blocks, GV);
+            if (s.clusters > 1 && !(a.workspace = merge_workspace())) s.clusters = 1;
+            a.clusters = s.clusters;
+            launch_cluster(attn_step_kv4_kernel<ng.value, nt.value>, dim3(units * s.clusters * s.cl, n_tok), dim3(AK_THREADS),
+                           (size_t)attn_kv4_smem(ng.value, nt.value, GV, s.cl).total, s.cl, a);
+        };
+        if (GV <= 4) go(std::integral_constant<int, 1>());
+        else go(std::integral_constant<int, 2>());
+    });
+}
+
 }  // namespace
 
 extern "C" {
@@ -233,22 +255,7 @@ void cuda_attn_step_kv4(float *out, const float *q, const float *k_new, const fl
         if (!activation_slot(out_slot, n_heads * head_dim, &a.o)) return;
         a.emit_q = 1;
     }
-    const int G = n_heads / n_kv_heads;
-    a.splits = (G + 7) / 8;
-    a.prefetch = pdl_enabled() && d_step;
-    a.status = status_word_if_ready();
-    const int GV = (G + a.splits - 1) / a.splits, units = n_kv_heads * a.splits;
-    by_groups(head_dim, [&](auto ng) {
-        auto go = [&](auto nt) {
-            StepShape s = step_shape<ng.value, nt.value>(units, a.n_blocks, GV);
-            if (s.clusters > 1 && !(a.workspace = merge_workspace())) s.clusters = 1;
-            a.clusters = s.clusters;
-            launch_cluster(attn_step_kv4_kernel<ng.value, nt.value>, dim3(units * s.clusters * s.cl), dim3(AK_THREADS),
-                           (size_t)attn_kv4_smem(ng.value, nt.value, GV, s.cl).total, s.cl, a);
-        };
-        if (GV <= 4) go(std::integral_constant<int, 1>());
-        else go(std::integral_constant<int, 2>());
-    });
+    launch_step(a, 1, head_dim);
 }
 
 void cuda_attn_prompt_kv4(float *out, const float *q, const void *d_cache, int n_tok, int n_heads, int n_kv_heads, int head_dim, int max_seq,
@@ -263,7 +270,20 @@ void cuda_attn_prompt_kv4(float *out, const float *q, const void *d_cache, int n
         refuse("cuda_attn_prompt_kv4: out and q must be 16-byte aligned device pointers");
         return;
     }
-    AttnPromptKv4Args a = {out, q, (const uint8_t *)d_cache, n_tok, n_heads, n_kv_heads, kv4_blocks(max_seq), pos0, window, UMMA_M / (n_heads / n_kv_heads),
+    // A few tokens on a long cache leave the prompt kernel, one CTA per kv head and 128 rows, with most SMs idle: there
+    // the step kernel takes them one by one, all in one launch.  Time of either in us, fitted to measurements (32 / 8 heads
+    // of 128; step: 16 tokens at 1000 12.6, 64 at 1000 35, 16 at 16000 89; prompt: 128 at 1000 40, 512 at 0 26, 512 at
+    // 16000 393): a wave of units and 3.7 TB/s of cache once per token, or 1.6 per 64 positions and wave of CTAs.
+    const int G = n_heads / n_kv_heads, ctas = n_kv_heads * ((n_tok + UMMA_M / G - 1) / (UMMA_M / G)), units = n_kv_heads * ((G + 7) / 8) * n_tok;
+    const double seen = window > 0 ? std::min(window, pos0 + n_tok) : pos0 + n_tok;
+    const double by_step = 2 + 4.5 * std::ceil(units / (2.0 * sm_count())) + n_tok * seen * n_kv_heads * head_dim * 1.25 / 3.7e6;
+    const double by_prompt = 9 + 1.6 * (seen / APK_BN + 1) * std::ceil(ctas / (double)sm_count());
+    if (by_step < by_prompt) {
+        AttnKv4Args s = {out, q, nullptr, nullptr, (uint8_t *)d_cache, nullptr, pos0, n_heads, n_kv_heads, max_seq, kv4_blocks(max_seq), window, scale, sinks};
+        launch_step(s, n_tok, head_dim);
+        return;
+    }
+    AttnPromptKv4Args a = {out, q, (const uint8_t *)d_cache, n_tok, n_heads, n_kv_heads, kv4_blocks(max_seq), pos0, window, UMMA_M / G,
                            scale, sinks, status_word_if_ready()};
     by_groups(head_dim, [&](auto ng) {
         static bool ready = false;

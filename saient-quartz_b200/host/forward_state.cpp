@@ -104,7 +104,11 @@ struct qh_model {
     // scratch (src/cuda.rs:312-354)
     GpuBuf d_hidden, d_norm_out, d_q, d_k, d_v, d_attn_out, d_scores, d_gate, d_up, d_expert_out, d_expert_acc;
     GpuBuf d_gate_all, d_up_all, d_expert_out_all, d_down_all, d_router_logits, d_logits;
-    std::vector<GpuBuf> kv_k, kv_v;
+    std::vector<GpuBuf> kv_k, kv_v;   // f32 caches, or
+    std::vector<GpuBuf> kv4;          // 4-bit ones (keys and values of a layer in one buffer)
+    int kv_bits = 0;                  // 0: nobody chose yet
+    GpuBuf g_u, g_tok;                // random numbers and tokens of a generation loop
+    int g_cap = 0;
     bool finalized = false;
     long long last_launches = 0;
     int n_recorded = 0;        // graph recordings made so far
@@ -208,11 +212,18 @@ int qh_finalize(qh_model *m)
     if (!ok) return -2;
     // the (cos, sin) table of a step's position is written together with the step words
     cuda_step_rope_table((int *)m->d_step.ptr, c.head_dim, c.rope_theta, c.yarn_scale, c.yarn_orig_ctx);
+    const char *bits = getenv("QUARTZ_KV_BITS");
+    if (m->kv_bits == 0) m->kv_bits = bits && atoi(bits) == 4 && cuda_attn_kv4_supported(nh, c.n_kv_heads, c.head_dim) ? 4 : 32;
     m->kv_k.resize(c.n_layers);
     m->kv_v.resize(c.n_layers);
+    m->kv4.resize(c.n_layers);
     std::vector<float> zeros(std::max(q_d, kv_d), 0.f), no_sink(nh, -INFINITY);
     for (int l = 0; l < c.n_layers; l++) {
-        if (!m->kv_k[l].alloc_f32(mseq * kv_d) || !m->kv_v[l].alloc_f32(mseq * kv_d)) return -3;
+        if (m->kv_bits == 4) {
+            if (!m->kv4[l].alloc_f32((cuda_kv4_bytes(c.max_seq, c.n_kv_heads, c.head_dim) + 3) / 4)) return -3;
+        } else if (!m->kv_k[l].alloc_f32(mseq * kv_d) || !m->kv_v[l].alloc_f32(mseq * kv_d)) {
+            return -3;
+        }
         Layer &L = m->L[l];
         // absent q/k/v biases are uploaded as zero vectors and added anyway (src/main.rs:366-368)
         if (L.q_bias.empty()) L.q_bias.upload(zeros.data(), (size_t)q_d * 4);
@@ -225,9 +236,26 @@ int qh_finalize(qh_model *m)
     return quartz_last_error() == 0 ? 0 : -4;
 }
 
+int qh_set_kv_bits(qh_model *m, int bits)
+{
+    if (!m || m->finalized || (bits != 32 && bits != 4)) return -1;
+    if (bits == 4 && !cuda_attn_kv4_supported(m->c.n_heads, m->c.n_kv_heads, m->c.head_dim)) return -2;
+    m->kv_bits = bits;
+    return 0;
+}
+
+int qh_kv_bits(qh_model *m) { return m ? m->kv_bits : 0; }
+
 int qh_set_kv(qh_model *m, int layer, const float *k, const float *v, int n_pos)
 {
     if (!m || !m->finalized || layer < 0 || layer >= m->c.n_layers || n_pos > m->c.max_seq) return -1;
+    if (m->kv_bits == 4) {   // quantised as they are written
+        GpuBuf dk, dv;
+        if (n_pos < 0 || !dk.upload(k, (size_t)n_pos * m->kv_d() * 4) || !dv.upload(v, (size_t)n_pos * m->kv_d() * 4)) return -2;
+        cuda_kv4_append_rows(m->kv4[layer].ptr, dk.f(), dv.f(), n_pos, m->c.n_kv_heads, m->c.head_dim, m->c.max_seq, 0);
+        cuda_sync();
+        return quartz_last_error() == 0 ? 0 : -10;
+    }
     cuda_h2d(m->kv_k[layer].ptr, k, (size_t)n_pos * m->kv_d() * 4);
     cuda_h2d(m->kv_v[layer].ptr, v, (size_t)n_pos * m->kv_d() * 4);
     return 0;
@@ -237,6 +265,17 @@ int qh_get_kv(qh_model *m, int layer, float *k, float *v, int pos0, int n_pos)
 {
     if (!m || !m->finalized || layer < 0 || layer >= m->c.n_layers || pos0 < 0 || n_pos < 0 || pos0 + n_pos > m->c.max_seq) return -1;
     const size_t off = (size_t)pos0 * m->kv_d() * 4, bytes = (size_t)n_pos * m->kv_d() * 4;
+    if (m->kv_bits == 4) {
+        GpuBuf dk, dv;
+        if (!dk.alloc_f32(bytes / 4) || !dv.alloc_f32(bytes / 4)) return -2;
+        cuda_kv4_read_rows(dk.f(), dv.f(), m->kv4[layer].ptr, n_pos, m->c.n_kv_heads, m->c.head_dim, m->c.max_seq, pos0);
+        if (bytes) {
+            cuda_d2h(k, dk.ptr, bytes);
+            cuda_d2h(v, dv.ptr, bytes);
+        }
+        cuda_sync();
+        return quartz_last_error() == 0 ? 0 : -10;
+    }
     cuda_d2h(k, (const uint8_t *)m->kv_k[layer].ptr + off, bytes);
     cuda_d2h(v, (const uint8_t *)m->kv_v[layer].ptr + off, bytes);
     cuda_sync();
@@ -248,6 +287,9 @@ static int attn_start(const qh_config &c, int layer, int pos)   // src/main.rs:2
     if (c.swa_window > 0 && layer % 2 == 0) return std::max(0, pos + 1 - c.swa_window);
     return 0;
 }
+
+// Sliding-window layers (src/main.rs:231-237): the window the attention kernel applies on the device.
+static int attn_window(const qh_config &c, int layer) { return (c.swa_window > 0 && layer % 2 == 0) ? c.swa_window : 0; }
 
 static float attn_scale(const qh_config &c)   // src/cuda.rs:532-536
 {
@@ -430,12 +472,17 @@ static void step_reference(qh_model *m, int token, int pos, bool need_logits)
         }
         cuda_rope_yarn(m->d_q.f(), h, hd, pos, c.rope_theta, c.yarn_scale, c.yarn_orig_ctx, c.rope_neox);
         cuda_rope_yarn(m->d_k.f(), kv, hd, pos, c.rope_theta, c.yarn_scale, c.yarn_orig_ctx, c.rope_neox);
-        cuda_kv_append(m->kv_k[l].f(), m->kv_v[l].f(), m->d_k.f(), m->d_v.f(), pos, kv_d);
-        const int k_start = attn_start(c, l, pos), seq_a = seq - k_start;
-        const float *kc = m->kv_k[l].f() + (size_t)k_start * kv_d, *vc = m->kv_v[l].f() + (size_t)k_start * kv_d;
-        cuda_attn_score_all(m->d_scores.f(), m->d_q.f(), kc, h, kv, seq_a, hd, kv_d, c.max_seq, scale);
-        cuda_softmax_sink_all(m->d_scores.f(), h, seq_a, c.max_seq, L.sinks.f());
-        cuda_attn_values_all(m->d_attn_out.f(), m->d_scores.f(), vc, h, kv, seq_a, hd, kv_d, c.max_seq);
+        if (m->kv_bits == 4) {   // q and k are rotated: theta 0
+            cuda_attn_step_kv4(m->d_attn_out.f(), m->d_q.f(), m->d_k.f(), m->d_v.f(), m->kv4[l].ptr, h, kv, hd, c.max_seq, nullptr, pos,
+                               attn_window(c, l), scale, L.sinks.f(), 0.f, 1.f, 0, 0, -1);
+        } else {
+            cuda_kv_append(m->kv_k[l].f(), m->kv_v[l].f(), m->d_k.f(), m->d_v.f(), pos, kv_d);
+            const int k_start = attn_start(c, l, pos), seq_a = seq - k_start;
+            const float *kc = m->kv_k[l].f() + (size_t)k_start * kv_d, *vc = m->kv_v[l].f() + (size_t)k_start * kv_d;
+            cuda_attn_score_all(m->d_scores.f(), m->d_q.f(), kc, h, kv, seq_a, hd, kv_d, c.max_seq, scale);
+            cuda_softmax_sink_all(m->d_scores.f(), h, seq_a, c.max_seq, L.sinks.f());
+            cuda_attn_values_all(m->d_attn_out.f(), m->d_scores.f(), vc, h, kv, seq_a, hd, kv_d, c.max_seq);
+        }
         cuda_gemv(L.o.ggml_type, L.o.u8(), m->d_attn_out.f(), m->d_norm_out.f(), q_d, d);
         if (!L.o_bias.empty()) cuda_vec_add(m->d_norm_out.f(), L.o_bias.f(), d);
         cuda_vec_add(m->d_hidden.f(), m->d_norm_out.f(), d);
@@ -477,14 +524,17 @@ static bool fusable(qh_model *m)
     return cuda_gemv_q_supported(m->lm_head.ggml_type, m->lm_head.u8(), c.embed_dim) != 0;
 }
 
-// Sliding-window layers (src/main.rs:231-237): the window the attention kernel applies on the device.
-static int attn_window(const qh_config &c, int layer) { return (c.swa_window > 0 && layer % 2 == 0) ? c.swa_window : 0; }
-
 // The attention block of layer l as one launch; token position comes from the device step words.
 static void attn_layer(qh_model *m, int l, int out_slot)
 {
     const qh_config &c = m->c;
     Layer &L = m->L[l];
+    if (m->kv_bits == 4) {
+        cuda_attn_step_kv4(m->d_attn_out.f(), m->d_q.f(), m->d_k.f(), m->d_v.f(), m->kv4[l].ptr, c.n_heads, c.n_kv_heads, c.head_dim, c.max_seq,
+                           (const int *)m->d_step.ptr, 0, attn_window(c, l), attn_scale(c), L.sinks.f(), c.rope_theta, c.yarn_scale,
+                           c.yarn_orig_ctx, c.rope_neox, out_slot);
+        return;
+    }
     cuda_attn_step(m->d_attn_out.f(), m->d_q.f(), m->d_k.f(), m->d_v.f(), m->kv_k[l].f(), m->kv_v[l].f(), c.n_heads,
                    c.n_kv_heads, c.head_dim, c.max_seq, (const int *)m->d_step.ptr, 0, attn_window(c, l), attn_scale(c),
                    L.sinks.f(), c.rope_theta, c.yarn_scale, c.yarn_orig_ctx, c.rope_neox, out_slot);
@@ -722,9 +772,14 @@ int qh_prefill(qh_model *m, const int *tokens, int n, int pos0, float *logits_ho
         cuda_gemm(L.q.ggml_type, L.q.u8(), Xn, Q, n, d, q_d);
         cuda_gemm(L.k.ggml_type, L.k.u8(), Xn, K, n, d, kv_d);
         cuda_gemm(L.v.ggml_type, L.v.u8(), Xn, V, n, d, kv_d);
-        cuda_rope_kv_rows(Q, K, V, m->kv_k[l].f(), m->kv_v[l].f(), n, h, kv, hd, pos0, c.rope_theta, c.yarn_scale, c.yarn_orig_ctx,
-                          c.rope_neox);
-        cuda_attn_prompt(A, Q, m->kv_k[l].f(), m->kv_v[l].f(), n, h, kv, hd, c.max_seq, pos0, attn_window(c, l), scale, L.sinks.f());
+        if (m->kv_bits == 4) {
+            cuda_rope_kv4_rows(Q, K, V, m->kv4[l].ptr, n, h, kv, hd, c.max_seq, pos0, c.rope_theta, c.yarn_scale, c.yarn_orig_ctx, c.rope_neox);
+            cuda_attn_prompt_kv4(A, Q, m->kv4[l].ptr, n, h, kv, hd, c.max_seq, pos0, attn_window(c, l), scale, L.sinks.f());
+        } else {
+            cuda_rope_kv_rows(Q, K, V, m->kv_k[l].f(), m->kv_v[l].f(), n, h, kv, hd, pos0, c.rope_theta, c.yarn_scale, c.yarn_orig_ctx,
+                              c.rope_neox);
+            cuda_attn_prompt(A, Q, m->kv_k[l].f(), m->kv_v[l].f(), n, h, kv, hd, c.max_seq, pos0, attn_window(c, l), scale, L.sinks.f());
+        }
         cuda_gemm(L.o.ggml_type, L.o.u8(), A, Xn, n, q_d, d);
         cuda_vec_add(X, Xn, n * d);
         cuda_rms_norm_rows(Xn, X, L.ffn_norm.f(), n, d);
@@ -750,6 +805,42 @@ int qh_prefill(qh_model *m, const int *tokens, int n, int pos0, float *logits_ho
     cuda_rms_norm(m->d_norm_out.f(), X + (size_t)(n - 1) * d, m->final_norm.f(), d);
     cuda_gemv(m->lm_head.ggml_type, m->lm_head.u8(), m->d_norm_out.f(), m->d_logits.f(), d, c.vocab_size);
     if (logits_host) cuda_d2h(logits_host, m->d_logits.ptr, (size_t)c.vocab_size * 4);
+    cuda_sync();
+    return quartz_last_error() == 0 ? 0 : -10;
+}
+
+int qh_generate(qh_model *m, int token, int pos, int n, float temperature, int top_k, float top_p, float min_p, const float *u,
+                int *tokens_out)
+{
+    if (!m || !m->finalized || !tokens_out || n <= 0 || pos < 0 || (long long)pos + n > m->c.max_seq || token < 0 || token >= m->c.vocab_size ||
+        (!u && temperature > 0.f))
+        return -1;
+    if (n > m->g_cap) {
+        if (!m->g_u.alloc_f32(n) || !m->g_tok.alloc_f32(n)) return -2;
+        m->g_cap = n;
+    }
+    if (u) cuda_h2d(m->g_u.ptr, u, (size_t)n * 4);
+    const bool on_device = fusable(m);
+    const int V = m->c.vocab_size;
+    int *tok = (int *)m->g_tok.ptr;
+    for (int i = 0; i < n; i++) {
+        if (i == 0 || !on_device) {
+            const int rc = qh_step_device(m, token, pos + i, 1);
+            if (rc) return rc;
+        } else {
+            quartz_graph_launch(m->graphs[1]);   // token and position are in the step words
+        }
+        cuda_sample(m->d_logits.f(), 1, V, (size_t)V, temperature, top_k, top_p, min_p, u ? m->g_u.f() + i : nullptr, tok + i, nullptr);
+        if (i + 1 == n) break;
+        if (on_device) {
+            cuda_step_advance((int *)m->d_step.ptr, tok + i);
+        } else {
+            int next = -1;
+            cuda_d2h(&next, tok + i, 4);
+            if (next >= 0) token = next;   // (a row without a token keeps the last one, as the step words do)
+        }
+    }
+    cuda_d2h(tokens_out, tok, (size_t)n * 4);
     cuda_sync();
     return quartz_last_error() == 0 ? 0 : -10;
 }

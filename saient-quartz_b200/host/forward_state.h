@@ -55,6 +55,11 @@ const char *qh_load_error(void);
 void qh_destroy(qh_model *m);
 /* upload one tensor (raw GGUF bytes, or f32 for norms/biases/router); repack=1 calls the repack hook */
 int qh_set_tensor(qh_model *m, int role, int layer, uint32_t ggml_type, const void *host, size_t bytes, int repack);
+/* The KV cache's precision, before qh_finalize: 32 (f32, default, as the reference) or 4 (cuda_kv4_*: 5 bits a value with its
+ * group's parameters, 6.4 times smaller; head_dim 32, 64, 96 or 128, at most 16 query heads per kv head).  0 on success.
+ * QUARTZ_KV_BITS=4 in the environment selects 4 for models of that geometry whose host calls nothing (qh_load_gguf). */
+int qh_set_kv_bits(qh_model *m, int bits);
+int qh_kv_bits(qh_model *m);
 /* allocate scratch + KV cache, default zero biases / no sinks (src/cuda.rs:361-492) */
 int qh_finalize(qh_model *m);
 /* write n_pos rows of K and V (f32 [n_pos x kv_dim]) into layer's caches (benchmark pre-fill) */
@@ -72,6 +77,13 @@ int qh_forward_step_chained(qh_model *m, int token, int pos, int need_logits, fl
  * logits_host (may be NULL) receives the LAST token's logits.  Models with QK-norm or projection biases run token
  * by token through the decode step.  0 on success. */
 int qh_prefill(qh_model *m, const int *tokens, int n, int pos0, float *logits_host);
+/* Generate n tokens: step at (token, pos), choose the next token from its logits (cuda_sample with the random number
+ * u[i], uniform in [0, 1), and the given settings), step with it at pos + 1, ...  Where the fused sequence serves the model
+ * the whole loop runs on the device -- sampled token and position go from one step to the next as device words
+ * (cuda_step_advance) -- and the host waits once, for tokens_out[0..n); otherwise it reads every token back.  The last
+ * token is chosen, not stepped: pos + n <= max_seq.  u may be NULL at temperature 0.  0 on success. */
+int qh_generate(qh_model *m, int token, int pos, int n, float temperature, int top_k, float top_p, float min_p, const float *u,
+                int *tokens_out);
 /* device-only variants for timing: no copies, the result stays in the device logits buffer; fused: 0 reference
  * sequence, 1 fused, 2 chained */
 int qh_step_device(qh_model *m, int token, int pos, int fused);

@@ -50,6 +50,9 @@ def host_lib():
         H.qh_graphs_recorded.argtypes = [C.c_void_p]
         H.qh_force_host_router.argtypes = [C.c_int]
         H.qh_prefill.argtypes = [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_void_p]
+        H.qh_set_kv_bits.argtypes = [C.c_void_p, C.c_int]
+        H.qh_kv_bits.argtypes = [C.c_void_p]
+        H.qh_generate.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_float, C.c_int, C.c_float, C.c_float, C.c_void_p, C.c_void_p]
         H.qh_get_kv.argtypes = [C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_int]
         _host = H
     return _host
@@ -65,7 +68,7 @@ Q4K_M_TYPES = dict(Q=12, K=12, V=12, O=12, GATE=12, UP=12, DOWN=14, LM_HEAD=14, 
 class HostModel:
     """A model resident on the GPU, driven through the C++ host mirror."""
 
-    def __init__(self, repack=True, types=Q4K_M_TYPES, seed=synth.DEFAULT_SEED, keep_host=False, **cfg):
+    def __init__(self, repack=True, types=Q4K_M_TYPES, seed=synth.DEFAULT_SEED, keep_host=False, kv_bits=32, **cfg):
         from . import ensure_iq_grids
         ensure_iq_grids()
         self.H = host_lib()
@@ -77,6 +80,8 @@ class HostModel:
         self.m = self.H.qh_create(C.byref(self.c))
         if not self.m:
             raise RuntimeError("qh_create failed")
+        if kv_bits != 32 and self.H.qh_set_kv_bits(self.m, kv_bits) != 0:
+            raise ValueError(f"qh_set_kv_bits: {kv_bits} bits are not served for this head geometry")
         self.types = dict(types)
         self.host = {} if keep_host else None
         self.repack = repack
@@ -173,6 +178,18 @@ class HostModel:
             from . import lib
             raise RuntimeError(f"prefill failed: {rc} ({lib().quartz_error_string().decode()})")
         return logits
+
+    def generate(self, token, pos, n, temperature=0.0, top_k=0, top_p=1.0, min_p=0.0, u=None):
+        """n tokens after (token, pos), chosen on the device (qh_generate); u: n random numbers in [0, 1)."""
+        out = np.empty(n, dtype=np.int32)
+        u = None if u is None else np.ascontiguousarray(u, dtype=np.float32)
+        if u is not None and u.size < n:
+            raise ValueError("generate: one random number per token")
+        rc = self.H.qh_generate(self.m, token, pos, n, temperature, top_k, top_p, min_p, None if u is None else u.ctypes.data, out.ctypes.data)
+        if rc != 0:
+            from . import lib
+            raise RuntimeError(f"generate failed: {rc} ({lib().quartz_error_string().decode()})")
+        return out
 
     def step(self, token, pos, fused=False):
         logits = np.empty(self.cfg["vocab_size"], dtype=np.float32)
