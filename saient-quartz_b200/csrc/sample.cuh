@@ -62,11 +62,9 @@ struct SampleExp {
         return (u64)__double_as_longlong(w + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;   // + 2^52: rounded to a whole number
     }
 };
-// Weight of logit z in units of 2^-44
-__device__ __forceinline__ u64 smp_weight(float z, float M, float inv_t, const SampleExp &e)
-{
-    return z == M ? (u64)SMP_ONE : (z - M) * inv_t < -31.5f ? 0 : e(z);
-}
+// Weights below exp(-9) are taken in 32 bits: their errors (2e-6 of a weight, either way) average out of sums to which
+// such tokens contribute by the thousand.
+__device__ __forceinline__ u64 smp_light(float x) { return x < -31.5f ? 0 : __float2uint_rn(exp2f(x * 1.44269504f) * (float)SMP_ONE); }
 
 // ---- the kernel -------------------------------------------------------------------------------------------------
 // A cluster of CL CTAs per row; each keeps a contiguous part of the row in shared memory, read once from HBM.  Nothing is
@@ -78,7 +76,10 @@ __device__ __forceinline__ u64 smp_weight(float z, float M, float inv_t, const S
 //   4. top_p: the counts bracket the bin in which the weights reach their goal (a bin's tokens weigh the same within 1/32);
 //      one pass sums the weights above the bracket and below it, and those inside bin by bin; the tokens of the right
 //      bin are gathered and ranked.
-//   5. the kept weights are summed warp by warp in the order of the vocabulary; the warp in whose range u falls walks it.
+//   5. the kept weights are summed warp by warp in the order of the vocabulary (above the bracket step 4 did that, only
+//      tokens inside it are looked at again); the warp in whose range u falls walks its part.
+// Tokens that need more than a few instructions (64-bit weights, histogram entries) are first collected, so that a warp
+// takes 32 of them at a time.
 // A bin with more tokens than the list takes (ties, high temperatures) is divided further, by the number itself.
 // A histogram is reduced in slices, one per CTA, that are pushed to every CTA: all find the same bin without asking.
 constexpr int SMP_BINS = 2 * SMP_THREADS, SMP_LIST = 512,   // (a thread looks after two bins, and one token of the list)
@@ -96,9 +97,11 @@ struct SampleShared {
     u64 from[2][SMP_MAX_CLUSTER][3];              // what the cluster's CTAs pushed last, and before
     u64 red[SMP_WARPS];
     double exp2_16[16];
+    u64 own[2], got[SMP_MAX_CLUSTER][2];          // sums beside a histogram: this CTA's, everybody's
     u64 result;
     u64 before;
     int n_mine, n_list, at, bin;
+    uint16_t later[SMP_WARPS][64];                // tokens that a warp has put off
 };
 
 // sum, or largest, over the block; every thread gets it
@@ -132,10 +135,11 @@ __device__ __forceinline__ T smp_warp_inclusive(T v)
     }
     return v;
 }
-// sum over the threads before this one; *total over all (T of 8 bytes)
+// sum over the threads before this one; *total over all
 template <class T>
 __device__ __forceinline__ T smp_before(T v, u64 *scratch, T *total)
 {
+    static_assert(sizeof(T) <= 8, "");
     T *sm = (T *)scratch;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const T inc = smp_warp_inclusive(v);
@@ -171,7 +175,38 @@ struct Sampler {
         const float t = (M - x) * per_bin;
         return x == M ? 0 : t < (float)(SMP_BINS - 1) ? (int)t : SMP_BINS - 1;
     }
-    __device__ __forceinline__ u64 weight(float x) const { return smp_weight(x, M, inv, e); }
+    __device__ __forceinline__ float log_weight(float x) const { return x == M ? 0.f : (x - M) * inv; }
+    __device__ __forceinline__ u64 weight(float x) const
+    {
+        const float y = log_weight(x);
+        return x == M ? (u64)SMP_ONE : y < -9.f ? smp_light(y) : e(x);
+    }
+    // Calls now(i) for tokens lo + lane, lo + 32 + lane, .. below hi; what it returns true for is done by put_off(i), 32 at a time.
+    template <class Now, class PutOff>
+    __device__ __forceinline__ void sweep(int lo, int hi, Now now, PutOff put_off) const
+    {
+        const int lane = threadIdx.x & 31;
+        uint16_t *later = s.later[threadIdx.x >> 5];
+        int held = 0;
+        for (int i0 = lo; i0 < hi; i0 += 32) {
+            const int i = i0 + lane;
+            const bool more = i < hi && now(i);
+            const unsigned mask = __ballot_sync(0xFFFFFFFFu, more);
+            if (more) later[held + __popc(mask & ((1u << lane) - 1))] = (uint16_t)i;
+            held += __popc(mask);
+            if (held >= 32) {
+                __syncwarp();
+                put_off((int)later[lane]);
+                held -= 32;
+                const uint16_t rest = later[32 + lane];
+                __syncwarp();
+                later[lane] = rest;
+            }
+        }
+        __syncwarp();
+        if (lane < held) put_off((int)later[lane]);
+        __syncwarp();
+    }
     __device__ __forceinline__ u64 weight_of(u64 number) const { return weight(smp_unkey((uint32_t)(number >> 32))); }
 
     // three values of this CTA to every CTA: afterwards s.from[turn][r] holds those of CTA r (two turns' worth are kept:
@@ -196,6 +231,10 @@ struct Sampler {
         if (threadIdx.x == 0) s.bin = -1;
         __syncthreads();
     }
+    __device__ __forceinline__ void no_list()
+    {
+        if (threadIdx.x == 0) s.n_mine = s.n_list = 0;   // (the cluster meets before the next tokens arrive)
+    }
     __device__ __forceinline__ void add(int b, bool weights, u64 w)
     {
         atomicAdd(&s.cnt[b], 1u);
@@ -214,6 +253,7 @@ struct Sampler {
             for (int t = threadIdx.x; t < SMP_BINS; t += SMP_THREADS) {
                 const SampleShared *from = peer(t / per);
                 const int b = rank * per + t % per;
+                if (what && t < 2 * CL) s.got[t >> 1][t & 1] = peer(t >> 1)->own[t & 1];
                 s.slice[t] = what ? (u64)from->part[0][b] + ((u64)from->part[1][b] << 15) + ((u64)from->part[2][b] << 30) : from->cnt[b];
             }
             __syncthreads();
@@ -252,8 +292,6 @@ struct Sampler {
     template <class Pred>
     __device__ __forceinline__ void gather(Pred pred)
     {
-        if (threadIdx.x == 0) s.n_mine = s.n_list = 0;
-        sync();
         for (int i = threadIdx.x; i < n; i += SMP_THREADS)
             if (pred(i)) s.mine[atomicAdd(&s.n_mine, 1)] = number(i);
         __syncthreads();
@@ -318,6 +356,7 @@ struct Sampler {
             if ((int)threadIdx.x < CL) peer(threadIdx.x)->result = last;
         }
         sync();
+        no_list();
         return s.result;
     }
 };
@@ -340,25 +379,33 @@ __global__ void __launch_bounds__(SMP_THREADS) sample_kernel(const SampleArgs a)
     pdl_trigger();
     // ---- 1. the row into shared memory; its first token ----
     const float *src = a.logits + (size_t)row * a.ld + c.base;
+    float top = -INFINITY;
+    int at = -1;
+    auto take = [&](float x, int i) {   // (in rising order of i: the first of equals stays)
+        z[i] = x;
+        if (x > top) {
+            top = x;
+            at = i;
+        }
+    };
     if (((uintptr_t)src & 15) == 0) {
-        for (int i = tid; i < n / 4; i += SMP_THREADS) ((float4 *)z)[i] = __ldcs((const float4 *)src + i);
-        if (tid < (n & 3)) z[(n & ~3) + tid] = src[(n & ~3) + tid];
+#pragma unroll 4
+        for (int i = tid; i < n / 4; i += SMP_THREADS) {
+            const float4 v = __ldcs((const float4 *)src + i);
+            take(v.x, 4 * i);
+            take(v.y, 4 * i + 1);
+            take(v.z, 4 * i + 2);
+            take(v.w, 4 * i + 3);
+        }
+        if (tid < (n & 3)) take(src[(n & ~3) + tid], (n & ~3) + tid);
     } else {
-        for (int i = tid; i < n; i += SMP_THREADS) z[i] = __ldcs(src + i);
+#pragma unroll 4
+        for (int i = tid; i < n; i += SMP_THREADS) take(__ldcs(src + i), i);
     }
     if (tid < 16) s.exp2_16[tid] = exp2((double)tid / 16.0);
+    c.no_list();
     c.clear(false);   // (synchronises)
-    u64 best = 0;
-    {
-        float top = -INFINITY;
-        int at = -1;
-        for (int i = tid; i < n; i += SMP_THREADS)
-            if (z[i] > top) {
-                top = z[i];
-                at = i;
-            }
-        if (at >= 0) best = c.number(at);
-    }
+    u64 best = at >= 0 ? c.number(at) : 0;
     best = smp_reduce<true>(best, s.red);
     c.exchange(best, 0, 0);
     for (int r = 0; r < c.CL; r++) best = max(best, s.from[c.turn][r][0]);
@@ -429,6 +476,9 @@ __global__ void __launch_bounds__(SMP_THREADS) sample_kernel(const SampleArgs a)
         }
         c.keep_to(c.last_in_bin(b, in_bin, before, (double)a.top_k, false));
     }
+    const int seg = ((n + SMP_WARPS - 1) / SMP_WARPS + 31) & ~31, lo = min(n, warp * seg), hi = min(n, lo + seg);   // this warp's part
+    int first = 0, last = -1;
+    u64 above_here = 0;   // weights above the bracket that this lane has summed
     if (by_p) {
         // ---- 4. top_p ----
         if (by_k) {   // the counts of the set (last_in_bin may have used the histogram)
@@ -437,43 +487,57 @@ __global__ void __launch_bounds__(SMP_THREADS) sample_kernel(const SampleArgs a)
                 if (c.in_set(i)) c.add(c.bin(z[i]), false, 0);
             c.collect(false);
         }
-        // a token of bin b weighs between exp(-(b + 1) / 32) and exp(-b / 32); 1e-4 covers the rounding of its bin
-        double most[2], least[2], most_all, least_all;
+        // a token of bin b weighs between exp(-(b + 1) / 32) and exp(-b / 32); 1e-3 covers the rounding of its bin and of these sums
+        float most[2], least[2], most_all, least_all;
         for (int k = 0; k < 2; k++) {
             const int b = 2 * tid + k;
-            const double count = (double)s.all_cnt[b];
-            most[k] = count * exp(-(double)b / 32.0) * 1.0001;
-            least[k] = b < SMP_BINS - 1 ? count * exp(-(double)(b + 1) / 32.0) * 0.9999 : 0.0;
+            const float count = (float)s.all_cnt[b];
+            most[k] = count * expf(-(float)b / 32.f) * 1.001f;
+            least[k] = b < SMP_BINS - 1 ? count * expf(-(float)(b + 1) / 32.f) * 0.999f : 0.f;
         }
-        double most_before = smp_before(most[0] + most[1], s.red, &most_all), least_before = smp_before(least[0] + least[1], s.red, &least_all);
+        float most_before = smp_before(most[0] + most[1], s.red, &most_all), least_before = smp_before(least[0] + least[1], s.red, &least_all);
         // the first bin that may hold the border is the last with most_before < goal, the last one the first with least up to it >= goal
-        int first = 0, from_end = 0;
+        int from_end = 0;
+        first = 0;
         for (int k = 0; k < 2; k++) {
-            if (most_before < (double)a.top_p * least_all) first = 2 * tid + k;
+            if (most_before < a.top_p * least_all) first = 2 * tid + k;
             least_before += least[k];
-            if (least_before >= (double)a.top_p * most_all) from_end = max(from_end, SMP_BINS - 1 - (2 * tid + k));
+            if (least_before >= a.top_p * most_all) from_end = max(from_end, SMP_BINS - 1 - (2 * tid + k));
             most_before += most[k];
         }
         first = (int)smp_reduce<true>((u64)first, s.red);
-        const int last = SMP_BINS - 1 - (int)smp_reduce<true>((u64)from_end, s.red);
+        last = SMP_BINS - 1 - (int)smp_reduce<true>((u64)from_end, s.red);
         c.clear(true);
         u64 above = 0, below = 0;
-        for (int i = tid; i < n; i += SMP_THREADS) {
+        c.sweep(lo, hi, [&](int i) {
+            const float x = z[i], y = c.log_weight(x);
+            const int b = c.bin(x);
+            const bool light = y < -9.f, inside = b >= first && b <= last, in = c.in_set(i);
+            if (in && light && !inside) {
+                if (b < first) above += smp_light(y);
+                else below += smp_light(y);
+            }
+            return in && (!light || inside);
+        }, [&](int i) {
             const int b = c.bin(z[i]);
-            const u64 w = c.in_set(i) ? c.weight(z[i]) : 0;   // (one evaluation for the three cases)
+            const u64 w = c.weight(z[i]);
             if (b < first) above += w;
             else if (b > last) below += w;
-            else if (c.in_set(i)) c.add(b, true, w);
-        }
+            else c.add(b, true, w);
+        });
+        above_here = above;
         above = smp_reduce<false>(above, s.red);
         below = smp_reduce<false>(below, s.red);
-        c.exchange(above, below, 0);
-        above = below = 0;
-        for (int r = 0; r < c.CL; r++) {
-            above += s.from[c.turn][r][0];
-            below += s.from[c.turn][r][1];
+        if (tid == 0) {
+            s.own[0] = above;
+            s.own[1] = below;
         }
         c.collect(true);
+        above = below = 0;
+        for (int r = 0; r < c.CL; r++) {
+            above += s.got[r][0];
+            below += s.got[r][1];
+        }
         u64 inside;
         smp_before(s.all_w[2 * tid] + s.all_w[2 * tid + 1], s.red, &inside);
         const double goal = (double)a.top_p * (double)(above + inside + below);
@@ -482,10 +546,21 @@ __global__ void __launch_bounds__(SMP_THREADS) sample_kernel(const SampleArgs a)
         if (b >= 0) c.keep_to(c.last_in_bin(b, s.all_cnt[b], before, goal, true));
     }
     // ---- 5. the token ----
-    const int seg = ((n + SMP_WARPS - 1) / SMP_WARPS + 31) & ~31, lo = min(n, warp * seg), hi = min(n, lo + seg);
-    auto kept = [&](int i) -> u64 { return c.in_set(i) && heavy(z[i]) ? c.weight(z[i]) : 0; };
     u64 mine = 0, cta;
-    for (int i = lo + lane; i < hi; i += 32) mine += kept(i);
+    if (by_p && lowest <= 0.0) {
+        mine = above_here;
+        c.sweep(lo, hi, [&](int i) {
+            const int b = c.bin(z[i]);
+            return b >= first && b <= last && c.in_set(i);
+        }, [&](int i) { mine += c.weight(z[i]); });
+    } else {
+        c.sweep(lo, hi, [&](int i) {
+            const float y = c.log_weight(z[i]);
+            const bool in = c.in_set(i) && heavy(z[i]);
+            if (in && y < -9.f) mine += smp_light(y);
+            return in && y >= -9.f;
+        }, [&](int i) { mine += c.weight(z[i]); });
+    }
     u64 warp_sum = mine;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) warp_sum += __shfl_xor_sync(0xFFFFFFFFu, warp_sum, o);
@@ -499,18 +574,26 @@ __global__ void __launch_bounds__(SMP_THREADS) sample_kernel(const SampleArgs a)
     }
     const u64 goal = min((u64)floor(u * (double)total), total - 1);
     if (goal < run || goal >= run + warp_sum) return;
-    for (int i0 = lo; i0 < hi; i0 += 32) {
-        const u64 w = i0 + lane < hi ? kept(i0 + lane) : 0;
-        const u64 inc = run + smp_warp_inclusive(w);
-        const unsigned hit = __ballot_sync(0xFFFFFFFFu, inc > goal);
-        if (hit) {
-            if (lane == __ffs(hit) - 1) {
-                a.tokens[row] = c.base + i0 + lane;
-                if (a.probs) a.probs[row] = (float)((double)w / (double)total);
-            }
-            return;
+    for (int i0 = lo; i0 < hi; i0 += 128) {   // four runs of 32 at once: their weights do not wait for one another
+        u64 w[4], sum[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int i = i0 + 32 * k + lane;
+            w[k] = i < hi && c.in_set(i) && heavy(z[i]) ? c.weight(z[i]) : 0;
+            sum[k] = smp_warp_inclusive(w[k]);
         }
-        run = __shfl_sync(0xFFFFFFFFu, inc, 31);
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const unsigned hit = __ballot_sync(0xFFFFFFFFu, run + sum[k] > goal);
+            if (hit) {
+                if (lane == __ffs(hit) - 1) {
+                    a.tokens[row] = c.base + i0 + 32 * k + lane;
+                    if (a.probs) a.probs[row] = (float)((double)w[k] / (double)total);
+                }
+                return;
+            }
+            run += __shfl_sync(0xFFFFFFFFu, sum[k], 31);
+        }
     }
 }
 
