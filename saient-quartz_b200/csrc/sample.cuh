@@ -74,8 +74,8 @@ __device__ __forceinline__ u64 smp_light(float x) { return x < -31.5f ? 0 : __fl
 //   3. top_k: the bin of the k-th token follows from the counts; its tokens are gathered and ranked against one another.
 //      When all tokens down to that bin fit the list (k up to some hundreds), everything else is done on the list.
 //   4. top_p: the counts bracket the bin in which the weights reach their goal (a bin's tokens weigh the same within 1/32);
-//      one pass sums the weights above the bracket and below it, and those inside bin by bin; the tokens of the right
-//      bin are gathered and ranked.
+//      one pass sums the weights above the bracket and below it, and those inside in 1024 finer bins; the tokens of the
+//      right bin are gathered and ranked.
 //   5. the kept weights are summed warp by warp in the order of the vocabulary (above the bracket step 4 did that, only
 //      tokens inside it are looked at again); the warp in whose range u falls walks its part.
 // Tokens that need more than a few instructions (64-bit weights, histogram entries) are first collected, so that a warp
@@ -157,6 +157,7 @@ struct Sampler {
     int n, base;          // tokens in it, index of the first
     int CL, rank, turn;
     float M, inv, per_bin;
+    float fine0, fine;    // inside the bracket: bin (t - fine0) * fine of t = (M - z) * per_bin
     SampleExp e;
     float keep_z;         // the set: logits above keep_z, and those equal to it with an index up to keep_i
     int keep_i;
@@ -174,6 +175,11 @@ struct Sampler {
     {
         const float t = (M - x) * per_bin;
         return x == M ? 0 : t < (float)(SMP_BINS - 1) ? (int)t : SMP_BINS - 1;
+    }
+    __device__ __forceinline__ int fine_bin(float x) const   // of a token inside the bracket
+    {
+        const float t = x == M ? 0.f : fminf((M - x) * per_bin, (float)SMP_BINS);
+        return max(0, min(SMP_BINS - 1, (int)((t - fine0) * fine)));
     }
     __device__ __forceinline__ float log_weight(float x) const { return x == M ? 0.f : (x - M) * inv; }
     __device__ __forceinline__ u64 weight(float x) const
@@ -301,15 +307,17 @@ struct Sampler {
         sync();
     }
     // Number of the last token with `above` + (weights, or count, of the set's tokens before it) < goal, given that it is
-    // among the `count` tokens of bin b.
-    __device__ __forceinline__ u64 last_in_bin(int b, uint32_t count, u64 above, double goal, bool weights)
+    // among the `count` tokens for which in_bin holds (a run of the order).
+    template <class Bin>
+    __device__ __forceinline__ u64 last_in_bin(Bin in_bin, uint32_t count, u64 above, double goal, bool weights)
     {
+        bool ranged = false;
         u64 lo = 0, hi = ~(u64)0;
         if (count > SMP_LIST) {
             u64 small = 0, large = 0;   // largest of ~number and of number
             for (int i = threadIdx.x; i < n; i += SMP_THREADS) {
                 const u64 x = number(i);
-                if (in_set(i) && bin(z[i]) == b) {
+                if (in_set(i) && in_bin(z[i])) {
                     small = max(small, ~x);
                     large = max(large, x);
                 }
@@ -337,10 +345,10 @@ struct Sampler {
                 lo = max(lo, hi - (((u64)1 << shift) - 1));
             }
             if (lo == hi) return hi;
-            b = -1;
+            ranged = true;
         }
         gather([&](int i) {
-            if (b >= 0) return in_set(i) && bin(z[i]) == b;
+            if (!ranged) return in_set(i) && in_bin(z[i]);
             const u64 x = number(i);
             return x >= lo && x <= hi;
         });
@@ -474,7 +482,7 @@ __global__ void __launch_bounds__(SMP_THREADS) sample_kernel(const SampleArgs a)
             }
             return;
         }
-        c.keep_to(c.last_in_bin(b, in_bin, before, (double)a.top_k, false));
+        c.keep_to(c.last_in_bin([&](float x) { return c.bin(x) == b; }, in_bin, before, (double)a.top_k, false));
     }
     const int seg = ((n + SMP_WARPS - 1) / SMP_WARPS + 31) & ~31, lo = min(n, warp * seg), hi = min(n, lo + seg);   // this warp's part
     int first = 0, last = -1;
@@ -507,6 +515,8 @@ __global__ void __launch_bounds__(SMP_THREADS) sample_kernel(const SampleArgs a)
         }
         first = (int)smp_reduce<true>((u64)first, s.red);
         last = SMP_BINS - 1 - (int)smp_reduce<true>((u64)from_end, s.red);
+        c.fine0 = (float)first;
+        c.fine = (float)SMP_BINS / (float)(last + 1 - first);
         c.clear(true);
         u64 above = 0, below = 0;
         c.sweep(lo, hi, [&](int i) {
@@ -523,7 +533,7 @@ __global__ void __launch_bounds__(SMP_THREADS) sample_kernel(const SampleArgs a)
             const u64 w = c.weight(z[i]);
             if (b < first) above += w;
             else if (b > last) below += w;
-            else c.add(b, true, w);
+            else c.add(c.fine_bin(z[i]), true, w);
         });
         above_here = above;
         above = smp_reduce<false>(above, s.red);
@@ -543,7 +553,8 @@ __global__ void __launch_bounds__(SMP_THREADS) sample_kernel(const SampleArgs a)
         const double goal = (double)a.top_p * (double)(above + inside + below);
         u64 before;
         const int b = c.boundary(true, above, goal, &before);
-        if (b >= 0) c.keep_to(c.last_in_bin(b, s.all_cnt[b], before, goal, true));
+        if (b >= 0)
+            c.keep_to(c.last_in_bin([&](float x) { const int k = c.bin(x); return k >= first && k <= last && c.fine_bin(x) == b; }, s.all_cnt[b], before, goal, true));
     }
     // ---- 5. the token ----
     u64 mine = 0, cta;
