@@ -280,7 +280,7 @@ void cuda_attn_prompt_kv4(float *out, const float *q, const void *d_cache, int n
  * <= 0: the first only), of those the ones that weigh at least min_p (<= 0: all; above 1 counts as 1).  The answer
  * is the first token in the order of the vocabulary at which the running sum of the kept weights exceeds u times their
  * total; u below 0 or NaN counts as 0, from 1 on the last token of weight is taken.  Weights are whole numbers of
- * units of 2^-44: a token below half a unit is never chosen.  temperature 0: the largest logit, ties to the lower index (d_u may be NULL), probability 1.  Logits of -inf
+ * units of 2^-44, rounded down: a token below one unit is never chosen.  temperature 0: the largest logit, ties to the lower index (d_u may be NULL), probability 1.  Logits of -inf
  * and NaN are never chosen; a row without any other gives token -1, probability 0.  The sums are exact integers: the
  * same inputs give the same token however the work is split.  vocab <= 524288, finite temperature >= 0.
  * cuda_step_advance: d_step[0] = *d_token (left as it is if that is negative), d_step[1] += 1, and the registered RoPE

@@ -24,7 +24,7 @@ def sample(z, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         order, w = order[:n], w[:n]
     keep = w >= min(min_p, 1.0)
     order, w = order[keep], w[keep]
-    w = np.where(w > 2.0 ** -45, w, 0.0)     # a weight is a whole number of units of 2^-44
+    w = np.where(w >= 2.0 ** -44, w, 0.0)    # a weight is a whole number of units of 2^-44, rounded down
     by = np.argsort(order)
     order, w = order[by], w[by]
     run = np.cumsum(w)

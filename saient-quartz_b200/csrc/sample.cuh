@@ -8,6 +8,13 @@
 //
 // Weights are held as 64-bit integers in units of 2^-44, so that every sum is exact and does not depend on its order:
 // 2^19 tokens of weight 1 still fit.  A logit of -inf or NaN has no weight and is never chosen.
+//
+// A weight is 2^(-t / 32), t = 32 log2(e) (M - z) / T.  With b the whole number next to t it is 2^(-b / 32), from a table of
+// 32 by b mod 32 and a shift, times 1 - r, r from four terms of the exponential's series (|y| < 0.011: 2e-11).  Only r E
+// is taken in 32 bits, so a weight is right to 2^-29, and t as a sum of two f32 numbers: M - z is exact as one, and no
+// 64-bit arithmetic is needed (CUDA's exp in 64 bits took twice the time of the rest).  Why so exact: with thousands of
+// tokens kept, an error of 1e-7 in their sums would move the border of top_p, or the token that u falls on, once in some
+// thousand rows.  b is also the bin in which tokens are counted: it follows the order of the logits.
 #pragma once
 
 #include <cooperative_groups.h>
@@ -45,59 +52,32 @@ __device__ __forceinline__ uint32_t smp_key(float z)
 
 __device__ __forceinline__ float smp_unkey(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k); }
 
-// exp of a weight's argument in units of 2^-44.  In 64 bits: with thousands of tokens kept, an error of 1e-7 in their sums
-// moves the border of top_p, or the token that u falls on, once in some thousand rows. 2^(n / 16) from a table, the rest (below ln 2 / 32) by its
-// Taylor series up to the fifth power (1.4e-13).  (CUDA's exp: 730 us, not 610, for 256 rows of 128256.)
-struct SampleExp {
-    double M, scale;        // scale = 16 log2(e) / temperature
-    const double *table;    // 2^(k / 16), k < 16
-    __device__ __forceinline__ u64 operator()(float z) const
-    {
-        const double t = ((double)z - M) * scale, whole = t + 6755399441055744.0;   // 1.5 * 2^52: the sum's low word is t's nearest integer
-        const int n = __double2loint(whole);
-        constexpr double A = 0.04332169878499658;   // ln(2) / 16
-        const double f = (t - (whole - 6755399441055744.0)) * A;
-        const double p = fma(f, fma(f, fma(f, fma(f, fma(f, 1.0 / 120, 1.0 / 24), 1.0 / 6), 0.5), 1.0), 1.0) * table[n & 15];
-        const double w = __hiloint2double(__double2hiint(p) + (((n >> 4) + 44) << 20), __double2loint(p));
-        return (u64)__double_as_longlong(w + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;   // + 2^52: rounded to a whole number
-    }
-};
-// Weights below exp(-9) are taken in 32 bits: their errors (2e-6 of a weight, either way) average out of sums to which
-// such tokens contribute by the thousand.
-__device__ __forceinline__ u64 smp_light(float x) { return x < -31.5f ? 0 : __float2uint_rn(exp2f(x * 1.44269504f) * (float)SMP_ONE); }
-
 // ---- the kernel -------------------------------------------------------------------------------------------------
 // A cluster of CL CTAs per row; each keeps a contiguous part of the row in shared memory, read once from HBM.  Nothing is
 // sorted: a threshold is the number of the last token kept, and is found by counting.
 //   1. the largest number of the row (M; at temperature 0 the answer)
-//   2. a histogram of the logits over 1024 bins of 1/32 of the temperature below M
-//   3. top_k: the bin of the k-th token follows from the counts; its tokens are gathered and ranked against one another.
-//      When all tokens down to that bin fit the list (k up to some hundreds), everything else is done on the list.
-//   4. top_p: the counts bracket the bin in which the weights reach their goal (a bin's tokens weigh the same within 1/32);
-//      one pass sums the weights above the bracket and below it, and those inside in 1024 finer bins; the tokens of the
-//      right bin are gathered and ranked.
-//   5. the kept weights are summed warp by warp in the order of the vocabulary (above the bracket step 4 did that, only
-//      tokens inside it are looked at again); the warp in whose range u falls walks its part.
-// Tokens that need more than a few instructions (64-bit weights, histogram entries) are first collected, so that a warp
-// takes 32 of them at a time.
+//   2. top_k: a histogram of the tokens over the bins b; the bin of the k-th token is known then, its tokens are gathered
+//      and ranked against one another.  When all tokens down to that bin fit the list (k up to some hundreds), everything
+//      else is done on the list.
+//   3. top_p: the same with a histogram of the weights, bin by bin in units of the bin's own size.
+//   4. the kept weights are summed warp by warp in the order of the vocabulary; the warp in whose range u falls walks its
+//      part.  (Few tokens are kept as a rule: a warp collects them and weighs 32 at a time.)
 // A bin with more tokens than the list takes (ties, high temperatures) is divided further, by the number itself.
 // A histogram is reduced in slices, one per CTA, that are pushed to every CTA: all find the same bin without asking.
-constexpr int SMP_BINS = 2 * SMP_THREADS, SMP_LIST = 512,   // (a thread looks after two bins, and one token of the list)
-              SMP_WARPS = SMP_THREADS / 32, SMP_MAX_CLUSTER = 16;
+constexpr int SMP_PER = 3, SMP_BINS = SMP_PER * SMP_THREADS, SMP_LIST = 512;   // (a thread looks after three bins, and one token of the list)
+constexpr int SMP_WARPS = SMP_THREADS / 32, SMP_MAX_CLUSTER = 16;
+static_assert(SMP_BINS >= 32 * 46 && SMP_BINS % SMP_MAX_CLUSTER == 0, "bins cover weights down to 2^-45");
 
 struct SampleShared {
-    uint32_t cnt[SMP_BINS], part[3][SMP_BINS];    // this CTA's histogram: tokens, and their weights in parts of 15 bits
-    uint32_t all_cnt[SMP_BINS];                   // the row's
-    u64 all_w[SMP_BINS];
+    uint32_t part[2][SMP_BINS];                   // this CTA's histogram: tokens in [0], or the two halves of their sizes
+    u64 all[SMP_BINS];                            // the row's: tokens, or weights
     union {
         u64 slice[SMP_BINS];                      // while a histogram is collected: this CTA's slice of everybody's
-        struct { u64 mine[SMP_LIST], list[SMP_LIST]; };   // gathered tokens: this CTA's; (CTA 0) the row's
+        struct { u64 mine[SMP_LIST], list[SMP_LIST], list_w[SMP_LIST]; };   // gathered tokens: this CTA's; (CTA 0) the row's, their weights
     };
-    u64 list_w[SMP_LIST];
-    u64 from[2][SMP_MAX_CLUSTER][3];              // what the cluster's CTAs pushed last, and before
+    u64 from[2][SMP_MAX_CLUSTER][2];              // what the cluster's CTAs pushed last, and before
     u64 red[SMP_WARPS];
-    double exp2_16[16];
-    u64 own[2], got[SMP_MAX_CLUSTER][2];          // sums beside a histogram: this CTA's, everybody's
+    uint2 table[32];                              // 2^27 * 2^(-k / 32): rounded to a whole number, and that as f32
     u64 result;
     u64 before;
     int n_mine, n_list, at, bin;
@@ -124,29 +104,25 @@ __device__ __forceinline__ u64 smp_reduce(u64 v, u64 *sm)
     }
     return v;
 }
-template <class T>
-__device__ __forceinline__ T smp_warp_inclusive(T v)
+__device__ __forceinline__ u64 smp_warp_inclusive(u64 v)
 {
     const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const T y = __shfl_up_sync(0xFFFFFFFFu, v, o);
+        const u64 y = __shfl_up_sync(0xFFFFFFFFu, v, o);
         if (lane >= o) v += y;
     }
     return v;
 }
 // sum over the threads before this one; *total over all
-template <class T>
-__device__ __forceinline__ T smp_before(T v, u64 *scratch, T *total)
+__device__ __forceinline__ u64 smp_before(u64 v, u64 *sm, u64 *total)
 {
-    static_assert(sizeof(T) <= 8, "");
-    T *sm = (T *)scratch;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const T inc = smp_warp_inclusive(v);
+    const u64 inc = smp_warp_inclusive(v);
     __syncthreads();
     if (lane == 31) sm[warp] = inc;
     __syncthreads();
-    const T w = lane < SMP_WARPS ? sm[lane] : T(0), winc = smp_warp_inclusive(w);
+    const u64 w = lane < SMP_WARPS ? sm[lane] : 0, winc = smp_warp_inclusive(w);
     *total = __shfl_sync(0xFFFFFFFFu, winc, 31);
     return __shfl_sync(0xFFFFFFFFu, winc - w, warp) + inc - v;
 }
@@ -156,9 +132,7 @@ struct Sampler {
     const float *z;       // this CTA's part of the row
     int n, base;          // tokens in it, index of the first
     int CL, rank, turn;
-    float M, inv, per_bin;
-    float fine0, fine;    // inside the bracket: bin (t - fine0) * fine of t = (M - z) * per_bin
-    SampleExp e;
+    float M, c_hi, c_lo;  // t = (M - z) * (c_hi + c_lo)
     float keep_z;         // the set: logits above keep_z, and those equal to it with an index up to keep_i
     int keep_i;
 
@@ -171,22 +145,33 @@ struct Sampler {
         keep_i = (int)~(uint32_t)last;
     }
     __device__ __forceinline__ u64 number(int i) const { return (u64)smp_key(z[i]) << 32 | (uint32_t)~(base + i); }
+    // the whole number next to t, at most SMP_BINS - 1 (which also takes M = inf and T = 0's neighbours, where t is not a number)
     __device__ __forceinline__ int bin(float x) const
     {
-        const float t = (M - x) * per_bin;
-        return x == M ? 0 : t < (float)(SMP_BINS - 1) ? (int)t : SMP_BINS - 1;
+        const float t = x == M ? 0.f : __fmul_rn(M - x, c_hi);
+        return t < (float)(SMP_BINS - 1) ? __float2int_rn(t) : SMP_BINS - 1;
     }
-    __device__ __forceinline__ int fine_bin(float x) const   // of a token inside the bracket
+    // the weight of logit x is size << 17 >> b / 32, b its bin
+    __device__ __forceinline__ uint32_t size(float x, int &b) const
     {
-        const float t = x == M ? 0.f : fminf((M - x) * per_bin, (float)SMP_BINS);
-        return max(0, min(SMP_BINS - 1, (int)((t - fine0) * fine)));
+        const float d = M - x, back = d - M, rest = (M - (d - back)) - (x + back);   // d + rest = M - x exactly
+        const float t = __fmul_rn(d, c_hi), t_lo = fmaf(d, c_hi, -t) + fmaf(d, c_lo, rest * c_hi);
+        const float whole = __fadd_rn(t, 12582912.f);   // 1.5 * 2^23: the sum's low bits are t's nearest integer
+        const bool far = !(t < (float)(SMP_BINS - 1)), top = x == M;
+        b = top ? 0 : far ? SMP_BINS - 1 : __float_as_int(whole) - 0x4B400000;
+        const float y = ((t - (whole - 12582912.f)) + t_lo) * 0.0216608494f;   // ln 2 / 32
+        const float r = y * fmaf(y, fmaf(y, fmaf(y, -1.f / 24, 1.f / 6), -0.5f), 1.f);
+        const uint2 e = s.table[b & 31];
+        const uint32_t v = e.x + (0x4B400000 - __float_as_uint(fmaf(__uint_as_float(e.y), r, 12582912.f)));
+        return top ? 1u << 27 : far ? 0 : v;
     }
-    __device__ __forceinline__ float log_weight(float x) const { return x == M ? 0.f : (x - M) * inv; }
     __device__ __forceinline__ u64 weight(float x) const
     {
-        const float y = log_weight(x);
-        return x == M ? (u64)SMP_ONE : y < -9.f ? smp_light(y) : e(x);
+        int b;
+        const uint32_t v = size(x, b);
+        return (u64)v << 17 >> (b >> 5);
     }
+    __device__ __forceinline__ u64 weight_of(u64 number) const { return weight(smp_unkey((uint32_t)(number >> 32))); }
     // Calls now(i) for tokens lo + lane, lo + 32 + lane, .. below hi; what it returns true for is done by put_off(i), 32 at a time.
     template <class Now, class PutOff>
     __device__ __forceinline__ void sweep(int lo, int hi, Now now, PutOff put_off) const
@@ -198,6 +183,7 @@ struct Sampler {
             const int i = i0 + lane;
             const bool more = i < hi && now(i);
             const unsigned mask = __ballot_sync(0xFFFFFFFFu, more);
+            if (!mask) continue;
             if (more) later[held + __popc(mask & ((1u << lane) - 1))] = (uint16_t)i;
             held += __popc(mask);
             if (held >= 32) {
@@ -213,27 +199,22 @@ struct Sampler {
         if (lane < held) put_off((int)later[lane]);
         __syncwarp();
     }
-    __device__ __forceinline__ u64 weight_of(u64 number) const { return weight(smp_unkey((uint32_t)(number >> 32))); }
 
-    // three values of this CTA to every CTA: afterwards s.from[turn][r] holds those of CTA r (two turns' worth are kept:
+    // two values of this CTA to every CTA: afterwards s.from[turn][r] holds those of CTA r (two turns' worth are kept:
     // a CTA may still read the last ones while another pushes the next)
-    __device__ __forceinline__ void exchange(u64 a, u64 b, u64 c)
+    __device__ __forceinline__ void exchange(u64 a, u64 b)
     {
         turn ^= 1;
         if ((int)threadIdx.x < CL) {
             u64 *to = peer(threadIdx.x)->from[turn][rank];
             to[0] = a;
             to[1] = b;
-            to[2] = c;
         }
         sync();
     }
-    __device__ __forceinline__ void clear(bool weights)
+    __device__ __forceinline__ void clear()
     {
-        for (int b = threadIdx.x; b < SMP_BINS; b += SMP_THREADS) {
-            s.cnt[b] = 0;
-            if (weights) s.part[0][b] = s.part[1][b] = s.part[2][b] = 0;
-        }
+        for (int b = threadIdx.x; b < SMP_BINS; b += SMP_THREADS) s.part[0][b] = s.part[1][b] = 0;
         if (threadIdx.x == 0) s.bin = -1;
         __syncthreads();
     }
@@ -241,49 +222,41 @@ struct Sampler {
     {
         if (threadIdx.x == 0) s.n_mine = s.n_list = 0;   // (the cluster meets before the next tokens arrive)
     }
-    __device__ __forceinline__ void add(int b, bool weights, u64 w)
+    __device__ __forceinline__ void add(int b, bool weights, uint32_t size)   // (sizes are below 2^28: 2^17 halves fit a sum)
     {
-        atomicAdd(&s.cnt[b], 1u);
-        if (weights) {
-            atomicAdd(&s.part[0][b], (uint32_t)(w & 0x7FFF));
-            atomicAdd(&s.part[1][b], (uint32_t)(w >> 15 & 0x7FFF));
-            atomicAdd(&s.part[2][b], (uint32_t)(w >> 30));
-        }
+        atomicAdd(&s.part[0][b], weights ? size & 0x3FFF : 1u);
+        if (weights) atomicAdd(&s.part[1][b], size >> 14);
     }
-    // the row's histogram into every CTA: this one sums a slice of all CTAs' bins and pushes it (lanes run over bins)
-    __device__ __forceinline__ void collect(bool weights)
+    // The row's histogram into every CTA: this one sums a slice of all CTAs' bins and pushes it (lanes run over bins).  Weights:
+    // the bins' sizes are in units of 2^(17 - shift), shift = b / 32 or (of a bin divided further) as given.
+    __device__ __forceinline__ void collect(bool weights, int shift = -1)
     {
         sync();
         const int per = SMP_BINS / CL;
-        for (int what = weights ? 1 : 0; what >= 0; what--) {   // weights, then tokens
-            for (int t = threadIdx.x; t < SMP_BINS; t += SMP_THREADS) {
-                const SampleShared *from = peer(t / per);
-                const int b = rank * per + t % per;
-                if (what && t < 2 * CL) s.got[t >> 1][t & 1] = peer(t >> 1)->own[t & 1];
-                s.slice[t] = what ? (u64)from->part[0][b] + ((u64)from->part[1][b] << 15) + ((u64)from->part[2][b] << 30) : from->cnt[b];
-            }
-            __syncthreads();
-            for (int t = threadIdx.x; t < SMP_BINS; t += SMP_THREADS) {
-                const int k = t % per, b = rank * per + k;
-                u64 sum = 0;
-                for (int r = 0; r < CL; r++) sum += s.slice[r * per + k];
-                if (what) peer(t / per)->all_w[b] = sum;
-                else peer(t / per)->all_cnt[b] = (uint32_t)sum;
-            }
-            if (what) __syncthreads();
+        for (int t = threadIdx.x; t < SMP_BINS; t += SMP_THREADS) {
+            const SampleShared *from = peer(t / per);
+            const int b = rank * per + t % per;
+            s.slice[t] = weights ? (u64)from->part[0][b] + ((u64)from->part[1][b] << 14) : from->part[0][b];
+        }
+        __syncthreads();
+        for (int t = threadIdx.x; t < SMP_BINS; t += SMP_THREADS) {
+            const int k = t % per, b = rank * per + k;
+            u64 sum = 0;
+            for (int r = 0; r < CL; r++) sum += s.slice[r * per + k];
+            peer(t / per)->all[b] = weights ? sum << 17 >> (shift < 0 ? b >> 5 : shift) : sum;
         }
         sync();
     }
     // The first bin at which `above` plus the sum up to and with it reaches the goal; *before: the sum above it.
     // (The last bin that holds anything where the goal is not reached: fewer tokens than top_k.)
-    __device__ __forceinline__ int boundary(bool weights, u64 above, double goal, u64 *before)
+    __device__ __forceinline__ int boundary(u64 above, double goal, u64 *before)
     {
-        u64 v[2], total;
-        for (int k = 0; k < 2; k++) v[k] = weights ? s.all_w[2 * threadIdx.x + k] : s.all_cnt[2 * threadIdx.x + k];
-        u64 sum = above + smp_before(v[0] + v[1], s.red, &total);
-        for (int k = 0; k < 2; k++) {
+        u64 v[SMP_PER], total, mine = 0;
+        for (int k = 0; k < SMP_PER; k++) mine += v[k] = s.all[SMP_PER * threadIdx.x + k];
+        u64 sum = above + smp_before(mine, s.red, &total);
+        for (int k = 0; k < SMP_PER; k++) {
             if (v[k] && (double)sum < goal && (goal <= (double)(sum + v[k]) || sum + v[k] == above + total)) {
-                s.bin = 2 * threadIdx.x + k;
+                s.bin = SMP_PER * threadIdx.x + k;
                 s.before = sum;
             }
             sum += v[k];
@@ -307,24 +280,23 @@ struct Sampler {
         sync();
     }
     // Number of the last token with `above` + (weights, or count, of the set's tokens before it) < goal, given that it is
-    // among the `count` tokens for which in_bin holds (a run of the order).
-    template <class Bin>
-    __device__ __forceinline__ u64 last_in_bin(Bin in_bin, uint32_t count, u64 above, double goal, bool weights)
+    // among the set's tokens of bin b, at most `count` of them.
+    __device__ __forceinline__ u64 last_in_bin(int b, u64 count, u64 above, double goal, bool weights)
     {
-        bool ranged = false;
         u64 lo = 0, hi = ~(u64)0;
+        bool ranged = false;
         if (count > SMP_LIST) {
             u64 small = 0, large = 0;   // largest of ~number and of number
             for (int i = threadIdx.x; i < n; i += SMP_THREADS) {
                 const u64 x = number(i);
-                if (in_set(i) && in_bin(z[i])) {
+                if (in_set(i) && bin(z[i]) == b) {
                     small = max(small, ~x);
                     large = max(large, x);
                 }
             }
             small = smp_reduce<true>(small, s.red);
             large = smp_reduce<true>(large, s.red);
-            exchange(small, large, 0);
+            exchange(small, large);
             for (int r = 0; r < CL; r++) {
                 small = max(small, s.from[turn][r][0]);
                 large = max(large, s.from[turn][r][1]);
@@ -333,22 +305,24 @@ struct Sampler {
             hi = large;
             while (count > SMP_LIST && lo < hi) {
                 const int shift = max(0, 54 - __clzll((long long)(hi - lo)));   // (hi - lo) >> shift < 1024
-                clear(weights);
+                clear();
                 for (int i = threadIdx.x; i < n; i += SMP_THREADS) {
                     const u64 x = number(i);
-                    if (x >= lo && x <= hi) add((int)((hi - x) >> shift), weights, weights ? weight(z[i]) : 0);
+                    int same;   // (all lie in bin b)
+                    if (x >= lo && x <= hi) add((int)((hi - x) >> shift), weights, weights ? size(z[i], same) : 0);
                 }
-                collect(weights);
-                const int sub = boundary(weights, above, goal, &above);
-                count = s.all_cnt[sub];
+                collect(weights, b >> 5);
+                const int sub = boundary(above, goal, &above);
+                count = held_by(s.all[sub], weights, b);
                 hi -= (u64)sub << shift;
                 lo = max(lo, hi - (((u64)1 << shift) - 1));
+                __syncthreads();
             }
             if (lo == hi) return hi;
             ranged = true;
         }
         gather([&](int i) {
-            if (!ranged) return in_set(i) && in_bin(z[i]);
+            if (!ranged) return in_set(i) && bin(z[i]) == b;
             const u64 x = number(i);
             return x >= lo && x <= hi;
         });
@@ -366,6 +340,13 @@ struct Sampler {
         sync();
         no_list();
         return s.result;
+    }
+    // At most so many tokens make up v, tokens or weights of bin b (a token's weight is 2^(-b / 32) within 1.1 per cent)
+    __device__ __forceinline__ u64 held_by(u64 v, bool weights, int b) const
+    {
+        if (!weights) return v;
+        const float one = __uint_as_float(s.table[b & 31].y) * (float)(1ull << 17) / (float)(1ull << (b >> 5));
+        return (u64)(((float)v + 1.f) / one * 1.02f) + 1;   // (the sum was rounded down to a unit)
     }
 };
 
@@ -410,12 +391,15 @@ __global__ void __launch_bounds__(SMP_THREADS) sample_kernel(const SampleArgs a)
 #pragma unroll 4
         for (int i = tid; i < n; i += SMP_THREADS) take(__ldcs(src + i), i);
     }
-    if (tid < 16) s.exp2_16[tid] = exp2((double)tid / 16.0);
+    if (tid < 32) {
+        const uint32_t e = (uint32_t)rint(exp2(27.0 - (double)tid / 32.0));
+        s.table[tid] = make_uint2(e, __float_as_uint((float)e));
+    }
     c.no_list();
-    c.clear(false);   // (synchronises)
+    c.clear();   // (synchronises)
     u64 best = at >= 0 ? c.number(at) : 0;
     best = smp_reduce<true>(best, s.red);
-    c.exchange(best, 0, 0);
+    c.exchange(best, 0);
     for (int r = 0; r < c.CL; r++) best = max(best, s.from[c.turn][r][0]);
     const bool none = best == 0;
     if (none || a.temperature == 0.f) {
@@ -426,34 +410,33 @@ __global__ void __launch_bounds__(SMP_THREADS) sample_kernel(const SampleArgs a)
         return;
     }
     c.M = smp_unkey((uint32_t)(best >> 32));
-    const double inv64 = 1.0 / (double)a.temperature;
-    c.inv = (float)inv64;
-    c.per_bin = (float)(32.0 * inv64);
-    c.e = {(double)c.M, 16.0 * 1.4426950408889634 * inv64, s.exp2_16};
+    const double inv64 = 1.0 / (double)a.temperature, scale = 32.0 * 1.4426950408889634 * inv64;
+    c.c_hi = (float)scale;
+    c.c_lo = isinf(c.c_hi) ? 0.f : (float)(scale - (double)c.c_hi);
     c.keep_z = -INFINITY;
     c.keep_i = -1;
+    const float inv = (float)inv64;
     const double u = (double)fminf(fmaxf(a.u[row], 0.f), 1.f), lowest = fmin((double)a.min_p, 1.0);
     const float log_lowest = lowest > 0.0 ? (float)log(lowest) : -INFINITY;
     auto heavy = [&](float x) {   // weight >= min_p: decided in 64 bits where 32 could be wrong
-        const float y = (x - c.M) * c.inv;
-        if (x == c.M || y > log_lowest + 1e-3f) return true;
+        if (lowest <= 0.0 || x == c.M) return true;
+        const float y = (x - c.M) * inv;
+        if (y > log_lowest + 1e-3f) return true;
         if (y < log_lowest - 1e-3f) return false;
         return exp(((double)x - (double)c.M) * inv64) >= lowest;
     };
     const bool by_k = a.top_k > 0 && a.top_k < a.vocab, by_p = a.top_p > 0.f && a.top_p < 1.f;
-    if (by_k || by_p) {
-        // ---- 2. counts ----
-        for (int i = tid; i < n; i += SMP_THREADS)
-            if (c.in_set(i)) c.add(c.bin(z[i]), false, 0);
-        c.collect(false);
-    }
     if (a.top_p <= 0.f) {
         c.keep_to(best);
     } else if (by_k) {
-        // ---- 3. top_k ----
+        // ---- 2. top_k ----
+#pragma unroll 4
+        for (int i = tid; i < n; i += SMP_THREADS)
+            if (c.in_set(i)) c.add(c.bin(z[i]), false, 0);
+        c.collect(false);
         u64 before;
-        const int b = c.boundary(false, 0, (double)a.top_k, &before);
-        const uint32_t in_bin = s.all_cnt[b];
+        const int b = c.boundary(0, (double)a.top_k, &before);
+        const u64 in_bin = s.all[b];
         if (before + in_bin <= SMP_LIST) {
             c.gather([&](int i) { return c.in_set(i) && c.bin(z[i]) <= b; });
             if (c.rank != 0) return;   // (nobody pushes to this CTA or reads from it any more)
@@ -482,102 +465,35 @@ __global__ void __launch_bounds__(SMP_THREADS) sample_kernel(const SampleArgs a)
             }
             return;
         }
-        c.keep_to(c.last_in_bin([&](float x) { return c.bin(x) == b; }, in_bin, before, (double)a.top_k, false));
+        c.keep_to(c.last_in_bin(b, in_bin, before, (double)a.top_k, false));
+        if (by_p) c.clear();
     }
-    const int seg = ((n + SMP_WARPS - 1) / SMP_WARPS + 31) & ~31, lo = min(n, warp * seg), hi = min(n, lo + seg);   // this warp's part
-    int first = 0, last = -1;
-    u64 above_here = 0;   // weights above the bracket that this lane has summed
     if (by_p) {
-        // ---- 4. top_p ----
-        if (by_k) {   // the counts of the set (last_in_bin may have used the histogram)
-            c.clear(false);
-            for (int i = tid; i < n; i += SMP_THREADS)
-                if (c.in_set(i)) c.add(c.bin(z[i]), false, 0);
-            c.collect(false);
-        }
-        // a token of bin b weighs between exp(-(b + 1) / 32) and exp(-b / 32); 1e-3 covers the rounding of its bin and of these sums
-        float most[2], least[2], most_all, least_all;
-        for (int k = 0; k < 2; k++) {
-            const int b = 2 * tid + k;
-            const float count = (float)s.all_cnt[b];
-            most[k] = count * expf(-(float)b / 32.f) * 1.001f;
-            least[k] = b < SMP_BINS - 1 ? count * expf(-(float)(b + 1) / 32.f) * 0.999f : 0.f;
-        }
-        float most_before = smp_before(most[0] + most[1], s.red, &most_all), least_before = smp_before(least[0] + least[1], s.red, &least_all);
-        // the first bin that may hold the border is the last with most_before < goal, the last one the first with least up to it >= goal
-        int from_end = 0;
-        first = 0;
-        for (int k = 0; k < 2; k++) {
-            if (most_before < a.top_p * least_all) first = 2 * tid + k;
-            least_before += least[k];
-            if (least_before >= a.top_p * most_all) from_end = max(from_end, SMP_BINS - 1 - (2 * tid + k));
-            most_before += most[k];
-        }
-        first = (int)smp_reduce<true>((u64)first, s.red);
-        last = SMP_BINS - 1 - (int)smp_reduce<true>((u64)from_end, s.red);
-        c.fine0 = (float)first;
-        c.fine = (float)SMP_BINS / (float)(last + 1 - first);
-        c.clear(true);
-        u64 above = 0, below = 0;
-        c.sweep(lo, hi, [&](int i) {
-            const float x = z[i], y = c.log_weight(x);
-            const int b = c.bin(x);
-            const bool light = y < -9.f, inside = b >= first && b <= last, in = c.in_set(i);
-            if (in && light && !inside) {
-                if (b < first) above += smp_light(y);
-                else below += smp_light(y);
-            }
-            return in && (!light || inside);
-        }, [&](int i) {
-            const int b = c.bin(z[i]);
-            const u64 w = c.weight(z[i]);
-            if (b < first) above += w;
-            else if (b > last) below += w;
-            else c.add(c.fine_bin(z[i]), true, w);
-        });
-        above_here = above;
-        above = smp_reduce<false>(above, s.red);
-        below = smp_reduce<false>(below, s.red);
-        if (tid == 0) {
-            s.own[0] = above;
-            s.own[1] = below;
+        // ---- 3. top_p ----
+#pragma unroll 4
+        for (int i = tid; i < n; i += SMP_THREADS) {
+            int b;
+            const uint32_t v = c.size(z[i], b);
+            if (c.in_set(i)) c.add(b, true, v);
         }
         c.collect(true);
-        above = below = 0;
-        for (int r = 0; r < c.CL; r++) {
-            above += s.got[r][0];
-            below += s.got[r][1];
-        }
-        u64 inside;
-        smp_before(s.all_w[2 * tid] + s.all_w[2 * tid + 1], s.red, &inside);
-        const double goal = (double)a.top_p * (double)(above + inside + below);
-        u64 before;
-        const int b = c.boundary(true, above, goal, &before);
-        if (b >= 0)
-            c.keep_to(c.last_in_bin([&](float x) { const int k = c.bin(x); return k >= first && k <= last && c.fine_bin(x) == b; }, s.all_cnt[b], before, goal, true));
+        u64 all = 0, before;
+        for (int k = 0; k < SMP_PER; k++) all += s.all[SMP_PER * tid + k];
+        all = smp_reduce<false>(all, s.red);
+        const double goal = (double)a.top_p * (double)all;
+        const int b = c.boundary(0, goal, &before);
+        c.keep_to(c.last_in_bin(b, c.held_by(s.all[b], true, b), before, goal, true));
     }
-    // ---- 5. the token ----
+    // ---- 4. the token ----
+    const int seg = ((n + SMP_WARPS - 1) / SMP_WARPS + 31) & ~31, lo = min(n, warp * seg), hi = min(n, lo + seg);   // this warp's part
     u64 mine = 0, cta;
-    if (by_p && lowest <= 0.0) {
-        mine = above_here;
-        c.sweep(lo, hi, [&](int i) {
-            const int b = c.bin(z[i]);
-            return b >= first && b <= last && c.in_set(i);
-        }, [&](int i) { mine += c.weight(z[i]); });
-    } else {
-        c.sweep(lo, hi, [&](int i) {
-            const float y = c.log_weight(z[i]);
-            const bool in = c.in_set(i) && heavy(z[i]);
-            if (in && y < -9.f) mine += smp_light(y);
-            return in && y >= -9.f;
-        }, [&](int i) { mine += c.weight(z[i]); });
-    }
+    c.sweep(lo, hi, [&](int i) { return c.in_set(i) && heavy(z[i]); }, [&](int i) { mine += c.weight(z[i]); });
     u64 warp_sum = mine;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) warp_sum += __shfl_xor_sync(0xFFFFFFFFu, warp_sum, o);
     u64 run = smp_before(lane == 0 ? warp_sum : 0, s.red, &cta);
     run = __shfl_sync(0xFFFFFFFFu, run, 0);
-    c.exchange(cta, 0, 0);
+    c.exchange(cta, 0);
     u64 total = 0;
     for (int r = 0; r < c.CL; r++) {
         if (r < c.rank) run += s.from[c.turn][r][0];
