@@ -487,7 +487,12 @@ __global__ void __launch_bounds__(SMP_THREADS) sample_kernel(const SampleArgs a)
     // ---- 4. the token ----
     const int seg = ((n + SMP_WARPS - 1) / SMP_WARPS + 31) & ~31, lo = min(n, warp * seg), hi = min(n, lo + seg);   // this warp's part
     u64 mine = 0, cta;
-    c.sweep(lo, hi, [&](int i) { return c.in_set(i) && heavy(z[i]); }, [&](int i) { mine += c.weight(z[i]); });
+    if (!by_k && !by_p && a.top_p > 0.f && lowest <= 0.0) {   // all of them
+#pragma unroll 4
+        for (int i = lo + lane; i < hi; i += 32) mine += z[i] > -INFINITY ? c.weight(z[i]) : 0;
+    } else {
+        c.sweep(lo, hi, [&](int i) { return c.in_set(i) && heavy(z[i]); }, [&](int i) { mine += c.weight(z[i]); });
+    }
     u64 warp_sum = mine;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) warp_sum += __shfl_xor_sync(0xFFFFFFFFu, warp_sum, o);
