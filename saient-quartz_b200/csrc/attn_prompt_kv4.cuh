@@ -8,7 +8,8 @@
 // A value is d (code - 8) + (m + 8 d).  The first term's two parts are exact and cost two packed instructions for two
 // values (hi = d c rounded, lo = d c - hi by one HFMA2: d has 11 bits, c four); the second is the same for the 32 dims of a
 // group, so it is a product of its own, with m and 8 d as they are: 8 more k of S against the sums of q over the groups, 8
-// more columns of O.  (Values split in f32, ten instructions for two, made unpacking the bottleneck: 182 us, not %s.)
+// more columns of O.  (Values split in f32 take ten instructions for two: 2048 tokens of 32 / 8 heads of
+// 128 took 182 us so, 171 with this.)
 // A operands live in tensor memory because a 64-wide MMA that fetched them from shared memory would be bound by that.
 // The tensor core rounds its sums towards zero, so O is never carried across tiles there: each tile's O starts from zero
 // and is added to f32 registers, where a raised softmax reference is also paid for (one factor per row and tile).
@@ -45,7 +46,7 @@ struct AttnPromptKv4Args {
 };
 
 struct AttnPromptKv4Shared {
-    uint64_t full[APK_STAGES], free_[APK_STAGES], s_full[2], p_full[2], o_free;
+    uint64_t full[APK_STAGES], free_[APK_STAGES], s_full[2], p_full[2], o_free, q_done;
     float corr[4][UMMA_M];           // factor of a row's earlier outputs at tile j (slot j % 4)
     float scale_k[4], scale_v[4];    // 1 / what the tile's K and V were multiplied with
     uint32_t nan_v[4][4][2];         // positions of the tile whose V group is NaN, by group
@@ -120,6 +121,7 @@ __global__ void __launch_bounds__(APK_THREADS, 1) attn_prompt_kv4_kernel(const A
             mbar_init(&s.p_full[i], 4);
         }
         mbar_init(&s.o_free, 8);
+        mbar_init(&s.q_done, 4);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (threadIdx.x < 32) ((uint32_t *)s.nan_v)[threadIdx.x] = 0;
@@ -146,14 +148,37 @@ __global__ void __launch_bounds__(APK_THREADS, 1) attn_prompt_kv4_kernel(const A
     if (warp < 4) {
         // ---- Q into tensor memory ----
         const uint32_t lanes = (uint32_t)(32 * warp) << 16;
-        const float *q = a.q + ((size_t)(t0 + tok) * a.n_heads + head) * HD;
         const float to_log2 = a.scale * 1.44269504f;
-        float top = 0.f;
-        if (is_row)
-            for (int i = 0; i < HD / 4; i++) {
-                const float4 v = __ldcg((const float4 *)q + i);
-                top = fmaxf(top, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
+        // rows come in one after the other, eight loads of 16 bytes on their way, through the last stage, which the filling warps
+        // leave alone until then (a thread that reads its own row touches 32 rows at once: 2048 tokens took 151 us so, 129 with
+        // this); 16-byte columns are rotated by the row against bank conflicts
+        constexpr int COLS = HD / 4;
+        float4 *stage_q = (float4 *)(ring + (APK_STAGES - 1) * STAGE) + warp * 32 * COLS;
+        const float4 *q0 = (const float4 *)(a.q + ((size_t)t0 * a.n_heads + (size_t)kvh * G) * HD);
+        const int my_row = is_row ? (tok * a.n_heads + row % G) * COLS : -1;
+        constexpr int AT_ONCE = 8;
+        static_assert(COLS % AT_ONCE == 0, "");
+        for (int k = 0; k < COLS; k += AT_ONCE) {
+            float4 v[AT_ONCE];
+#pragma unroll
+            for (int b = 0; b < AT_ONCE; b++) {
+                const int i = 32 * (k + b) + lane, from = __shfl_sync(0xFFFFFFFFu, my_row, i / COLS);
+                v[b] = from >= 0 ? __ldcg(q0 + from + i % COLS) : make_float4(0.f, 0.f, 0.f, 0.f);
             }
+#pragma unroll
+            for (int b = 0; b < AT_ONCE; b++) {
+                const int i = 32 * (k + b) + lane, r = i / COLS;
+                stage_q[r * COLS + (i % COLS + r) % COLS] = v[b];
+            }
+        }
+        __syncwarp();
+        auto q_at = [&](int c) { return stage_q[lane * COLS + (c + lane) % COLS]; };
+        float top = 0.f;
+#pragma unroll 8
+        for (int c = 0; c < COLS; c++) {
+            const float4 v = q_at(c);
+            top = fmaxf(top, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
+        }
         top *= fabsf(to_log2);
         const int e = top > 0.f ? max(-100, min(100, 127 + 8 - (int)(__float_as_uint(top) >> 23))) : 0;   // the largest element into [2^8, 2^9): 32 of them fit f16
         const float up = __uint_as_float((uint32_t)(127 + e) << 23), back = __uint_as_float((uint32_t)(127 - e) << 23);
@@ -163,11 +188,7 @@ __global__ void __launch_bounds__(APK_THREADS, 1) attn_prompt_kv4_kernel(const A
             uint32_t hi[16], lo[16];
 #pragma unroll
             for (int c = 0; c < 4; c++) {
-                float4 u = make_float4(0.f, 0.f, 0.f, 0.f), v = u;
-                if (is_row) {
-                    u = __ldcg((const float4 *)q + 8 * g + 2 * c);
-                    v = __ldcg((const float4 *)q + 8 * g + 2 * c + 1);
-                }
+                const float4 u = q_at(8 * g + 2 * c), v = q_at(8 * g + 2 * c + 1);
                 const float x[4] = {u.x, u.y, u.z, u.w}, y[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
@@ -196,6 +217,7 @@ __global__ void __launch_bounds__(APK_THREADS, 1) attn_prompt_kv4_kernel(const A
         tc_wait_st();
         tc_fence_before();
         asm volatile("bar.sync 1, 160;" ::: "memory");   // with the issuing warp: Q is in place
+        if (lane == 0) mbar_arrive(&s.q_done);           // the last stage may be filled
         // ---- tiles ----
         const int p_row = p_first + tok, lo_row = a.window > 0 ? max(0, p_row + 1 - a.window) : 0;
         float ref = -3.0e38f, l = 0.f;
@@ -422,6 +444,7 @@ __global__ void __launch_bounds__(APK_THREADS, 1) attn_prompt_kv4_kernel(const A
                 s.scale_v[j & 3] = 1.f / uv;
             }
             unsigned char *stage = ring + (j % APK_STAGES) * STAGE;
+            if (j == APK_STAGES - 1) ok = ok && mbar_wait(&s.q_done, 0);
 #pragma unroll
             for (int g = 0; g < NG; g++) {
                 // odd positions take a pair of groups the other way round: eight lanes then fill eight different 16-byte columns

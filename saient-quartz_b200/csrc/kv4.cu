@@ -272,8 +272,8 @@ void cuda_attn_prompt_kv4(float *out, const float *q, const void *d_cache, int n
     }
     // A few tokens on a long cache leave the prompt kernel, one CTA per kv head and 128 rows, with most SMs idle: there
     // the step kernel takes them one by one, all in one launch.  Time of either in us, fitted to measurements (32 / 8 heads
-    // of 128; step: 16 tokens at 1000 12.6, 64 at 1000 35, 16 at 16000 89; prompt: 128 at 1000 40, 512 at 0 26, 512 at
-    // 16000 393): a wave of units and 3.7 TB/s of cache once per token, or 1.6 per 64 positions and wave of CTAs.
+    // of 128; step: 16 tokens at 1000 12.5, 64 at 1000 35, 16 at 16000 89; prompt: 128 at 1000 37, 512 at 0 22, 512 at
+    // 16000 398): a wave of units and 3.7 TB/s of cache once per token, or 1.6 per 64 positions and wave of CTAs.
     const int G = n_heads / n_kv_heads, ctas = n_kv_heads * ((n_tok + UMMA_M / G - 1) / (UMMA_M / G)), units = n_kv_heads * ((G + 7) / 8) * n_tok;
     const double seen = window > 0 ? std::min(window, pos0 + n_tok) : pos0 + n_tok;
     const double by_step = 2 + 4.5 * std::ceil(units / (2.0 * sm_count())) + n_tok * seen * n_kv_heads * head_dim * 1.25 / 3.7e6;
