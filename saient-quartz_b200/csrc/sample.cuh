@@ -73,12 +73,11 @@ struct SampleShared {
     u64 all[SMP_BINS];                            // the row's: tokens, or weights
     union {
         u64 slice[SMP_BINS];                      // while a histogram is collected: this CTA's slice of everybody's
-        struct { u64 mine[SMP_LIST], list[SMP_LIST], list_w[SMP_LIST]; };   // gathered tokens: this CTA's; (CTA 0) the row's, their weights
+        struct { u64 mine[SMP_LIST], list[SMP_LIST], list_w[SMP_LIST]; };   // gathered tokens: this CTA's; the row's, their weights
     };
     u64 from[2][SMP_MAX_CLUSTER][2];              // what the cluster's CTAs pushed last, and before
     u64 red[SMP_WARPS];
     uint2 table[32];                              // 2^27 * 2^(-k / 32): rounded to a whole number, and that as f32
-    u64 result;
     u64 before;
     int n_mine, n_list, at, bin;
     uint16_t later[SMP_WARPS][64];                // tokens that a warp has put off
@@ -227,18 +226,15 @@ struct Sampler {
         atomicAdd(&s.part[0][b], weights ? size & 0x3FFF : 1u);
         if (weights) atomicAdd(&s.part[1][b], size >> 14);
     }
-    // The row's histogram into every CTA: this one sums a slice of all CTAs' bins and pushes it (lanes run over bins).  Weights:
+    // The row's histogram into every CTA: each gets a slice of all CTAs' bins, sums it and pushes it (lanes run over bins).  Weights:
     // the bins' sizes are in units of 2^(17 - shift), shift = b / 32 or (of a bin divided further) as given.
     __device__ __forceinline__ void collect(bool weights, int shift = -1)
     {
-        sync();
         const int per = SMP_BINS / CL;
-        for (int t = threadIdx.x; t < SMP_BINS; t += SMP_THREADS) {
-            const SampleShared *from = peer(t / per);
-            const int b = rank * per + t % per;
-            s.slice[t] = weights ? (u64)from->part[0][b] + ((u64)from->part[1][b] << 14) : from->part[0][b];
-        }
         __syncthreads();
+        for (int t = threadIdx.x; t < SMP_BINS; t += SMP_THREADS)
+            peer(t / per)->slice[rank * per + t % per] = weights ? (u64)s.part[0][t] + ((u64)s.part[1][t] << 14) : s.part[0][t];
+        sync();
         for (int t = threadIdx.x; t < SMP_BINS; t += SMP_THREADS) {
             const int k = t % per, b = rank * per + k;
             u64 sum = 0;
@@ -248,12 +244,14 @@ struct Sampler {
         sync();
     }
     // The first bin at which `above` plus the sum up to and with it reaches the goal; *before: the sum above it.
-    // (The last bin that holds anything where the goal is not reached: fewer tokens than top_k.)
-    __device__ __forceinline__ int boundary(u64 above, double goal, u64 *before)
+    // (The last bin that holds anything where the goal is not reached: fewer tokens than top_k.)  part < 0: `goal` is the goal,
+    // else that part of the sum over all bins, and becomes it.
+    __device__ __forceinline__ int boundary(u64 above, double &goal, u64 *before, double part = -1.0)
     {
         u64 v[SMP_PER], total, mine = 0;
         for (int k = 0; k < SMP_PER; k++) mine += v[k] = s.all[SMP_PER * threadIdx.x + k];
         u64 sum = above + smp_before(mine, s.red, &total);
+        if (part >= 0.0) goal = part * (double)total;
         for (int k = 0; k < SMP_PER; k++) {
             if (v[k] && (double)sum < goal && (goal <= (double)(sum + v[k]) || sum + v[k] == above + total)) {
                 s.bin = SMP_PER * threadIdx.x + k;
@@ -267,16 +265,17 @@ struct Sampler {
         __syncthreads();   // (read before the next clear)
         return b;
     }
-    // The tokens for which pred holds, as numbers, in CTA 0's list (it takes them all: the caller has counted)
+    // The tokens for which pred holds, as numbers, in the first `lists` CTAs' lists (a list takes them all: the caller has counted)
     template <class Pred>
-    __device__ __forceinline__ void gather(Pred pred)
+    __device__ __forceinline__ void gather(int lists, Pred pred)
     {
         for (int i = threadIdx.x; i < n; i += SMP_THREADS)
             if (pred(i)) s.mine[atomicAdd(&s.n_mine, 1)] = number(i);
         __syncthreads();
         if (threadIdx.x == 0) s.at = atomicAdd(&peer(0)->n_list, s.n_mine);
         __syncthreads();
-        for (int i = threadIdx.x; i < s.n_mine; i += SMP_THREADS) peer(0)->list[s.at + i] = s.mine[i];
+        for (int i = threadIdx.x; i < s.n_mine; i += SMP_THREADS)
+            for (int r = 0; r < lists; r++) peer(r)->list[s.at + i] = s.mine[i];
         sync();
     }
     // Number of the last token with `above` + (weights, or count, of the set's tokens before it) < goal, given that it is
@@ -321,25 +320,25 @@ struct Sampler {
             if (lo == hi) return hi;
             ranged = true;
         }
-        gather([&](int i) {
+        gather(CL, [&](int i) {
             if (!ranged) return in_set(i) && bin(z[i]) == b;
             const u64 x = number(i);
             return x >= lo && x <= hi;
         });
-        if (rank == 0) {
-            const int c = s.n_list;
-            const u64 x = (int)threadIdx.x < c ? s.list[threadIdx.x] : 0;
-            if ((int)threadIdx.x < c) s.list_w[threadIdx.x] = weights ? weight_of(x) : 1;
-            __syncthreads();
-            u64 before = above;
-            if ((int)threadIdx.x < c)
-                for (int j = 0; j < c; j++) before += s.list[j] > x ? s.list_w[j] : 0;
-            const u64 last = ~smp_reduce<true>((int)threadIdx.x < c && (double)before < goal ? ~x : 0, s.red);
-            if ((int)threadIdx.x < CL) peer(threadIdx.x)->result = last;
-        }
-        sync();
+        // each CTA ranks every CL-th token of the list, CL threads to a token
+        const int c = peer(0)->n_list, e = rank + CL * ((int)threadIdx.x / CL), first = (int)threadIdx.x % CL;
+        if ((int)threadIdx.x < c) s.list_w[threadIdx.x] = weights ? weight_of(s.list[threadIdx.x]) : 1;
+        __syncthreads();
+        const u64 x = e < c ? s.list[e] : 0;
+        u64 before = 0;
+        if (e < c)
+            for (int j = first; j < c; j += CL) before += s.list[j] > x ? s.list_w[j] : 0;
+        for (int o = CL >> 1; o > 0; o >>= 1) before += __shfl_xor_sync(0xFFFFFFFFu, before, o);
+        u64 last = smp_reduce<true>(e < c && (double)(above + before) < goal ? ~x : 0, s.red);
+        exchange(last, 0);
+        for (int r = 0; r < CL; r++) last = max(last, s.from[turn][r][0]);
         no_list();
-        return s.result;
+        return ~last;
     }
     // At most so many tokens make up v, tokens or weights of bin b (a token's weight is 2^(-b / 32) within 1.1 per cent)
     __device__ __forceinline__ u64 held_by(u64 v, bool weights, int b) const
@@ -435,10 +434,11 @@ __global__ void __launch_bounds__(SMP_THREADS) sample_kernel(const SampleArgs a)
             if (c.in_set(i)) c.add(c.bin(z[i]), false, 0);
         c.collect(false);
         u64 before;
-        const int b = c.boundary(0, (double)a.top_k, &before);
+        double goal = a.top_k;
+        const int b = c.boundary(0, goal, &before);
         const u64 in_bin = s.all[b];
         if (before + in_bin <= SMP_LIST) {
-            c.gather([&](int i) { return c.in_set(i) && c.bin(z[i]) <= b; });
+            c.gather(1, [&](int i) { return c.in_set(i) && c.bin(z[i]) <= b; });
             if (c.rank != 0) return;   // (nobody pushes to this CTA or reads from it any more)
             const int m = s.n_list;
             const u64 x = tid < m ? s.list[tid] : 0;
@@ -465,7 +465,7 @@ __global__ void __launch_bounds__(SMP_THREADS) sample_kernel(const SampleArgs a)
             }
             return;
         }
-        c.keep_to(c.last_in_bin(b, in_bin, before, (double)a.top_k, false));
+        c.keep_to(c.last_in_bin(b, in_bin, before, goal, false));
         if (by_p) c.clear();
     }
     if (by_p) {
@@ -477,11 +477,9 @@ __global__ void __launch_bounds__(SMP_THREADS) sample_kernel(const SampleArgs a)
             if (c.in_set(i)) c.add(b, true, v);
         }
         c.collect(true);
-        u64 all = 0, before;
-        for (int k = 0; k < SMP_PER; k++) all += s.all[SMP_PER * tid + k];
-        all = smp_reduce<false>(all, s.red);
-        const double goal = (double)a.top_p * (double)all;
-        const int b = c.boundary(0, goal, &before);
+        u64 before;
+        double goal;
+        const int b = c.boundary(0, goal, &before, (double)a.top_p);
         c.keep_to(c.last_in_bin(b, c.held_by(s.all[b], true, b), before, goal, true));
     }
     // ---- 4. the token ----
