@@ -258,7 +258,9 @@ void cuda_attn_prompt(float *out, const float *q, const float *k_cache, const fl
  *                           in one launch whose shape does not depend on the position.  The new position takes part
  *                           with the values that it has in the cache.  theta <= 0: q and k_new are taken as they are
  *                           (already rotated, or a layer without rotation); k_new and v_new NULL: nothing is
- *                           appended, the cache holds the position already.
+ *                           appended, the cache holds the position already.  Long contexts are merged in a workspace
+ *                           of the library, one for every stream and for every graph that is being captured: graphs
+ *                           may replay side by side, two executables of one captured graph may not.
  *   cuda_attn_prompt_kv4    cuda_attn_prompt over such a cache (rows appended before, e.g. by cuda_rope_kv4_rows) */
 size_t cuda_kv4_bytes(int max_seq, int n_kv_heads, int head_dim);
 void cuda_kv4_append_rows(void *d_cache, const float *k, const float *v, int n_tok, int n_kv_heads, int head_dim, int max_seq, int pos0);
@@ -280,9 +282,10 @@ void cuda_attn_prompt_kv4(float *out, const float *q, const void *d_cache, int n
  * <= 0: the first only), of those the ones that weigh at least min_p (<= 0: all; above 1 counts as 1).  The answer
  * is the first token in the order of the vocabulary at which the running sum of the kept weights exceeds u times their
  * total; u below 0 or NaN counts as 0, from 1 on the last token of weight is taken.  Weights are whole numbers of
- * units of 2^-44, rounded down: a token below one unit is never chosen.  temperature 0: the largest logit, ties to the lower index (d_u may be NULL), probability 1.  Logits of -inf
- * and NaN are never chosen; a row without any other gives token -1, probability 0.  The sums are exact integers: the
- * same inputs give the same token however the work is split.  vocab <= 524288, finite temperature >= 0.
+ * units of 2^-44, rounded down: a token below one unit is never chosen, nor is one whose logit lies further below the
+ * largest than f32 reaches.  temperature 0: the largest logit, ties to the lower index (d_u may be NULL), probability 1.
+ * Logits of -inf and NaN are never chosen; a row without any other gives token -1, probability 0.  The sums are exact
+ * integers: the same inputs give the same token however the work is split.  vocab <= 524288, finite temperature >= 0.
  * cuda_step_advance: d_step[0] = *d_token (left as it is if that is negative), d_step[1] += 1, and the registered RoPE
  * tables of d_step (cuda_step_rope_table) for the new position: the device-side cuda_step_set, on the same stream. */
 void cuda_sample(const float *d_logits, int n_rows, int vocab, size_t row_stride, float temperature, int top_k, float top_p, float min_p,

@@ -563,7 +563,7 @@ __global__ void __launch_bounds__(AK_THREADS, NT == 1 ? 2 : 1) attn_step_kv4_ker
             for (int j = 0; j < NG; j++) x[j] = 0.f;
         }
         // 2^e brings the largest element into [2^13, 2^14)
-        const int e = top > 0.f ? max(-100, min(100, 127 + 13 - (int)(__float_as_uint(top) >> 23))) : 0;
+        const int e = top > 0.f ? max(-120, min(100, 127 + 13 - (int)(__float_as_uint(top) >> 23))) : 0;
         const float up = __uint_as_float((uint32_t)(127 + e) << 23);
         float *head_qs = qs + h * (NG + 1);
         if (lane == 0) head_qs[NG] = 1.f / up;

@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(APK_THREADS, 1) attn_prompt_kv4_kernel(const A
             top = fmaxf(top, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
         }
         top *= fabsf(to_log2);
-        const int e = top > 0.f ? max(-100, min(100, 127 + 8 - (int)(__float_as_uint(top) >> 23))) : 0;   // the largest element into [2^8, 2^9): 32 of them fit f16
+        const int e = top > 0.f ? max(-120, min(100, 127 + 8 - (int)(__float_as_uint(top) >> 23))) : 0;   // the largest element into [2^8, 2^9): 32 of them fit f16
         const float up = __uint_as_float((uint32_t)(127 + e) << 23), back = __uint_as_float((uint32_t)(127 - e) << 23);
         float sum[4] = {0.f, 0.f, 0.f, 0.f};   // of q over the groups
 #pragma unroll
@@ -351,8 +351,8 @@ __global__ void __launch_bounds__(APK_THREADS, 1) attn_prompt_kv4_kernel(const A
         uint32_t kw[NG], vw[NG], kp[NG], vp[NG], kw1[NG], vw1[NG], kp1[NG], vp1[NG];
         const uint8_t *at0 = head_blocks + (size_t)(b0 + p_tile / KV4_BLOCK) * (40 * HD) + 4 * NG * (p_tile % KV4_BLOCK);   // (a tile is two blocks on)
         auto fetch = [&](int j) {
-            const int pos = base0 + APK_BN * j + p_tile;
-            if ((unsigned)(pos - k_lo) <= (unsigned)(p_last - k_lo)) {
+            const unsigned pos = (unsigned)base0 + APK_BN * j + p_tile;   // (may pass 2^31 where a cache ends there)
+            if (pos - k_lo <= (unsigned)(p_last - k_lo)) {
                 const uint8_t *at = at0 + (size_t)j * (2 * 40 * HD);
                 ldg_words<NG>(at + 16 * HD, kp1);
                 ldg_words<NG>(at + 36 * HD, vp1);

@@ -14,6 +14,20 @@ bool activation_slot(int slot, int n, XQOut *o);
 // the (cos, sin) table registered for these step words and parameters, or NULL
 const float2 *step_rope_table(const int *d_step, int head_dim, float theta, float yarn_scale, int yarn_orig_ctx);
 
+// What is set once per device, as a kernel's attributes are.  (Devices beyond the table: every time.)
+struct PerDevice {
+    bool done[16] = {};
+    template <class F>
+    void once(F f)
+    {
+        int device = 0;
+        if (cudaGetDevice(&device) != cudaSuccess) cudaGetLastError();
+        if (device < 16 && done[device]) return;
+        f();
+        if (device < 16) done[device] = true;
+    }
+};
+
 // Ordinary launch, or programmatic dependent launch when enabled; cluster > 1: clusters of that many CTAs along x.
 template <class... KArgs, class... Args>
 static void launch_cluster(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, int cluster, Args... args)

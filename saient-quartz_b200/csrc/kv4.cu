@@ -44,11 +44,14 @@ struct StepShape {
 template <int NG, int NT>
 StepShape step_shape(int units, int n_blocks, int GV)
 {
-    static int fit[4 * NT + 1][4] = {};   // clusters of 1, 2, 4, 8 CTAs that the device holds at once
+    static int fit[4 * NT + 1][4] = {};   // clusters of 1, 2, 4, 8 CTAs that the device holds at once (every B200 alike)
+    static PerDevice ready;
     int (&f)[4] = fit[GV];
-    if (!f[0]) {
-        const auto kernel = attn_step_kv4_kernel<NG, NT>;
+    const auto kernel = attn_step_kv4_kernel<NG, NT>;
+    ready.once([&] {
         QZ_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, attn_kv4_smem(NG, NT, 4 * NT, 8).total));
+    });
+    if (!f[0]) {
         for (int i = 0; i < 4; i++) {
             cudaLaunchConfig_t cfg = {};
             cudaLaunchAttribute at[1];
@@ -286,11 +289,10 @@ void cuda_attn_prompt_kv4(float *out, const float *q, const void *d_cache, int n
     AttnPromptKv4Args a = {out, q, (const uint8_t *)d_cache, n_tok, n_heads, n_kv_heads, kv4_blocks(max_seq), pos0, window, UMMA_M / G,
                            scale, sinks, status_word_if_ready()};
     by_groups(head_dim, [&](auto ng) {
-        static bool ready = false;
-        if (!ready) {
+        static PerDevice ready;
+        ready.once([&] {
             QZ_CUDA_CHECK(cudaFuncSetAttribute(attn_prompt_kv4_kernel<ng.value>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)attn_prompt_kv4_smem(ng.value)));
-            ready = true;
-        }
+        });
         launch(attn_prompt_kv4_kernel<ng.value>, dim3(n_kv_heads, (n_tok + a.tq - 1) / a.tq), dim3(APK_THREADS), attn_prompt_kv4_smem(ng.value), a);
     });
 }

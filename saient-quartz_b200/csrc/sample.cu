@@ -8,16 +8,15 @@ namespace {
 
 size_t sample_smem(int chunk) { return ((sizeof(SampleShared) + 15) & ~(size_t)15) + (size_t)chunk * 4; }
 
-// CTAs per row: enough for two CTAs and their parts of rows to fit an SM (16 for the longest rows), then, while that leaves SMs idle, more of them as long as a
-// thread keeps four tokens (the device holds 7 clusters of 16).
+// CTAs per row: enough for two CTAs and their parts of rows to fit an SM (16 for the longest rows), then, while that leaves
+// SMs idle, more of them as long as a thread keeps four tokens (the device holds 7 clusters of 16).
 int sample_cluster(int n_rows, int vocab)
 {
-    static bool ready = false;
-    if (!ready) {
+    static PerDevice ready;
+    ready.once([] {
         QZ_CUDA_CHECK(cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
         if (cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) cudaGetLastError();
-        ready = true;
-    }
+    });
     int cl = 1;
     while (cl < SMP_MAX_CLUSTER && sample_smem((vocab + cl - 1) / cl + 3) > 112 * 1024) cl *= 2;
     while (cl < SMP_MAX_CLUSTER && (long long)n_rows * cl * 2 <= (cl == 8 ? 112 : sm_count()) && vocab / (cl * 2) >= 4 * SMP_THREADS) cl *= 2;

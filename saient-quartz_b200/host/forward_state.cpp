@@ -267,12 +267,11 @@ int qh_get_kv(qh_model *m, int layer, float *k, float *v, int pos0, int n_pos)
     const size_t off = (size_t)pos0 * m->kv_d() * 4, bytes = (size_t)n_pos * m->kv_d() * 4;
     if (m->kv_bits == 4) {
         GpuBuf dk, dv;
+        if (n_pos == 0) return 0;
         if (!dk.alloc_f32(bytes / 4) || !dv.alloc_f32(bytes / 4)) return -2;
         cuda_kv4_read_rows(dk.f(), dv.f(), m->kv4[layer].ptr, n_pos, m->c.n_kv_heads, m->c.head_dim, m->c.max_seq, pos0);
-        if (bytes) {
-            cuda_d2h(k, dk.ptr, bytes);
-            cuda_d2h(v, dv.ptr, bytes);
-        }
+        cuda_d2h(k, dk.ptr, bytes);
+        cuda_d2h(v, dv.ptr, bytes);
         cuda_sync();
         return quartz_last_error() == 0 ? 0 : -10;
     }

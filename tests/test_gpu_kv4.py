@@ -328,6 +328,103 @@ def run_prompt(gpu, nh, n_kv, hd, n, pos0, window, sinks, sharp=1.0):
     assert np.array_equal(cache.download(np.uint8), raw)
 
 
+# Long enough that the call takes the tensor-core kernel (fewer tokens go through the step kernel).
+@pytest.mark.parametrize("nh,n_kv,hd,n", [(8, 2, 64, 700), (32, 8, 128, 515), (5, 1, 96, 1100), (6, 3, 32, 801), (16, 1, 128, 1000), (3, 3, 64, 703),
+                                          (14, 2, 96, 700), (24, 3, 128, 690)])
+@pytest.mark.parametrize("pos0,window", [(0, 0), (93, 0), (0, 33), (450, 100), (31, 129)])
+def test_prompt_tiles(gpu, nh, n_kv, hd, n, pos0, window):
+    run_prompt(gpu, nh, n_kv, hd, n, pos0, window, sinks=pos0 % 2 == 1, sharp=4.0 if window == 100 else 1.0)
+
+
+def test_prompt_queries_of_any_size(gpu):
+    """Scores that single one position out, scores that all but vanish, and queries near both ends of f32."""
+    L, r = gpu.lib(), rng(31)
+    nh, n_kv, hd, n = 16, 8, 64, 515
+    k, v = rows(r, n, n_kv, hd, True), rows(r, n, n_kv, hd, False)
+    cache = upload(gpu, kv4.store(np.full(kv4.nbytes(n, n_kv, hd), 0xFF, np.uint8), k, v, 0, n))
+    q = r.standard_normal((n, nh, hd), dtype=np.float32)
+    q *= np.exp2(r.integers(-10, 11, (n, nh, 1))).astype(np.float32)
+    dq, out = upload(gpu, q), gpu.GpuBuf.alloc_f32(q.size)
+    L.cuda_attn_prompt_kv4(out.ptr, dq.ptr, cache.ptr, n, nh, n_kv, hd, n, 0, 0, 0.125, None)
+    got = out.download().reshape(q.shape)
+    gpu.check_error()
+    want, bound = kv4.attention(q, kv4.values(k), kv4.values(v), 0, 0, 0.125, None)
+    # A value is summed as p d (code - 8) and p (m + 8 d), which cancel where one position decides and its value is near zero
+    # (the bound above counts |value|).  With A the larger end of the group's range, 15 d <= 2 A, the two are at most 16 / 15 A
+    # and A; either carries 22 bits of p and one f32 rounding, 2^-22 + 2^-24: in all (31 / 15) 1.25 2^-22 A < 2^-20 A a position,
+    # and the weights sum to one.  A exceeds the group's largest value by the rounding of d only (2^-10).
+    seen = np.maximum.accumulate(np.abs(kv4.values(v)).max(-1), 0).repeat(nh // n_kv, 1)[..., None]
+    assert (np.abs(got - want) <= bound + 2.0 ** -20 * seen).all()
+    # one key towers over the others: with |q| = 2^120 its row is the answer, with 2^-120 the mean is
+    k = np.zeros_like(k)
+    k[0] = 1.0
+    put(gpu, cache, kv4.store(np.full(kv4.nbytes(n, n_kv, hd), 0xFF, np.uint8), k, v, 0, n))
+    vv = kv4.values(v)
+    for e, answer in ((120, np.broadcast_to(vv[:1], vv.shape)), (-120, np.cumsum(vv, 0) / np.arange(1, n + 1)[:, None, None])):
+        put(gpu, dq, np.full(q.shape, 2.0 ** e, np.float32))
+        for tokens in (n, 1):       # the step kernel too
+            L.cuda_attn_prompt_kv4(out.ptr, dq.ptr, cache.ptr, tokens, nh, n_kv, hd, n, n - tokens, 0, 0.125, None)
+            got = out.download(count=tokens * nh * hd).reshape(tokens, nh, hd)
+            want = answer[n - tokens:].repeat(nh // n_kv, 1)
+            # a mean of n values of about 1: n roundings of 2^-24 each at most, and 2^-22 of each term
+            assert np.abs(got - want).max() <= (n * 2.0 ** -24 + 2.0 ** -21) * np.abs(vv).max(), (e, tokens)
+    gpu.check_error()
+
+
+def test_prompt_scales_of_values_far_apart(gpu):
+    """Steps that differ by 2^20 between positions and groups, some of them past 8188 in keys or in values; minima past f16's range."""
+    L, r = gpu.lib(), rng(32)
+    for nh, n_kv, hd, n in ((16, 8, 128, 515), (12, 6, 96, 515)):
+        k, v = rows(r, n, n_kv, hd, False), rows(r, n, n_kv, hd, False)
+        g = hd // 32
+        v *= np.exp2(r.integers(-10, 11, (n, n_kv, g))).repeat(32, -1).astype(np.float32)
+        v[100:103] *= 65000.0                    # spans of up to 2^17 and more: the largest step f16 holds
+        v[300, :, :32] = np.linspace(-65504, 65504, 32)
+        k[200, :, :32] = np.linspace(-65504, 65504, 32)
+        k[201, :, 3] = 9e4
+        q = r.standard_normal((n, nh, hd), dtype=np.float32) * np.float32(2.0 ** -14)
+        cache = upload(gpu, kv4.store(np.full(kv4.nbytes(n, n_kv, hd), 0xFF, np.uint8), k, v, 0, n))
+        dq, out = upload(gpu, q), gpu.GpuBuf.alloc_f32(q.size)
+        L.cuda_attn_prompt_kv4(out.ptr, dq.ptr, cache.ptr, n, nh, n_kv, hd, n, 0, 0, 0.088, None)
+        got = out.download().reshape(q.shape)
+        gpu.check_error()
+        want, bound = kv4.attention(q, kv4.values(k), kv4.values(v), 0, 0, float(np.float32(0.088)), None)
+        # weights carry 22 bits; a tile's values are scaled by its largest (2^-20 of what the row has seen)
+        seen = np.maximum.accumulate(np.abs(kv4.values(v)).max(-1), 0).repeat(nh // n_kv, 1)[..., None]
+        assert (np.abs(got - want) <= bound + 2.0 ** -20 * seen).all()
+
+
+def test_prompt_propagates_nan(gpu):
+    """A NaN among a group's keys reaches every output of the rows that see it, one among its values that group's alone; rows
+    before it, rows whose window has passed it and other heads are untouched."""
+    L, r = gpu.lib(), rng(33)
+    for nh, n_kv, hd, n in ((16, 8, 128, 515), (12, 6, 96, 515)):
+        G = nh // n_kv
+        k, v = rows(r, n, n_kv, hd, True), rows(r, n, n_kv, hd, False)
+        q = r.standard_normal((n, nh, hd), dtype=np.float32)
+        dq, out = upload(gpu, q), gpu.GpuBuf.alloc_f32(q.size)
+        bad_k, bad_v = k.copy(), v.copy()
+        bad_k[300, 2, 5] = np.nan
+        bad_v[131, 4, 40] = np.inf               # group 1 of kv head 4
+        bad_v[400, 4, 70] = np.nan               # and group 2, later
+        for window in (0, 60):
+            raw = kv4.store(np.full(kv4.nbytes(n + 40, n_kv, hd), 0xFF, np.uint8), bad_k, bad_v, 0, n + 40)
+            cache = upload(gpu, raw)
+            L.cuda_attn_prompt_kv4(out.ptr, dq.ptr, cache.ptr, n, nh, n_kv, hd, n + 40, 0, window, 0.088, None)
+            got = out.download().reshape(q.shape)
+            gpu.check_error()
+            want, bound = kv4.attention(q, kv4.values(k), kv4.values(v), 0, window, float(np.float32(0.088)), None)
+            t = np.arange(n)
+            hit = np.zeros(q.shape, bool)
+            sees = lambda p: (t >= p) & (t < p + window if window else True)
+            hit[sees(300), 2 * G:3 * G] = True
+            hit[sees(131), 4 * G:5 * G, 32:64] = True
+            hit[sees(400), 4 * G:5 * G, 64:96] = True
+            assert (np.isnan(got) == hit).all()
+            # (the clean values differ where a NaN is hit only: rows elsewhere do not see positions 300, 131 or 400 of those heads' groups)
+            assert (np.abs(got - want) <= bound)[~hit].all()
+
+
 # ---- together, and where the machinery can go wrong --------------------------------------------------------------
 def test_prompt_then_steps(gpu):
     """A prompt appended and attended to, then tokens one at a time, each through one recorded graph: the run of a

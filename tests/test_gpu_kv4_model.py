@@ -165,3 +165,10 @@ def test_generate_to_the_last_position_and_refusals(gpu, oracle_mod):
         HostModel(kv_bits=4, vocab_size=320, embed_dim=2048, n_heads=32, n_kv_heads=1, n_layers=1, ffn_dim=4096, head_dim=64, rope_theta=1e4, max_seq=8)
     assert m.H.qh_set_kv_bits(m.m, 32) == -1      # too late
     gpu.lib().quartz_clear_error()
+
+
+def test_no_positions(gpu, oracle_mod):
+    m = _model(n_layers=1, max_seq=40)
+    k, v = m.read_kv(0, 3, 0)
+    assert k.size == v.size == 0
+    gpu.check_error()
