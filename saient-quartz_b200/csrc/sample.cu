@@ -1,4 +1,7 @@
 // C entry point of the token sampler.
+#include <algorithm>
+#include <cmath>
+
 #include "host.cuh"
 #include "sample.cuh"
 
@@ -42,6 +45,8 @@ extern "C" void cuda_sample(const float *d_logits, int n_rows, int vocab, size_t
         return;
     }
     const int cl = sample_cluster(n_rows, vocab), chunk = ((vocab + cl - 1) / cl + 3) & ~3;
-    const SampleArgs a = {d_logits, row_stride, vocab, temperature, top_k, top_p, min_p, d_u, d_tokens, d_probs, chunk};
+    const double inv_t = 1.0 / (double)temperature, c = 32.0 * 1.4426950408889634 * inv_t, lowest = std::min((double)min_p, 1.0);
+    const SampleArgs a = {d_logits, row_stride, vocab, temperature, inv_t, c, 1.0 / c, top_k, top_p, lowest,
+                          lowest > 0.0 ? (float)std::log(lowest) : 0.f, d_u, d_tokens, d_probs, chunk};
     launch_cluster(sample_kernel, dim3((unsigned)n_rows * cl), dim3(SMP_THREADS), sample_smem(chunk), cl, a);
 }

@@ -9,12 +9,14 @@
 // Weights are held as 64-bit integers in units of 2^-44, so that every sum is exact and does not depend on its order:
 // 2^19 tokens of weight 1 still fit.  A logit of -inf or NaN has no weight and is never chosen.
 //
-// A weight is 2^(-t / 32), t = 32 log2(e) (M - z) / T.  With b the whole number next to t it is 2^(-b / 32), from a table of
-// 32 by b mod 32 and a shift, times 1 - r, r from four terms of the exponential's series (|y| < 0.011: 2e-11).  Only r E
-// is taken in 32 bits, so a weight is right to 2^-29, and t as a sum of two f32 numbers: M - z is exact as one, and no
-// 64-bit arithmetic is needed (CUDA's exp in 64 bits took twice the time of the rest).  Why so exact: with thousands of
-// tokens kept, an error of 1e-7 in their sums would move the border of top_p, or the token that u falls on, once in some
-// thousand rows.  b is also the bin in which tokens are counted: it follows the order of the logits.
+// With c = 32 log2(e) / T as a sum of two f32 numbers, z c is a whole number k and a rest f, |f| < 0.8: one FMA rounds z c to
+// k, two more give f with an error of 2^-26.  The weight is then 2^((k - k_M) / 32), from a table of 32 and a shift, times
+// 2^((f - f_M) / 32): the table carries f_M, four terms of the exponential's series give the rest (|y| < 0.017: 1e-11), and
+// only table times series is taken in 32 bits, so a weight is right to 2^-28.  (CUDA's exp in 64 bits took twice the time
+// of the rest.)  Where z c passes 2^22, at temperatures near 0 or logits of any size, M - z takes the place of z, exact as two
+// f32 numbers.  Why so exact: with thousands of tokens kept, an error of 1e-7 in their sums would move the border of top_p, or
+// the token that u falls on, once in some thousand rows.  b = k_M - k is also the bin in which tokens are counted: it follows
+// the order of the logits.
 #pragma once
 
 #include <cooperative_groups.h>
@@ -33,8 +35,11 @@ struct SampleArgs {
     size_t ld;
     int vocab;
     float temperature;
+    double inv_t, c, one_over_c;   // 1 / temperature; 32 log2(e) / temperature
     int top_k;
-    float top_p, min_p;
+    float top_p;
+    double min_p;        // (at most 1)
+    float log_min_p;
     const float *u;
     int *tokens;
     float *probs;
@@ -60,8 +65,8 @@ __device__ __forceinline__ float smp_unkey(uint32_t k) { return __uint_as_float(
 //      and ranked against one another.  When all tokens down to that bin fit the list (k up to some hundreds), everything
 //      else is done on the list.
 //   3. top_p: the same with a histogram of the weights, bin by bin in units of the bin's own size.
-//   4. the kept weights are summed warp by warp in the order of the vocabulary; the warp in whose range u falls walks its
-//      part.  (Few tokens are kept as a rule: a warp collects them and weighs 32 at a time.)
+//   4. the kept weights are summed warp by warp in the order of the vocabulary; the part of the warp in whose
+//      range u falls is weighed again, token by token.  (Few are kept as a rule: a warp collects them and weighs 32 at a time.)
 // A bin with more tokens than the list takes (ties, high temperatures) is divided further, by the number itself.
 // A histogram is reduced in slices, one per CTA, that are pushed to every CTA: all find the same bin without asking.
 constexpr int SMP_PER = 3, SMP_BINS = SMP_PER * SMP_THREADS, SMP_LIST = 512;   // (a thread looks after three bins, and one token of the list)
@@ -77,31 +82,25 @@ struct SampleShared {
     };
     u64 from[2][SMP_MAX_CLUSTER][2];              // what the cluster's CTAs pushed last, and before
     u64 red[SMP_WARPS];
-    uint2 table[32];                              // 2^27 * 2^(-k / 32): rounded to a whole number, and that as f32
+    uint2 table[32];                              // 2^27 * 2^(-(k + f_M) / 32): rounded to a whole number, and that as f32
     u64 before;
     int n_mine, n_list, at, bin;
-    uint16_t later[SMP_WARPS][64];                // tokens that a warp has put off
+    uint16_t later[SMP_WARPS][160];               // tokens that a warp has put off
 };
 
-// sum, or largest, over the block; every thread gets it
-template <bool MAX>
-__device__ __forceinline__ u64 smp_reduce(u64 v, u64 *sm)
+// largest over the warp, and over the block; every thread gets it
+__device__ __forceinline__ u64 smp_warp_largest(u64 v)
 {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const u64 y = __shfl_xor_sync(0xFFFFFFFFu, v, o);
-        v = MAX ? (v > y ? v : y) : v + y;
-    }
+    const uint32_t hi = __reduce_max_sync(0xFFFFFFFFu, (uint32_t)(v >> 32));
+    return (u64)hi << 32 | __reduce_max_sync(0xFFFFFFFFu, (uint32_t)(v >> 32) == hi ? (uint32_t)v : 0);
+}
+__device__ __forceinline__ u64 smp_largest(u64 v, u64 *sm)
+{
+    v = smp_warp_largest(v);
     __syncthreads();
     if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = v;
     __syncthreads();
-    v = (threadIdx.x & 31) < SMP_WARPS ? sm[threadIdx.x & 31] : 0;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const u64 y = __shfl_xor_sync(0xFFFFFFFFu, v, o);
-        v = MAX ? (v > y ? v : y) : v + y;
-    }
-    return v;
+    return smp_warp_largest((threadIdx.x & 31) < SMP_WARPS ? sm[threadIdx.x & 31] : 0);
 }
 __device__ __forceinline__ u64 smp_warp_inclusive(u64 v)
 {
@@ -131,38 +130,85 @@ struct Sampler {
     const float *z;       // this CTA's part of the row
     int n, base;          // tokens in it, index of the first
     int CL, rank, turn;
-    float M, c_hi, c_lo;  // t = (M - z) * (c_hi + c_lo)
+    float M, c_hi, c_lo;  // c = c_hi + c_lo
+    bool plain;           // z c stays below 2^22
+    float low;            // plain: all logits up to here share the last bin
+    int top;              // plain: the bits of 1.5 * 2^23 + k_M
     float keep_z;         // the set: logits above keep_z, and those equal to it with an index up to keep_i
     int keep_i;
 
     __device__ __forceinline__ SampleShared *peer(int r) const { return cooperative_groups::this_cluster().map_shared_rank(&s, r); }
     __device__ __forceinline__ void sync() const { cooperative_groups::this_cluster().sync(); }
-    __device__ __forceinline__ bool in_set(int i) const { return z[i] > keep_z || (z[i] == keep_z && base + i <= keep_i); }
+    __device__ __forceinline__ bool in_set(float x, int i) const { return x > keep_z || (x == keep_z && base + i <= keep_i); }
+    // f(logit, i) for this CTA's tokens i, in any order (-inf behind the last)
+    template <class F>
+    __device__ __forceinline__ void each(F f) const
+    {
+#pragma unroll 2
+        for (int i = threadIdx.x; 4 * i < n; i += SMP_THREADS) {
+            const float4 v = ((const float4 *)z)[i];
+            f(v.x, 4 * i);
+            f(v.y, 4 * i + 1);
+            f(v.z, 4 * i + 2);
+            f(v.w, 4 * i + 3);
+        }
+    }
     __device__ __forceinline__ void keep_to(u64 last)
     {
         keep_z = smp_unkey((uint32_t)(last >> 32));
         keep_i = (int)~(uint32_t)last;
     }
     __device__ __forceinline__ u64 number(int i) const { return (u64)smp_key(z[i]) << 32 | (uint32_t)~(base + i); }
-    // the whole number next to t, at most SMP_BINS - 1 (which also takes M = inf and T = 0's neighbours, where t is not a number)
+    // (ends with the threads synchronised)
+    __device__ __forceinline__ void scale(double c, double one_over_c)
+    {
+        constexpr double LAST = SMP_BINS - 1;
+        const double Mc = (double)M * c;
+        c_hi = (float)c;
+        c_lo = isinf(c_hi) ? 0.f : (float)(c - (double)c_hi);
+        plain = fabs(Mc) < 4190000.0 && c_hi < 1e30f && c_hi > 1e-30f;
+        low = -INFINITY;
+        top = __float_as_int(fmaf(M, c_hi, 12582912.f));   // 1.5 * 2^23: the sum's low bits are the nearest integer
+        if (plain) {
+            const float last = (float)((Mc - LAST) * one_over_c);   // (its product is off by 1/4 at most: bin LAST - 1, LAST or LAST + 1)
+            low = bin(last) == SMP_BINS - 1 ? last : (float)((Mc - LAST + 0.75) * one_over_c);
+        }
+        if (threadIdx.x < 32) {
+            const double f = plain ? Mc - (double)(top - 0x4B400000) : 0.0;
+            const uint32_t e = (uint32_t)rint(exp2(27.0 - ((double)threadIdx.x + f) / 32.0));
+            s.table[threadIdx.x] = make_uint2(e, __float_as_uint((float)e));
+        }
+        __syncthreads();
+    }
+    // b, at most SMP_BINS - 1
     __device__ __forceinline__ int bin(float x) const
     {
-        const float t = x == M ? 0.f : __fmul_rn(M - x, c_hi);
+        if (plain) return top - __float_as_int(fmaf(fmaxf(x, low), c_hi, 12582912.f));   // (NaN goes with the lowest)
+        const float t = x == M ? 0.f : __fmul_rn(M - x, c_hi);   // (M = inf, T = 0's neighbours: t may not be a number)
         return t < (float)(SMP_BINS - 1) ? __float2int_rn(t) : SMP_BINS - 1;
     }
     // the weight of logit x is size << 17 >> b / 32, b its bin
     __device__ __forceinline__ uint32_t size(float x, int &b) const
     {
-        const float d = M - x, back = d - M, rest = (M - (d - back)) - (x + back);   // d + rest = M - x exactly
-        const float t = __fmul_rn(d, c_hi), t_lo = fmaf(d, c_hi, -t) + fmaf(d, c_lo, rest * c_hi);
-        const float whole = __fadd_rn(t, 12582912.f);   // 1.5 * 2^23: the sum's low bits are t's nearest integer
-        const bool far = !(t < (float)(SMP_BINS - 1)), top = x == M;
-        b = top ? 0 : far ? SMP_BINS - 1 : __float_as_int(whole) - 0x4B400000;
-        const float y = ((t - (whole - 12582912.f)) + t_lo) * 0.0216608494f;   // ln 2 / 32
-        const float r = y * fmaf(y, fmaf(y, fmaf(y, -1.f / 24, 1.f / 6), -0.5f), 1.f);
+        float f;
+        bool far = false;
+        if (plain) {
+            const float y = fmaxf(x, low), whole = fmaf(y, c_hi, 12582912.f);
+            b = top - __float_as_int(whole);
+            f = fmaf(y, c_lo, fmaf(y, c_hi, 12582912.f - whole));
+        } else {
+            const float d = M - x, back = d - M, rest = (M - (d - back)) - (x + back);   // d + rest = M - x exactly
+            const float t = __fmul_rn(d, c_hi), t_lo = fmaf(d, c_hi, -t) + fmaf(d, c_lo, rest * c_hi);
+            const bool first = x == M;
+            far = !first && !(t < (float)(SMP_BINS - 1));
+            b = first ? 0 : far ? SMP_BINS - 1 : __float2int_rn(t);
+            f = first || far ? 0.f : ((float)b - t) - t_lo;
+        }
+        constexpr float L = 0.0216608494f;   // ln 2 / 32
+        const float r = f * fmaf(f, fmaf(f, fmaf(f, L * L * L * L / 24, L * L * L / 6), L * L / 2), L);
         const uint2 e = s.table[b & 31];
-        const uint32_t v = e.x + (0x4B400000 - __float_as_uint(fmaf(__uint_as_float(e.y), r, 12582912.f)));
-        return top ? 1u << 27 : far ? 0 : v;
+        const uint32_t v = e.x + (__float_as_uint(fmaf(__uint_as_float(e.y), r, 12582912.f)) - 0x4B400000);
+        return far ? 0 : v;
     }
     __device__ __forceinline__ u64 weight(float x) const
     {
@@ -171,30 +217,31 @@ struct Sampler {
         return (u64)v << 17 >> (b >> 5);
     }
     __device__ __forceinline__ u64 weight_of(u64 number) const { return weight(smp_unkey((uint32_t)(number >> 32))); }
-    // Calls now(i) for tokens lo + lane, lo + 32 + lane, .. below hi; what it returns true for is done by put_off(i), 32 at a time.
+    // Tokens lo .. below hi for which now(logit, i) holds are passed to put_off(i), 32 at a time.
     template <class Now, class PutOff>
     __device__ __forceinline__ void sweep(int lo, int hi, Now now, PutOff put_off) const
     {
         const int lane = threadIdx.x & 31;
         uint16_t *later = s.later[threadIdx.x >> 5];
         int held = 0;
-        for (int i0 = lo; i0 < hi; i0 += 32) {
-            const int i = i0 + lane;
-            const bool more = i < hi && now(i);
-            const unsigned mask = __ballot_sync(0xFFFFFFFFu, more);
-            if (!mask) continue;
-            if (more) later[held + __popc(mask & ((1u << lane) - 1))] = (uint16_t)i;
-            held += __popc(mask);
-            if (held >= 32) {
-                __syncwarp();
-                put_off((int)later[lane]);
-                held -= 32;
-                const uint16_t rest = later[32 + lane];
-                __syncwarp();
-                later[lane] = rest;
+        for (int i0 = lo; i0 < hi; i0 += 128) {
+            const int i = i0 + 4 * lane;
+            const float4 v = i < hi ? *(const float4 *)(z + i) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const bool more = now(x[k], i + k);
+                const unsigned mask = __ballot_sync(0xFFFFFFFFu, more);
+                if (more) later[held + __popc(mask & ((1u << lane) - 1))] = (uint16_t)(i + k);
+                held += __popc(mask);
             }
+            __syncwarp();
+            while (held >= 32) {
+                held -= 32;
+                put_off((int)later[held + lane]);
+            }
+            __syncwarp();
         }
-        __syncwarp();
         if (lane < held) put_off((int)later[lane]);
         __syncwarp();
     }
@@ -210,6 +257,11 @@ struct Sampler {
             to[1] = b;
         }
         sync();
+    }
+    // the largest of what the CTAs pushed last
+    __device__ __forceinline__ u64 largest(int which = 0) const
+    {
+        return smp_warp_largest((int)(threadIdx.x & 31) < CL ? s.from[turn][threadIdx.x & 31][which] : 0);
     }
     __device__ __forceinline__ void clear()
     {
@@ -230,16 +282,20 @@ struct Sampler {
     // the bins' sizes are in units of 2^(17 - shift), shift = b / 32 or (of a bin divided further) as given.
     __device__ __forceinline__ void collect(bool weights, int shift = -1)
     {
-        const int per = SMP_BINS / CL;
+        const int log_third = 10 - __ffs(CL), per = 3 << log_third;   // (SMP_BINS = 3 * 512)
         __syncthreads();
-        for (int t = threadIdx.x; t < SMP_BINS; t += SMP_THREADS)
-            peer(t / per)->slice[rank * per + t % per] = weights ? (u64)s.part[0][t] + ((u64)s.part[1][t] << 14) : s.part[0][t];
-        sync();
         for (int t = threadIdx.x; t < SMP_BINS; t += SMP_THREADS) {
-            const int k = t % per, b = rank * per + k;
+            const int to = (t >> log_third) / 3;
+            peer(to)->slice[(rank - to) * per + t] = weights ? (u64)s.part[0][t] + ((u64)s.part[1][t] << 14) : s.part[0][t];
+        }
+        sync();
+        for (int k = threadIdx.x; k < per; k += SMP_THREADS) {
+            const int b = rank * per + k;
             u64 sum = 0;
+#pragma unroll 4
             for (int r = 0; r < CL; r++) sum += s.slice[r * per + k];
-            peer(t / per)->all[b] = weights ? sum << 17 >> (shift < 0 ? b >> 5 : shift) : sum;
+            if (weights) sum = sum << 17 >> (shift < 0 ? b >> 5 : shift);
+            for (int r = 0; r < CL; r++) peer(r)->all[b] = sum;
         }
         sync();
     }
@@ -269,8 +325,9 @@ struct Sampler {
     template <class Pred>
     __device__ __forceinline__ void gather(int lists, Pred pred)
     {
-        for (int i = threadIdx.x; i < n; i += SMP_THREADS)
-            if (pred(i)) s.mine[atomicAdd(&s.n_mine, 1)] = number(i);
+        each([&](float x, int i) {
+            if (pred(x, i)) s.mine[atomicAdd(&s.n_mine, 1)] = number(i);
+        });
         __syncthreads();
         if (threadIdx.x == 0) s.at = atomicAdd(&peer(0)->n_list, s.n_mine);
         __syncthreads();
@@ -288,18 +345,16 @@ struct Sampler {
             u64 small = 0, large = 0;   // largest of ~number and of number
             for (int i = threadIdx.x; i < n; i += SMP_THREADS) {
                 const u64 x = number(i);
-                if (in_set(i) && bin(z[i]) == b) {
+                if (in_set(z[i], i) && bin(z[i]) == b) {
                     small = max(small, ~x);
                     large = max(large, x);
                 }
             }
-            small = smp_reduce<true>(small, s.red);
-            large = smp_reduce<true>(large, s.red);
+            small = smp_largest(small, s.red);
+            large = smp_largest(large, s.red);
             exchange(small, large);
-            for (int r = 0; r < CL; r++) {
-                small = max(small, s.from[turn][r][0]);
-                large = max(large, s.from[turn][r][1]);
-            }
+            small = largest();
+            large = largest(1);
             lo = ~small;
             hi = large;
             while (count > SMP_LIST && lo < hi) {
@@ -320,11 +375,10 @@ struct Sampler {
             if (lo == hi) return hi;
             ranged = true;
         }
-        gather(CL, [&](int i) {
-            if (!ranged) return in_set(i) && bin(z[i]) == b;
-            const u64 x = number(i);
-            return x >= lo && x <= hi;
-        });
+        if (ranged)
+            gather(CL, [&](float, int i) { return i < n && number(i) >= lo && number(i) <= hi; });
+        else
+            gather(CL, [&](float x, int i) { return in_set(x, i) && bin(x) == b; });
         // each CTA ranks every CL-th token of the list, CL threads to a token
         const int c = peer(0)->n_list, e = rank + CL * ((int)threadIdx.x / CL), first = (int)threadIdx.x % CL;
         if ((int)threadIdx.x < c) s.list_w[threadIdx.x] = weights ? weight_of(s.list[threadIdx.x]) : 1;
@@ -334,11 +388,9 @@ struct Sampler {
         if (e < c)
             for (int j = first; j < c; j += CL) before += s.list[j] > x ? s.list_w[j] : 0;
         for (int o = CL >> 1; o > 0; o >>= 1) before += __shfl_xor_sync(0xFFFFFFFFu, before, o);
-        u64 last = smp_reduce<true>(e < c && (double)(above + before) < goal ? ~x : 0, s.red);
-        exchange(last, 0);
-        for (int r = 0; r < CL; r++) last = max(last, s.from[turn][r][0]);
+        exchange(smp_largest(e < c && (double)(above + before) < goal ? ~x : 0, s.red), 0);
         no_list();
-        return ~last;
+        return ~largest();
     }
     // At most so many tokens make up v, tokens or weights of bin b (a token's weight is 2^(-b / 32) within 1.1 per cent)
     __device__ __forceinline__ u64 held_by(u64 v, bool weights, int b) const
@@ -367,39 +419,40 @@ __global__ void __launch_bounds__(SMP_THREADS) sample_kernel(const SampleArgs a)
     pdl_trigger();
     // ---- 1. the row into shared memory; its first token ----
     const float *src = a.logits + (size_t)row * a.ld + c.base;
+    const float4 *z4 = (const float4 *)z;
     float top = -INFINITY;
-    int at = -1;
-    auto take = [&](float x, int i) {   // (in rising order of i: the first of equals stays)
-        z[i] = x;
-        if (x > top) {
-            top = x;
+    int at = 0;
+    auto look = [&](const float4 &v, int i) {   // (in rising order of i: the first of equals stays)
+        const float m = fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w));
+        if (m > top) {
+            top = m;
             at = i;
         }
     };
-    if (((uintptr_t)src & 15) == 0) {
+    const bool vectors = ((uintptr_t)src & 15) == 0;
+    if (vectors) {
 #pragma unroll 4
         for (int i = tid; i < n / 4; i += SMP_THREADS) {
             const float4 v = __ldcs((const float4 *)src + i);
-            take(v.x, 4 * i);
-            take(v.y, 4 * i + 1);
-            take(v.z, 4 * i + 2);
-            take(v.w, 4 * i + 3);
+            *((float4 *)z + i) = v;
+            look(v, i);
         }
-        if (tid < (n & 3)) take(src[(n & ~3) + tid], (n & ~3) + tid);
+        if (tid < (n & 3)) z[(n & ~3) + tid] = __ldcs(src + (n & ~3) + tid);
     } else {
 #pragma unroll 4
-        for (int i = tid; i < n; i += SMP_THREADS) take(__ldcs(src + i), i);
+        for (int i = tid; i < n; i += SMP_THREADS) z[i] = __ldcs(src + i);
     }
-    if (tid < 32) {
-        const uint32_t e = (uint32_t)rint(exp2(27.0 - (double)tid / 32.0));
-        s.table[tid] = make_uint2(e, __float_as_uint((float)e));
-    }
+    if (tid < ((n + 3) & ~3) - n) z[n + tid] = -INFINITY;   // up to a vector
     c.no_list();
     c.clear();   // (synchronises)
-    u64 best = at >= 0 ? c.number(at) : 0;
-    best = smp_reduce<true>(best, s.red);
-    c.exchange(best, 0);
-    for (int r = 0; r < c.CL; r++) best = max(best, s.from[c.turn][r][0]);
+    for (int i = vectors ? n / 4 + (tid - n / 4 & SMP_THREADS - 1) : tid; 4 * i < n; i += SMP_THREADS) look(z4[i], i);   // what was not looked at
+    u64 best = 0;
+    if (top > -INFINITY) {
+        const float4 v = z4[at];
+        best = c.number(4 * at + (v.x == top ? 0 : v.y == top ? 1 : v.z == top ? 2 : 3));
+    }
+    c.exchange(smp_largest(best, s.red), 0);
+    best = c.largest();
     const bool none = best == 0;
     if (none || a.temperature == 0.f) {
         if (c.rank == 0 && tid == 0) {
@@ -409,36 +462,33 @@ __global__ void __launch_bounds__(SMP_THREADS) sample_kernel(const SampleArgs a)
         return;
     }
     c.M = smp_unkey((uint32_t)(best >> 32));
-    const double inv64 = 1.0 / (double)a.temperature, scale = 32.0 * 1.4426950408889634 * inv64;
-    c.c_hi = (float)scale;
-    c.c_lo = isinf(c.c_hi) ? 0.f : (float)(scale - (double)c.c_hi);
     c.keep_z = -INFINITY;
     c.keep_i = -1;
-    const float inv = (float)inv64;
-    const double u = (double)fminf(fmaxf(a.u[row], 0.f), 1.f), lowest = fmin((double)a.min_p, 1.0);
-    const float log_lowest = lowest > 0.0 ? (float)log(lowest) : -INFINITY;
+    c.scale(a.c, a.one_over_c);
+    const float inv = (float)a.inv_t;
+    const double u = (double)fminf(fmaxf(a.u[row], 0.f), 1.f);
     auto heavy = [&](float x) {   // weight >= min_p: decided in 64 bits where 32 could be wrong
-        if (lowest <= 0.0 || x == c.M) return true;
+        if (a.min_p <= 0.0 || x == c.M) return true;
         const float y = (x - c.M) * inv;
-        if (y > log_lowest + 1e-3f) return true;
-        if (y < log_lowest - 1e-3f) return false;
-        return exp(((double)x - (double)c.M) * inv64) >= lowest;
+        if (y > a.log_min_p + 1e-3f) return true;
+        if (y < a.log_min_p - 1e-3f) return false;
+        return exp(((double)x - (double)c.M) * a.inv_t) >= a.min_p;
     };
     const bool by_k = a.top_k > 0 && a.top_k < a.vocab, by_p = a.top_p > 0.f && a.top_p < 1.f;
     if (a.top_p <= 0.f) {
         c.keep_to(best);
     } else if (by_k) {
         // ---- 2. top_k ----
-#pragma unroll 4
-        for (int i = tid; i < n; i += SMP_THREADS)
-            if (c.in_set(i)) c.add(c.bin(z[i]), false, 0);
+        c.each([&](float x, int i) {
+            if (c.in_set(x, i)) c.add(c.bin(x), false, 0);
+        });
         c.collect(false);
         u64 before;
         double goal = a.top_k;
         const int b = c.boundary(0, goal, &before);
         const u64 in_bin = s.all[b];
         if (before + in_bin <= SMP_LIST) {
-            c.gather(1, [&](int i) { return c.in_set(i) && c.bin(z[i]) <= b; });
+            c.gather(1, [&](float x, int i) { return c.in_set(x, i) && c.bin(x) <= b; });
             if (c.rank != 0) return;   // (nobody pushes to this CTA or reads from it any more)
             const int m = s.n_list;
             const u64 x = tid < m ? s.list[tid] : 0;
@@ -447,13 +497,14 @@ __global__ void __launch_bounds__(SMP_THREADS) sample_kernel(const SampleArgs a)
                 for (int j = 0; j < m; j++) place += s.list[j] > x;
             const u64 w = tid < m && place < a.top_k ? c.weight_of(x) : 0;
             if (tid < m) s.list_w[tid] = w;
-            u64 total = smp_reduce<false>(w, s.red), earlier = 0;
+            u64 total, earlier = 0;
+            smp_before(w, s.red, &total);
             if (w && a.top_p < 1.f)
                 for (int j = 0; j < m; j++) earlier += s.list[j] > x ? s.list_w[j] : 0;
             const bool in = w && (a.top_p >= 1.f || (double)earlier < (double)a.top_p * (double)total) && heavy(smp_unkey((uint32_t)(x >> 32)));
             __syncthreads();
             if (tid < m) s.list_w[tid] = in ? w : 0;
-            total = smp_reduce<false>(in ? w : 0, s.red);
+            smp_before(in ? w : 0, s.red, &total);
             const u64 goal = min((u64)floor(u * (double)total), total - 1);
             if (in) {
                 u64 run = 0;   // weights of lower indices (larger low words)
@@ -470,12 +521,11 @@ __global__ void __launch_bounds__(SMP_THREADS) sample_kernel(const SampleArgs a)
     }
     if (by_p) {
         // ---- 3. top_p ----
-#pragma unroll 4
-        for (int i = tid; i < n; i += SMP_THREADS) {
+        c.each([&](float x, int i) {
             int b;
-            const uint32_t v = c.size(z[i], b);
-            if (c.in_set(i)) c.add(b, true, v);
-        }
+            const uint32_t v = c.size(x, b);
+            if (c.in_set(x, i)) c.add(b, true, v);
+        });
         c.collect(true);
         u64 before;
         double goal;
@@ -483,47 +533,52 @@ __global__ void __launch_bounds__(SMP_THREADS) sample_kernel(const SampleArgs a)
         c.keep_to(c.last_in_bin(b, c.held_by(s.all[b], true, b), before, goal, true));
     }
     // ---- 4. the token ----
-    const int seg = ((n + SMP_WARPS - 1) / SMP_WARPS + 31) & ~31, lo = min(n, warp * seg), hi = min(n, lo + seg);   // this warp's part
+    const int seg = ((n + SMP_WARPS - 1) / SMP_WARPS + 127) & ~127, lo = min(n, warp * seg), hi = min(n, lo + seg);   // this warp's part
     u64 mine = 0, cta;
-    if (!by_k && !by_p && a.top_p > 0.f && lowest <= 0.0) {   // all of them
+    if (!by_k && !by_p && a.top_p > 0.f && a.min_p <= 0.0) {   // all of them
 #pragma unroll 4
         for (int i = lo + lane; i < hi; i += 32) mine += z[i] > -INFINITY ? c.weight(z[i]) : 0;
     } else {
-        c.sweep(lo, hi, [&](int i) { return c.in_set(i) && heavy(z[i]); }, [&](int i) { mine += c.weight(z[i]); });
+        c.sweep(lo, hi, [&](float x, int i) { return c.in_set(x, i) && heavy(x); }, [&](int i) { mine += c.weight(z[i]); });
     }
     u64 warp_sum = mine;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) warp_sum += __shfl_xor_sync(0xFFFFFFFFu, warp_sum, o);
     u64 run = smp_before(lane == 0 ? warp_sum : 0, s.red, &cta);
-    run = __shfl_sync(0xFFFFFFFFu, run, 0);
+    run = __shfl_sync(0xFFFFFFFFu, run, 0);   // of the warps before this one
     c.exchange(cta, 0);
-    u64 total = 0;
+    u64 total = 0, before = 0;
     for (int r = 0; r < c.CL; r++) {
-        if (r < c.rank) run += s.from[c.turn][r][0];
+        if (r < c.rank) before += s.from[c.turn][r][0];
         total += s.from[c.turn][r][0];
     }
     const u64 goal = min((u64)floor(u * (double)total), total - 1);
-    if (goal < run || goal >= run + warp_sum) return;
-    for (int i0 = lo; i0 < hi; i0 += 128) {   // four runs of 32 at once: their weights do not wait for one another
-        u64 w[4], sum[4];
+    if (goal < before || goal >= before + cta) return;   // another CTA's
+    run += before;
+    if (lane == 0 && goal >= run && goal < run + warp_sum) {
+        s.at = warp;
+        s.before = run;
+    }
+    __syncthreads();
+    // the part of the warp in whose range the goal lies, by all threads: up to four tokens each
+    constexpr int MOST = SMP_MAX_VOCAB / SMP_MAX_CLUSTER / SMP_WARPS / SMP_THREADS;
+    const int from = s.at * seg, each = (seg + SMP_THREADS - 1) / SMP_THREADS, end = min(n, from + seg);
+    run = s.before;
+    u64 w[MOST], sum = 0, all;
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const int i = i0 + 32 * k + lane;
-            w[k] = i < hi && c.in_set(i) && heavy(z[i]) ? c.weight(z[i]) : 0;
-            sum[k] = smp_warp_inclusive(w[k]);
-        }
+    for (int k = 0; k < MOST; k++) {
+        const int i = from + each * tid + k;
+        w[k] = k < each && i < end && c.in_set(z[i], i) && heavy(z[i]) ? c.weight(z[i]) : 0;
+        sum += w[k];
+    }
+    run += smp_before(sum, s.red, &all);
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const unsigned hit = __ballot_sync(0xFFFFFFFFu, run + sum[k] > goal);
-            if (hit) {
-                if (lane == __ffs(hit) - 1) {
-                    a.tokens[row] = c.base + i0 + 32 * k + lane;
-                    if (a.probs) a.probs[row] = (float)((double)w[k] / (double)total);
-                }
-                return;
-            }
-            run += __shfl_sync(0xFFFFFFFFu, sum[k], 31);
+    for (int k = 0; k < MOST; k++) {
+        if (goal >= run && goal < run + w[k]) {
+            a.tokens[row] = c.base + from + each * tid + k;
+            if (a.probs) a.probs[row] = (float)((double)w[k] / (double)total);
         }
+        run += w[k];
     }
 }
 
