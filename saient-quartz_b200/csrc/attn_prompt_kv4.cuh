@@ -149,28 +149,19 @@ __global__ void __launch_bounds__(APK_THREADS, 1) attn_prompt_kv4_kernel(const A
         // ---- Q into tensor memory ----
         const uint32_t lanes = (uint32_t)(32 * warp) << 16;
         const float to_log2 = a.scale * 1.44269504f;
-        // rows come in one after the other, eight loads of 16 bytes on their way, through the last stage, which the filling warps
+        // rows come in one after the other, copied to the last stage, which the filling warps
         // leave alone until then (a thread that reads its own row touches 32 rows at once: 2048 tokens took 151 us so, 129 with
         // this); 16-byte columns are rotated by the row against bank conflicts
         constexpr int COLS = HD / 4;
         float4 *stage_q = (float4 *)(ring + (APK_STAGES - 1) * STAGE) + warp * 32 * COLS;
         const float4 *q0 = (const float4 *)(a.q + ((size_t)t0 * a.n_heads + (size_t)kvh * G) * HD);
         const int my_row = is_row ? (tok * a.n_heads + row % G) * COLS : -1;
-        constexpr int AT_ONCE = 8;
-        static_assert(COLS % AT_ONCE == 0, "");
-        for (int k = 0; k < COLS; k += AT_ONCE) {
-            float4 v[AT_ONCE];
-#pragma unroll
-            for (int b = 0; b < AT_ONCE; b++) {
-                const int i = 32 * (k + b) + lane, from = __shfl_sync(0xFFFFFFFFu, my_row, i / COLS);
-                v[b] = from >= 0 ? __ldcg(q0 + from + i % COLS) : make_float4(0.f, 0.f, 0.f, 0.f);
-            }
-#pragma unroll
-            for (int b = 0; b < AT_ONCE; b++) {
-                const int i = 32 * (k + b) + lane, r = i / COLS;
-                stage_q[r * COLS + (i % COLS + r) % COLS] = v[b];
-            }
+#pragma unroll 8
+        for (int i = lane; i < 32 * COLS; i += 32) {
+            const int r = i / COLS, from = __shfl_sync(0xFFFFFFFFu, my_row, r);
+            cp_async16(stage_q + r * COLS + (i % COLS + r) % COLS, q0 + max(from, 0) + i % COLS, from >= 0);
         }
+        cp_async_wait_all();
         __syncwarp();
         auto q_at = [&](int c) { return stage_q[lane * COLS + (c + lane) % COLS]; };
         float top = 0.f;

@@ -22,6 +22,7 @@
 
 #include <cooperative_groups.h>
 
+#include "async_copy.cuh"
 #include "fused_ops.cuh"
 
 namespace qz {
@@ -57,12 +58,6 @@ struct AttnStepArgs {
     const float2 *rope_tab;
 };
 
-__device__ __forceinline__ void cp_async16(void *smem_dst, const void *gmem_src)
-{
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(smem_dst)), "l"(gmem_src)
-                 : "memory");
-}
-__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 // split cluster barrier (every thread of the CTA executes both halves)
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
