@@ -62,6 +62,12 @@ __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.w
 // one mma.m16n8k16; both parts are scaled by powers of two (per head for q, per warp for d) that keep them clear of
 // f16's ends.  Sums are f32.
 // The softmax reference of a head is raised only when a score exceeds it by 2^8; until then weights up to 2^8 do no harm.
+//
+// Measured (32 / 8 heads of 128, replayed): context 18 4.4 us, 1024 with rotation and append 9.0 (without 6.3), 4096 10.6,
+// 16384 13.9, 131072 51 us = 3.3 TB/s of the cache.  Short contexts are bound by the launch, two cluster barriers and one
+// block's latency; long ones by instruction issue: a warp spends some 400 instructions on a tile of 16 positions (unpacking,
+// the hi / lo parts, 24 MMAs) at 0.55 per cycle and scheduler; the same launch that only loads takes 32 us.
+// Clusters join a unit only when every warp still has a block: at twice that 16384 positions take 14.2 us, 8192 13.4 (12.3).
 __host__ __device__ constexpr int attn_kv4_stages(int NG) { return NG == 1 ? 8 : NG == 2 ? 4 : 2; }   // ~10 KB in flight per warp
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)

@@ -17,6 +17,10 @@
 //   K  32-bit word t * NG + g, t < 4: dims 32 g + 8 t + i in nibbles i < 8   (K is the row operand: k runs over dims)
 //   V  16-bit word r * NG + g, r < 8: dims 32 g + 4 r + i in nibbles i < 4   (V^T is: k runs over positions)
 //   parameters: NG halves m, then NG halves d.
+//
+// Writing and reading are bound by HBM: 4 bytes on one side, 0.625 on the other.  Eight dims per thread make every access
+// of a warp whole sectors.  8192 rows of 8 heads of 128, appended and read back: 36 us, 4.3 TB/s; 8189 of 4 heads of 96:
+// 17.0 us, 3.4 TB/s; a few rows are bound by the two launches (2.8 us in a replayed graph).
 #pragma once
 
 #include "activation.cuh"

@@ -69,6 +69,11 @@ __device__ __forceinline__ float smp_unkey(uint32_t k) { return __uint_as_float(
 //      range u falls is weighed again, token by token.  (Few are kept as a rule: a warp collects them and weighs 32 at a time.)
 // A bin with more tokens than the list takes (ties, high temperatures) is divided further, by the number itself.
 // A histogram is reduced in slices, one per CTA, that are pushed to every CTA: all find the same bin without asking.
+//
+// Measured (128256 tokens, replayed): one row, top_k 40 12.3 us, top_p alone 20.8, no filter 8.3; 256 rows, top_k 139 us,
+// top_p 255, no filter 114, temperature 0 47 us = 2.8 TB/s.  One row is bound by cluster barriers (five or six, 1 to 2 us each),
+// many rows by instruction issue and the histogram's shared-memory atomics (two per token) between the same barriers: two
+// CTAs of an SM, of different rows, are all there is to overlap them (a part of a row and the histograms take 107 KB).
 constexpr int SMP_PER = 3, SMP_BINS = SMP_PER * SMP_THREADS, SMP_LIST = 512;   // (a thread looks after three bins, and one token of the list)
 constexpr int SMP_WARPS = SMP_THREADS / 32, SMP_MAX_CLUSTER = 16;
 static_assert(SMP_BINS >= 32 * 46 && SMP_BINS % SMP_MAX_CLUSTER == 0, "bins cover weights down to 2^-45");
