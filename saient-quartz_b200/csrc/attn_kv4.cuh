@@ -63,7 +63,7 @@ __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.w
 // f16's ends.  Sums are f32.
 // The softmax reference of a head is raised only when a score exceeds it by 2^8; until then weights up to 2^8 do no harm.
 //
-// Measured (32 / 8 heads of 128, replayed): context 18 4.4 us, 1024 with rotation and append 9.0 (without 6.3), 4096 10.6,
+// Measured (32 / 8 heads of 128, replayed): context 1024 6.3 us (8 / 2 heads of 64, context 18: 4.4), 4096 10.6,
 // 16384 13.9, 131072 51 us = 3.3 TB/s of the cache.  Short contexts are bound by the launch, two cluster barriers and one
 // block's latency; long ones by instruction issue: a warp spends some 400 instructions on a tile of 16 positions (unpacking,
 // the hi / lo parts, 24 MMAs) at 0.55 per cycle and scheduler; the same launch that only loads takes 32 us.
