@@ -156,6 +156,12 @@ def test_step_long(gpu, nh, n_kv, hd, ctx):
     run_step(gpu, nh, n_kv, hd, ctx, max_seq=ctx + 64, window=0, sinks=False, append=True, sharp=8.0)
 
 
+@pytest.mark.parametrize("nh,n_kv,hd,max_seq", [(64, 8, 64, 9000), (40, 8, 32, 8200), (28, 4, 96, 33000), (48, 8, 128, 8192)])
+@pytest.mark.parametrize("ctx", [1, 70, 1500, 8111])
+def test_step_wide_groups_in_a_long_cache(gpu, nh, n_kv, hd, max_seq, ctx):
+    run_step(gpu, nh, n_kv, hd, ctx, max_seq=max_seq, window=0, sinks=ctx == 70, append=ctx != 1500)
+
+
 def run_step(gpu, nh, n_kv, hd, ctx, max_seq, window, sinks, append, sharp=1.0):
     L, r = gpu.lib(), rng(nh, n_kv, hd, ctx, window)
     pos, scale = ctx - 1, np.float32(1 / np.sqrt(hd))
