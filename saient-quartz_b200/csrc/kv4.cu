@@ -283,13 +283,17 @@ void cuda_attn_prompt_kv4(float *out, const float *q, const void *d_cache, int n
         return;
     }
     // A few tokens on a long cache leave the prompt kernel, one CTA per kv head and 128 rows, with most SMs idle: there
-    // the step kernel takes them one by one, all in one launch.  Time of either in us, fitted to measurements (32 / 8 heads
-    // of 128; step: 16 tokens at 1000 12.5, 64 at 1000 35, 16 at 16000 89; prompt: 128 at 1000 37, 512 at 0 22, 512 at
-    // 16000 398): a wave of units and 3.7 TB/s of cache once per token, or 1.6 per 64 positions and wave of CTAs.
-    const int G = n_heads / n_kv_heads, ctas = n_kv_heads * ((n_tok + UMMA_M / G - 1) / (UMMA_M / G)), units = n_kv_heads * ((G + 7) / 8) * n_tok;
-    const double seen = window > 0 ? std::min(window, pos0 + n_tok) : pos0 + n_tok;
-    const double by_step = 2 + 4.5 * std::ceil(units / (2.0 * sm_count())) + n_tok * seen * n_kv_heads * head_dim * 1.25 / 3.7e6;
-    const double by_prompt = 9 + 1.6 * (seen / APK_BN + 1) * std::ceil(ctas / (double)sm_count());
+    // the step kernel takes them one by one, all in one launch.  Time of either in us, fitted to measurements: waves of units
+    // (more than four query heads: one to an SM, else two) and what a unit spends on a position, or what a CTA spends on a
+    // tile of 64.  Step / prompt, 32 / 8 heads of 128: 32 tokens at 0 7.7 / 10.4, 64 at 0 14.7 / 10.8, 64 at 2000 56 / 58, 64
+    // at 16000 338 / 384; 64 / 8: 16 at 200 13 / 15, 32 at 0 21 / 11, 16 at 2000 30 / 56, 64 at 2000 119 / 58; 12 / 6 of 64:
+    // 32 at 0 4.7 / 6.3, 64 at 0 8.5 / 7.1, 64 at 16000 178 / 259.
+    const int G = n_heads / n_kv_heads, ctas = n_kv_heads * ((n_tok + UMMA_M / G - 1) / (UMMA_M / G)), splits = (G + 7) / 8, units = n_kv_heads * splits * n_tok;
+    const bool wide = (G + splits - 1) / splits > 4;
+    const double h = head_dim / 128.0, sms = sm_count(), most = pos0 + (double)n_tok, mean = pos0 + 0.5 * n_tok;
+    const double by_step = 2 + (wide ? 1.8 + 7.6 * h : 1 + 5 * h) * std::ceil(units / (wide ? sms : 2 * sms)) +
+                           (wide ? 51 + 26 * h : 16 + 24 * h) * 1e-6 * units * (window > 0 ? std::min((double)window, mean) : mean);
+    const double by_prompt = 3 + 6 * h + (0.5 + h) * std::ceil((window > 0 ? std::min((double)window + UMMA_M / G, most) : most) / APK_BN) * std::ceil(ctas / sms);
     if (by_step < by_prompt) {
         AttnKv4Args s = {out, q, nullptr, nullptr, (uint8_t *)d_cache, nullptr, pos0, n_heads, n_kv_heads, max_seq, kv4_blocks(max_seq), window, scale, sinks};
         launch_step(s, n_tok, head_dim);
