@@ -232,12 +232,15 @@ void cuda_rope_kv4_rows(float *q, float *k, const float *v, void *d_cache, int n
         refuse("cuda_rope_kv4_rows: 0 <= pos0, pos0 + n_tok <= max_seq, n_tok <= 65535");
         return;
     }
-    if (!q || !k || !v) {
-        refuse("cuda_rope_kv4_rows: q, k and v must be device pointers");
+    if (!q || !k || !v || !aligned16(q) || !aligned16(k) || !aligned16(v)) {
+        refuse("cuda_rope_kv4_rows: q, k and v must be 16-byte aligned device pointers");
         return;
     }
     by_groups(head_dim, [&](auto ng) {
-        launch(rope_kv4_rows_kernel<ng.value>, dim3(n_heads + n_kv_heads, n_tok), dim3(64), 0, q, k, v, (uint8_t *)d_cache, n_heads, n_kv_heads,
+        // blocks of a token: all of its rows at once while they still find room on the chip, one from there on
+        const int at_once = RK4_THREADS / 32 * (8 / ng.value), rows = (theta > 0.f ? n_heads : 0) + 2 * n_kv_heads;
+        const int share = std::max(1, std::min((rows + at_once - 1) / at_once, 8 * sm_count() / n_tok));
+        launch(rope_kv4_rows_kernel<ng.value>, dim3(n_tok, share), dim3(RK4_THREADS), 0, q, k, v, (uint8_t *)d_cache, n_heads, n_kv_heads,
                kv4_blocks(max_seq), pos0, theta, yarn_scale, yarn_orig_ctx, neox);
     });
 }

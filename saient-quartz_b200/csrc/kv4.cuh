@@ -173,50 +173,90 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(float *__restrict__ k, fl
     dst[1] = make_float4(x[4], x[5], x[6], x[7]);
 }
 
-// rope_kv_rows_kernel with a 4-bit cache: token t = blockIdx.y at position pos0 + t; q and k rotated in place (theta <= 0:
-// left as they are), then warp 0 of a key head quantises its k and warp 1 its v.  grid.x = query heads, then kv heads.
+// cuda_rope_kv_rows with a 4-bit cache: token blockIdx.x at position pos0 + blockIdx.x; q and k rotated in place (theta <= 0: left
+// as they are), k and v quantised.  The angles of a token are computed once for all of its rows: 512 tokens of 32 / 8
+// heads of 128 take 5.7 us (4.2 TB/s), 8192 take 66 (5.8 TB/s); one block per row, as the f32 form has it, took 21.7 and 338, most
+// of it for angles and for starting blocks.
+// Rows are q's, k's, then v's; 4 NG threads share one, each with four pairs, two vectors of four dims.  grid.y blocks share
+// a token's rows where there are few tokens.
+constexpr int RK4_THREADS = 256;
+
 template <int NG>
-__global__ void __launch_bounds__(64) rope_kv4_rows_kernel(float *q, float *k, const float *__restrict__ v, uint8_t *__restrict__ cache,
-                                                           int n_heads, int n_kv, int n_blocks, int pos0, float theta,
-                                                           float yarn_scale, int yarn_orig_ctx, int neox)
+__global__ void __launch_bounds__(RK4_THREADS) rope_kv4_rows_kernel(float *q, float *k, const float *__restrict__ v, uint8_t *__restrict__ cache,
+                                                                    int n_heads, int n_kv, int n_blocks, int pos0, float theta,
+                                                                    float yarn_scale, int yarn_orig_ctx, int neox)
 {
-    constexpr int HD = 32 * NG, half = HD / 2;
-    __shared__ __align__(16) float ks[HD];
+    constexpr int HD = 32 * NG, half = HD / 2, PER = 4 * NG, ROWS = 32 / PER;   // threads per row, rows per warp
+    __shared__ float2 cs[half];   // (cos, sin)
     pdl_wait();
     pdl_trigger();
-    const int i = threadIdx.x, tok = blockIdx.y, pos = pos0 + tok;
-    const bool is_k = (int)blockIdx.x >= n_heads;
-    const int head = is_k ? blockIdx.x - n_heads : blockIdx.x;
-    float *xh = is_k ? k + ((size_t)tok * n_kv + head) * HD : q + ((size_t)tok * n_heads + head) * HD;
-    if (i < half) {
-        const int i0 = neox ? i : 2 * i, i1 = neox ? i + half : 2 * i + 1;
-        float a = xh[i0], b = xh[i1];
-        if (theta > 0.f) {
+    const int tok = blockIdx.x, pos = pos0 + tok, lane = threadIdx.x & 31;
+    const bool rotate = theta > 0.f;
+    if (rotate) {
+        if (threadIdx.x < half) {
             const RopeArgsLite r{pos, theta, yarn_scale, yarn_orig_ctx};
             float s, c;
-            rope_cs_lite(r, i, HD, c, s);
-            const float r0 = a * c - b * s, r1 = a * s + b * c;
-            a = r0;
-            b = r1;
-            xh[i0] = a;
-            xh[i1] = b;
+            rope_cs_lite(r, threadIdx.x, HD, c, s);
+            cs[threadIdx.x] = make_float2(c, s);
         }
-        if (is_k) {
-            ks[i0] = a;
-            ks[i1] = b;
-        }
+        __syncthreads();
     }
-    if (!is_k) return;
-    __syncthreads();
-    const int lane = i & 31;
-    if (lane >= 4 * NG) return;
-    const bool is_v = i >= 32;
-    const float *src = (is_v ? v + ((size_t)tok * n_kv + head) * HD : ks) + 8 * lane;
-    float x[8];
+    const int in_warp = lane / PER, j = lane % PER, n_q = rotate ? n_heads : 0, n_rows = n_q + 2 * n_kv;
+    const int at0 = neox ? 4 * j : 8 * j, at1 = neox ? half + 4 * j : 8 * j + 4;
+    for (int r0 = ((int)blockIdx.y * (RK4_THREADS / 32) + (threadIdx.x >> 5)) * ROWS; r0 < n_rows; r0 += gridDim.y * (RK4_THREADS / 32) * ROWS) {
+        const int row = r0 + in_warp;
+        const bool there = in_warp < ROWS && row < n_rows;
+        const unsigned mask = __ballot_sync(0xFFFFFFFFu, there);
+        if (!there) continue;
+        const bool is_q = row < n_q, is_v = row >= n_q + n_kv;
+        const int head = is_q ? row : is_v ? row - n_q - n_kv : row - n_q;
+        float x[8];
+        if (is_v) {
+            const float4 *src = (const float4 *)(v + ((size_t)tok * n_kv + head) * HD + 8 * j);
+            const float4 a = __ldg(src), b = __ldg(src + 1);
+            x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+        } else {
+            float *at = is_q ? q + ((size_t)tok * n_heads + head) * HD : k + ((size_t)tok * n_kv + head) * HD;
+            const float4 a = *(const float4 *)(at + at0), b = *(const float4 *)(at + at1);
+            x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+            if (rotate) {
+                auto turn = [&](float &x0, float &x1, int pair) {
+                    const float2 w = cs[pair];
+                    const float y0 = x0 * w.x - x1 * w.y, y1 = x0 * w.y + x1 * w.x;
+                    x0 = y0;
+                    x1 = y1;
+                };
+                if (neox) {
 #pragma unroll
-    for (int e = 0; e < 8; e++) x[e] = src[e];
-    kv4_store8<NG>(x, kv4_block(cache, n_blocks, head, pos / KV4_BLOCK, HD), pos % KV4_BLOCK, lane >> 2, lane & 3, is_v,
-                   4 * NG == 32 ? 0xFFFFFFFFu : (1u << (4 * NG)) - 1u);
+                    for (int c = 0; c < 4; c++) turn(x[c], x[4 + c], 4 * j + c);
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 4; c++) turn(x[2 * c], x[2 * c + 1], 4 * j + c);
+                }
+                *(float4 *)(at + at0) = make_float4(x[0], x[1], x[2], x[3]);
+                *(float4 *)(at + at1) = make_float4(x[4], x[5], x[6], x[7]);
+            }
+        }
+        // all threads of the warp's rows take part in the exchange; a query's have nothing to store
+        if (neox) {   // dims 8 j ..: vectors 2 j and 2 j + 1 of the row, which threads 2 j .. of its first or second half hold
+            const int from = in_warp * PER + (2 * j) % PER;
+            float y[8];
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                const float a0 = __shfl_sync(mask, x[c], from), a1 = __shfl_sync(mask, x[c], from + 1);
+                const float b0 = __shfl_sync(mask, x[4 + c], from), b1 = __shfl_sync(mask, x[4 + c], from + 1);
+                y[c] = 2 * j < PER ? a0 : b0;
+                y[4 + c] = 2 * j < PER ? a1 : b1;
+            }
+            if (!is_v) {
+#pragma unroll
+                for (int c = 0; c < 8; c++) x[c] = y[c];
+            }
+        }
+        const unsigned stored = __ballot_sync(mask, !is_q);
+        if (!is_q)
+            kv4_store8<NG>(x, kv4_block(cache, n_blocks, head, pos / KV4_BLOCK, HD), pos % KV4_BLOCK, j >> 2, j & 3, is_v, stored);
+    }
 }
 
 }  // namespace qz

@@ -136,6 +136,14 @@ def test_rope_rows_equal_rotation_then_append(gpu, n, nh, n_kv, hd, pos0, neox, 
     assert np.array_equal(c1.download(np.uint8), c2.download(np.uint8))
 
 
+@pytest.mark.parametrize("neox", [0, 1])
+@pytest.mark.parametrize("nh,n_kv,hd", GEOMETRY)
+@pytest.mark.parametrize("n", [1, 3, 700])
+def test_rope_rows_of_every_geometry(gpu, nh, n_kv, hd, n, neox):
+    test_rope_rows_equal_rotation_then_append(gpu, n, nh, n_kv, hd, 5, neox, 1e4)
+    test_rope_rows_equal_rotation_then_append(gpu, n, nh, n_kv, hd, 5, neox, 0.0)
+
+
 # ---- one token -------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("nh,n_kv,hd", GEOMETRY)
 @pytest.mark.parametrize("ctx", [1, 2, 31, 32, 33, 64, 95, 300, 1025])

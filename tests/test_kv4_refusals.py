@@ -102,3 +102,11 @@ def test_nothing_to_do_is_not_an_error(L):
     L.cuda_attn_prompt_kv4(P, P, P, 0, 8, 2, 64, 40, 0, 0, 0.1, None)
     L.cuda_sample(P, 0, 100, 100, 0.8, 5, 0.9, 0.0, P, P, None)
     assert L.quartz_last_error() == 0 and L.quartz_launch_count() == before
+
+
+@pytest.mark.parametrize("bad", [0, 1, 2])
+def test_rope_rows_refuse_unaligned_rows(L, bad):
+    before = L.quartz_launch_count()
+    a = [P + 4 * (i == bad) for i in range(3)]
+    L.cuda_rope_kv4_rows(*a, P, 3, 4, 2, 64, 40, 0, 1e4, 1.0, 0, 0)
+    assert refused(L) == before
