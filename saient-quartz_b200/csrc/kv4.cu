@@ -200,8 +200,12 @@ void cuda_kv4_append_rows(void *d_cache, const float *k, const float *v, int n_t
         return;
     }
     const long long rows = (long long)n_tok * n_kv_heads, threads = rows * (head_dim / 8);
+    if (rows >= 1ll << 31) {
+        set_error(QZ_ERR_TOO_LARGE, "cuda_kv4_append_rows: n_tok * n_kv_heads must be below 2^31");
+        return;
+    }
     by_groups(head_dim, [&](auto ng) {
-        launch(kv4_append_kernel<ng.value>, dim3((unsigned)((threads + 255) / 256), 2), dim3(256), 0, (uint8_t *)d_cache, k, v, rows, n_kv_heads,
+        launch(kv4_append_kernel<ng.value>, dim3((unsigned)((threads + 255) / 256), 2), dim3(256), 0, (uint8_t *)d_cache, k, v, (unsigned)rows, n_kv_heads,
                kv4_blocks(max_seq), pos0);
     });
 }
@@ -218,8 +222,12 @@ void cuda_kv4_read_rows(float *k, float *v, const void *d_cache, int n_tok, int 
         return;
     }
     const long long rows = (long long)n_tok * n_kv_heads, threads = rows * (head_dim / 8);
+    if (rows >= 1ll << 31) {
+        set_error(QZ_ERR_TOO_LARGE, "cuda_kv4_read_rows: n_tok * n_kv_heads must be below 2^31");
+        return;
+    }
     by_groups(head_dim, [&](auto ng) {
-        launch(kv4_read_kernel<ng.value>, dim3((unsigned)((threads + 255) / 256), 2), dim3(256), 0, k, v, (const uint8_t *)d_cache, rows, n_kv_heads,
+        launch(kv4_read_kernel<ng.value>, dim3((unsigned)((threads + 255) / 256), 2), dim3(256), 0, k, v, (const uint8_t *)d_cache, (unsigned)rows, n_kv_heads,
                kv4_blocks(max_seq), pos0);
     });
 }

@@ -121,20 +121,19 @@ __device__ __forceinline__ void kv4_store8(const float (&x)[8], uint8_t *blk, in
 // Rows k, v [n_tok][n_kv_heads * head_dim] into positions pos0 .. : one thread per eight dims; grid.y 0 keys, 1 values.
 template <int NG>
 __global__ void __launch_bounds__(256) kv4_append_kernel(uint8_t *__restrict__ cache, const float *__restrict__ k,
-                                                         const float *__restrict__ v, long long n_rows, int n_kv, int n_blocks, int pos0)
+                                                         const float *__restrict__ v, unsigned n_rows, int n_kv, int n_blocks, int pos0)
 {
     constexpr int PER = 4 * NG;   // threads per row
     pdl_wait();
     pdl_trigger();
-    const long long e = (long long)blockIdx.x * 256 + threadIdx.x;
-    const long long row = e / PER;
-    const int j = (int)(e - row * PER), g = j >> 2, t = j & 3;
+    const unsigned row = (blockIdx.x * 256ull + threadIdx.x) / PER;   // (memory holds less than 2^31 rows)
+    const int j = (int)((blockIdx.x * 256ull + threadIdx.x) % PER), g = j >> 2, t = j & 3;
     const unsigned mask = __ballot_sync(0xFFFFFFFFu, row < n_rows);
     if (row >= n_rows) return;
-    const float *src = (blockIdx.y ? v : k) + row * (32 * NG) + 32 * g + 8 * t;
+    const float *src = (blockIdx.y ? v : k) + (size_t)row * (32 * NG) + 32 * g + 8 * t;
     const float4 a = __ldg((const float4 *)src), b = __ldg((const float4 *)src + 1);
     const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-    const long long tok = row / n_kv;
+    const unsigned tok = row / (unsigned)n_kv;
     const int head = (int)(row - tok * n_kv);
     const int pos = pos0 + (int)tok;
     kv4_store8<NG>(x, kv4_block(cache, n_blocks, head, pos / KV4_BLOCK, 32 * NG), pos % KV4_BLOCK, g, t, blockIdx.y != 0, mask);
@@ -143,16 +142,15 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(uint8_t *__restrict__ c
 // The reverse: the values of positions pos0 .. as f32 rows.
 template <int NG>
 __global__ void __launch_bounds__(256) kv4_read_kernel(float *__restrict__ k, float *__restrict__ v, const uint8_t *__restrict__ cache,
-                                                       long long n_rows, int n_kv, int n_blocks, int pos0)
+                                                       unsigned n_rows, int n_kv, int n_blocks, int pos0)
 {
     constexpr int PER = 4 * NG, HD = 32 * NG;
     pdl_wait();
     pdl_trigger();
-    const long long e = (long long)blockIdx.x * 256 + threadIdx.x;
-    const long long row = e / PER;
+    const unsigned row = (blockIdx.x * 256ull + threadIdx.x) / PER;
     if (row >= n_rows) return;
-    const int j = (int)(e - row * PER), g = j >> 2, t = j & 3;
-    const long long tok = row / n_kv;
+    const int j = (int)((blockIdx.x * 256ull + threadIdx.x) % PER), g = j >> 2, t = j & 3;
+    const unsigned tok = row / (unsigned)n_kv;
     const int head = (int)(row - tok * n_kv);
     const int pos = pos0 + (int)tok, r = pos % KV4_BLOCK;
     const uint8_t *side = kv4_block(const_cast<uint8_t *>(cache), n_blocks, head, pos / KV4_BLOCK, HD) + (blockIdx.y ? 20 * HD : 0);
@@ -168,7 +166,7 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(float *__restrict__ k, fl
     float x[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) x[i] = fmaf(d, (float)((w >> (4 * i)) & 15u), m);
-    float4 *dst = (float4 *)((blockIdx.y ? v : k) + row * HD + 32 * g + 8 * t);
+    float4 *dst = (float4 *)((blockIdx.y ? v : k) + (size_t)row * HD + 32 * g + 8 * t);
     dst[0] = make_float4(x[0], x[1], x[2], x[3]);
     dst[1] = make_float4(x[4], x[5], x[6], x[7]);
 }

@@ -110,3 +110,10 @@ def test_rope_rows_refuse_unaligned_rows(L, bad):
     a = [P + 4 * (i == bad) for i in range(3)]
     L.cuda_rope_kv4_rows(*a, P, 3, 4, 2, 64, 40, 0, 1e4, 1.0, 0, 0)
     assert refused(L) == before
+
+
+@pytest.mark.parametrize("name", ["append", "read"])
+def test_rows_refuse_more_than_memory_holds(L, name):
+    before = L.quartz_launch_count()
+    rows(L, name, n_tok=2 ** 26, n_kv=32, hd=32, max_seq=2 ** 26)
+    assert refused(L, 5) == before
