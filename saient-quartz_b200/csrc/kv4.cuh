@@ -19,8 +19,9 @@
 //   parameters: NG halves m, then NG halves d.
 //
 // Writing and reading are bound by HBM: 4 bytes on one side, 0.625 on the other.  Eight dims per thread make every access
-// of a warp whole sectors.  8192 rows of 8 heads of 128, appended and read back: 36 us, 4.3 TB/s; 8189 of 4 heads of 96:
-// 17.0 us, 3.4 TB/s; a few rows are bound by the two launches (2.8 us in a replayed graph).
+// of a warp whole sectors.  8192 rows of 8 heads of 128: written 20.1 us, 3.9 TB/s (bound by the quantiser's issue slots as much as
+// by HBM; 64-bit borders for every code and clamps took 21.3), read back 15.6 us, 5.0 TB/s; 8189 of 4 heads of 96: 8.7 and 7.6
+// us; a few rows are bound by the launches (1.4 and 1.0 us in a replayed graph).
 #pragma once
 
 #include "activation.cuh"
@@ -38,35 +39,37 @@ __device__ __forceinline__ uint8_t *kv4_block(uint8_t *cache, int n_blocks, int 
     return cache + ((size_t)head * n_blocks + block) * kv4_block_bytes(head_dim);
 }
 
-// Parameters of a group from its extremes.  The two borders (is m + 15 d >= hi, would one f16 less do) are decided in
-// 64 bits, where every quantity is exact for operands within 2^29 of one another.
+// Does m + 15 d reach hi?  Decided exactly: 15 d is exact, its sum with m is taken with the error that it leaves.
+__device__ __forceinline__ bool kv4_reaches(float m, __half d, float hi)
+{
+    const float t = 15.f * __half2float(d), s = __fadd_rn(t, m), b = __fadd_rn(s, -t), err = __fadd_rn(__fadd_rn(t, -__fadd_rn(s, -b)), __fadd_rn(m, -b));
+    return __fadd_rn(__fadd_rn(s, -hi), err) >= 0.f;   // (where s and hi differ by more than err, their difference has its sign)
+}
+// Parameters of a group from its extremes.  The f32 quotient is right to 2^-22 of itself: only if it lies that close to an
+// f16 number can that number, or the one above it, be the answer instead, and is asked exactly.
 __device__ __forceinline__ void kv4_params(float lo, float hi, __half &m, __half &d)
 {
     m = __float2half_rd(fmaxf(lo, -65504.f) + 0.f);   // (+ 0: a minimum of -0 is stored as 0)
-    const double span = fmax((double)hi - (double)__half2float(m), 0.0);
-    float df = __half2float(__float2half_ru(fminf((float)(span * (1.0 / 15.0)), 65504.f)));
-    // the product above may be one ulp (of f32) to either side of span / 15: at most one f16 away from the answer
-    if (15.0 * (double)df < span && df < 65504.f) df = __half2float(__ushort_as_half((unsigned short)(__half_as_ushort(__float2half_rn(df)) + 1)));
-    if (df > 0.f) {
-        const float less = __half2float(__ushort_as_half((unsigned short)(__half_as_ushort(__float2half_rn(df)) - 1)));
-        if (15.0 * (double)less >= span) df = less;
+    const float mf = __half2float(m), q = fmaxf(hi - mf, 0.f) * (1.f / 15.f), near = q * (1.f / (1 << 20));
+    d = __float2half_ru(fminf(q, 65504.f));
+    const unsigned short bits = __half_as_ushort(d);
+    const __half less = __ushort_as_half((unsigned short)(bits - 1));   // (of 0: NaN, which nothing is near to)
+    if (__half2float(d) - q < near || q - __half2float(less) < near) {
+        if (!kv4_reaches(mf, d, hi)) {
+            if (bits < 0x7BFF) d = __ushort_as_half((unsigned short)(bits + 1));
+        } else if (bits && kv4_reaches(mf, less, hi)) {
+            d = less;
+        }
     }
-    d = __float2half_rn(df);
 }
 
-// (x - m) / d to nearest, ties to even.  The f32 quotient is off by less than 2^-18 (15 * 2^-22), so only a quotient
-// that close to a border needs the exact comparison, in 64 bits; it is rare.
-__device__ __forceinline__ uint32_t kv4_code(float x, float m, float d, float inv)
+// (x - m) / d to nearest, ties to even, where its f32 value y, off by less than 2^-18 (15 * 2^-22), is too close to a border
+// to tell: in 64 bits.
+__device__ __forceinline__ float kv4_code_exact(float x, float m, float d, float y)
 {
-    const float y = fminf(fmaxf((x - m) * inv, 0.f), 15.f);
-    float c = rintf(y);
-    if (fabsf(fabsf(y - c) - 0.5f) < 1e-5f) {
-        const float below = floorf(y), half = below + 0.5f;
-        const double r = ((double)x - (double)m) - (double)half * (double)d;
-        c = r > 0.0 ? below + 1.f : (r < 0.0 ? below : ((((int)below) & 1) ? below + 1.f : below));
-        c = fminf(c, 15.f);
-    }
-    return (uint32_t)c;
+    const float below = floorf(y), half = below + 0.5f;
+    const double r = ((double)x - (double)m) - (double)half * (double)d;
+    return r > 0.0 || (r == 0.0 && ((int)below & 1)) ? fminf(below + 1.f, 15.f) : below;
 }
 
 // Quantise eight consecutive dims (32 g + 8 t ..) of a row; the four lanes of a group (t = 0..3, consecutive lanes of
@@ -83,22 +86,37 @@ __device__ __forceinline__ void kv4_store8(const float (&x)[8], uint8_t *blk, in
         hi = fmaxf(hi, x[i]);
         ok = ok && isfinite(x[i]);
     }
-    int all_ok = ok ? 1 : 0;
+    if (!ok) lo = -INFINITY;
 #pragma unroll
     for (int s = 1; s < 4; s <<= 1) {
         lo = fminf(lo, __shfl_xor_sync(mask, lo, s));
         hi = fmaxf(hi, __shfl_xor_sync(mask, hi, s));
-        all_ok &= __shfl_xor_sync(mask, all_ok, s);
     }
     __half m, d;
     uint32_t w = 0;
-    if (all_ok) {
+    if (lo > -INFINITY) {
         kv4_params(lo, hi, m, d);
         const float mf = __half2float(m), df = __half2float(d), inv = df > 0.f ? 1.f / df : 0.f;
-        if (df > 0.f) {
+        constexpr float WHOLE = 12582912.f;   // 1.5 * 2^23: a sum's low bits are the nearest integer
+        bool odd = lo < -65504.f || df >= 65504.f;   // rare: saturated (codes may lie outside 0 .. 15), or close to a border
+        float c[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) w |= kv4_code(x[i], mf, df, inv) << (4 * i);
+        for (int i = 0; i < 8; i++) {
+            const float y = (x[i] - mf) * inv;
+            c[i] = (y + WHOLE) - WHOLE;
+            odd |= fabsf(fabsf(y - c[i]) - 0.5f) < 1e-5f;
         }
+        if (odd) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float y = fminf(fmaxf((x[i] - mf) * inv, 0.f), 15.f);
+                c[i] = (y + WHOLE) - WHOLE;
+                if (fabsf(fabsf(y - c[i]) - 0.5f) < 1e-5f) c[i] = kv4_code_exact(x[i], mf, df, y);
+            }
+        }
+        // four codes as one number of 16 bits
+        const float a = fmaf(fmaf(fmaf(c[3], 16.f, c[2]), 16.f, c[1]), 16.f, c[0]) + WHOLE, b = fmaf(fmaf(fmaf(c[7], 16.f, c[6]), 16.f, c[5]), 16.f, c[4]) + WHOLE;
+        w = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x5410);
     } else {
         m = __ushort_as_half((unsigned short)0x7FFF);
         d = __ushort_as_half((unsigned short)0);
@@ -173,14 +191,14 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(float *__restrict__ k, fl
 
 // cuda_rope_kv_rows with a 4-bit cache: token blockIdx.x at position pos0 + blockIdx.x; q and k rotated in place (theta <= 0: left
 // as they are), k and v quantised.  The angles of a token are computed once for all of its rows: 512 tokens of 32 / 8
-// heads of 128 take 5.7 us (4.2 TB/s), 8192 take 66 (5.8 TB/s); one block per row, as the f32 form has it, took 21.7 and 338, most
+// heads of 128 take 5.4 us (4.4 TB/s), 8192 take 61 (6.3 TB/s; at 57 registers instead of 40 69 us); one block per row, as the f32 form has it, took 21.7 and 338, most
 // of it for angles and for starting blocks.
 // Rows are q's, k's, then v's; 4 NG threads share one, each with four pairs, two vectors of four dims.  grid.y blocks share
 // a token's rows where there are few tokens.
 constexpr int RK4_THREADS = 256;
 
 template <int NG>
-__global__ void __launch_bounds__(RK4_THREADS) rope_kv4_rows_kernel(float *q, float *k, const float *__restrict__ v, uint8_t *__restrict__ cache,
+__global__ void __launch_bounds__(RK4_THREADS, 6) rope_kv4_rows_kernel(float *q, float *k, const float *__restrict__ v, uint8_t *__restrict__ cache,
                                                                     int n_heads, int n_kv, int n_blocks, int pos0, float theta,
                                                                     float yarn_scale, int yarn_orig_ctx, int neox)
 {
