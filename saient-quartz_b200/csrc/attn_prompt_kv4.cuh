@@ -145,8 +145,8 @@ __global__ void __launch_bounds__(APK_THREADS, 1) attn_prompt_kv4_kernel(const A
     const int tok = row / G, head = kvh * G + row % G;
     const bool is_row = row < nt * G;
 
-    // registers: 128 a thread at launch; the issuing warpgroup gives 64 of each of its threads away (8192), the others
-    // take 16 (2048) and 24 (2 x 3072)
+    // registers: 128 a thread at launch; the issuing warpgroup gives 64 of each of its threads away, the others take 16, 24 and
+    // 24 a thread: as many together
     if (warp < 4) asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
     else if (warp < 12) asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
     else asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
