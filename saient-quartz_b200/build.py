@@ -40,9 +40,11 @@ def included(src, seen=None):
     return seen
 
 
-def object_current(src, obj):
-    """The object is newer than its source, all that it includes and this file (compiler flags)."""
-    return os.path.exists(obj) and all(os.path.getmtime(f) <= os.path.getmtime(obj) for f in included(src) | {os.path.abspath(__file__)})
+def object_current(src, obj, cmd):
+    """The object is newer than its source, all that it includes and this file, and was made by the same command."""
+    if not os.path.exists(obj) or any(os.path.getmtime(f) > os.path.getmtime(obj) for f in included(src) | {os.path.abspath(__file__)}):
+        return False
+    return os.path.exists(obj + ".cmd") and open(obj + ".cmd").read() == " ".join(cmd)
 
 
 def build_host(force=False):
@@ -69,16 +71,21 @@ def build(force=False, verbose=False):
     cc = arch.replace("sm_", "compute_")
     cmd = [nvcc, "-O3", "-std=c++17", "-gencode", f"arch={cc},code={arch}", "-lineinfo", "-Xcompiler", "-fPIC", "-c"]
     cmd += os.environ.get("QUARTZ_NVCC_FLAGS", "").split()   # extra compiler flags (e.g. -DNAME=value)
-    if verbose:
-        cmd[1:1] = ["-Xptxas", "-v"]
+    show = ["-Xptxas", "-v"] if verbose else []
     objs, running = [], []
     for src in (s for s in sources() if s.endswith(".cu")):
         obj = os.path.join(HERE, os.path.splitext(os.path.basename(src))[0] + ".o")
         objs.append(obj)
-        if not force and object_current(src, obj):
+        if not force and object_current(src, obj, cmd):
             continue
-        running.append((src, subprocess.Popen(cmd + ["-o", obj, src])))
-    failed = [src for src, p in running if p.wait() != 0]
+        running.append((src, obj, subprocess.Popen(cmd + show + ["-o", obj, src])))
+    failed = []
+    for src, obj, p in running:
+        if p.wait() != 0:
+            failed.append(src)
+        else:
+            with open(obj + ".cmd", "w") as f:
+                f.write(" ".join(cmd))
     if failed:
         raise RuntimeError("nvcc failed on " + ", ".join(failed))
     tmp = LIB + ".tmp"
