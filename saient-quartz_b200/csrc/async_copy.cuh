@@ -1,4 +1,4 @@
-// Bulk asynchronous copies and the mbarriers they complete on.
+// Bulk asynchronous copies, the mbarriers they complete on, and the split cluster barrier.
 #pragma once
 
 #include "common.cuh"
@@ -66,5 +66,9 @@ __device__ __forceinline__ void cp_async16(void *smem_dst, const void *gmem_src,
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(smem_dst)), "l"(gmem_src), "r"(there ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// split cluster barrier (every thread of the CTA executes both halves)
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 }  // namespace qz

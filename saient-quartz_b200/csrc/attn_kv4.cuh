@@ -37,10 +37,6 @@ struct AttnKv4Args {
     int *status;
 };
 
-// split cluster barrier (every thread of the CTA executes both halves)
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-
 // ---- one token ---------------------------------------------------------------------------------------------------
 // One launch whose shape does not depend on the position.  A unit is a kv head (two units when more than eight query heads
 // share it); it has NC clusters of CL CTAs, of which as many work as the context has a block for every warp of.  Warp w of

@@ -58,10 +58,6 @@ struct AttnStepArgs {
     const float2 *rope_tab;
 };
 
-// split cluster barrier (every thread of the CTA executes both halves)
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-
 // dynamic shared memory (floats): ks [AS_ROWS][AS_KS_STRIDE], vs [AS_ROWS][ATT_MAX_HD], qs [G][ATT_MAX_HD],
 // ps [AS_WARPS][32], wres [AS_WARPS][2][ATT_MAX_HD + 2] (per-warp partials), recv [CL][2 G + S] (what the cluster's
 // CTAs push here: their (max, sum) of every head and their part of this CTA's S outputs), cs_tab [ATT_MAX_HD / 2] x 2
