@@ -21,7 +21,7 @@
 
 #include <cooperative_groups.h>
 
-#include "common.cuh"
+#include "async_copy.cuh"
 
 namespace qz {
 
@@ -420,6 +420,7 @@ __global__ void __launch_bounds__(SMP_THREADS) sample_kernel(const SampleArgs a)
     c.base = c.rank * a.chunk;
     c.n = max(0, min(a.chunk, a.vocab - c.base));
     const int row = blockIdx.x / c.CL, n = c.n;
+    cluster_arrive();   // another CTA's shared memory may be written once it runs: waited for before the first exchange
     pdl_wait();
     pdl_trigger();
     // ---- 1. the row into shared memory; its first token ----
@@ -456,7 +457,9 @@ __global__ void __launch_bounds__(SMP_THREADS) sample_kernel(const SampleArgs a)
         const float4 v = z4[at];
         best = c.number(4 * at + (v.x == top ? 0 : v.y == top ? 1 : v.z == top ? 2 : 3));
     }
-    c.exchange(smp_largest(best, s.red), 0);
+    best = smp_largest(best, s.red);
+    cluster_wait();   // (arrived at the top; the row was loaded meanwhile)
+    c.exchange(best, 0);
     best = c.largest();
     const bool none = best == 0;
     if (none || a.temperature == 0.f) {

@@ -121,6 +121,19 @@ def test_same_answer_however_the_rows_are_batched(gpu):
     assert np.array_equal(call(gpu, z, u, probs=False, **kw)[0], tok)
 
 
+def test_many_clusters_at_once(gpu):
+    """Rows of two and four CTAs in far more clusters than the device holds at once: the CTAs of a cluster start at different times,
+    and write to one another's shared memory only once all of them run.  Every row against the oracle, several times over."""
+    r = rng(10)
+    for rows, vocab in ((700, 20003), (300, 60007)):
+        z = (r.standard_normal((rows, vocab), dtype=np.float32) * 3)
+        u = r.random(rows)
+        for kw in (dict(temperature=0.0), dict(top_k=3, temperature=0.7), dict(top_p=0.8)):
+            tok = check(gpu, z, u, **kw)
+            for _ in range(3):
+                assert np.array_equal(call(gpu, z, u, **kw)[0], tok)
+
+
 def test_frequencies(gpu):
     """10,000 draws from eight tokens: a token's count is binomial; six standard deviations (2e-9 a token)."""
     p = np.array([0.3, 0.2, 0.15, 0.1, 0.1, 0.08, 0.05, 0.02])
