@@ -286,8 +286,11 @@ void cuda_attn_prompt_kv4(float *out, const float *q, const void *d_cache, int n
  * largest than f32 reaches.  temperature 0: the largest logit, ties to the lower index (d_u may be NULL), probability 1.
  * Logits of -inf and NaN are never chosen; a row without any other gives token -1, probability 0.  The sums are exact
  * integers: the same inputs give the same token however the work is split.  vocab <= 524288, finite temperature >= 0.
+ * cuda_sample_supported: 1 if cuda_sample takes this vocabulary and these settings (top_p and min_p are numbers); what it
+ * does not take it refuses, and writes no token.
  * cuda_step_advance: d_step[0] = *d_token (left as it is if that is negative), d_step[1] += 1, and the registered RoPE
  * tables of d_step (cuda_step_rope_table) for the new position: the device-side cuda_step_set, on the same stream. */
+int cuda_sample_supported(int vocab, float temperature, float top_p, float min_p);
 void cuda_sample(const float *d_logits, int n_rows, int vocab, size_t row_stride, float temperature, int top_k, float top_p, float min_p,
                  const float *d_u, int *d_tokens, float *d_probs);
 void cuda_step_advance(int *d_step, const int *d_token);

@@ -115,6 +115,7 @@ _SIGS = {
     "cuda_attn_step_kv4": (None, [C.c_void_p] * 5 + [C.c_int] * 4 + [C.c_void_p, C.c_int, C.c_int, C.c_float, C.c_void_p, C.c_float,
                                   C.c_float, C.c_int, C.c_int, C.c_int]),
     "cuda_attn_prompt_kv4": (None, [C.c_void_p] * 3 + [C.c_int] * 7 + [C.c_float, C.c_void_p]),
+    "cuda_sample_supported": (C.c_int, [C.c_int, C.c_float, C.c_float, C.c_float]),
     "cuda_sample": (None, [C.c_void_p, C.c_int, C.c_int, C.c_size_t, C.c_float, C.c_int, C.c_float, C.c_float] + [C.c_void_p] * 3),
     "cuda_step_advance": (None, [C.c_void_p, C.c_void_p]),
     "cuda_gemv_experts": (None, [C.c_uint32, C.c_void_p, C.c_size_t, C.c_void_p, C.c_int, C.c_void_p, C.c_size_t, C.c_void_p,

@@ -28,6 +28,11 @@ int sample_cluster(int n_rows, int vocab)
 
 }  // namespace
 
+extern "C" int cuda_sample_supported(int vocab, float temperature, float top_p, float min_p)
+{
+    return vocab >= 1 && vocab <= SMP_MAX_VOCAB && temperature >= 0.f && std::isfinite(temperature) && top_p == top_p && min_p == min_p ? 1 : 0;
+}
+
 extern "C" void cuda_sample(const float *d_logits, int n_rows, int vocab, size_t row_stride, float temperature, int top_k, float top_p,
                             float min_p, const float *d_u, int *d_tokens, float *d_probs)
 {
@@ -36,7 +41,7 @@ extern "C" void cuda_sample(const float *d_logits, int n_rows, int vocab, size_t
         set_error(vocab > SMP_MAX_VOCAB ? QZ_ERR_TOO_LARGE : QZ_ERR_BAD_SHAPE, "cuda_sample: 1 <= vocab <= 524288 and row_stride >= vocab");
         return;
     }
-    if (!(temperature >= 0.f) || !isfinite(temperature) || !(top_p == top_p) || !(min_p == min_p)) {
+    if (!cuda_sample_supported(vocab, temperature, top_p, min_p)) {
         set_error(QZ_ERR_BAD_SHAPE, "cuda_sample: temperature must be finite and at least 0, top_p and min_p must be numbers");
         return;
     }

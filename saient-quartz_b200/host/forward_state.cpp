@@ -812,7 +812,7 @@ int qh_generate(qh_model *m, int token, int pos, int n, float temperature, int t
                 int *tokens_out)
 {
     if (!m || !m->finalized || !tokens_out || n <= 0 || pos < 0 || (long long)pos + n > m->c.max_seq || token < 0 || token >= m->c.vocab_size ||
-        (!u && temperature > 0.f))
+        (!u && temperature > 0.f) || !cuda_sample_supported(m->c.vocab_size, temperature, top_p, min_p))
         return -1;
     if (n > m->g_cap) {
         if (!m->g_u.alloc_f32(n) || !m->g_tok.alloc_f32(n)) return -2;

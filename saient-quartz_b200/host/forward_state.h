@@ -81,7 +81,8 @@ int qh_prefill(qh_model *m, const int *tokens, int n, int pos0, float *logits_ho
  * u[i], uniform in [0, 1), and the given settings), step with it at pos + 1, ...  Where the fused sequence serves the model
  * the whole loop runs on the device -- sampled token and position go from one step to the next as device words
  * (cuda_step_advance) -- and the host waits once, for tokens_out[0..n); otherwise it reads every token back.  The last
- * token is chosen, not stepped: pos + n <= max_seq.  u may be NULL at temperature 0.  0 on success. */
+ * token is chosen, not stepped: pos + n <= max_seq.  u may be NULL at temperature 0.  Settings or a vocabulary that
+ * cuda_sample does not take (cuda_sample_supported) are refused before anything runs.  0 on success. */
 int qh_generate(qh_model *m, int token, int pos, int n, float temperature, int top_k, float top_p, float min_p, const float *u,
                 int *tokens_out);
 /* device-only variants for timing: no copies, the result stays in the device logits buffer; fused: 0 reference

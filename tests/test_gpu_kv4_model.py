@@ -167,6 +167,21 @@ def test_generate_to_the_last_position_and_refusals(gpu, oracle_mod):
     gpu.lib().quartz_clear_error()
 
 
+@pytest.mark.parametrize("bad", [dict(temperature=-1.0), dict(temperature=float("nan")), dict(temperature=float("inf")), dict(top_p=float("nan")),
+                                 dict(min_p=float("nan"))])
+def test_generate_refuses_what_the_sampler_does_not_take(gpu, oracle_mod, bad):
+    m = _model(n_layers=1, max_seq=40)
+    m.fill_kv(10)
+    before = gpu.lib().quartz_launch_count()
+    a = dict(temperature=0.5, u=np.full(5, 0.5, np.float32))
+    a.update(bad)
+    with pytest.raises(RuntimeError):
+        m.generate(1, 10, 5, **a)
+    assert gpu.lib().quartz_launch_count() == before and gpu.lib().quartz_last_error() == 0
+    assert len(m.generate(1, 10, 5)) == 5
+    gpu.check_error()
+
+
 def test_no_positions(gpu, oracle_mod):
     m = _model(n_layers=1, max_seq=40)
     k, v = m.read_kv(0, 3, 0)

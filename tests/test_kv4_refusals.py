@@ -117,3 +117,12 @@ def test_rows_refuse_more_than_memory_holds(L, name):
     before = L.quartz_launch_count()
     rows(L, name, n_tok=2 ** 26, n_kv=32, hd=32, max_seq=2 ** 26)
     assert refused(L, 5) == before
+
+
+def test_sampler_settings(L):
+    assert all(L.cuda_sample_supported(*a) == 1 for a in ((1, 0.0, 1.0, 0.0), (1 << 19, 0.8, 0.9, 0.05), (100, 3e38, -1.0, 7.0)))
+    nan, inf = float("nan"), float("inf")
+    for bad in ((0, 0.8, 0.9, 0.0), (-5, 0.8, 0.9, 0.0), ((1 << 19) + 1, 0.8, 0.9, 0.0), (100, -0.5, 0.9, 0.0), (100, nan, 0.9, 0.0), (100, inf, 0.9, 0.0),
+                (100, -inf, 0.9, 0.0), (100, 0.8, nan, 0.0), (100, 0.8, 0.9, nan), (100, 0.0, nan, 0.0)):
+        assert L.cuda_sample_supported(*bad) == 0, bad
+    assert L.quartz_last_error() == 0
