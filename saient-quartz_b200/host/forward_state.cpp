@@ -815,6 +815,7 @@ int qh_generate(qh_model *m, int token, int pos, int n, float temperature, int t
         (!u && temperature > 0.f) || !cuda_sample_supported(m->c.vocab_size, temperature, top_p, min_p))
         return -1;
     if (n > m->g_cap) {
+        m->g_cap = 0;   // (growing drops the old buffers first)
         if (!m->g_u.alloc_f32(n) || !m->g_tok.alloc_f32(n)) return -2;
         m->g_cap = n;
     }

@@ -27,8 +27,13 @@ void *cuda_alloc(size_t n)
     return p;
 }
 void cuda_drop(void *p) { free(p); }
-void cuda_h2d(void *d, const void *s, size_t n) { memcpy(d, s, n); }
-void cuda_d2h(void *d, const void *s, size_t n) { memcpy(d, s, n); }
+static void copy(void *d, const void *s, size_t n)
+{
+    if (valid(d) && valid(s)) memcpy(d, s, n);
+    else fake_bad_writes++;
+}
+void cuda_h2d(void *d, const void *s, size_t n) { copy(d, s, n); }
+void cuda_d2h(void *d, const void *s, size_t n) { copy(d, s, n); }
 int quartz_last_error(void) { return fake_error; }
 int quartz_graph_begin(void) { return 1; }
 void *quartz_graph_end(void) { return &step_words; }
@@ -146,3 +151,14 @@ def test_a_vocabulary_that_the_sampler_does_not_take_is_refused(H):
     assert m.generate(20)[0] == -1 and m.get("error") == 0
     assert [m.get(n) for n in ("samples", "replays", "bad_rows")] == [0, 0, 0]
     H.qh_destroy(m.m)
+
+
+@pytest.mark.parametrize("which", [1, 2])
+def test_buffers_that_could_not_grow(model, which):
+    """The first or the second of the two does not fit: refused, and a later, shorter call has buffers of its own again."""
+    assert model.generate(4)[0] == 0
+    model.set("fail_alloc", which)
+    assert model.generate(100)[0] == -2
+    for n in (1, 3, 4, 100):
+        assert model.generate(n) == (0, model.expected(n))
+    assert model.get("bad_writes") == 0 and model.get("bad_rows") == 0
