@@ -820,6 +820,9 @@ int qh_generate(qh_model *m, int token, int pos, int n, float temperature, int t
         m->g_cap = n;
     }
     if (u) cuda_h2d(m->g_u.ptr, u, (size_t)n * 4);
+    // -1: where a launch of the sampler fails, the step words keep their token
+    const std::vector<int> none(n, -1);
+    cuda_h2d(m->g_tok.ptr, none.data(), (size_t)n * 4);
     const bool on_device = fusable(m);
     const int V = m->c.vocab_size;
     int *tok = (int *)m->g_tok.ptr;

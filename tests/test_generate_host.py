@@ -162,3 +162,16 @@ def test_buffers_that_could_not_grow(model, which):
     for n in (1, 3, 4, 100):
         assert model.generate(n) == (0, model.expected(n))
     assert model.get("bad_writes") == 0 and model.get("bad_rows") == 0
+
+
+def test_a_sampler_that_did_not_run(model):
+    """Its launch failed: the steps go on with the last token, never with what the buffer held, and the call fails."""
+    assert model.generate(4)[0] == 0
+    model.set("fail_sample", 1)
+    for n in (4, 40):
+        rc, tokens = model.generate(n)
+        assert rc != 0 and model.get("bad_rows") == 0
+        assert set(tokens) <= {-1, -77}
+    model.set("fail_sample", 0)
+    model.set("error", 0)
+    assert model.generate(40) == (0, model.expected(40))
