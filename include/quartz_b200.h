@@ -365,7 +365,8 @@ void cuda_host_free(void *p);
  * instead of executed; cuda_h2d / cuda_d2h / cuda_sync must stay outside (cuda_h2d_async and
  * cuda_d2h_async may be recorded), and every scratch buffer must
  * already exist (run the sequence once eagerly first).  end returns an executable graph (NULL on
- * failure); launch replays it, ordered with the default stream. */
+ * failure); launch replays it, ordered with the library's stream (the default one, or what quartz_set_stream
+ * set): behind the calls before it, ahead of those after it.  Replays of all graphs follow one another. */
 /* 1 (default): kernels recorded into a graph are launched as programmatic dependents, so each
  * may begin (and a GEMV may start streaming its weights) while its predecessor drains; 0: plain
  * serial edges.  Results are identical. */

@@ -6,7 +6,7 @@
 namespace qz {
 
 bool pdl_enabled();            // kernels are being recorded into a graph as programmatic dependents
-cudaStream_t replay_stream();  // stream on which recorded graphs replay (step words are written there)
+cudaStream_t replay_stream();  // stream on which the step words are written, in order with the replays of recorded graphs
 int *status_word();            // device word that bounded waits set when they run out; NULL if it cannot be created
 int *status_word_if_ready();   // the same for calls that may be captured before anything created it (then NULL)
 // activation-form scratch slot 0..3 for a vector of n values; false (and the sticky error) if there is none

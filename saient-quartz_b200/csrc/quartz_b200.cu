@@ -46,7 +46,8 @@ void set_error(int code, const char *what)
 }
 cudaStream_t stream() { return g_stream; }
 static cudaStream_t g_graph_stream = nullptr, g_saved_stream = nullptr;
-// the stream the recorded graphs replay on (when there is one), so that the step words are ordered with the replays
+// Where the step words are written: on the stream the recorded graphs replay on, or on the stream that is set, with which
+// quartz_graph_launch orders every replay.
 cudaStream_t replay_stream() { return (g_graph_stream && g_stream == 0) ? g_graph_stream : g_stream; }
 int sm_count()
 {
@@ -2091,7 +2092,23 @@ void quartz_set_pdl(int on) { g_pdl_in_graphs = on != 0; }
 void quartz_graph_launch(void *graph_exec)
 {
     if (!graph_exec) return;
+    // All replays run on one stream, one after the other (the recorded calls share the library's scratch).  The legacy default
+    // stream is ordered with it by itself, any other one that is set by events on both sides of the replay.
+    static cudaEvent_t event = nullptr;
+    const bool join = g_stream != 0 && g_stream != g_graph_stream;
+    if (join && !event) {
+        QZ_CUDA_CHECK(cudaEventCreateWithFlags(&event, cudaEventDisableTiming));
+        if (!event) return;
+    }
+    if (join) {
+        QZ_CUDA_CHECK(cudaEventRecord(event, g_stream));
+        QZ_CUDA_CHECK(cudaStreamWaitEvent(g_graph_stream, event, 0));
+    }
     QZ_CUDA_CHECK(cudaGraphLaunch((cudaGraphExec_t)graph_exec, g_graph_stream));
+    if (join) {
+        QZ_CUDA_CHECK(cudaEventRecord(event, g_graph_stream));
+        QZ_CUDA_CHECK(cudaStreamWaitEvent(g_stream, event, 0));
+    }
 }
 
 void quartz_graph_destroy(void *graph_exec)

@@ -127,6 +127,58 @@ def test_generate_equals_steps_and_the_oracle_sampler(gpu, oracle_mod, kv_bits, 
     gpu.check_error()
 
 
+def test_a_replay_is_ordered_with_the_stream_that_is_set(gpu):
+    """On a non-blocking stream held up by a long kernel: what is issued before a replay runs before it, what follows after it."""
+    import torch
+    L, n = gpu.lib(), 1 << 16
+    a, b, c = (gpu.GpuBuf.upload(np.full(n, x, np.float32)) for x in (5.0, 3.0, 0.0))
+    L.quartz_set_stream(None)
+    assert L.quartz_graph_begin()
+    L.cuda_vec_add(a.ptr, b.ptr, n)          # a += 3
+    graph = L.quartz_graph_end()
+    st = torch.cuda.Stream()
+    L.quartz_set_stream(st.cuda_stream)
+    try:
+        with torch.cuda.stream(st):
+            torch.cuda._sleep(100_000_000)
+            L.cuda_vec_zero(a.ptr, n)
+            L.quartz_graph_launch(graph)     # a = 3
+            L.quartz_graph_launch(graph)     # a = 6
+            L.cuda_vec_add(c.ptr, a.ptr, n)  # c = 6
+            L.quartz_graph_launch(graph)     # a = 9
+        st.synchronize()                     # waits for the last replay as well
+    finally:
+        L.quartz_set_stream(None)
+    assert (a.download() == 9).all() and (c.download() == 6).all()
+    L.quartz_graph_destroy(graph)
+    gpu.check_error()
+
+
+@pytest.mark.parametrize("kv_bits", [4, 32])
+def test_generate_on_a_stream_of_the_callers(gpu, oracle_mod, kv_bits):
+    import torch
+    L, n = gpu.lib(), 24
+    m = _model(kv_bits=kv_bits)
+    m.fill_kv(30)
+    u = np.random.Generator(np.random.PCG64(6)).random(n).astype(np.float32)
+    kw = dict(temperature=1.1, top_k=50, top_p=0.9, u=u)
+    want = list(m.generate(7, 30, n, **kw))
+    step = m.step(9, 40, fused=True)
+    try:
+        for st in (torch.cuda.Stream(), torch.cuda.Stream()):
+            L.quartz_set_stream(st.cuda_stream)
+            for _ in range(3):
+                assert list(m.generate(7, 30, n, **kw)) == want
+            assert np.array_equal(m.step(9, 40, fused=True), step)
+        fresh = _model(kv_bits=kv_bits)      # recorded while the stream is set
+        fresh.fill_kv(30)
+        assert list(fresh.generate(7, 30, n, **kw)) == want
+    finally:
+        torch.cuda.synchronize()
+        L.quartz_set_stream(None)
+    gpu.check_error()
+
+
 def test_generate_without_the_fused_sequence(gpu, oracle_mod):
     r = np.random.Generator(np.random.PCG64(4))
     m = _model(extra=[("Q_BIAS", 0, r.standard_normal(2048).astype(np.float32))])
