@@ -711,7 +711,9 @@ __global__ void __launch_bounds__(AK_THREADS, NT == 1 ? 2 : 1) attn_step_kv4_ker
             int before = 0;
             // releases the warp's stores (ordered before it by the warp barrier), acquires the other clusters'
             if (lane == 0) asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(before) : "l"(count) : "memory");
-            if (__shfl_sync(0xFFFFFFFFu, before, 0) != NC - 1) continue;
+            before = __shfl_sync(0xFFFFFFFFu, before, 0);
+            __syncwarp();   // (the shuffle orders no memory: lane 0's acquire is the warp's from here on)
+            if (before != NC - 1) continue;
             if (lane == 0) *count = 0;   // for the next call
             float all_top = -3.0e38f;
             for (int c = 0; c < NC; c++) all_top = fmaxf(all_top, __ldcg(ws + 34 * c));

@@ -531,3 +531,136 @@ def test_cache_past_32_bits(gpu):
         gpu.check_error()
     finally:
         L.cuda_drop(ptr)
+
+
+# ---- several clusters and their merge, recorded ------------------------------------------------------------------
+def merge_setup(gpu, r, nh, n_kv, hd, max_seq, filled_to):
+    cache, raw, k, v = filled(gpu, r, filled_to, n_kv, hd, max_seq)
+    q, kn, vn = r.standard_normal((1, nh, hd), dtype=np.float32), rows(r, 1, n_kv, hd, True), rows(r, 1, n_kv, hd, False)
+    return cache, raw, k, v, q, kn, vn
+
+
+@pytest.mark.parametrize("nh,n_kv,hd,max_seq", [(32, 8, 128, 9000), (8, 2, 64, 20000), (64, 8, 128, 9000), (12, 2, 96, 12000)])
+def test_recorded_step_of_a_long_cache(gpu, nh, n_kv, hd, max_seq):
+    """As a model with a long context issues it: rotation with the table, append, position words, activation slot, recorded, at positions
+    that one, some and all clusters of a unit work on, several replays each."""
+    from saient_quartz_b200 import synth
+    L, r = gpu.lib(), rng(50, nh, hd)
+    cache, raw, k, v, q, kn, vn = merge_setup(gpu, r, nh, n_kv, hd, max_seq, max_seq)
+    dq, dk, dv = upload(gpu, q), upload(gpu, kn), upload(gpu, vn)
+    K, N, scale = nh * hd, 64, 0.09
+    out, out2, step = gpu.GpuBuf.alloc_f32(K), gpu.GpuBuf.alloc_f32(K), gpu.GpuBuf.alloc_f32(4)
+    w = upload(gpu, synth.make_weights(8, K, N, tensor_id=3))
+    y = [gpu.GpuBuf.alloc_f32(N) for _ in range(2)]
+
+    def call():
+        L.cuda_attn_step_kv4(out.ptr, dq.ptr, dk.ptr, dv.ptr, cache.ptr, nh, n_kv, hd, max_seq, step.ptr, 0, 0, scale, None, 5e5, 1.0, 0, 0, 2)
+    L.cuda_step_rope_table(step.ptr, hd, 5e5, 1.0, 0)
+    L.cuda_step_set(step.ptr, 0, 0)
+    call()
+    assert L.quartz_graph_begin()
+    call()
+    graph = L.quartz_graph_end()
+    assert graph
+    for pos in (7, 2000, 3199, max_seq // 2, max_seq - 1):
+        L.cuda_step_set(step.ptr, 5, pos)
+        got = []
+        for _ in range(4):
+            put(gpu, cache, raw)
+            L.quartz_graph_launch(graph)
+            got.append(out.download())
+        assert all(np.array_equal(g, got[0]) for g in got)
+        after = cache.download(np.uint8)
+        # the same by parts: rotation and append by the rows' call, attention without either
+        put(gpu, cache, raw)
+        q2, k2 = upload(gpu, q), upload(gpu, kn)
+        L.cuda_rope_kv4_rows(q2.ptr, k2.ptr, dv.ptr, cache.ptr, 1, nh, n_kv, hd, max_seq, pos, 5e5, 1.0, 0, 0)
+        assert np.array_equal(cache.download(np.uint8), after)
+        L.cuda_attn_step_kv4(out2.ptr, q2.ptr, None, None, cache.ptr, nh, n_kv, hd, max_seq, None, pos, 0, scale, None, 0.0, 1.0, 0, 0, -1)
+        kk, vv = k[:pos + 1].copy(), v[:pos + 1].copy()
+        kk[pos], vv[pos] = kv4.values(k2.download().reshape(1, n_kv, hd))[0], kv4.values(vn)[0]
+        want, bound = kv4.attention(q2.download().reshape(1, nh, hd), kk, vv, pos, 0, float(np.float32(scale)), None)
+        held(out2.download().reshape(1, nh, hd), want, bound)
+        # the rotation may round differently by an ulp where the compiler contracts it: 2^-22 of a score's terms
+        assert np.abs(got[0] - out2.download()).max() <= 2.0 ** -18 * np.abs(want).max()
+        if L.cuda_gemv_q_supported(8, w.ptr, K):      # the slot holds what cuda_quantize_x makes of the result
+            put(gpu, cache, raw)
+            L.quartz_graph_launch(graph)
+            L.cuda_quantize_x(out.ptr, K, 1)
+            for slot, b in ((2, y[0]), (1, y[1])):
+                L.cuda_gemv_q(8, 1, (C.c_void_p * 1)(w.ptr), (C.c_int * 1)(slot), (C.c_void_p * 1)(b.ptr), K, N, 0)
+            assert np.array_equal(y[0].download(), y[1].download())
+    L.quartz_graph_destroy(graph)
+    gpu.check_error()
+
+
+def test_graphs_of_long_caches_side_by_side(gpu):
+    """Two captured steps that merge, replayed at the same time on two streams, and two eager ones: each has a workspace of its own."""
+    import torch
+    L, sets = gpu.lib(), []
+    nh, n_kv, hd, max_seq = 16, 4, 128, 9000
+    for i in range(2):
+        r = rng(51, i)
+        cache, _, k, v, q, _, _ = merge_setup(gpu, r, nh, n_kv, hd, max_seq, max_seq)
+        out = gpu.GpuBuf.alloc_f32(nh * hd)
+        want = kv4.attention(q, k, v, max_seq - 1, 0, float(np.float32(0.09)), None)
+        sets.append((cache, upload(gpu, q), out, want, torch.cuda.Stream(), torch.cuda.CUDAGraph()))
+
+    def call(s):
+        L.cuda_attn_step_kv4(s[2].ptr, s[1].ptr, None, None, s[0].ptr, nh, n_kv, hd, max_seq, None, max_seq - 1, 0, 0.09, None, 0.0, 1.0, 0, 0, -1)
+
+    def check():
+        torch.cuda.synchronize()
+        got = [s[2].download() for s in sets]
+        for g, s in zip(got, sets):
+            held(g.reshape(1, nh, hd), *s[3])
+            put(gpu, s[2], np.zeros(nh * hd, np.float32))
+        return got
+    try:
+        for s in sets:
+            call(s)
+        first = check()
+        for s in sets:
+            with torch.cuda.graph(s[5], stream=s[4]):
+                L.quartz_set_stream(torch.cuda.current_stream().cuda_stream)
+                call(s)
+            L.quartz_set_stream(None)
+        for _ in range(3):
+            for _ in range(50):
+                for s in sets:
+                    with torch.cuda.stream(s[4]):
+                        s[5].replay()
+            assert all(np.array_equal(a, b) for a, b in zip(check(), first))
+            for _ in range(50):
+                for s in sets:
+                    L.quartz_set_stream(s[4].cuda_stream)
+                    call(s)
+            L.quartz_set_stream(None)
+            assert all(np.array_equal(a, b) for a, b in zip(check(), first))
+    finally:
+        torch.cuda.synchronize()
+        L.quartz_set_stream(None)
+    gpu.check_error()
+
+
+def test_workspaces_of_graphs_that_are_gone_are_used_again(gpu):
+    import torch
+    L, r = gpu.lib(), rng(52)
+    nh, n_kv, hd, max_seq = 16, 4, 128, 9000
+    cache, _, k, v, q, _, _ = merge_setup(gpu, r, nh, n_kv, hd, max_seq, max_seq)
+    dq, out = upload(gpu, q), gpu.GpuBuf.alloc_f32(nh * hd)
+    want = kv4.attention(q, k, v, max_seq - 1, 0, float(np.float32(0.09)), None)
+    free = []
+    for i in range(40):
+        assert L.quartz_graph_begin()
+        L.cuda_attn_step_kv4(out.ptr, dq.ptr, None, None, cache.ptr, nh, n_kv, hd, max_seq, None, max_seq - 1, 0, 0.09, None, 0.0, 1.0, 0, 0, -1)
+        graph = L.quartz_graph_end()
+        put(gpu, out, np.zeros(nh * hd, np.float32))
+        for _ in range(3):
+            L.quartz_graph_launch(graph)
+        held(out.download().reshape(1, nh, hd), *want)
+        L.quartz_graph_destroy(graph)
+        torch.cuda.synchronize()
+        free.append(torch.cuda.mem_get_info()[0])
+    assert free[4] - free[-1] <= 4 << 20          # 35 workspaces of their own would take 20 MB
+    gpu.check_error()
