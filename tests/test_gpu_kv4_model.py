@@ -234,6 +234,30 @@ def test_generate_refuses_what_the_sampler_does_not_take(gpu, oracle_mod, bad):
     gpu.check_error()
 
 
+def test_a_long_context_in_every_sequence(gpu, oracle_mod):
+    """A cache in which several clusters of a kv head work and merge: recorded steps, generation, short and long positions."""
+    m = _model(max_seq=9000, n_layers=2)
+    m.fill_kv(8900)
+    ref = _ref(m, 8900)
+    for pos, tok in ((8900, 17), (8901, 300)):
+        want = ref.forward(tok, pos)
+        plain = m.step(tok, pos, fused=False)
+        assert _rel(plain, want) < 5e-3
+        _rows_match(m, ref, pos)
+        for seq in (1, 2):
+            got = m.step(tok, pos, fused=seq)
+            assert _rel(got, want) < 5e-3 and _rel(got, plain) < 2e-3, seq
+    u = np.random.Generator(np.random.PCG64(9)).random(12).astype(np.float32)
+    for at in (40, 4000, 8902):
+        got = m.generate(7, at, 12, temperature=0.9, top_k=30, u=u)
+        tok, want = 7, []
+        for i in range(12):
+            tok = sampling.sample(m.step(tok, at + i, fused=True), u[i], temperature=0.9, top_k=30)[0]
+            want.append(tok)
+        assert list(got) == want
+    gpu.check_error()
+
+
 def test_no_positions(gpu, oracle_mod):
     m = _model(n_layers=1, max_seq=40)
     k, v = m.read_kv(0, 3, 0)
