@@ -651,7 +651,7 @@ def test_workspaces_of_graphs_that_are_gone_are_used_again(gpu):
     dq, out = upload(gpu, q), gpu.GpuBuf.alloc_f32(nh * hd)
     want = kv4.attention(q, k, v, max_seq - 1, 0, float(np.float32(0.09)), None)
     free = []
-    for i in range(40):
+    for i in range(200):
         assert L.quartz_graph_begin()
         L.cuda_attn_step_kv4(out.ptr, dq.ptr, None, None, cache.ptr, nh, n_kv, hd, max_seq, None, max_seq - 1, 0, 0.09, None, 0.0, 1.0, 0, 0, -1)
         graph = L.quartz_graph_end()
@@ -662,5 +662,7 @@ def test_workspaces_of_graphs_that_are_gone_are_used_again(gpu):
         L.quartz_graph_destroy(graph)
         torch.cuda.synchronize()
         free.append(torch.cuda.mem_get_info()[0])
-    assert free[4] - free[-1] <= 4 << 20          # 35 workspaces of their own would take 20 MB
+    # 195 workspaces of their own, 4 * (128 * 32 + 128 * 32 * 34) bytes each, would take 107 MiB; the driver's own pools take chunks
+    # of some MiB at times (8 were seen)
+    assert free[4] - free[-1] <= 32 << 20
     gpu.check_error()
