@@ -11,6 +11,8 @@ namespace qz {
 // six warps: two CTAs of them per SM leave 168 registers a thread (eight: 128, which spill; 131072 positions take 58 us, not 51)
 constexpr int AK_THREADS = 192, AK_WARPS = AK_THREADS / 32;
 constexpr int AK_MAX_G = 16;
+constexpr float AK_RAISE = 2.f;                       // weights are at most 2^AK_RAISE,
+constexpr float AK_STEP_TOP = 8192.f;                 // scaled steps at most this, set to [1/4, 1/2) of it: products below 2^15
 constexpr int AK_MAX_CLUSTERS = 128;                  // of all units together when a unit has several
 constexpr int AK_COUNTERS = AK_MAX_CLUSTERS * 32;     // one per run of 32 outputs of a unit
 constexpr size_t AK_WORKSPACE = sizeof(float) * (AK_COUNTERS + (size_t)AK_MAX_CLUSTERS * 32 * 34);
@@ -55,9 +57,11 @@ struct AttnKv4Args {
 // the mantissa) and one exact HADD2 / HFMA2.  (The nibbles alone, as f16 subnormals, would need no second step, but the
 // tensor core aligns products by their nominal exponents: 6 to 10 bits of the sum were lost, 5e-6 of the output.)
 // q and p * d are split into two f16 parts, hi + lo, in neighbouring columns of the 8-column operand, so four heads fill
-// one mma.m16n8k16; both parts are scaled by powers of two (per head for q, per warp for d) that keep them clear of
-// f16's ends.  Sums are f32.
-// The softmax reference of a head is raised only when a score exceeds it by 2^8; until then weights up to 2^8 do no harm.
+// one mma.m16n8k16; both parts are scaled by powers of two (per head for q, per group of 32 dims for d: a group's outputs
+// owe nothing to the other groups) that keep them clear of f16's ends.  Sums are f32.
+// The softmax reference of a head is raised only when a score exceeds it by 2^AK_RAISE; until then weights up to that do no
+// harm, and f16 has as many binades more for small ones.  With the largest step that the warp has met in a group at 2^11 or
+// above, 22 bits of p d are whole down to 2^-14 of that step (p d = 2^-3), and below that the error is 2^-35 of it at most.
 //
 // Measured (32 / 8 heads of 128, replayed): context 1024 6.3 us (8 / 2 heads of 64, context 18: 4.4), 4096 10.6,
 // 16384 13.9, 131072 51 us = 3.3 TB/s of the cache.  Short contexts are bound by the launch, two cluster barriers and one
@@ -187,7 +191,8 @@ __device__ __forceinline__ void lds_floats(const float *p, float (&x)[N])
 // 32 j + 4 gr + i of head t.  Weights as operand: head gr / 2 (part gr % 2), positions t, t + 4, t + 8, t + 12 of a tile.
 template <int NG, int NT>
 struct Kv4Warp {
-    static constexpr int SCRATCH = 4 * 32 * NG;   // floats of shared memory a warp needs: d, m + 8 d of K and of V per position
+    // floats of shared memory a warp needs: d, m + 8 d of K and of V per position, powers of two that p * d of group j carries
+    static constexpr int VE = 4 * 32 * NG, SCRATCH = VE + 4;
     uint32_t qf[NT][NG][4];   // q as the column operand: dims (0,4) (1,5) (2,6) (3,7) of 32 j + 8 t, column gr
     float qs[NT][NG];         // sum of q over group j, head t
     float back[NT];           // scores in log2 units = back * what the products give, head t
@@ -195,12 +200,12 @@ struct Kv4Warp {
     float o[NT][2 * NG][4];   // sums of the tensor core since the last flush
     float acc[NT][2 * NG][2]; // flushed sums (hi + lo)
     float mo[NT][NG];         // partial sums of p * (m + 8 d), head gr / 2
-    float ve;                 // power of two that p * d carries
     Nibbles nib;
 
-    __device__ __forceinline__ void clear()
+    __device__ __forceinline__ void clear(float *scratch, int lane)
     {
-        ve = 1.2676506e30f;   // 2^100: the first block with a step above zero sets it
+        if (lane < NG) scratch[VE + lane] = 1.2676506e30f;   // 2^100: the first block with a step above zero sets it
+        __syncwarp();
 #pragma unroll
         for (int n = 0; n < NT; n++) {
             ref[n] = -3.0e38f;
@@ -238,7 +243,9 @@ struct Kv4Warp {
         // ---- parameters: lane = position, converted once for the warp ----
         const bool whole = lo == 0 && hi == KV4_BLOCK - 1;
         {
-            float m[NG], d[NG], dm = 0.f;
+            float m[NG], d[NG], ve[NG];
+            bool above = false;
+            lds_floats<NG>(scratch + VE, ve);
             const bool seen = lane >= lo && lane <= hi;
 #pragma unroll
             for (int side = 0; side < 2; side++) {
@@ -250,21 +257,27 @@ struct Kv4Warp {
                     for (int j = 0; j < NG; j++) m[j] = d[j] = 0.f;
                 }
                 float *dd = (side ? vd : kd) + lane * NG, *mm = (side ? vm : km) + lane * NG;
+#pragma unroll
+                for (int j = 0; j < NG; j++) m[j] = fmaf(8.f, d[j], m[j]);
+                if (side) {   // values: d as p will meet it, scaled
+#pragma unroll
+                    for (int j = 0; j < NG; j++) {
+                        d[j] *= ve[j];
+                        above |= d[j] > AK_STEP_TOP;
+                    }
+                }
                 if constexpr (NG == 4) {
                     *(float4 *)dd = make_float4(d[0], d[1], d[2], d[3]);
-                    *(float4 *)mm = make_float4(fmaf(8.f, d[0], m[0]), fmaf(8.f, d[1], m[1]), fmaf(8.f, d[2], m[2]), fmaf(8.f, d[3], m[3]));
+                    *(float4 *)mm = make_float4(m[0], m[1], m[2], m[3]);
                 } else {
 #pragma unroll
                     for (int j = 0; j < NG; j++) {
                         dd[j] = d[j];
-                        mm[j] = fmaf(8.f, d[j], m[j]);
+                        mm[j] = m[j];
                     }
                 }
             }
-            // scale of p * d: the largest d stays below 2^7 (weights are at most 2^8: products below 2^15)
-#pragma unroll
-            for (int j = 0; j < NG; j++) dm = fmaxf(dm, d[j]);
-            if (__any_sync(0xFFFFFFFFu, dm * ve > 128.f)) set_scale(dm);
+            if (__any_sync(0xFFFFFFFFu, above)) set_scale(d, ve, vd + lane * NG, scratch + VE);   // (rare)
         }
         __syncwarp();
         // ---- scores ----
@@ -310,7 +323,7 @@ struct Kv4Warp {
         // ---- weights ----
         bool raise = false;
 #pragma unroll
-        for (int n = 0; n < NT; n++) raise |= fmaxf(fmaxf(s[0][n][0], s[0][n][1]), fmaxf(s[1][n][0], s[1][n][1])) * back[n] > ref[n] + 8.f;
+        for (int n = 0; n < NT; n++) raise |= fmaxf(fmaxf(s[0][n][0], s[0][n][1]), fmaxf(s[1][n][0], s[1][n][1])) * back[n] > ref[n] + AK_RAISE;
         if (__any_sync(0xFFFFFFFFu, raise)) {
 #pragma unroll
             for (int n = 0; n < NT; n++) {
@@ -362,8 +375,6 @@ struct Kv4Warp {
                 const float a = part ? p[n][2] : p[n][0], b = part ? p[n][3] : p[n][1];
 #pragma unroll
                 for (int j = 0; j < NG; j++) mo[n][j] = fmaf(a, m[0][j], fmaf(b, m[1][j], mo[n][j]));
-#pragma unroll
-                for (int i = 0; i < 4; i++) p[n][i] *= ve;
             }
 #pragma unroll
             for (int j = 0; j < NG; j++) {
@@ -395,16 +406,25 @@ struct Kv4Warp {
             acc[n][j][0] *= f; acc[n][j][1] *= f;
         }
     }
-    // the power of two that brings the warp's largest dm into [32, 64)
-    __device__ __forceinline__ void set_scale(float dm)
+    // `scaled`: the block's steps times ve, this lane's position.  Groups that need it get the power of two that brings the largest
+    // into [1/4, 1/2) of AK_STEP_TOP; the scaled steps once more, to dst.  (ve lives in shared memory: in registers 64 / 8 heads at
+    // 131072 positions take 97 us, not 95.)
+    __device__ __forceinline__ void set_scale(const float (&scaled)[NG], const float (&ve)[NG], float *dst, float *ve_dst)
     {
 #pragma unroll
-        for (int x = 1; x < 32; x <<= 1) dm = fmaxf(dm, __shfl_xor_sync(0xFFFFFFFFu, dm, x));
-        const float to = __uint_as_float((uint32_t)(127 + 5 + 127 - (int)(__float_as_uint(dm) >> 23)) << 23);
-        const float f = to / ve;
-        ve = to;
+        for (int j = 0; j < NG; j++) {
+            const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(scaled[j]));   // (steps are not negative)
+            const float f = __uint_as_float(top) > AK_STEP_TOP ? __uint_as_float((127 + 11 + 127 - (top >> 23)) << 23) : 1.f;
+            ve_dst[j] = ve[j] * f;   // (all lanes the same)
+            dst[j] = scaled[j] * f;
 #pragma unroll
-        for (int n = 0; n < NT; n++) scale_outputs(n, f);
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int k = 2 * j; k < 2 * j + 2; k++) {
+                    o[n][k][0] *= f; o[n][k][1] *= f; o[n][k][2] *= f; o[n][k][3] *= f;
+                    acc[n][k][0] *= f; acc[n][k][1] *= f;
+                }
+        }
     }
 
     // after the last flush: the sum of weights of head t, and outputs (times it) of dims 32 j + 4 gr .. + 3 of head t
@@ -415,13 +435,13 @@ struct Kv4Warp {
         for (int k = 4; k < 32; k <<= 1) x += __shfl_xor_sync(0xFFFFFFFFu, x, k);
         return x;
     }
-    __device__ __forceinline__ float4 out(int n, int j, int lane) const
+    __device__ __forceinline__ float4 out(int n, int j, int lane, const float *scratch) const
     {
         float m = mo[n][j];
 #pragma unroll
         for (int k = 1; k < 8; k <<= 1) m += __shfl_xor_sync(0xFFFFFFFFu, m, k);
         m = __shfl_sync(0xFFFFFFFFu, m, 8 * (lane & 3));
-        const float e = 1.f / ve;
+        const float e = __uint_as_float((254u << 23) - __float_as_uint(scratch[VE + j]));   // 1 / ve (a division a group costs 0.3 us)
         return make_float4(fmaf(acc[n][2 * j][0], e, m), fmaf(acc[n][2 * j][1], e, m), fmaf(acc[n][2 * j + 1][0], e, m),
                            fmaf(acc[n][2 * j + 1][1], e, m));
     }
@@ -436,8 +456,8 @@ __host__ __device__ constexpr AttnKv4Smem attn_kv4_smem(int NG, int NT, int GV, 
     const int HD = 32 * NG;
     s.ring = 0;                                               // [warps][stages] blocks; a warp's results replace its own
     int at = AK_WARPS * attn_kv4_stages(NG) * 40 * HD;
-    s.params = at;                                            // [warps][4][32][NG] floats
-    at += AK_WARPS * 4 * 32 * NG * 4;
+    s.params = at;                                            // [warps]{[4][32][NG], 4} floats
+    at += AK_WARPS * (4 * 32 * NG + 4) * 4;
     s.qf = at;                                                // [8 NT columns][HD] halves
     at += 8 * NT * HD * 2;
     s.qs = at;                                                // [4 NT heads][NG + 1] floats
@@ -584,7 +604,8 @@ __global__ void __launch_bounds__(AK_THREADS, NT == 1 ? 2 : 1) attn_step_kv4_ker
     }
     __syncthreads();
     Kv4Warp<NG, NT> w;
-    w.clear();
+    float *scratch = (float *)(smem + at.params) + warp * w.SCRATCH;
+    w.clear(scratch, lane);
 #pragma unroll
     for (int n = 0; n < NT; n++) {
         const float *head_qs = qs + (4 * n + (lane & 3)) * (NG + 1);
@@ -636,7 +657,7 @@ __global__ void __launch_bounds__(AK_THREADS, NT == 1 ? 2 : 1) attn_step_kv4_ker
             }
             __syncwarp();
         }
-        w.block(blk, (float *)(smem + at.params) + warp * w.SCRATCH, lo, hi, lane);
+        w.block(blk, scratch, lo, hi, lane);
         if ((i & 3) == 3) w.flush();
         __syncwarp();   // every lane is done with the stage
         if (lane == 0 && i + STAGES < n_mine) {
@@ -656,7 +677,7 @@ __global__ void __launch_bounds__(AK_THREADS, NT == 1 ? 2 : 1) attn_step_kv4_ker
         float *dst = part + warp * WS + h * RS;
 #pragma unroll
         for (int j = 0; j < NG; j++) {
-            const float4 v = w.out(n, j, lane);
+            const float4 v = w.out(n, j, lane, scratch);
             if (h < n_h) {
                 *(float2 *)(dst + 2 + 32 * j + 4 * (lane >> 2)) = make_float2(v.x, v.y);
                 *(float2 *)(dst + 4 + 32 * j + 4 * (lane >> 2)) = make_float2(v.z, v.w);

@@ -666,3 +666,59 @@ def test_workspaces_of_graphs_that_are_gone_are_used_again(gpu):
     # of some MiB at times (8 were seen)
     assert free[4] - free[-1] <= 32 << 20
     gpu.check_error()
+
+
+# ---- groups and positions of very different sizes ----------------------------------------------------------------
+def test_step_groups_far_apart_are_each_as_accurate(gpu):
+    """Groups whose values lie up to 2^20 below another's: each is held to its own size."""
+    L = gpu.lib()
+    for nh, n_kv, exps in ((4, 1, (0, -9, -16, -20)), (8, 1, (-20, 0, -12, 3)), (6, 3, (-18, 0)), (16, 2, (0, -15, -20))):
+        r, hd, ctx = rng(40, nh), 32 * len(exps), 200
+        k, v = rows(r, ctx, n_kv, hd, False), rows(r, ctx, n_kv, hd, False)
+        v *= np.exp2(np.array(exps, np.float32)).repeat(32)
+        cache = upload(gpu, kv4.store(np.zeros(kv4.nbytes(ctx, n_kv, hd), np.uint8), k, v, 0, ctx))
+        out, scale = gpu.GpuBuf.alloc_f32(nh * hd), float(np.float32(hd ** -0.5))
+        for sharp in (1e-20, 1.0, 8.0):
+            q = r.standard_normal((1, nh, hd), dtype=np.float32) * np.float32(sharp)
+            dq = upload(gpu, q)
+            L.cuda_attn_step_kv4(out.ptr, dq.ptr, None, None, cache.ptr, nh, n_kv, hd, ctx, None, ctx - 1, 0, scale, None, 0.0, 1.0, 0, 0, -1)
+            kk, vv = kv4.values(k), kv4.values(v)
+            want, bound = kv4.attention(q, kk, vv, ctx - 1, 0, scale, None)
+            # A value is p d (code - 8) + p (m + 8 d); with A the larger end of a group's range 15 d <= 2 A, so the two are at most
+            # 16 / 15 A and A.  Each carries 22 bits and one f32 rounding: (31 / 15) 1.25 2^-22 A < 2^-20 A a position, taken with
+            # the weights.  p d itself: |code - 8| 2^-35 of the group's largest step D at most, 2^-32 D a position, the largest weight
+            # of all being 1.
+            A = np.abs(vv.reshape(ctx, n_kv, -1, 32)).max(-1).repeat(32, -1)
+            D = kv4.quantise(v)[2].max(0).repeat(32, -1).repeat(nh // n_kv, 0)
+            own = 2.0 ** -20 * kv4.attention(q, kk, A, ctx - 1, 0, scale, None)[0] + ctx * 2.0 ** -32 * D
+            err = np.abs(out.download().reshape(1, nh, hd) - want)
+            assert (err <= bound + own).all(), (nh, sharp, (err / (bound + own)).max())
+            # and in the norm, group by group, as the other tests hold all of them together
+            by = lambda x: np.linalg.norm(x.reshape(nh, -1, 32), axis=(0, 2))
+            assert (by(err) <= 2.0 ** -19 * by(want)).all(), (nh, sharp, by(err) / by(want))
+    gpu.check_error()
+
+
+def test_step_position_far_above_the_others(gpu):
+    """One position's values are 2^16 times the others' and its weight is next to nothing: the others keep their bits.  A position's error
+    in p d is two roundings to 2^-24 of a scale on which the largest step D is at least 2^11, uniform: 2^-24 0.41 / 2^11 D with codes of 4.6 on
+    average, 2^-34 D; that of n positions over the sum l of their weights sqrt(n) 2^-34 D / l.  Twice that, beside 2^-20 of the output."""
+    L, r = gpu.lib(), rng(41)
+    nh, n_kv, hd, ctx, scale = 4, 1, 128, 200, float(np.float32(0.0883))
+    for at in (0, 17, 199):
+        k, v = np.abs(rows(r, ctx, n_kv, hd, False)), rows(r, ctx, n_kv, hd, False)
+        k[at] = -3
+        v[at] *= 2.0 ** 16
+        q = np.full((1, nh, hd), 0.5, np.float32)
+        cache = upload(gpu, kv4.store(np.zeros(kv4.nbytes(ctx, n_kv, hd), np.uint8), k, v, 0, ctx))
+        dq, out = upload(gpu, q), gpu.GpuBuf.alloc_f32(nh * hd)
+        L.cuda_attn_step_kv4(out.ptr, dq.ptr, None, None, cache.ptr, nh, n_kv, hd, ctx, None, ctx - 1, 0, scale, None, 0.0, 1.0, 0, 0, -1)
+        kk, vv = kv4.values(k), kv4.values(v)
+        want, _ = kv4.attention(q, kk, vv, ctx - 1, 0, scale, None)
+        s = kk[:, 0].astype(np.float64) @ q[0, 0] * scale
+        l = np.exp(s - s.max()).sum()
+        D = kv4.quantise(v)[2].max(0).repeat(32, -1).repeat(nh, 0)
+        err = out.download().reshape(1, nh, hd) - want
+        allowed = 2 * np.linalg.norm(np.sqrt(ctx) * 2.0 ** -34 * D / l) + 2.0 ** -20 * np.linalg.norm(want)
+        assert np.linalg.norm(err) <= allowed, (at, np.linalg.norm(err) / allowed, np.linalg.norm(err) / np.linalg.norm(want))
+    gpu.check_error()
