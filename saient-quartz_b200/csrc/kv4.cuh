@@ -45,12 +45,13 @@ __device__ __forceinline__ bool kv4_reaches(float m, __half d, float hi)
     const float t = 15.f * __half2float(d), s = __fadd_rn(t, m), b = __fadd_rn(s, -t), err = __fadd_rn(__fadd_rn(t, -__fadd_rn(s, -b)), __fadd_rn(m, -b));
     return __fadd_rn(__fadd_rn(s, -hi), err) >= 0.f;   // (where s and hi differ by more than err, their difference has its sign)
 }
-// Parameters of a group from its extremes.  The f32 quotient is right to 2^-22 of itself: only if it lies that close to an
-// f16 number can that number, or the one above it, be the answer instead, and is asked exactly.
+// Parameters of a group from its extremes.  The f32 quotient (rounded up: a range of a few subnormals is not none) is right to
+// 2^-22 of itself: only if it lies that close to an f16 number can that number, or the one above it, be the answer instead, and is
+// asked exactly.
 __device__ __forceinline__ void kv4_params(float lo, float hi, __half &m, __half &d)
 {
     m = __float2half_rd(fmaxf(lo, -65504.f) + 0.f);   // (+ 0: a minimum of -0 is stored as 0)
-    const float mf = __half2float(m), q = fmaxf(hi - mf, 0.f) * (1.f / 15.f), near = q * (1.f / (1 << 20));
+    const float mf = __half2float(m), q = __fmul_ru(fmaxf(hi - mf, 0.f), 1.f / 15.f), near = q * (1.f / (1 << 20));
     d = __float2half_ru(fminf(q, 65504.f));
     const unsigned short bits = __half_as_ushort(d);
     const __half less = __ushort_as_half((unsigned short)(bits - 1));   // (of 0: NaN, which nothing is near to)

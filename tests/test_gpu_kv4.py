@@ -722,3 +722,29 @@ def test_step_position_far_above_the_others(gpu):
         allowed = 2 * np.linalg.norm(np.sqrt(ctx) * 2.0 ** -34 * D / l) + 2.0 ** -20 * np.linalg.norm(want)
         assert np.linalg.norm(err) <= allowed, (at, np.linalg.norm(err) / allowed, np.linalg.norm(err) / np.linalg.norm(want))
     gpu.check_error()
+
+
+def test_rows_of_subnormal_numbers(gpu):
+    """Ranges of a few f32 subnormals: the step is the smallest one, not none."""
+    L, r = gpu.lib(), rng(42)
+    tiny = np.float32(2.0 ** -149)
+    x = np.zeros((70, 1, 32), np.float32)
+    for i in range(10):
+        x[i, 0, 3 * i] = (i + 1) * tiny
+        x[10 + i, 0, i] = -(i + 1) * tiny
+        x[20 + i, 0] = r.integers(0, 2 ** i + 1, 32).astype(np.float32) * tiny
+    x[30] = np.float32(2.0 ** -24)
+    x[30, 0, 5] = np.nextafter(np.float32(2.0 ** -24), np.float32(1))
+    for i in range(31, 70):
+        x[i, 0] = (r.standard_normal(32) * 2.0 ** -r.integers(100, 149)).astype(np.float32)
+    raw = np.full(kv4.nbytes(70, 1, 32), 7, np.uint8)
+    cache, dk, dv = upload(gpu, raw), upload(gpu, x), upload(gpu, x[::-1])
+    L.cuda_kv4_append_rows(cache.ptr, dk.ptr, dv.ptr, 70, 1, 32, 70, 0)
+    gpu.check_error()
+    assert np.array_equal(cache.download(np.uint8), kv4.store(raw, x, x[::-1], 0, 70))
+    ok, ov = gpu.GpuBuf.alloc_f32(x.size), gpu.GpuBuf.alloc_f32(x.size)
+    L.cuda_kv4_read_rows(ok.ptr, ov.ptr, cache.ptr, 70, 1, 32, 70, 0)
+    for got, want in ((ok, x), (ov, x[::-1])):
+        assert np.array_equal(got.download(), kv4.values(want).reshape(-1))
+        step = kv4.quantise(want)[2].repeat(32, -1).reshape(-1)
+        assert (np.abs(got.download().astype(np.float64) - want.reshape(-1)) <= step / 2).all()
