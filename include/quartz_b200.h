@@ -259,8 +259,9 @@ void cuda_attn_prompt(float *out, const float *q, const float *k_cache, const fl
  *                           with the values that it has in the cache.  theta <= 0: q and k_new are taken as they are
  *                           (already rotated, or a layer without rotation); k_new and v_new NULL: nothing is
  *                           appended, the cache holds the position already.  Long contexts are merged in a workspace
- *                           of the library, one for every stream and for every graph that is being captured: graphs
- *                           may replay side by side, two executables of one captured graph may not.
+ *                           of the library, one for every graph that is being captured (graphs may replay side by side,
+ *                           two executables of one captured graph may not), one for each of the first 16 streams of a
+ *                           device that ask for it, one for all later ones, whose calls then follow one another.
  *                           Products carry 22 bits and sums are f32.  Of a position's weight times its step in a
  *                           group, these are 22 bits down to 2^-14 of the largest step that the group has in the
  *                           context, and an error of 2^-35 of that step below.

@@ -86,31 +86,57 @@ StepShape step_shape(int units, int n_blocks, int GV)
 
 // The workspace in which the clusters of a unit meet.  Calls on one stream follow one another and share one; every graph
 // that is being captured gets one of its own (graphs may be replayed side by side), which returns to the pool when the
-// last executable form of the graph is gone.  NULL if it cannot be had (then one cluster per unit works).
+// last executable form of the graph is gone.  Streams are told apart by their ids: a handle may come back for a new stream while
+// work of the old one is still running.  Nothing tells when a stream is gone, so only the first AK_OWN_STREAMS of a device have
+// their own; all later ones share one more, which an event passes from call to call.
+// ptr NULL: it cannot be had (then one cluster per unit works).
+constexpr int AK_OWN_STREAMS = 16;   // (0.57 MB each; the event costs a call a microsecond or two on the host)
 struct Workspace {
     int device;
-    cudaStream_t stream;
+    unsigned long long stream;    // its id (its handle in a capture); 0: shared
     unsigned long long capture;   // 0: calls that run at once
     float *ptr;
+    cudaEvent_t passed;           // shared: recorded behind the last call
     std::atomic<bool> in_use;
 };
-float *merge_workspace()
+struct MergeWorkspace {
+    float *ptr;
+    cudaEvent_t record;           // to be recorded behind the launch, or NULL
+};
+MergeWorkspace merge_workspace()
 {
     static std::vector<std::unique_ptr<Workspace>> all;
     cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
-    unsigned long long id = 0;
+    unsigned long long capture = 0, id = 0;
     cudaGraph_t graph = nullptr;
-    if (cudaStreamGetCaptureInfo_v2(stream(), &status, &id, &graph, nullptr, nullptr) != cudaSuccess) cudaGetLastError();
-    if (status == cudaStreamCaptureStatusInvalidated) return nullptr;
+    if (cudaStreamGetCaptureInfo_v2(stream(), &status, &capture, &graph, nullptr, nullptr) != cudaSuccess) cudaGetLastError();
+    if (status == cudaStreamCaptureStatusInvalidated) return {};
     const bool capturing = status == cudaStreamCaptureStatusActive;
-    if (!capturing) id = 0;
+    if (!capturing) capture = 0;
     int device = 0;
-    cudaGetDevice(&device);
-    Workspace *w = nullptr;
-    for (auto &e : all)
-        if (e->device == device && e->in_use && e->stream == stream() && e->capture == id) return e->ptr;
-    for (auto &e : all)
-        if (e->device == device && !e->in_use) w = e.get();
+    // (asked for its id, a stream loses its capture; while that lasts the handle will do)
+    if (capturing) id = (uintptr_t)stream();
+    if (cudaGetDevice(&device) != cudaSuccess || (!capturing && cudaStreamGetId(stream(), &id) != cudaSuccess)) {
+        cudaGetLastError();
+        return {};
+    }
+    Workspace *w = nullptr, *shared = nullptr;
+    int owners = 0;
+    for (auto &e : all) {
+        if (e->device != device) continue;
+        if (!e->in_use) w = e.get();
+        else if (e->passed) shared = e.get();
+        else if (e->stream == id && e->capture == capture) return {e->ptr, nullptr};
+        else if (!e->capture) owners++;
+    }
+    const bool share = !capturing && owners >= AK_OWN_STREAMS;
+    if (share && shared) {
+        if (cudaStreamWaitEvent(stream(), shared->passed, 0) != cudaSuccess) {
+            cudaGetLastError();
+            return {};
+        }
+        return {shared->ptr, shared->passed};
+    }
     if (!w) {
         cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;   // allocating does not disturb a capture
         cudaThreadExchangeStreamCaptureMode(&mode);
@@ -124,7 +150,7 @@ float *merge_workspace()
             if (p) cudaFree(p);
         }
         cudaThreadExchangeStreamCaptureMode(&mode);
-        if (!ok) return nullptr;
+        if (!ok) return {};
         all.push_back(std::make_unique<Workspace>());
         w = all.back().get();
         w->device = device;
@@ -136,13 +162,18 @@ float *merge_workspace()
         if (cudaUserObjectCreate(&owner, w, release, 1, cudaUserObjectNoDestructorSync) != cudaSuccess ||
             cudaGraphRetainUserObject(graph, owner, 1, cudaGraphUserObjectMove) != cudaSuccess) {
             cudaGetLastError();
-            return nullptr;
+            return {};
         }
     }
-    w->stream = stream();
-    w->capture = id;
+    if (share && cudaEventCreateWithFlags(&w->passed, cudaEventDisableTiming) != cudaSuccess) {
+        cudaGetLastError();
+        w->passed = nullptr;
+        return {};
+    }
+    w->stream = share ? 0 : id;
+    w->capture = capture;
     w->in_use = true;
-    return w->ptr;
+    return {w->ptr, w->passed};
 }
 
 // NG = head_dim / 32 as a template argument
@@ -168,10 +199,13 @@ void launch_step(AttnKv4Args &a, int n_tok, int head_dim)
     by_groups(head_dim, [&](auto ng) {
         auto go = [&](auto nt) {
             StepShape s = step_shape<ng.value, nt.value>(units * n_tok, a.n_blocks, GV);
-            if (s.clusters > 1 && !(a.workspace = merge_workspace())) s.clusters = 1;
+            MergeWorkspace w = {};
+            if (s.clusters > 1 && !(w = merge_workspace()).ptr) s.clusters = 1;
+            a.workspace = w.ptr;
             a.clusters = s.clusters;
             launch_cluster(attn_step_kv4_kernel<ng.value, nt.value>, dim3(units * s.clusters * s.cl, n_tok), dim3(AK_THREADS),
                            (size_t)attn_kv4_smem(ng.value, nt.value, GV, s.cl).total, s.cl, a);
+            if (w.record) QZ_CUDA_CHECK(cudaEventRecord(w.record, stream()));
         };
         if (GV <= 4) go(std::integral_constant<int, 1>());
         else go(std::integral_constant<int, 2>());

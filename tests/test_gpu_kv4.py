@@ -748,3 +748,60 @@ def test_rows_of_subnormal_numbers(gpu):
         assert np.array_equal(got.download(), kv4.values(want).reshape(-1))
         step = kv4.quantise(want)[2].repeat(32, -1).reshape(-1)
         assert (np.abs(got.download().astype(np.float64) - want.reshape(-1)) <= step / 2).all()
+
+
+def test_many_streams_that_come_and_go(gpu):
+    """Forty streams with calls that merge in flight at once, then two hundred that are destroyed with their call still running (their
+    handles come back): every result is right, and what the library keeps does not grow with them."""
+    import torch
+    from cuda.bindings import runtime as rt
+    L, r = gpu.lib(), rng(53)
+    nh, n_kv, hd, max_seq, n = 16, 4, 128, 9000, 40
+
+    def new():
+        err, s = rt.cudaStreamCreateWithFlags(rt.cudaStreamNonBlocking)
+        assert err == rt.cudaError_t.cudaSuccess
+        return int(s)
+    cache, _, k, v, _, _, _ = merge_setup(gpu, r, nh, n_kv, hd, max_seq, max_seq)
+    q = r.standard_normal((n, nh, hd), dtype=np.float32)
+    dq, out, want = [upload(gpu, x) for x in q], [gpu.GpuBuf.alloc_f32(nh * hd) for _ in q], []
+
+    def call(i):
+        L.cuda_attn_step_kv4(out[i].ptr, dq[i].ptr, None, None, cache.ptr, nh, n_kv, hd, max_seq, None, max_seq - 1, 0, 0.09, None, 0.0, 1.0, 0, 0, -1)
+
+    def check():
+        torch.cuda.synchronize()
+        for i in range(n):
+            assert np.array_equal(out[i].download(), want[i]), i
+            put(gpu, out[i], np.zeros(nh * hd, np.float32))
+    for i in range(n):
+        call(i)
+        want.append(out[i].download())
+    held(want[3].reshape(1, nh, hd), *kv4.attention(q[3:4], k, v, max_seq - 1, 0, float(np.float32(0.09)), None))
+    streams = [new() for _ in range(n)]
+    try:
+        for _ in range(5):
+            for _ in range(10):
+                for i, s in enumerate(streams):
+                    L.quartz_set_stream(s)
+                    call(i)
+            L.quartz_set_stream(None)
+            check()
+        free = torch.cuda.mem_get_info()[0]
+        for turn in range(5):
+            for i in range(n):
+                s = new()
+                L.quartz_set_stream(s)
+                for _ in range(3):
+                    call(i)
+                rt.cudaStreamDestroy(s)
+            L.quartz_set_stream(None)
+            check()
+        # 200 workspaces would be 109 MiB
+        assert free - torch.cuda.mem_get_info()[0] <= 32 << 20
+    finally:
+        torch.cuda.synchronize()
+        L.quartz_set_stream(None)
+        for s in streams:
+            rt.cudaStreamDestroy(s)
+    gpu.check_error()
