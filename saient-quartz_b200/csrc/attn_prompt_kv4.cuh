@@ -504,7 +504,7 @@ __global__ void __launch_bounds__(APK_THREADS, 1) attn_prompt_kv4_kernel(const A
         const bool leader = elect_one();
         constexpr uint32_t i_s = umma_idesc_f16(APK_BN, false), i_o = umma_idesc_f16(64 * NH + 16, true), i_lo = umma_idesc_f16(64 * NH, true);
         const uint32_t ring_addr = smem_u32(ring), t_base = __shfl_sync(0xFFFFFFFFu, tmem, 0);
-        int done = -1;   // last tile whose P V was issued
+        int scored = -1, done = -1;   // last tiles whose S and whose P V were issued
         for (int j = 0; j <= n_tiles; j++) {
             if (j < n_tiles) {
                 // S(j) may overwrite P(j - 2): the MMAs that read it were issued before and execute in order
@@ -522,6 +522,7 @@ __global__ void __launch_bounds__(APK_THREADS, 1) attn_prompt_kv4_kernel(const A
                     if (m != 1) tc_mma_f16_ta(leader, d, t_base + T_Q + (m == 0 ? 136 : 128), stage + ((AT_X + 64) >> 4), i_s, 1u);
                 }
                 if (leader) tc_commit(&s.s_full[j & 1]);
+                scored = j;
             }
             if (j > 0) {
                 const int i = j - 1;
@@ -540,7 +541,9 @@ __global__ void __launch_bounds__(APK_THREADS, 1) attn_prompt_kv4_kernel(const A
                 done = i;
             }
         }
-        if (done >= 0) mbar_wait(&s.free_[done % APK_STAGES], (done / APK_STAGES) & 1);   // nothing in flight at the exit
+        // nothing in flight at the exit, also where a wait gave up between the two
+        if (scored >= 0) mbar_wait(&s.s_full[scored & 1], (scored >> 1) & 1);
+        if (done >= 0) mbar_wait(&s.free_[done % APK_STAGES], (done / APK_STAGES) & 1);
         __syncwarp();
     }
     if (!ok && a.status) *a.status = QZ_ERR_TIMEOUT;
