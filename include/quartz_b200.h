@@ -265,7 +265,9 @@ void cuda_attn_prompt(float *out, const float *q, const float *k_cache, const fl
  *                           Products carry 22 bits and sums are f32.  Of a position's weight times its step in a
  *                           group, these are 22 bits down to 2^-14 of the largest step that the group has in the
  *                           context, and an error of 2^-35 of that step below.
- *   cuda_attn_prompt_kv4    cuda_attn_prompt over such a cache (rows appended before, e.g. by cuda_rope_kv4_rows) */
+ *   cuda_attn_prompt_kv4    cuda_attn_prompt over such a cache (rows appended before, e.g. by cuda_rope_kv4_rows).  Products
+ *                           carry 22 bits, sums are f32; where 64 neighbouring positions hold a step above 8188 (values
+ *                           that span 122820), their steps and minima below 2^-11 are taken to 2^-22 */
 size_t cuda_kv4_bytes(int max_seq, int n_kv_heads, int head_dim);
 void cuda_kv4_append_rows(void *d_cache, const float *k, const float *v, int n_tok, int n_kv_heads, int head_dim, int max_seq, int pos0);
 void cuda_rope_kv4_rows(float *q, float *k, const float *v, void *d_cache, int n_tok, int n_heads, int n_kv_heads, int head_dim,

@@ -16,9 +16,10 @@
 //
 //   warps 0-3   one row per thread: S from tensor memory, mask, weights 64 exp2(s - ref), their sum, P back.  The
 //               reference is raised only when a score exceeds it by 2^8.
-//   warps 4-11  fill a ring of three (K, V) stages from the cache, 8 dims of a position at a time.  A tile with a step
-//               above 8188 (8 d would overflow) is scaled by a power of two.  Between two stages
-//               they add a finished O tile to their half of a row.
+//   warps 4-11  fill a ring of three (K, V) stages from the cache, 8 dims of a position at a time.  The keys, or the values, of
+//               a tile with a step above 8188 (8 d would overflow) are taken by an eighth: exact but for steps and minima
+//               below 2^-11, which are then off by 2^-22 at most.  Between two stages they add a finished O tile to their
+//               half of a row.
 //   warp 12     issues S(j), then P V of tile j - 1: the tensor core works while the weights are computed.
 // Columns of tensor memory: Q 144 (hi, lo, sums over groups), S / P 2 x 64, O 144 (two halves of 64 dims, 16 for m and 8 d).
 // Within every 8 dims the tiles' order is (0,4,1,5,2,6,3,7), which unpacking produces for free; Q is put in that order,
@@ -55,7 +56,6 @@ struct AttnPromptKv4Shared {
     float corr[4][UMMA_M];           // factor of a row's earlier outputs at tile j (slot j % 4)
     float scale_k[4], scale_v[4];    // 1 / what the tile's K and V were multiplied with
     uint32_t nan_v[4][4][2];         // positions of the tile whose V group is NaN, by group
-    uint32_t top[2][2][8];           // largest magnitude per warp, as bits
     float inv[UMMA_M];               // 1 / sum of weights
     uint32_t nan_row[UMMA_M];        // groups of the row's output that are NaN
     uint32_t tmem;
@@ -360,35 +360,27 @@ __global__ void __launch_bounds__(APK_THREADS, 1) attn_prompt_kv4_kernel(const A
                 for (int i = 0; i < NG; i++) kp1[i] = vp1[i] = kw1[i] = vw1[i] = 0;   // m = d = 0
             }
         };
-        // (rare) note V groups that are NaN and take them as zero; bring the tile's parameters into range: times the power of
-        // two that takes its largest magnitude to [2^12, 2^13)
+        // is it so for any of these warps' threads?
+        auto any_thread = [](bool x) {
+            uint32_t any;
+            asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 3, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}\n"
+                         : "=r"(any) : "r"((uint32_t)x) : "memory");
+            return any != 0;
+        };
+        // (rare) note V groups that are NaN and take them as zero; bring steps whose eightfold overflows into range
         auto mend = [&](int j, float &uk, float &uv) {
-            float top_k = 0.f, top_v = 0.f;
+            bool big_k = false, big_v = false;
 #pragma unroll
-            for (int g = 0; g < NG; g++)
+            for (int g = 0; g < NG; g++) {
                 if ((bits_of(vp, g) & 0x7FFFu) > 0x7C00u) {
                     if (t == 0) atomicOr(&s.nan_v[j & 3][g][p_tile >> 5], 1u << (p_tile & 31));
                     vp[g >> 1] &= g & 1 ? 0x0000FFFFu : 0xFFFF0000u;
                 }
-#pragma unroll
-            for (int g = 0; g < NG; g++) {
-                top_k = fmaxf(top_k, fabsf(half_of(kp, g)) + 15.f * half_of(kp, NG + g));
-                top_v = fmaxf(top_v, fabsf(half_of(vp, g)) + 15.f * half_of(vp, NG + g));
+                big_k |= bits_of(kp, NG + g) > 0x6FFFu;
+                big_v |= bits_of(vp, NG + g) > 0x6FFFu;
             }
-            const uint32_t wk = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(top_k)), wv = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(top_v));
-            if (lane == 0) {
-                s.top[j & 1][0][w8] = wk;
-                s.top[j & 1][1][w8] = wv;
-            }
-            asm volatile("bar.sync 3, 256;" ::: "memory");
-            uint32_t tk = 0, tv = 0;
-            for (int i = 0; i < 8; i++) {
-                tk = max(tk, s.top[j & 1][0][i]);
-                tv = max(tv, s.top[j & 1][1][i]);
-            }
-            const int ek = tk ? 127 + 12 - (int)(tk >> 23) : 0, ev = tv ? 127 + 12 - (int)(tv >> 23) : 0;
-            uk = __uint_as_float((uint32_t)(127 + ek) << 23);
-            uv = __uint_as_float((uint32_t)(127 + ev) << 23);
+            if (any_thread(big_k)) uk = 0.125f;
+            if (any_thread(big_v)) uv = 0.125f;
             auto times = [](uint32_t w, float u) {
                 const float2 x = __half22float2(*(const __half2 *)&w);
                 return pack_half2(x.x * u, x.y * u);
@@ -430,11 +422,8 @@ __global__ void __launch_bounds__(APK_THREADS, 1) attn_prompt_kv4_kernel(const A
                 for (int g = 0; g < NG; g++)
                     odd |= bits_of(kp, NG + g) > 0x6FFFu || bits_of(vp, NG + g) > 0x6FFFu || (bits_of(vp, g) & 0x7FFFu) > 0x7C00u;
             }
-            uint32_t any;
-            asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 3, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}\n"
-                         : "=r"(any) : "r"((uint32_t)odd) : "memory");
             float uk = 1.f, uv = 1.f;
-            if (any) mend(j, uk, uv);
+            if (any_thread(odd)) mend(j, uk, uv);
             if (tid == 0) {
                 s.scale_k[j & 3] = 1.f / uk;
                 s.scale_v[j & 3] = 1.f / uv;

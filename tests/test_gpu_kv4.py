@@ -805,3 +805,37 @@ def test_many_streams_that_come_and_go(gpu):
         for s in streams:
             rt.cudaStreamDestroy(s)
     gpu.check_error()
+
+
+def test_prompt_groups_far_apart_are_each_as_accurate(gpu):
+    """Tiles with steps above 8188 in one group, of the values or of the keys: the small groups beside it are held to their own size."""
+    L = gpu.lib()
+    for nh, n_kv, hd, n in ((16, 8, 128, 515), (12, 6, 96, 515), (8, 4, 64, 700)):
+        r, g, scale = rng(43, hd), hd // 32, float(np.float32(hd ** -0.5))
+        k, v = rows(r, n, n_kv, hd, False), rows(r, n, n_kv, hd, False)
+        v[..., 32:] *= np.float32(2.0 ** -8)
+        v[100:400:37, :, :32] = np.linspace(-65504, 65504, 32)     # a step of 8734
+        k[90:420:55, :, :32] = np.linspace(65504, -65504, 32)
+        k[..., 32:] *= np.float32(2.0 ** -2)
+        q = r.standard_normal((n, nh, hd), dtype=np.float32) * 4
+        q[..., :32] = 0                          # (the towering keys weigh nothing: the others decide)
+        cache = upload(gpu, kv4.store(np.full(kv4.nbytes(n, n_kv, hd), 0xFF, np.uint8), k, v, 0, n))
+        dq, out = upload(gpu, q), gpu.GpuBuf.alloc_f32(q.size)
+        L.cuda_attn_prompt_kv4(out.ptr, dq.ptr, cache.ptr, n, nh, n_kv, hd, n, 0, 0, scale, None)
+        got = out.download().reshape(q.shape)
+        gpu.check_error()
+        kk, vv = kv4.values(k), kv4.values(v)
+        want, bound = kv4.attention(q, kk, vv, 0, 0, scale, None)
+        # bound: its score error is that of the largest key, here one that q does not touch; so that of the dims q has
+        e_s = (np.abs(q[..., 32:]).sum(-1) * np.abs(kk[..., 32:]).max() * scale * (hd + 16) * 2.0 ** -23)[..., None]
+        # A: the larger end of a group's range, weighed: 2^-20 of it for the two terms of a value, which may cancel; the weights' errors
+        # 4 e_s and n 2^-22 of |value| <= A.  (An eighth of a step or minimum is exact down to 2^-11: the small groups' are above that.)
+        A = np.abs(vv.reshape(n, n_kv, g, 32)).max(-1).repeat(32, -1)
+        own = kv4.attention(q, kk, A, 0, 0, scale, None)[0]
+        allowed = own * (2.0 ** -20 + 4 * e_s + (np.arange(n)[:, None, None] + 33) * 2.0 ** -22)
+        err = np.abs(got - want)[..., 32:]
+        assert (err <= allowed[..., 32:]).all(), (hd, (err / allowed[..., 32:]).max())
+        # and in the norm, as the other tests hold all groups together
+        assert np.linalg.norm(err) <= 2.0 ** -19 * np.linalg.norm(want[..., 32:]), np.linalg.norm(err) / np.linalg.norm(want[..., 32:])
+        assert (np.abs(got - want) <= bound + 2.0 ** -20 * np.maximum.accumulate(np.abs(vv).max(-1), 0).repeat(nh // n_kv, 1)[..., None]).all()
+    gpu.check_error()
