@@ -20,12 +20,39 @@ def sources():
     return sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cu", ".cuh")))
 
 
-def up_to_date():
-    if not os.path.exists(LIB) or not os.path.exists(ARCHIVE):
+def compiler():
+    return os.path.join(os.environ.get("CUDA_HOME", "/usr/local/cuda"), "bin", "nvcc")
+
+
+def compile_command():
+    arch = os.environ.get("QUARTZ_CUDA_ARCH", "sm_100a")   # same variable as the reference's build.rs:33
+    cc = arch.replace("sm_", "compute_")
+    cmd = [compiler(), "-O3", "-std=c++17", "-gencode", f"arch={cc},code={arch}", "-lineinfo", "-Xcompiler", "-fPIC", "-c"]
+    return cmd + os.environ.get("QUARTZ_NVCC_FLAGS", "").split()   # extra compiler flags (e.g. -DNAME=value)
+
+
+def made_by(path, cmd):
+    """Was `path` made by this command?  (Recorded beside it once it was finished.)"""
+    return os.path.exists(path) and os.path.exists(path + ".cmd") and open(path + ".cmd").read() == " ".join(cmd)
+
+
+def forget(path):
+    if os.path.exists(path + ".cmd"):
+        os.remove(path + ".cmd")
+
+
+def record(path, cmd):
+    with open(path + ".cmd", "w") as f:
+        f.write(" ".join(cmd))
+
+
+def up_to_date(cmd):
+    """The library and the archive are newer than all they are made from, this file too, and come from the same command."""
+    if not made_by(LIB, cmd) or not os.path.exists(ARCHIVE):
         return False
     t = os.path.getmtime(LIB)
     hdr = os.path.join(HERE, "..", "include", "quartz_b200.h")
-    return all(os.path.getmtime(s) <= t for s in sources() + [hdr])
+    return all(os.path.getmtime(s) <= t for s in sources() + [hdr, os.path.abspath(__file__)])
 
 
 def included(src, seen=None):
@@ -44,7 +71,7 @@ def object_current(src, obj, cmd):
     """The object is newer than its source, all that it includes and this file, and was made by the same command."""
     if not os.path.exists(obj) or any(os.path.getmtime(f) > os.path.getmtime(obj) for f in included(src) | {os.path.abspath(__file__)}):
         return False
-    return os.path.exists(obj + ".cmd") and open(obj + ".cmd").read() == " ".join(cmd)
+    return made_by(obj, cmd)
 
 
 def build_host(force=False):
@@ -63,14 +90,11 @@ def build_host(force=False):
 
 
 def build(force=False, verbose=False):
-    if not force and up_to_date():
+    cmd = compile_command()
+    if not force and up_to_date(cmd):
         build_host()
         return LIB
-    nvcc = os.path.join(os.environ.get("CUDA_HOME", "/usr/local/cuda"), "bin", "nvcc")
-    arch = os.environ.get("QUARTZ_CUDA_ARCH", "sm_100a")   # same variable as the reference's build.rs:33
-    cc = arch.replace("sm_", "compute_")
-    cmd = [nvcc, "-O3", "-std=c++17", "-gencode", f"arch={cc},code={arch}", "-lineinfo", "-Xcompiler", "-fPIC", "-c"]
-    cmd += os.environ.get("QUARTZ_NVCC_FLAGS", "").split()   # extra compiler flags (e.g. -DNAME=value)
+    forget(LIB)
     show = ["-Xptxas", "-v"] if verbose else []
     objs, running = [], []
     for src in (s for s in sources() if s.endswith(".cu")):
@@ -78,24 +102,25 @@ def build(force=False, verbose=False):
         objs.append(obj)
         if not force and object_current(src, obj, cmd):
             continue
+        forget(obj)
         running.append((src, obj, subprocess.Popen(cmd + show + ["-o", obj, src])))
     failed = []
     for src, obj, p in running:
         if p.wait() != 0:
             failed.append(src)
         else:
-            with open(obj + ".cmd", "w") as f:
-                f.write(" ".join(cmd))
+            record(obj, cmd)
     if failed:
         raise RuntimeError("nvcc failed on " + ", ".join(failed))
     tmp = LIB + ".tmp"
-    subprocess.check_call([nvcc, "-gencode", f"arch={cc},code={arch}", "-shared", "-o", tmp] + objs)
+    subprocess.check_call(cmd[:1] + cmd[3:5] + ["-shared", "-o", tmp] + objs)
     os.replace(tmp, LIB)   # a reader never sees a half-written library
     tmp = ARCHIVE + ".tmp"
     if os.path.exists(tmp):
         os.remove(tmp)
     subprocess.check_call(["ar", "rcs", tmp] + objs)
     os.replace(tmp, ARCHIVE)
+    record(LIB, cmd)
     build_host(force=True)
     return LIB
 

@@ -30,3 +30,77 @@ def test_objects_are_used_again_only_as_they_are(build, tmp_path):
     assert not build.object_current(src, obj, cmd + ["-DX"])
     os.utime(str(tmp_path / "b.cuh"), (now + 1, now + 1))     # a header of a header
     assert not build.object_current(src, obj, cmd)
+
+
+class Compiler:
+    """Stands in for the compiler and the linker: writes what it was asked for, `made` names the objects compiled."""
+    def __init__(self, fail=()):
+        self.made, self.fail = [], fail
+
+    def Popen(self, cmd):
+        src, obj = cmd[-1], cmd[-2]
+        assert not os.path.exists(obj + ".cmd")       # nothing claims to know how an object was made while it is made
+        self.made.append(os.path.basename(obj))
+        with open(obj, "w") as f:
+            f.write("object")
+        bad = os.path.basename(src) in self.fail
+
+        class Done:
+            def wait(self):
+                return 1 if bad else 0
+        return Done()
+
+    def check_call(self, cmd):
+        out = cmd[cmd.index("-o") + 1] if "-o" in cmd else cmd[2]
+        with open(out, "w") as f:
+            f.write("library")
+
+
+@pytest.fixture()
+def tree(build, tmp_path, monkeypatch):
+    (tmp_path / "pkg" / "csrc").mkdir(parents=True)
+    (tmp_path / "include").mkdir()
+    (tmp_path / "include" / "quartz_b200.h").write_text("")
+    for n in ("a.cu", "b.cu"):
+        (tmp_path / "pkg" / "csrc" / n).write_text("int x;\n")
+    pkg = tmp_path / "pkg"
+    for name, path in (("HERE", pkg), ("CSRC", pkg / "csrc"), ("LIB", pkg / "libquartz_b200.so"), ("ARCHIVE", pkg / "libkernels.a")):
+        monkeypatch.setattr(build, name, str(path))
+    monkeypatch.setattr(build, "build_host", lambda force=False: None)
+    for name in ("QUARTZ_NVCC_FLAGS", "QUARTZ_CUDA_ARCH", "CUDA_HOME"):
+        monkeypatch.delenv(name, raising=False)
+
+    def run(fail=(), **kw):
+        c = Compiler(fail)
+        monkeypatch.setattr(build.subprocess, "Popen", c.Popen)
+        monkeypatch.setattr(build.subprocess, "check_call", c.check_call)
+        build.build(**kw)
+        return sorted(c.made)
+    return run
+
+
+def test_another_command_builds_again(build, tree, monkeypatch):
+    assert tree() == ["a.o", "b.o"]
+    assert tree() == []
+    for name, value in (("QUARTZ_NVCC_FLAGS", "-DX=1"), ("QUARTZ_CUDA_ARCH", "sm_103a"), ("CUDA_HOME", "/opt/other")):
+        monkeypatch.setenv(name, value)
+        assert tree() == ["a.o", "b.o"], name
+        assert tree() == []
+    for name in ("QUARTZ_NVCC_FLAGS", "QUARTZ_CUDA_ARCH", "CUDA_HOME"):
+        monkeypatch.delenv(name)
+    assert tree() == ["a.o", "b.o"]                  # and back
+    now = os.path.getmtime(build.LIB) + 100
+    os.utime(os.path.join(build.CSRC, "a.cu"), (now, now))
+    made = tree()
+    assert "a.o" in made
+    assert tree(force=True) == ["a.o", "b.o"]
+
+
+def test_a_build_that_failed_is_not_taken_for_one_that_did_not(build, tree, monkeypatch):
+    assert tree() == ["a.o", "b.o"]
+    monkeypatch.setenv("QUARTZ_NVCC_FLAGS", "-DX=1")
+    with pytest.raises(RuntimeError):
+        tree(fail=("b.cu",))
+    monkeypatch.delenv("QUARTZ_NVCC_FLAGS")          # b.o is the other command's, whatever was recorded before
+    assert tree() == ["a.o", "b.o"]
+    assert tree() == []
