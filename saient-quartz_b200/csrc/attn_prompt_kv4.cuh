@@ -14,8 +14,9 @@
 // The tensor core rounds its sums towards zero, so O is never carried across tiles there: each tile's O starts from zero
 // and is added to f32 registers, where a raised softmax reference is also paid for (one factor per row and tile).
 //
-//   warps 0-3   one row per thread: S from tensor memory, mask, weights 64 exp2(s - ref), their sum, P back.  The
-//               reference is raised only when a score exceeds it by 2^8.
+//   warps 0-3   one row per thread: S from tensor memory, mask, weights 2^11 exp2(s - ref), their sum, P back.  The
+//               reference is raised only when a score exceeds it by 2^4: weights stay below 2^15, and their lo parts keep
+//               clear of f16's subnormals down to weights of 2^-14 (many small ones beside a large one, as a sink has, add up).
 //   warps 4-11  fill a ring of three (K, V) stages from the cache, 8 dims of a position at a time.  The keys, or the values, of
 //               a tile with a step above 8188 (8 d would overflow) are taken by an eighth: exact but for steps and minima
 //               below 2^-11, which are then off by 2^-22 at most.  Between two stages they add a finished O tile to their
@@ -40,6 +41,7 @@
 namespace qz {
 
 constexpr int APK_BN = 64, APK_STAGES = 3, APK_THREADS = 512;
+constexpr float APK_RAISE = 4.f, APK_CARRY = 11.f;   // log2: how far a score may exceed the reference, what weights carry
 
 struct AttnPromptKv4Args {
     float *out;
@@ -244,7 +246,7 @@ __global__ void __launch_bounds__(APK_THREADS, 1) attn_prompt_kv4_kernel(const A
             }
             const float y = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * f;
             float corr = 1.f;
-            if (y > ref + 8.f) {
+            if (y > ref + APK_RAISE) {
                 corr = ex2(ref - y);
                 l *= corr;
                 ref = y;
@@ -259,7 +261,7 @@ __global__ void __launch_bounds__(APK_THREADS, 1) attn_prompt_kv4_kernel(const A
                 }
             }
             float l4[4] = {0.f, 0.f, 0.f, 0.f};
-            const float minus = 6.f - ref;   // weights carry 2^6: their lo parts stay clear of f16's subnormals
+            const float minus = APK_CARRY - ref;
 #pragma unroll
             for (int c = 0; c < 2; c++) {
                 uint32_t v[32], ph[16], pl[16];
@@ -284,7 +286,7 @@ __global__ void __launch_bounds__(APK_THREADS, 1) attn_prompt_kv4_kernel(const A
         }
         if (a.sinks && is_row) {
             const float sink = a.sinks[head] * 1.44269504f, all = fmaxf(ref, sink), down = ex2(ref - all);
-            s.inv[row] = down / fmaf(l, down, ex2(sink - all + 6.f));
+            s.inv[row] = down / fmaf(l, down, ex2(sink - all + APK_CARRY));
         } else {
             s.inv[row] = 1.f / l;
         }

@@ -839,3 +839,41 @@ def test_prompt_groups_far_apart_are_each_as_accurate(gpu):
         assert np.linalg.norm(err) <= 2.0 ** -19 * np.linalg.norm(want[..., 32:]), np.linalg.norm(err) / np.linalg.norm(want[..., 32:])
         assert (np.abs(got - want) <= bound + 2.0 ** -20 * np.maximum.accumulate(np.abs(vv).max(-1), 0).repeat(nh // n_kv, 1)[..., None]).all()
     gpu.check_error()
+
+
+@pytest.mark.parametrize("mass", [0.5, 0.99])
+@pytest.mark.parametrize("nh,n_kv,hd", [(32, 8, 128), (8, 2, 64), (12, 6, 96)])
+def test_many_small_weights_beside_a_large_one(gpu, nh, n_kv, hd, mass):
+    """The first position takes most of the mass and has no values, as in trained models; the outputs are the sum of the others' small
+    weights, 2^-17 of the largest at the end.
+
+    In the norm: 2^-19 of the output for independent errors of some 2^-22 a term, as elsewhere.  The output is a mean of n values of
+    both signs here, 1 / sqrt(n) = 0.03 of the sums of p m and of 8 p d that it is made of (about -2 and 2.1 times the sum s of p): what
+    errs in these with one sign weighs 33 times as much.  The tensor core rounds towards zero, 12 steps of half an ulp on a sum that grows from nothing: 3 2^-23
+    of either, with opposite signs, 3 2^-23 of their difference of 0.1 s together = 3.6e-8 s, 1.2e-6 of the output.  With 2^-19 = 1.9e-6
+    that is 3.1e-6 < 2^-18."""
+    L, r = gpu.lib(), rng(44, nh)
+    n, scale = 1100, float(np.float32(hd ** -0.5))
+    k, v = rows(r, n, n_kv, hd, False), rows(r, n, n_kv, hd, False)
+    k[..., 0] = 0
+    k[0, :, :] = 0
+    k[0, :, 0] = np.log(mass / (1 - mass) * n) / (8 * scale)
+    v[0] = 0
+    q = r.standard_normal((n, nh, hd), dtype=np.float32) * np.float32(0.2)
+    q[..., 0] = 8
+    cache = upload(gpu, kv4.store(np.full(kv4.nbytes(n, n_kv, hd), 0xFF, np.uint8), k, v, 0, n))
+    dq, out = upload(gpu, q), gpu.GpuBuf.alloc_f32(q.size)
+    L.cuda_attn_prompt_kv4(out.ptr, dq.ptr, cache.ptr, n, nh, n_kv, hd, n, 0, 0, scale, None)
+    got = out.download().reshape(q.shape)
+    want, bound = kv4.attention(q, kv4.values(k), kv4.values(v), 0, 0, scale, None)
+
+    def near(a, b, bound):
+        assert (np.abs(a - b) <= bound).all()
+        assert np.linalg.norm(a - b) <= 2.0 ** -18 * np.linalg.norm(b), np.linalg.norm(a - b) / np.linalg.norm(b)
+    near(got, want, bound)
+    for t in (n - 1, n // 2):
+        near(got[t], want[t], bound[t])
+        one = upload(gpu, q[t])
+        L.cuda_attn_step_kv4(out.ptr, one.ptr, None, None, cache.ptr, nh, n_kv, hd, n, None, t, 0, scale, None, 0.0, 1.0, 0, 0, -1)
+        near(out.download(count=nh * hd).reshape(nh, hd), want[t], bound[t])
+    gpu.check_error()
