@@ -14,7 +14,7 @@
 // 2^((f - f_M) / 32): the table carries f_M, four terms of the exponential's series give the rest (|y| < 0.017: 1e-11), and
 // only table times series is taken in 32 bits, so a weight is right to 2^-28.  (CUDA's exp in 64 bits took twice the time
 // of the rest.)  Where z c passes 2^22, at temperatures near 0 or logits of any size, M - z takes the place of z, exact as two
-// f32 numbers.  Why so exact: with thousands of tokens kept, an error of 1e-7 in their sums would move the border of top_p, or
+// f32 numbers, times a power of two that brings c to [1, 2) (c itself leaves f32 at temperatures below 2^-122).  Why so exact: with thousands of tokens kept, an error of 1e-7 in their sums would move the border of top_p, or
 // the token that u falls on, once in some thousand rows.  b = k_M - k is also the bin in which tokens are counted: it follows
 // the order of the logits.
 #pragma once
@@ -135,7 +135,8 @@ struct Sampler {
     const float *z;       // this CTA's part of the row
     int n, base;          // tokens in it, index of the first
     int CL, rank, turn;
-    float M, c_hi, c_lo;  // c = c_hi + c_lo
+    float M, c_hi, c_lo;  // c = up (c_hi + c_lo)
+    float up;             // plain: 1
     bool plain;           // z c stays below 2^22
     float low;            // plain: all logits up to here share the last bin
     int top;              // plain: the bits of 1.5 * 2^23 + k_M
@@ -170,8 +171,16 @@ struct Sampler {
         constexpr double LAST = SMP_BINS - 1;
         const double Mc = (double)M * c;
         c_hi = (float)c;
-        c_lo = isinf(c_hi) ? 0.f : (float)(c - (double)c_hi);
+        c_lo = (float)(c - (double)c_hi);
         plain = fabs(Mc) < 4190000.0 && c_hi < 1e30f && c_hi > 1e-30f;
+        up = 1.f;
+        if (!plain) {
+            const int e = max(-126, min(127, ilogb(c)));
+            const double rest = ldexp(c, -e);
+            up = (float)ldexp(1.0, e);
+            c_hi = (float)rest;
+            c_lo = (float)(rest - (double)c_hi);
+        }
         low = -INFINITY;
         top = __float_as_int(fmaf(M, c_hi, 12582912.f));   // 1.5 * 2^23: the sum's low bits are the nearest integer
         if (plain) {
@@ -189,7 +198,7 @@ struct Sampler {
     __device__ __forceinline__ int bin(float x) const
     {
         if (plain) return top - __float_as_int(fmaf(fmaxf(x, low), c_hi, 12582912.f));   // (NaN goes with the lowest)
-        const float t = x == M ? 0.f : __fmul_rn(M - x, c_hi);   // (M = inf, T = 0's neighbours: t may not be a number)
+        const float t = x == M ? 0.f : __fmul_rn((M - x) * up, c_hi);   // (M = inf: t may not be a number)
         return t < (float)(SMP_BINS - 1) ? __float2int_rn(t) : SMP_BINS - 1;
     }
     // the weight of logit x is size << 17 >> b / 32, b its bin
@@ -202,7 +211,7 @@ struct Sampler {
             b = top - __float_as_int(whole);
             f = fmaf(y, c_lo, fmaf(y, c_hi, 12582912.f - whole));
         } else {
-            const float d = M - x, back = d - M, rest = (M - (d - back)) - (x + back);   // d + rest = M - x exactly
+            const float diff = M - x, back = diff - M, d = diff * up, rest = ((M - (diff - back)) - (x + back)) * up;   // d + rest = up (M - x)
             const float t = __fmul_rn(d, c_hi), t_lo = fmaf(d, c_hi, -t) + fmaf(d, c_lo, rest * c_hi);
             const bool first = x == M;
             far = !first && !(t < (float)(SMP_BINS - 1));
@@ -473,11 +482,11 @@ __global__ void __launch_bounds__(SMP_THREADS) sample_kernel(const SampleArgs a)
     c.keep_z = -INFINITY;
     c.keep_i = -1;
     c.scale(a.c, a.one_over_c);
-    const float inv = (float)a.inv_t;
+    const float inv = (float)(a.inv_t / c.up);
     const double u = (double)fminf(fmaxf(a.u[row], 0.f), 1.f);
     auto heavy = [&](float x) {   // weight >= min_p: decided in 64 bits where 32 could be wrong
         if (a.min_p <= 0.0 || x == c.M) return true;
-        const float y = (x - c.M) * inv;
+        const float y = (x - c.M) * c.up * inv;
         if (y > a.log_min_p + 1e-3f) return true;
         if (y < a.log_min_p - 1e-3f) return false;
         return exp(((double)x - (double)c.M) * a.inv_t) >= a.min_p;

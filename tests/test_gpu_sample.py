@@ -100,6 +100,17 @@ def test_masked_and_odd_logits(gpu):
             check(gpu, z, r.random(12), **kw)
 
 
+@pytest.mark.parametrize("t", [1.4e-45, 1e-44, 1e-40, 1e-38, 1.3e-37, 1e-36, 1e30, 1e37, 3.4e38])
+def test_temperatures_at_the_ends(gpu, t):
+    """Logits of the temperature's own size, near both ends of f32: their quotients are ordinary numbers."""
+    r = rng(11)
+    for vocab in (40, 3000, 30001):
+        z = (r.standard_normal((5, vocab)) * 2.5 * np.float64(np.float32(t))).clip(-1.5e38, 1.5e38).astype(np.float32)
+        z[2] += z[2].max()
+        for kw in (dict(), dict(top_k=7), dict(top_p=0.8), dict(min_p=0.05), dict(top_k=700, top_p=0.9, min_p=0.01)):
+            check(gpu, z, r.random(5), temperature=t, **kw)
+
+
 def test_random_numbers_at_the_ends(gpu):
     r = rng(6)
     z = (r.standard_normal((6, 900)) * 2).astype(np.float32)
