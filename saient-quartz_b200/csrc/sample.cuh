@@ -224,6 +224,8 @@ struct Sampler {
         const uint32_t v = e.x + (__float_as_uint(fmaf(__uint_as_float(e.y), r, 12582912.f)) - 0x4B400000);
         return far ? 0 : v;
     }
+    // a size of bin b without what its weight is rounded down by: the sum over a bin is then the sum of its weights
+    __device__ __forceinline__ static uint32_t whole(uint32_t size, int b) { return size & 0xFFFFFFFFu << max((b >> 5) - 17, 0); }
     __device__ __forceinline__ u64 weight(float x) const
     {
         int b;
@@ -377,7 +379,7 @@ struct Sampler {
                 for (int i = threadIdx.x; i < n; i += SMP_THREADS) {
                     const u64 x = number(i);
                     int same;   // (all lie in bin b)
-                    if (x >= lo && x <= hi) add((int)((hi - x) >> shift), weights, weights ? size(z[i], same) : 0);
+                    if (x >= lo && x <= hi) add((int)((hi - x) >> shift), weights, weights ? whole(size(z[i], same), b) : 0);
                 }
                 collect(weights, b >> 5);
                 const int sub = boundary(above, goal, &above);
@@ -406,12 +408,13 @@ struct Sampler {
         no_list();
         return ~largest();
     }
-    // At most so many tokens make up v, tokens or weights of bin b (a token's weight is 2^(-b / 32) within 1.1 per cent)
+    // At most so many tokens make up v, tokens or weights of bin b (a token's weight is 2^(-b / 32) within 1.7 per cent, rounded down
+    // to a unit; where that can be none, v tells nothing)
     __device__ __forceinline__ u64 held_by(u64 v, bool weights, int b) const
     {
         if (!weights) return v;
-        const float one = __uint_as_float(s.table[b & 31].y) * (float)(1ull << 17) / (float)(1ull << (b >> 5));
-        return (u64)(((float)v + 1.f) / one * 1.02f) + 1;   // (the sum was rounded down to a unit)
+        const float least = floorf(__uint_as_float(s.table[b & 31].y) * (float)(1ull << 17) / (float)(1ull << (b >> 5)) * (1 / 1.02f));
+        return least < 1.f ? SMP_MAX_VOCAB : (u64)((float)v / least * 1.0001f) + 1;
     }
 };
 
@@ -541,7 +544,7 @@ __global__ void __launch_bounds__(SMP_THREADS) sample_kernel(const SampleArgs a)
         c.each([&](float x, int i) {
             int b;
             const uint32_t v = c.size(x, b);
-            if (c.in_set(x, i)) c.add(b, true, v);
+            if (c.in_set(x, i)) c.add(b, true, c.whole(v, b));
         });
         c.collect(true);
         u64 before;

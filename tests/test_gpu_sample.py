@@ -100,6 +100,25 @@ def test_masked_and_odd_logits(gpu):
             check(gpu, z, r.random(12), **kw)
 
 
+@pytest.mark.parametrize("vocab", [700, 9001, 128256, 400001])
+def test_a_prefix_that_reaches_top_p_exactly(gpu, vocab):
+    """Some equal logits and the rest so far below that it weighs nothing (each token less than a unit of 2^-44, as the call defines its
+    weights): half of the equal ones reach one half, no token more."""
+    r = rng(12)
+    for far in (-1000.0, -60.0, -41.0, -28.0):
+        for n, parts in ((2, (0.5,)), (4, (0.25, 0.5, 0.75)), (8, (0.125, 0.625)), (64, (0.5, 0.25))):
+            z = np.full((4, vocab), far, np.float32)
+            for row in z:
+                row[r.choice(vocab, n, replace=False)] = 3.0
+            for p in parts:
+                for kw in (dict(), dict(top_k=650), dict(top_k=n), dict(min_p=1e-3)):
+                    tok, probs = call(gpu, z, [0.0, 0.3, 0.7, 1 - 2.0 ** -24], top_p=p, **kw)
+                    want = [sorted(np.flatnonzero(row == 3.0)[:int(n * p)]) for row in z]
+                    at = [0, int(0.3 * n * p), int(0.7 * n * p), int(n * p) - 1]
+                    assert list(tok) == [w[i] for w, i in zip(want, at)], (far, n, p, kw)
+                    assert (np.abs(probs - 1 / (n * p)) <= 2.0 ** -23).all()
+
+
 @pytest.mark.parametrize("t", [1.4e-45, 1e-44, 1e-40, 1e-38, 1.3e-37, 1e-36, 1e30, 1e37, 3.4e38])
 def test_temperatures_at_the_ends(gpu, t):
     """Logits of the temperature's own size, near both ends of f32: their quotients are ordinary numbers."""
