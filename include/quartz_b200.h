@@ -262,9 +262,9 @@ void cuda_attn_prompt(float *out, const float *q, const float *k_cache, const fl
  *                           of the library, one for every graph that is being captured (graphs may replay side by side,
  *                           two executables of one captured graph may not), one for each of the first 16 streams of a
  *                           device that ask for it, one for all later ones, whose calls then follow one another.
- *                           Products carry 22 bits and sums are f32.  Of a position's weight times its step in a
- *                           group, these are 22 bits down to 2^-14 of the largest step that the group has in the
- *                           context, and an error of 2^-35 of that step below.
+ *                           Products carry 22 bits and sums are f32.  Of a position's weight (the largest counting as
+ *                           1) times its step in a group, these are 22 bits down to 2^-14 of the largest step that the
+ *                           group has in the context, and an error of 2^-35 of that step below.
  *   cuda_attn_prompt_kv4    cuda_attn_prompt over such a cache (rows appended before, e.g. by cuda_rope_kv4_rows).  Products
  *                           carry 22 bits, sums are f32; where 64 neighbouring positions hold a step above 8188 (values
  *                           that span 122820), their steps and minima below 2^-11 are taken to 2^-22 */

@@ -8,7 +8,8 @@
 
 namespace qz {
 
-// six warps: two CTAs of them per SM leave 168 registers a thread (eight: 128, which spill; 131072 positions take 58 us, not 51)
+// six warps: two CTAs of them per SM leave 168 registers a thread (12 bytes of a thread are spilled; eight warps leave 128, which
+// spill far more: 131072 positions take 58 us, not 51)
 constexpr int AK_THREADS = 192, AK_WARPS = AK_THREADS / 32;
 constexpr int AK_MAX_G = 16;
 constexpr float AK_RAISE = 2.f;                       // weights are at most 2^AK_RAISE,
@@ -63,10 +64,11 @@ struct AttnKv4Args {
 // harm, and f16 has as many binades more for small ones.  With the largest step that the warp has met in a group at 2^11 or
 // above, 22 bits of p d are whole down to 2^-14 of that step (p d = 2^-3), and below that the error is 2^-35 of it at most.
 //
-// Measured (32 / 8 heads of 128, replayed): context 1024 6.3 us (8 / 2 heads of 64, context 18: 4.4), 4096 10.6,
-// 16384 13.9, 131072 51 us = 3.3 TB/s of the cache.  Short contexts are bound by the launch, two cluster barriers and one
-// block's latency; long ones by instruction issue: a warp spends some 400 instructions on a tile of 16 positions (unpacking,
-// the hi / lo parts, 24 MMAs) at 0.55 per cycle and scheduler; the same launch that only loads takes 32 us.
+// Measured (32 / 8 heads of 128, replayed over caches that together exceed L2): context 1024 6.0 us (8 / 2 heads of 64, context 18:
+// 4.0), 4096 10.7, 16384 14.9 (13.4 from L2), 131072 51 us = 3.3 TB/s of the cache.  Short contexts are bound by the launch, two cluster
+// barriers and one block's latency; long ones by the warps' dependent instructions: a warp spends some 400 on a tile of 16
+// positions (unpacking, the hi / lo parts, 24 MMAs), three warps a scheduler issue 0.52 a cycle; the same launch that only loads
+// takes 32 us.
 // Clusters join a unit only when every warp still has a block: at twice that 16384 positions take 14.2 us, 8192 13.4 (12.3).
 __host__ __device__ constexpr int attn_kv4_stages(int NG) { return NG == 1 ? 8 : NG == 2 ? 4 : 2; }   // ~10 KB in flight per warp
 

@@ -29,10 +29,11 @@
 // group that is NaN is taken as zero by the MMA (0 * NaN would reach rows that do not see it) and noted in a bit mask,
 // from which the rows that see it are set to NaN.
 //
-// Measured (32 / 8 heads of 128, replayed): 512 tokens 20.7 us, 2048 123 us = 168 TF of attention, 505 TF with the three
-// products; 512 tokens at 16000 398 us.  Bound by the unpacking and softmax warps' issue and by shared memory: a tile takes
-// some 3000 cycles, of which the MMAs need 816, its operands' way through shared memory some 1350.  Tried: weights before
-// the maximum is known, repeated when it rises (2048 tokens: 137 us); parameters checked by a warp of their own (124 us).
+// Measured (32 / 8 heads of 128, replayed): 512 tokens 21.8 us, 2048 122 us = 281 TF of attention, 843 TF with the three
+// products; 512 tokens at 16000 404 us, 338 TF.  Bound by the unpacking and softmax warps' issue and by shared memory: a tile takes
+// some 3600 cycles, of which the MMAs need 1660 (13.6 MFLOP at 8192 a cycle), its operands' way through shared memory some
+// 1350; the tensor pipe is active 44 % of the time.  Tried: weights before the maximum is known, repeated when it rises (2048
+// tokens: 137 us); parameters checked by a warp of their own (124 us).
 #pragma once
 
 #include "attn_kv4.cuh"

@@ -74,8 +74,9 @@ StepShape step_shape(int units, int n_blocks, int GV)
     while (i > 0 && (f[i] < units || (1 << (i - 1)) >= n_blocks)) i--;
     // Of more than four query heads per kv head one CTA fits an SM, and clusters of 8 may leave half of them out (8 units: 64
     // CTAs against 128).  Narrower ones pay once a context is long, which the shape knows by the cache only: 64 / 8 heads
-    // of 128 at 131072 positions 94 us against 172, at 8192 16.5 against 18.4, at 2048 15.0 against 10.8; 28 / 4 (96 CTAs
-    // against 128) 53 against 64, 16.4 against 16.3 at 16384, 14.5 against 10.2 at 2048.
+    // of 128 at 131072 positions 95 us against 172, at 8192 16.9 against 18.4; 28 / 4 (96 CTAs against 128) 54 against 64, at 16384
+    // 16.4 against 16.3.  The price is paid where the context is short and the cache is not: at 2048 of 131072 positions 15.4 us
+    // against 10.7, 28 / 4 14.4 against 10.2.
     if (i == 3) {
         const int wide = (f[3] / units) << 3, narrow = (f[2] / units) << 2;
         if (2 * narrow >= 3 * wide ? n_blocks >= 256 : 4 * narrow >= 5 * wide && n_blocks >= 1024) i = 2;

@@ -19,9 +19,9 @@
 //   parameters: NG halves m, then NG halves d.
 //
 // Writing and reading are bound by HBM: 4 bytes on one side, 0.625 on the other.  Eight dims per thread make every access
-// of a warp whole sectors.  8192 rows of 8 heads of 128: written 20.1 us, 3.9 TB/s (bound by the quantiser's issue slots as much as
-// by HBM; 64-bit borders for every code and clamps took 21.3), read back 15.6 us, 5.0 TB/s; 8189 of 4 heads of 96: 8.7 and 7.6
-// us; a few rows are bound by the launches (1.4 and 1.0 us in a replayed graph).
+// of a warp whole sectors.  Over rows that together exceed L2, 8192 of 8 heads of 128: written 20.3 us, 3.8 TB/s (bound by the
+// quantiser's issue slots as much as by HBM; 64-bit borders for every code and clamps took 21.3), read back 15.8 us, 4.9 TB/s; 8189 of 4
+// heads of 96: 8.8 and 7.9 us; a few rows are bound by the launches (1.3 and 1.0 us in a replayed graph).
 #pragma once
 
 #include "activation.cuh"
@@ -192,7 +192,7 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(float *__restrict__ k, fl
 
 // cuda_rope_kv_rows with a 4-bit cache: token blockIdx.x at position pos0 + blockIdx.x; q and k rotated in place (theta <= 0: left
 // as they are), k and v quantised.  The angles of a token are computed once for all of its rows: 512 tokens of 32 / 8
-// heads of 128 take 5.4 us (4.4 TB/s), 8192 take 61 (6.3 TB/s; at 57 registers instead of 40 69 us); one block per row, as the f32 form has it, took 21.7 and 338, most
+// heads of 128 take 6.1 us (3.9 TB/s; 5.4 from L2), 8192 take 61 (6.2 TB/s; at 57 registers instead of 40 69 us); one block per row, as the f32 form has it, took 21.7 and 338, most
 // of it for angles and for starting blocks.
 // Rows are q's, k's, then v's; 4 NG threads share one, each with four pairs, two vectors of four dims.  grid.y blocks share
 // a token's rows where there are few tokens.

@@ -12,7 +12,8 @@
 // With c = 32 log2(e) / T as a sum of two f32 numbers, z c is a whole number k and a rest f, |f| < 0.8: one FMA rounds z c to
 // k, two more give f with an error of 2^-26.  The weight is then 2^((k - k_M) / 32), from a table of 32 and a shift, times
 // 2^((f - f_M) / 32): the table carries f_M, four terms of the exponential's series give the rest (|y| < 0.017: 1e-11), and
-// only table times series is taken in 32 bits, so a weight is right to 2^-28.  (CUDA's exp in 64 bits took twice the time
+// only table times series is taken in 32 bits, two roundings of half a unit in 2^26 to 2^27: a weight is right to 2^-26, to 2^-28 as a
+// rule.  (CUDA's exp in 64 bits took twice the time
 // of the rest.)  Where z c passes 2^22, at temperatures near 0 or logits of any size, M - z takes the place of z, exact as two
 // f32 numbers, times a power of two that brings c to [1, 2) (c itself leaves f32 at temperatures below 2^-122).  Why so exact: with thousands of tokens kept, an error of 1e-7 in their sums would move the border of top_p, or
 // the token that u falls on, once in some thousand rows.  b = k_M - k is also the bin in which tokens are counted: it follows
@@ -70,10 +71,11 @@ __device__ __forceinline__ float smp_unkey(uint32_t k) { return __uint_as_float(
 // A bin with more tokens than the list takes (ties, high temperatures) is divided further, by the number itself.
 // A histogram is reduced in slices, one per CTA, that are pushed to every CTA: all find the same bin without asking.
 //
-// Measured (128256 tokens, replayed): one row, top_k 40 12.3 us, top_p alone 20.8, no filter 8.3; 256 rows, top_k 139 us,
-// top_p 255, no filter 114, temperature 0 47 us = 2.8 TB/s.  One row is bound by cluster barriers (five or six, 1 to 2 us each),
-// many rows by instruction issue and the histogram's shared-memory atomics (two per token) between the same barriers: two
-// CTAs of an SM, of different rows, are all there is to overlap them (a part of a row and the histograms take 107 KB).
+// Measured (128256 tokens, replayed): one row, top_k 40 12.3 us, top_p alone 21.4, no filter 8.2; 256 rows, top_k 142 us,
+// top_p 266, no filter 117, temperature 0 47 us = 2.8 TB/s.  One row is bound by cluster barriers (five or six, 1 to 2 us each),
+// many rows by instruction issue (150 a warp and 32 tokens with top_p) and the histogram's shared-memory atomics (two per token)
+// between the same barriers: two CTAs of an SM, of different rows, are all there is to overlap them (a part of a row and the
+// histograms take 107 KB).  Sizes cut to whole units cost 2 per cent of top_p, the barrier that every CTA runs 1.
 constexpr int SMP_PER = 3, SMP_BINS = SMP_PER * SMP_THREADS, SMP_LIST = 512;   // (a thread looks after three bins, and one token of the list)
 constexpr int SMP_WARPS = SMP_THREADS / 32, SMP_MAX_CLUSTER = 16;
 static_assert(SMP_BINS >= 32 * 46 && SMP_BINS % SMP_MAX_CLUSTER == 0, "bins cover weights down to 2^-45");
