@@ -295,7 +295,8 @@ void cuda_attn_prompt_kv4(float *out, const float *q, const void *d_cache, int n
  * cuda_sample_supported: 1 if cuda_sample takes this vocabulary and these settings (top_p and min_p are numbers); what it
  * does not take it refuses, and writes no token.
  * cuda_step_advance: d_step[0] = *d_token (left as it is if that is negative), d_step[1] += 1, and the registered RoPE
- * tables of d_step (cuda_step_rope_table) for the new position: the device-side cuda_step_set, on the same stream. */
+ * tables of d_step (cuda_step_rope_table) for the new position: the device-side cuda_step_set, on the same stream.  What
+ * follows looks the token up unchecked: *d_token is negative or a token of the vocabulary, as cuda_sample writes it. */
 int cuda_sample_supported(int vocab, float temperature, float top_p, float min_p);
 void cuda_sample(const float *d_logits, int n_rows, int vocab, size_t row_stride, float temperature, int top_k, float top_p, float min_p,
                  const float *d_u, int *d_tokens, float *d_probs);
@@ -372,7 +373,8 @@ void cuda_host_free(void *p);
  * cuda_d2h_async may be recorded), and every scratch buffer must
  * already exist (run the sequence once eagerly first).  end returns an executable graph (NULL on
  * failure); launch replays it, ordered with the library's stream (the default one, or what quartz_set_stream
- * set): behind the calls before it, ahead of those after it.  Replays of all graphs follow one another. */
+ * set): behind the calls before it, ahead of those after it.  Replays of all graphs follow one another.  A graph is not
+ * launched inside a capture, its own or one of that stream's: that is refused, and the capture goes on. */
 /* 1 (default): kernels recorded into a graph are launched as programmatic dependents, so each
  * may begin (and a GEMV may start streaming its weights) while its predecessor drains; 0: plain
  * serial edges.  Results are identical. */

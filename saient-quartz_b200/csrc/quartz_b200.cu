@@ -2096,6 +2096,12 @@ void quartz_graph_launch(void *graph_exec)
     // stream is ordered with it by itself, any other one that is set by events on both sides of the replay.
     static cudaEvent_t event = nullptr;
     const bool join = g_stream != 0 && g_stream != g_graph_stream;
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    if (join && cudaStreamIsCapturing(g_stream, &status) != cudaSuccess) cudaGetLastError();
+    if (g_capturing || status != cudaStreamCaptureStatusNone) {   // (the launch would end that capture)
+        set_error(QZ_ERR_BAD_SHAPE, "quartz_graph_launch: a recorded graph cannot be launched while the stream is being captured");
+        return;
+    }
     if (join && !event) {
         QZ_CUDA_CHECK(cudaEventCreateWithFlags(&event, cudaEventDisableTiming));
         if (!event) return;

@@ -154,6 +154,46 @@ def test_a_replay_is_ordered_with_the_stream_that_is_set(gpu):
     gpu.check_error()
 
 
+def test_a_replay_inside_a_capture_is_refused(gpu):
+    """In the library's own recording and in one of the caller's stream: nothing is launched, and what is captured stays whole."""
+    import torch
+    L, n = gpu.lib(), 1 << 10
+    a, b = (gpu.GpuBuf.upload(np.full(n, x, np.float32)) for x in (5.0, 3.0))
+
+    def refused():
+        assert L.quartz_last_error() == 2 and b"captured" in L.quartz_error_string()
+        L.quartz_clear_error()
+    assert L.quartz_graph_begin()
+    L.cuda_vec_add(a.ptr, b.ptr, n)
+    graph = L.quartz_graph_end()
+    assert L.quartz_graph_begin()
+    L.quartz_graph_launch(graph)
+    L.cuda_vec_add(a.ptr, b.ptr, n)
+    other = L.quartz_graph_end()
+    assert other
+    refused()
+    L.quartz_graph_launch(other)
+    assert (a.download() == 8).all()
+    st, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    try:
+        with torch.cuda.graph(g, stream=st):
+            L.quartz_set_stream(torch.cuda.current_stream().cuda_stream)
+            L.cuda_vec_add(a.ptr, b.ptr, n)
+            L.quartz_graph_launch(graph)
+            L.cuda_vec_add(a.ptr, b.ptr, n)
+    finally:
+        L.quartz_set_stream(None)
+    refused()
+    g.replay()
+    torch.cuda.synchronize()
+    assert (a.download() == 14).all()
+    L.quartz_graph_launch(graph)
+    assert (a.download() == 17).all()
+    for x in (graph, other):
+        L.quartz_graph_destroy(x)
+    gpu.check_error()
+
+
 @pytest.mark.parametrize("kv_bits", [4, 32])
 def test_generate_on_a_stream_of_the_callers(gpu, oracle_mod, kv_bits):
     import torch
